@@ -298,8 +298,8 @@ class ALSEngine:
         self._parts_cache = {}
         self._side = None
         # Overlap of the exchange of row chunk c with the sweep of chunk c + 1, as measured on one MI355X with a stand-in
-        # of RCCL's kernel (tools/overlap_probe.py; its workgroups of 256 threads and 261-280 registers need a wholly
-        # free compute unit each):
+        # for its kernel at the worst-case size (tools/overlap_probe.py; workgroups of 256 threads and 288 registers, which
+        # need a wholly free compute unit each):
         #  * the collective and the next sweep become runnable at the same instant, when the chip drains - and the sweep's
         #    tens of thousands of small workgroups take every unit first, after which the collective finds no free
         #    unit until that sweep has ENDED (f = 64: done 10.8 ms after the event instead of 4.5).  Hence the gap: the

@@ -8,8 +8,8 @@ collective: user half-sweep of the 1.25 M x 1 M block (f = 128) on the main stre
 side stream submitted `--delay-ms` after the sweep was queued, i.e. while its persistent kernel runs; reported per reserve_cus: the sweep's duration and the time from
 the sweep's start to the copy's end (alone, the copy takes `copy_alone_ms`).  Two stand-ins: the runtime's own copy
 kernel (a handful of registers: it fits into the 40 registers the stream kernel leaves on a SIMD) and
-tools/ubench/probe_copy.hip with the footprint of an RCCL kernel (`--blocks` workgroups of 256 threads, 288 vector
-registers, 16 KB of LDS: one workgroup fills a compute unit, as rcclGenericKernel does), built with the hipcc line in that file.
+tools/ubench/probe_copy.hip at the worst-case size (`--blocks` workgroups of 256 threads, 288 vector
+registers, 16 KB of LDS: one workgroup fills a compute unit), built with the hipcc line in that file.
 
     python tools/overlap_probe.py [--reserve 0 4 8 16 32] [--mb 640] [--blocks 32]
 """
@@ -79,12 +79,12 @@ def main():
             assert rc == 0, rc
 
     out = {"f": f, "high_priority_side_stream": args.high_priority, "copy_mb": args.mb, "blocks": args.blocks, "threads": args.threads, "delay_ms": args.delay_ms, "runs": []}
-    for kind in ("runtime", "rccl_like"):
+    for kind in ("runtime", "whole_unit"):
         copy(kind); torch.cuda.synchronize()
         a, b = ev(), ev()
         a.record(); copy(kind); b.record(); torch.cuda.synchronize()
         out["copy_alone_ms_" + kind] = a.elapsed_time(b)
-    for kind, short in (("runtime", True), ("rccl_like", True), ("rccl_like", False)):
+    for kind, short in (("runtime", True), ("whole_unit", True), ("whole_unit", False)):
         if short and not (can_short and f > 64):
             continue
         for res in args.reserve:
@@ -123,7 +123,7 @@ def main():
                 with torch.cuda.stream(side):
                     h0.record(side)
                     if held:
-                        copy("rccl_like", blocks=held, passes=args.hold_passes)
+                        copy("whole_unit", blocks=held, passes=args.hold_passes)
                     h1.record(side)
                 time.sleep(0.0005)
                 e0.record(main_s)
@@ -152,7 +152,7 @@ def main():
                 side.wait_event(e1)
                 with torch.cuda.stream(side):
                     released = side.record_event() if args.gap_event else None
-                    copy("rccl_like", passes=args.pattern_passes)
+                    copy("whole_unit", passes=args.pattern_passes)
                     c1.record(side)
                 if released is not None:
                     main_s.wait_event(released)             # main stream: goes on when the side stream has been released
