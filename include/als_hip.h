@@ -381,6 +381,44 @@ int32_t als_recommend_topk_prepared_f32(const float *X, int64_t ldx, const int64
                                         const void *prepared, int64_t M, int32_t f, int32_t k, const int64_t *ex_rowptr,
                                         const int32_t *ex_col, int32_t ex_by_user_id, int32_t *idx_out, float *score_out,
                                         int32_t *overflow_out, void *workspace, size_t ws_bytes, void *stream);
+/* ------------------------------------------------------------------------------------
+ * Random draws from score rows (no reference counterpart: the reference always shows the ranked list).
+ *
+ * als_sample_rows draws n_draws columns, with replacement, from every row of `scores` ([n_rows, lds] row major, dtype
+ * float32, float16 or bfloat16; as als_scores_f32 leaves them) by the softmax of the row at a temperature T, cut by
+ * min-p, top-k and top-p in this order.  With x_i = (s_i - max s) / T and w_i = exp(x_i), rank order = score descending,
+ * ties by ascending column:
+ *     items with w_i < min_p are dropped; of the rest the first top_k stay; of those the shortest prefix in rank order
+ *     whose weight reaches top_p of theirs (at least one item);
+ *     with W the weight of what is left, draw d of row r is the first item in rank order at which the running weight
+ *     exceeds u[r, d] W, and logp_out[r, d] = ln(w / W) of that item.
+ * min_p <= 0, top_k <= 0 and top_p >= 1 switch a filter off, as a NaN does; min_p > 1 acts as 1, top_p < 0 as 0.  T not
+ * above 0 (or NaN) takes the best item, logp 0.  u is float32 or float64 in [0, 1), row major [n_rows, n_draws]; a value
+ * outside is taken as the nearer end, NaN as 0.  -inf and NaN scores are never drawn; a row of nothing else gives
+ * column -1 and logp -inf.  +inf scores share all the weight.  Weights are summed as integers of 2^-Q of the largest,
+ * Q = min(51, 62 - ceil(log2 M)); an item below half of that counts as dropped.  The answer depends on the row and its
+ * parameters alone.
+ * opts      [host] one value for all rows, or a [device] array with one per row where the pointer is not NULL.
+ * ex_*      as als_topk_rows_f32: those columns are set to -inf first, in place; columns outside [0, M) are ignored.
+ * All other pointers are [device].
+ * ------------------------------------------------------------------------------------ */
+#define ALS_DTYPE_F32 0
+#define ALS_DTYPE_F16 1
+#define ALS_DTYPE_BF16 2
+typedef struct {
+    float temperature;
+    int32_t top_k;
+    float top_p;
+    float min_p;
+    const float *temperature_rows;
+    const int32_t *top_k_rows;
+    const float *top_p_rows;
+    const float *min_p_rows;
+} als_sample_opts_t;
+int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows, int64_t M, const int64_t *ex_rowptr,
+                        const int32_t *ex_col, const int64_t *ex_row_ids, const als_sample_opts_t *opts, const void *u,
+                        int32_t u_is_f64, int32_t n_draws, int32_t *idx_out, float *logp_out, void *stream);
+
 int32_t als_predict_pairs_f32(const float *X, int64_t ldx, const float *Y, int64_t ldy, const int64_t *u,
                               const int64_t *i, int64_t n, int32_t f, float *out, void *stream);
 int32_t als_normalize_rows_f32(const float *E, int64_t lde, int64_t n, int32_t f, float *out, int64_t ldo,

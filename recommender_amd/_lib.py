@@ -26,6 +26,7 @@ SHORT_MAX_GROUPS = 8
 ABI_VERSION = 8          # als_abi_version() of the library this binding is written for (struct layouts included)
 ACCUMULATE_MODES = {"default": 0, "bf16x3": 1, "fp32": 2, "fp16x2": 3}
 ROW_KERNELS = {"auto": 0, "wave": 1, "stream": 2}
+DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}      # score rows of the softmax operators
 CG_FORMS = {"auto": 0, "lock_step": 1, "matrix": 2}
 
 c_i32, c_i64, c_f32, c_sz, c_vp = ctypes.c_int32, ctypes.c_int64, ctypes.c_float, ctypes.c_size_t, ctypes.c_void_p
@@ -52,6 +53,7 @@ SIGNATURES = {
                                                 c_vp, c_vp, c_vp, c_sz, c_vp]),
     "als_recommend_topk_f32": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i32, c_i32, c_vp, c_vp, c_i32, c_vp,
                                        c_vp, c_vp, c_vp, c_sz, c_vp]),
+    "als_sample_rows": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp]),
     "als_predict_pairs_f32": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_vp, c_vp]),
     "als_normalize_rows_f32": (c_i32, [c_vp, c_i64, c_i64, c_i32, c_vp, c_i64, c_vp]),
     "als_half_sweep_workspace_bytes": (c_sz, [c_i64, c_i64, c_i32]),
@@ -78,6 +80,12 @@ class SweepOpts(ctypes.Structure):
     _fields_ = [("accumulate", c_i32), ("row_kernel", c_i32), ("tap_begin", c_vp), ("tap_end", c_vp),
                 ("max_rating", c_f32), ("whitened", c_vp), ("ld_whitened", c_i64), ("short_bounds", c_vp),
                 ("reserve_cus", c_i32)]
+
+
+class SampleOpts(ctypes.Structure):
+    """als_sample_opts_t of include/als_hip.h."""
+    _fields_ = [("temperature", c_f32), ("top_k", c_i32), ("top_p", c_f32), ("min_p", c_f32), ("temperature_rows", c_vp),
+                ("top_k_rows", c_vp), ("top_p_rows", c_vp), ("min_p_rows", c_vp)]
 
 
 class AlsHipError(RuntimeError):

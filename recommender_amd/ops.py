@@ -599,6 +599,89 @@ def topk_rows(score_rows, k, exclude=None, exclude_rows=None):
     return idx, val
 
 
+def _score_rows(t, name):
+    """Row-major score rows of one of the three score types; returns (dtype code, leading dimension)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda:
+        raise ValueError("%s must be a CUDA/HIP tensor" % name)
+    if t.dtype not in _lib.DTYPES:
+        raise ValueError("%s must be float32, float16 or bfloat16, got %s" % (name, t.dtype))
+    if t.dim() != 2:
+        raise ValueError("%s must be 2-dimensional" % name)
+    n, M = t.shape
+    if M < 1:
+        raise ValueError("%s have no columns" % name)
+    if (M > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < M):
+        raise ValueError("%s must be row-major with unit inner stride (rows that overlap are not)" % name)
+    return _lib.DTYPES[t.dtype], (t.stride(0) if n > 1 else M)
+
+
+def _row_param(v, n, dtype, name, like):
+    """A parameter of the sampling: (scalar, None), or (0, tensor) with one value per row."""
+    if torch.is_tensor(v) and v.dim():
+        _index(v, dtype, name)
+        if v.shape[0] != n:
+            raise ValueError("%s must have one value per row" % name)
+        _same_device(like, v)
+        return 0, v
+    return (int(v) if dtype == torch.int32 else float(v)), None
+
+
+def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, exclude=None, exclude_rows=None):
+    """Random columns of every score row (float32, float16 or bfloat16), drawn from the row's softmax at `temperature` cut
+    by min_p, top_k and top_p in this order (als_sample_rows in include/als_hip.h has the definition).  u: the random
+    numbers, float32 or float64 in [0, 1), [n] for one draw per row or [n, d] for d draws with replacement.
+    temperature, top_k, top_p, min_p: one value for all rows, or a device tensor with one per row (float32; top_k int32);
+    top_k = 0, top_p = 1 and min_p = 0 are off, temperature = 0 takes the best item.
+    exclude / exclude_rows: as topk_rows (those columns are set to -inf in the score rows first).
+    Returns (idx int32, logp float32), shaped like u: the column and the logarithm of its probability; a row with
+    nothing to draw (all -inf or NaN) gives -1 and -inf.  The same inputs give the same draws, whatever else the call
+    holds."""
+    dtype, ld = _score_rows(score_rows, "score_rows")
+    n, M = score_rows.shape
+    if not isinstance(u, torch.Tensor) or u.dtype not in (torch.float32, torch.float64):
+        raise ValueError("u must be a float32 or float64 tensor")
+    if u.dim() not in (1, 2) or u.shape[0] != n or (u.dim() == 2 and u.shape[1] < 1):
+        raise ValueError("u must be [n_rows] or [n_rows, n_draws]")
+    if not u.is_cuda or not u.is_contiguous():
+        raise ValueError("u must be a contiguous CUDA/HIP tensor")
+    t, t_rows = _row_param(temperature, n, torch.float32, "temperature", score_rows)
+    k, k_rows = _row_param(top_k, n, torch.int32, "top_k", score_rows)
+    p, p_rows = _row_param(top_p, n, torch.float32, "top_p", score_rows)
+    m, m_rows = _row_param(min_p, n, torch.float32, "min_p", score_rows)
+    if not t >= 0:
+        raise ValueError("temperature must be >= 0")
+    if not 0 <= k < 2 ** 31:
+        raise ValueError("top_k must be >= 0 (0: off)")
+    if not (0 <= p <= 1 and 0 <= m <= 1):
+        raise ValueError("top_p and min_p must lie in [0, 1]")
+    ex_ptr = ex_col = None
+    if exclude is not None:
+        ex_ptr, ex_col = exclude
+        _index(ex_ptr, torch.int64, "exclude rowptr")
+        _index(ex_col, torch.int32, "exclude col")
+        if exclude_rows is not None:
+            _index(exclude_rows, torch.int64, "exclude_rows")
+            if exclude_rows.shape[0] != n:
+                raise ValueError("exclude_rows must have one entry per score row")
+            if n and (int(exclude_rows.min()) < 0 or int(exclude_rows.max()) + 1 >= ex_ptr.shape[0]):
+                raise ValueError("exclude_rows points outside the exclusion CSR")
+        elif ex_ptr.shape[0] != n + 1:
+            raise ValueError("exclude rowptr must have n_rows + 1 entries")
+    elif exclude_rows is not None:
+        raise ValueError("exclude_rows without exclude")
+    _same_device(score_rows, u, ex_ptr, ex_col, exclude_rows)
+    idx = torch.empty(u.shape, dtype=torch.int32, device=score_rows.device)
+    logp = torch.empty(u.shape, dtype=torch.float32, device=score_rows.device)
+    if n == 0:
+        return idx, logp
+    opts = _lib.SampleOpts(t, k, p, m, *(x.data_ptr() if x is not None else None for x in (t_rows, k_rows, p_rows, m_rows)))
+    with torch.cuda.device(score_rows.device):
+        check(lib.als_sample_rows(_ptr(score_rows), dtype, ld, n, M, _ptr(ex_ptr), _ptr(ex_col), _ptr(exclude_rows),
+                                  ctypes.byref(opts), _ptr(u), int(u.dtype == torch.float64), u.numel() // n, _ptr(idx),
+                                  _ptr(logp), _stream()), "als_sample_rows")
+    return idx, logp
+
+
 def predict_pairs(X, Y, u, i):
     """out[p] = <X[u[p]], Y[i[p]]>: the ALS model's output for explicit (user, item) pairs
     (reclibwh/core/ALS.py:359-362)."""
