@@ -419,6 +419,26 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
                         const int32_t *ex_col, const int64_t *ex_row_ids, const als_sample_opts_t *opts, const void *u,
                         int32_t u_is_f64, int32_t n_draws, int32_t *idx_out, float *logp_out, void *stream);
 
+/* ------------------------------------------------------------------------------------
+ * Following a teacher's ranked lists (no reference counterpart): how far a student's softmax over all items is from a
+ * teacher's softmax over the few items it lists (what als_recommend_topk_f32 returned for a larger model, say), and the
+ * gradient of that.  Per row, at temperature T (> 0, finite):
+ *     t_j = softmax of teacher_val / T over the row's list,   q_i = softmax of the student's scores / T over all M items
+ *     loss = sum_j t_j (ln t_j - ln q_j),                     slope_i = weight (q_i - t_i) / T   (t_i = 0 off the list)
+ * teacher_idx / teacher_val [n_rows, ld_teacher] int32 / float32, the first k (<= 1024) of a row; an index outside [0, M)
+ * is padding, of an item listed twice the first entry stands.  A list without entries (or whose values are all -inf)
+ * gives loss 0 and gradient 0.  weight: float32 per row, or NULL for 1.  A student score of -inf has q = 0 (and makes the
+ * loss +inf if the teacher lists it with t > 0); NaN or +inf scores make their row NaN.
+ *
+ * als_distill_rows   the scores are given, [n_rows, lds] row major in float32, float16 or bfloat16; grad_out [n_rows, ldg]
+ *                    of the same type receives slope and may be `scores` itself (same ld).  Sums are float32 in runs of 4
+ *                    or 8 items, float64 above, in an order set by M and the row's address modulo 16 alone.
+ * ------------------------------------------------------------------------------------ */
+size_t als_distill_rows_workspace_bytes(int32_t dtype, int64_t n_rows, int64_t M, int32_t k);
+int32_t als_distill_rows(const void *scores, int32_t dtype, int64_t lds, int64_t n_rows, int64_t M, const int32_t *teacher_idx,
+                         const float *teacher_val, int64_t ld_teacher, int32_t k, float temperature, const float *weight,
+                         float *loss_out, void *grad_out, int64_t ldg, void *workspace, size_t ws_bytes, void *stream);
+
 int32_t als_predict_pairs_f32(const float *X, int64_t ldx, const float *Y, int64_t ldy, const int64_t *u,
                               const int64_t *i, int64_t n, int32_t f, float *out, void *stream);
 int32_t als_normalize_rows_f32(const float *E, int64_t lde, int64_t n, int32_t f, float *out, int64_t ldo,

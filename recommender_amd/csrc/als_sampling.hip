@@ -63,7 +63,7 @@ __device__ __forceinline__ uint32_t rank_key(const float s) {
 
 struct Picked {
     u64 before, weight;       // running weight in front of the item, its own
-    int64_t index;
+    int32_t index;
 };
 
 struct SampleShared {
@@ -169,77 +169,62 @@ template <int TYPE, int NV>
 struct RowStore {
     RowView<TYPE> view;
     row_u32x4 held[NV ? NV : 1];
+    float extra;
+    int32_t extra_at;
 
     __device__ __forceinline__ RowStore(const RowView<TYPE> &v) : view(v) {
         if constexpr (NV > 0) {
 #pragma unroll
-            for (int q = 0; q < NV; ++q) held[q] = view.load((int64_t)q * SR_THREADS + threadIdx.x);
+            for (int q = 0; q < NV; ++q) {
+                held[q] = RowView<TYPE>::nothing();
+                if (q * SR_THREADS + (int)threadIdx.x < view.n_chunks) held[q] = view.load(q * SR_THREADS + threadIdx.x);
+            }
         }
+        extra_at = view.extra(threadIdx.x);
+        extra = extra_at >= 0 ? view.at(extra_at) : -__builtin_inff();
     }
-    // f(score, index) for this thread's elements, in index order
+    // f(score, index) for this thread's elements; what lies outside the row comes as -inf
     template <class F>
     __device__ __forceinline__ void each(F f) const {
         if constexpr (NV > 0) {
 #pragma unroll
             for (int q = 0; q < NV; ++q) {
-                const int64_t i0 = view.index0((int64_t)q * SR_THREADS + threadIdx.x);
+                const int32_t i0 = view.index0(q * SR_THREADS + threadIdx.x);
 #pragma unroll
                 for (int e = 0; e < RowView<TYPE>::VEC; ++e) f(RowView<TYPE>::value(held[q], e), i0 + e);
             }
         } else {
-            for (int64_t q = threadIdx.x; q < view.n_chunks; q += SR_THREADS) {
+            for (int32_t q = threadIdx.x; q < view.n_chunks; q += SR_THREADS) {
                 const row_u32x4 v = view.load(q);
-                const int64_t i0 = view.index0(q);
+                const int32_t i0 = view.index0(q);
 #pragma unroll
                 for (int e = 0; e < RowView<TYPE>::VEC; ++e) f(RowView<TYPE>::value(v, e), i0 + e);
             }
         }
+        if ((int)threadIdx.x < view.head + view.tail) f(extra, extra_at);
     }
 };
 
 // Index of the m-th element (from 0, in index order) whose key is `key`; the rarest path: more than SR_LIST items of one
-// bucket share one score.
+// bucket share one score.  An element per thread and round.
 template <int TYPE>
-__device__ int64_t nth_of_key(const RowView<TYPE> &view, const uint32_t key, u64 m, SampleShared &sh) {
+__device__ int32_t nth_of_key(const RowView<TYPE> &view, const uint32_t key, const u64 m, SampleShared &sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (tid == 0) sh.picked.index = -1;
     u64 seen = 0;
-    for (int64_t q0 = 0; q0 < view.n_chunks; q0 += SR_THREADS) {
-        const row_u32x4 v = view.load(q0 + tid);
-        unsigned mask = 0;
-#pragma unroll
-        for (int e = 0; e < RowView<TYPE>::VEC; ++e)
-            if (rank_key(RowView<TYPE>::value(v, e)) == key) mask |= 1u << e;
-        if (!view.whole(q0 + tid)) {                         // what reads as -inf beyond the row's ends is no item
-#pragma unroll
-            for (int e = 0; e < RowView<TYPE>::VEC; ++e) {
-                const int64_t i = view.index0(q0 + tid) + e;
-                if (i < 0 || i >= view.M) mask &= ~(1u << e);
-            }
-        }
-        const uint32_t own = __popc(mask);
-        uint32_t c = own;
-#pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const uint32_t cc = (uint32_t)__shfl_up((int)c, o);
-            if (lane >= o) c += cc;
-        }
+    for (int64_t i0 = 0; i0 < view.M; i0 += SR_THREADS) {
+        const int64_t i = i0 + tid;
+        const bool hit = i < view.M && rank_key(view.at(i)) == key;
+        const u64 mask = __ballot(hit);
         __syncthreads();                                     // the last round's wave sums have been read
-        if (lane == 63) sh.wave_c[wave] = c;
+        if (lane == 0) sh.wave_c[wave] = __popcll(mask);
         __syncthreads();
-        u64 before = seen + c - own;
-        u64 total = 0;
+        u64 before = seen + __popcll(mask & ((1ull << lane) - 1));
         for (int x = 0; x < SR_WAVES; ++x) {
             if (x < wave) before += sh.wave_c[x];
-            total += sh.wave_c[x];
+            seen += sh.wave_c[x];
         }
-        if (before <= m && m < before + own) {
-            int64_t i = view.index0(q0 + tid);
-            for (u64 left = m - before;; ++i, mask >>= 1)
-                if ((mask & 1u) && left-- == 0) break;
-            sh.picked.index = i;
-        }
-        seen += total;
+        if (hit && before == m) sh.picked.index = (int32_t)i;
         if (m < seen) break;                                 // uniform: `seen` is the same in every thread
     }
     __syncthreads();
@@ -266,7 +251,7 @@ __device__ Picked find(const RowStore<TYPE, NV> &row, const RowScale &c, const b
         sh.csub[2 * tid] = sh.csub[2 * tid + 1] = 0;
         sh.wsub[2 * tid] = sh.wsub[2 * tid + 1] = 0;
         __syncthreads();
-        row.each([&](const float s, const int64_t) {
+        row.each([&](const float s, const int32_t) {
             if (bucket_of(s, c) != b) return;
             const uint32_t key = rank_key(s);
             if (shift < 32 && (key >> shift) != prefix) return;
@@ -299,7 +284,7 @@ __device__ Picked find(const RowStore<TYPE, NV> &row, const RowScale &c, const b
     }
     if (tid == 0) sh.n_list = 0;
     __syncthreads();
-    row.each([&](const float s, const int64_t i) {
+    row.each([&](const float s, const int32_t i) {
         if (bucket_of(s, c) != b) return;
         const uint32_t key = rank_key(s);
         if (shift < 32 && (key >> shift) != prefix) return;
@@ -319,7 +304,7 @@ __device__ Picked find(const RowStore<TYPE, NV> &row, const RowScale &c, const b
         for (uint32_t q = 0; q < n; ++q)
             if (sh.list[q][0] > mine) { before += sh.list[q][1]; ++rank; }
         const bool here = by_count ? rank == target : (before <= target && target < before + w);
-        if (here) { sh.picked.before = before; sh.picked.weight = w; sh.picked.index = (int64_t)(uint32_t)~(uint32_t)mine; }
+        if (here) { sh.picked.before = before; sh.picked.weight = w; sh.picked.index = (int32_t)~(uint32_t)mine; }
     }
     __syncthreads();
     out = sh.picked;
@@ -349,7 +334,7 @@ __global__ __launch_bounds__(SR_THREADS) void sample_rows_kernel(const SampleArg
 
     // the largest score, and the smallest that is no mask value (it only sets the buckets' width)
     float hi = -__builtin_inff(), lo = __builtin_inff();
-    row.each([&](const float s, const int64_t) {
+    row.each([&](const float s, const int32_t) {
         hi = fmaxf(hi, s);
         lo = s > -1e30f ? fminf(lo, s) : lo;
     });
@@ -372,7 +357,7 @@ __global__ __launch_bounds__(SR_THREADS) void sample_rows_kernel(const SampleArg
     if (!(T > 0.f)) {                                         // the best item: lowest column of the largest score
         if (tid == 0) sh.base_w = ~0ull;
         __syncthreads();
-        row.each([&](const float s, const int64_t i) { if (s == hi) atomicMin(&sh.base_w, (u64)i); });
+        row.each([&](const float s, const int32_t i) { if (s == hi) atomicMin(&sh.base_w, (u64)i); });
         __syncthreads();
         for (int d = tid; d < a.n_draws; d += SR_THREADS) { idx[d] = (int32_t)sh.base_w; logp[d] = 0.f; }
         return;
@@ -390,7 +375,7 @@ __global__ __launch_bounds__(SR_THREADS) void sample_rows_kernel(const SampleArg
         const float width = fminf((float)fmin(span * (double)T, 3e38), hi - lo);
         c.per_score = (float)SR_BUCKETS / fmaxf(width, 1e-30f);
     }
-    row.each([&](const float s, const int64_t) {
+    row.each([&](const float s, const int32_t) {
         u64 w;
         if (!weigh(s, c, sh.pow2, w)) return;
         const uint32_t b = bucket_of(s, c);
@@ -417,7 +402,7 @@ __global__ __launch_bounds__(SR_THREADS) void sample_rows_kernel(const SampleArg
         const double t = u > 0.0 ? fmin(u, 1.0) * (double)W : 0.0;
         const u64 target = t >= (double)W ? W - 1 : (u64)t;
         const Picked p = find<TYPE, NV>(row, c, false, target < W ? target : W - 1, sh);
-        if (tid == 0) { idx[d] = (int32_t)p.index; logp[d] = (float)log((double)p.weight / (double)W); }
+        if (tid == 0) { idx[d] = p.index; logp[d] = (float)log((double)p.weight / (double)W); }
     }
 }
 

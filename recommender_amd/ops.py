@@ -682,6 +682,73 @@ def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, e
     return idx, logp
 
 
+def _teacher_lists(idx, val, n, like):
+    """(k, leading dimension) of the teacher's lists: int32 columns and float32 scores, [n, k], rows of one stride."""
+    _need(idx, torch.int32, "teacher_idx", 2)
+    _need(val, torch.float32, "teacher_val", 2)
+    if idx.shape != val.shape or idx.shape[0] != n:
+        raise ValueError("teacher_idx and teacher_val must both be [n_rows, k]")
+    k = idx.shape[1]
+    if not (1 <= k <= 1024):
+        raise ValueError("lists of 1 to 1024 items, got %d" % k)
+    lds = []
+    for t in (idx, val):
+        if (k > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < k):
+            raise ValueError("teacher lists must be row-major with unit inner stride")
+        lds.append(t.stride(0) if n > 1 else k)
+    if lds[0] != lds[1]:
+        raise ValueError("teacher_idx and teacher_val must have the same row stride")
+    _same_device(like, idx, val)
+    return k, lds[0]
+
+
+def _temperature(t):
+    t = float(t)
+    if not (1e-30 <= t <= 1e30):
+        raise ValueError("temperature must lie in [1e-30, 1e30]")
+    return t
+
+
+def distill_rows(score_rows, teacher_idx, teacher_val, temperature=1.0, weight=None, out=None):
+    """Loss and gradient of a student's scores following a teacher's ranked lists (als_distill_rows in
+    include/als_hip.h): per row KL(softmax(teacher_val / T) over the list || softmax(scores / T) over all columns).
+    score_rows: float32, float16 or bfloat16.  teacher_idx int32 / teacher_val float32 [n, k], k <= 1024, as
+    recommend_topk and topk_rows return them; an index outside the columns (-1) is padding, of a column listed twice the
+    first entry stands.  weight: float32 [n], the factor each row's gradient is multiplied by (1 / n for the mean loss).
+    out: where the gradient goes (same shape and type; score_rows itself is allowed), a new tensor by default.
+    Returns (loss float32 [n], unweighted; gradient [n, M] in the scores' type, = weight (q - t) / T)."""
+    dtype, ld = _score_rows(score_rows, "score_rows")
+    n, M = score_rows.shape
+    k, ldt = _teacher_lists(teacher_idx, teacher_val, n, score_rows)
+    T = _temperature(temperature)
+    if weight is not None:
+        _index(weight, torch.float32, "weight")
+        if weight.shape[0] != n:
+            raise ValueError("weight must have one value per row")
+    if out is None:
+        out = torch.empty((n, M), dtype=score_rows.dtype, device=score_rows.device)
+    odt, ldo = _score_rows(out, "out")
+    if odt != dtype or out.shape != score_rows.shape:
+        raise ValueError("out must have the scores' shape and type")
+    if out.data_ptr() == score_rows.data_ptr():
+        if ldo != ld:
+            raise ValueError("out is laid over score_rows with another row stride")
+    elif n and out.untyped_storage().data_ptr() == score_rows.untyped_storage().data_ptr():
+        a, b = score_rows.data_ptr(), out.data_ptr()
+        size = score_rows.element_size()
+        if a < b + ((n - 1) * ldo + M) * size and b < a + ((n - 1) * ld + M) * size:
+            raise ValueError("out overlaps score_rows without being it")
+    _same_device(score_rows, weight, out)
+    loss = torch.empty(n, dtype=torch.float32, device=score_rows.device)
+    if n == 0:
+        return loss, out
+    ws = torch.empty(lib.als_distill_rows_workspace_bytes(dtype, n, M, k), dtype=torch.uint8, device=score_rows.device)
+    with torch.cuda.device(score_rows.device):
+        check(lib.als_distill_rows(_ptr(score_rows), dtype, ld, n, M, _ptr(teacher_idx), _ptr(teacher_val), ldt, k, T, _ptr(weight),
+                                   _ptr(loss), _ptr(out), ldo, _ptr(ws), ws.numel(), _stream()), "als_distill_rows")
+    return loss, out
+
+
 def predict_pairs(X, Y, u, i):
     """out[p] = <X[u[p]], Y[i[p]]>: the ALS model's output for explicit (user, item) pairs
     (reclibwh/core/ALS.py:359-362)."""

@@ -1,0 +1,243 @@
+"""GPU tests of the distillation loss on score rows (csrc/als_distill.hip, ops.distill_rows) against its formula in
+float64.  No reference counterpart: parity is with the formula, and the gradient also with differences of the loss.
+
+Tolerances, u = 2^-24 (float32's half step): a term exp((s - max) / T) carries the rounding of its argument - a few u of
+|s - max| / T, the range R of the row - and of the exponential; the sums add a few u; so q is within (4 R + 16) u of
+itself, a slope within that of weight / T max(q, t), plus half a step of the type it is stored in (bf16 2^-8, fp16 2^-11,
+below fp16's normal range half its smallest step).  The loss is a t-weighted sum of terms of size up to R + ln M."""
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+U = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from recommender_amd import ops
+    return ops
+
+
+def definition(s, idx, val, T, w):
+    """One row in float64: loss, slope, q."""
+    M = len(s)
+    s, val = s.astype(np.float64), val.astype(np.float64)
+    seen, keep = set(), []
+    for p, j in enumerate(idx):
+        if 0 <= j < M and j not in seen:
+            seen.add(int(j)); keep.append(p)
+    with np.errstate(all="ignore"):
+        top = s.max()
+        e = np.exp((s - (top if top > -np.inf else 0.0)) / T)
+        z = e.sum()
+        q = e / z if z > 0 else e
+        if not keep or val[keep].max() == -np.inf:
+            return 0.0, np.zeros(M), q
+        v = val[keep]
+        t = np.exp((v - v.max()) / T)
+        t /= t.sum()
+        js = idx[keep].astype(np.int64)
+        terms = [tj * (np.log(tj) - (np.log(q[j]) if q[j] == 0 else (s[j] - top) / T - np.log(z))) for tj, j in zip(t, js) if tj > 0]
+        slope = q.copy()
+        slope[js] -= t
+    return float(np.sum(terms)), slope * (w / T), q
+
+
+def check(ops, S, idx, val, T=1.0, weight=None, **kw):
+    s0, i0, v0 = S.float().cpu().numpy(), idx.cpu().numpy(), val.cpu().numpy()
+    w0 = np.ones(len(s0), np.float32) if weight is None else weight.cpu().numpy()
+    dt = S.dtype
+    loss, grad = ops.distill_rows(S, idx, val, temperature=T, weight=weight, **kw)
+    assert loss.dtype == torch.float32 and grad.dtype == dt and grad.shape == S.shape
+    step = {torch.float32: 2.0 ** -24, torch.float16: 2.0 ** -11, torch.bfloat16: 2.0 ** -8}[dt]
+    floor = {torch.float32: 2.0 ** -126, torch.float16: 2.0 ** -25, torch.bfloat16: 2.0 ** -126}[dt]
+    T32 = float(np.float32(T))
+    for r in range(len(s0)):
+        wl, wg, q = definition(s0[r], i0[r], v0[r], T32, float(w0[r]))
+        fin = s0[r][np.isfinite(s0[r])]
+        R = (fin.max() - fin.min()) / T32 if fin.size else 0.0
+        # exp(-R) far below the sum: what is smaller than 2^-100 of the largest cannot matter and is not bounded by R
+        R = min(R, 70.0)
+        vals = v0[r][np.isfinite(v0[r])]
+        R2 = min((vals.max() - vals.min()) / T32 if vals.size else 0.0, 70.0)
+        got_l, got = float(loss[r]), grad[r].double().cpu().numpy()
+        if np.isfinite(wl):
+            assert abs(got_l - wl) <= (4 * R + 4 * R2 + 32) * U * (R + R2 + np.log(len(s0[r])) + 2), (r, got_l, wl)
+        else:
+            assert got_l == wl, (r, got_l, wl)
+        t = np.abs(q * (w0[r] / T32) - wg)                 # t w / T where listed
+        tol = ((4 * R + 16) * U * q + (4 * R2 + 16) * U * t / max(abs(w0[r]) / T32, 1e-300)) * abs(w0[r]) / T32 + step * np.abs(wg) + floor
+        bad = np.abs(got - wg) > tol
+        assert not bad.any(), (r, int(np.argmax(bad)), got[bad][:4], wg[bad][:4], tol[bad][:4])
+    return loss, grad
+
+
+def lists(rng, n, M, k):
+    idx = np.stack([rng.choice(M, size=k, replace=False) for _ in range(n)]).astype(np.int32)
+    val = -np.sort(-rng.normal(size=(n, k)).astype(np.float32), axis=1)
+    return torch.from_numpy(idx).cuda(), torch.from_numpy(np.ascontiguousarray(val)).cuda()
+
+
+def scores(rng, n, M, dtype, spread=1.0):
+    return torch.from_numpy((spread * rng.normal(size=(n, M))).astype(np.float32)).cuda().to(TYPES[dtype])
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("n,M,k", [(1, 1, 1), (2, 3, 2), (3, 7, 7), (4, 64, 5), (5, 65, 64), (3, 1023, 1000), (2, 9724, 50), (2, 16385, 100),
+                                   (2, 16391, 1024), (1, 32773, 64), (1, 65541, 200), (2, 65543, 10), (1, 131079, 100), (2, 300007, 50)])
+def test_sizes_and_types(ops, dtype, n, M, k):
+    rng = np.random.default_rng(M + k)
+    S = scores(rng, n, M, dtype, 1.5)
+    idx, val = lists(rng, n, M, k)
+    w = torch.from_numpy(rng.uniform(0.1, 2.0, n).astype(np.float32)).cuda()
+    check(ops, S, idx, val, 0.7, w)
+    check(ops, S, idx, val, 3.0)
+
+
+def test_padding_repeats_and_empty_lists(ops):
+    rng = np.random.default_rng(1)
+    for Mx in (2000, 90001):
+        S = scores(rng, 8, Mx, "f32")
+        idx, val = lists(rng, 8, Mx, 40)
+        idx[0, 20:] = -1
+        idx[1] = -1
+        idx[2, ::3] = -7
+        idx[3, 5:] = idx[3, 0]                     # one item over and over: its first entry stands
+        idx[4, 1::2] = idx[4, 0::2]
+        idx[5, 3] = Mx; idx[5, 9] = 2 ** 31 - 1       # outside: padding
+        val[6, 10:] = float("-inf")
+        val[7] = float("-inf")
+        loss, grad = check(ops, S, idx, val, 0.5)
+        for r in (1, 7):
+            assert float(loss[r]) == 0.0 and not grad[r].any()
+
+
+def test_masked_student_rows(ops):
+    rng = np.random.default_rng(2)
+    inf, low = float("inf"), torch.finfo(torch.float32).min
+    for M in (3000, 70001):
+        S = scores(rng, 6, M, "f32")
+        idx, val = lists(rng, 6, M, 30)
+        S[0, ::2] = -inf
+        S[0].scatter_(0, idx[0].long(), 0.25)
+        S[1] = -inf                                # nothing: loss +inf, slope -t w / T
+        S[2, ::2] = low
+        S[2].scatter_(0, idx[2].long(), -0.25)
+        S[3] = low                                 # a mask value everywhere: uniform
+        S[4, 5:] = -inf                            # the list's items are masked: +inf
+        S[5] = 0.0
+        loss, grad = check(ops, S, idx, val, 0.8)
+        assert loss[1] == inf and loss[4] == inf and torch.isfinite(grad).all()
+
+
+def test_nan_stays_in_its_row(ops):
+    rng = np.random.default_rng(3)
+    S = scores(rng, 3, 1500, "f32")
+    idx, val = lists(rng, 3, 1500, 20)
+    S[1, 7] = float("nan")
+    loss, grad = ops.distill_rows(S, idx, val)
+    assert torch.isnan(loss[1]) and torch.isnan(grad[1]).any()
+    keep = torch.tensor([0, 2], device="cuda")
+    l2, g2 = ops.distill_rows(S[keep], idx[keep], val[keep])
+    assert torch.equal(loss[keep], l2) and torch.equal(grad[keep], g2)
+
+
+def test_gradient_is_the_loss_difference(ops):
+    """Central differences of the float32 loss: the loss is a few u of its size off, so a step h gives the slope to about
+    16 u loss / h + h^2; h = 2^-6 keeps both below 5e-4."""
+    rng = np.random.default_rng(4)
+    M, h = 40, 2.0 ** -6
+    S = scores(rng, 1, M, "f32")
+    idx, val = lists(rng, 1, M, 8)
+    _, grad = ops.distill_rows(S, idx, val, temperature=0.9)
+    up = (S + h * torch.eye(M, device="cuda")).contiguous(); down = (S - h * torch.eye(M, device="cuda")).contiguous()
+    lu, _ = ops.distill_rows(up, idx.repeat(M, 1), val.repeat(M, 1), temperature=0.9)
+    ld, _ = ops.distill_rows(down, idx.repeat(M, 1), val.repeat(M, 1), temperature=0.9)
+    assert float(((lu.double() - ld.double()) / (2 * h) - grad[0].double()).abs().max()) < 5e-4
+    assert abs(float(grad.double().sum())) < 1e-5              # a shift of all scores changes nothing
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("M", [1201, 70003, 140003])
+def test_in_place_strided_and_misaligned(ops, dtype, M):
+    rng = np.random.default_rng(5)
+    big = scores(rng, 3, M + 16, dtype)
+    idx, val = lists(rng, 3, M, 30)
+    wide = torch.full((3, M + 16), 7.0, device="cuda", dtype=TYPES[dtype])
+    for a, b in [(0, 0), (1, 0), (0, 3), (5, 2), (7, 7)]:
+        S = big[:, a:a + M]
+        want = ops.distill_rows(S.contiguous(), idx, val, temperature=0.6)
+        wide.fill_(7.0)
+        out = wide[:, b:b + M]
+        loss, grad = ops.distill_rows(S, idx, val, temperature=0.6, out=out)
+        assert grad is out
+        # another alignment walks the row in other chunks: the sums may differ in their last bits
+        assert torch.allclose(loss, want[0], rtol=1e-6, atol=0) and torch.allclose(grad.float(), want[1].float(), rtol=2e-2, atol=1e-9)
+        assert (wide[:, :b] == 7.0).all() and (wide[:, b + M:] == 7.0).all()
+        inplace = big.clone()
+        view = inplace[:, a:a + M]
+        l2, g2 = ops.distill_rows(view, idx, val, temperature=0.6, out=view)
+        assert torch.equal(l2, loss) and torch.equal(g2, grad)
+        assert torch.equal(inplace[:, :a], big[:, :a]) and torch.equal(inplace[:, a + M:], big[:, a + M:])
+
+
+def test_same_bits_in_a_block_on_a_stream_and_in_a_graph(ops):
+    rng = np.random.default_rng(6)
+    for M in (20011, 100003):
+        S = scores(rng, 12, M, "f32")
+        S = torch.nn.functional.pad(S, (0, (-M) % 4))[:, :M]        # rows of one alignment: a row alone is walked the same
+        idx, val = lists(rng, 12, M, 60)
+        want = ops.distill_rows(S, idx, val, temperature=0.6)
+        for r in (0, 5, 11):
+            one = ops.distill_rows(S[r:r + 1], idx[r:r + 1], val[r:r + 1], temperature=0.6)
+            assert torch.equal(one[0], want[0][r:r + 1]) and torch.equal(one[1], want[1][r:r + 1])
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            there = ops.distill_rows(S, idx, val, temperature=0.6)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(there[0], want[0]) and torch.equal(there[1], want[1])
+        Sg = S.clone()
+        ops.distill_rows(Sg, idx, val, temperature=0.6)
+        torch.cuda.synchronize()
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = ops.distill_rows(Sg, idx, val, temperature=0.6)
+        for step in range(4):
+            Sg.copy_(S.roll(step, 0))
+            graph.replay()
+            eager = ops.distill_rows(Sg, idx, val, temperature=0.6)
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], eager[0]) and torch.equal(out[1], eager[1]), step
+
+
+def test_no_rows_and_refusals(ops):
+    S = torch.zeros(4, 10, device="cuda")
+    idx = torch.zeros(4, 3, dtype=torch.int32, device="cuda")
+    val = torch.zeros(4, 3, device="cuda")
+    loss, grad = ops.distill_rows(S[:0], idx[:0], val[:0])
+    assert loss.shape == (0,) and grad.shape == (0, 10)
+    buf = torch.zeros(100, device="cuda")
+    for bad in [lambda: ops.distill_rows(S.cpu(), idx, val), lambda: ops.distill_rows(S.double(), idx, val),
+                lambda: ops.distill_rows(S, idx.long(), val), lambda: ops.distill_rows(S, idx, val.half()),
+                lambda: ops.distill_rows(S, idx[:3], val[:3]), lambda: ops.distill_rows(S, idx, val[:, :2]),
+                lambda: ops.distill_rows(S, idx.cpu(), val), lambda: ops.distill_rows(S, idx[:, :0], val[:, :0]),
+                lambda: ops.distill_rows(S, torch.zeros(4, 1025, dtype=torch.int32, device="cuda"), torch.zeros(4, 1025, device="cuda")),
+                lambda: ops.distill_rows(S, idx, val, temperature=0.0), lambda: ops.distill_rows(S, idx, val, temperature=-1.0),
+                lambda: ops.distill_rows(S, idx, val, temperature=float("nan")),
+                lambda: ops.distill_rows(S, idx, val, temperature=float("inf")),
+                lambda: ops.distill_rows(S, idx, val, weight=torch.ones(3, device="cuda")),
+                lambda: ops.distill_rows(S, idx, val, weight=torch.ones(4, device="cuda").double()),
+                lambda: ops.distill_rows(S, idx, val, out=torch.zeros(4, 9, device="cuda")),
+                lambda: ops.distill_rows(S, idx, val, out=S.half()), lambda: ops.distill_rows(S.t(), idx, val),
+                lambda: ops.distill_rows(buf[:40].view(4, 10), idx, val, out=buf[20:60].view(4, 10)),
+                lambda: ops.distill_rows(buf[:80].view(4, 20)[:, :10], idx, val, out=buf[:40].view(4, 10)),
+                lambda: ops.distill_rows(S[:1].expand(4, 10), idx, val)]:
+        with pytest.raises(ValueError):
+            bad()
