@@ -433,7 +433,22 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  * als_distill_rows   the scores are given, [n_rows, lds] row major in float32, float16 or bfloat16; grad_out [n_rows, ldg]
  *                    of the same type receives slope and may be `scores` itself (same ld).  Sums are float32 in runs of 4
  *                    or 8 items, float64 above, in an order set by M and the row's address modulo 16 alone.
+ * als_distill_topk_f32   the scores are those of the factors, s_ui = <X[user_ids[u]], Y[i]> for i < M (user_ids NULL: rows
+ *                    0..n_users-1), and never stored: loss_out [n_users], and the gradients of sum_u weight_u loss_u
+ *                        dX_out [n_users, f]: sum_i slope_ui Y[i]    (a user listed twice has two rows),
+ *                        dY_out [M, f]:       sum_u slope_ui X[user_ids[u]],
+ *                    both dense row major.  A user id outside [0, x_rows) gives NaN for its loss and dX row and adds nothing
+ *                    to dY.  Any f <= ALS_MAX_FACTORS and alignment; temperature in [1e-6, 1e6]; the
+ *                    factors must be finite.  Products of 22-bit operands (two fp16 pieces of a value scaled by one power
+ *                    of two per factor; values below 2^-18 of the factor's largest lose bits) accumulated in float32.
+ *                    8 n M f operations, three products each.  Workspace: about 8 (n + M) F bytes, F = f rounded up to 32,
+ *                    64, 128 or 256, plus the parts of split sums.
  * ------------------------------------------------------------------------------------ */
+size_t als_distill_topk_workspace_bytes(int64_t n_users, int64_t M, int32_t f, int32_t k);
+int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const int64_t *user_ids, int64_t n_users, const float *Y,
+                             int64_t ldy, int64_t M, int32_t f, const int32_t *teacher_idx, const float *teacher_val, int64_t ld_teacher,
+                             int32_t k, float temperature, const float *weight, float *loss_out, float *dX_out, float *dY_out,
+                             void *workspace, size_t ws_bytes, void *stream);
 size_t als_distill_rows_workspace_bytes(int32_t dtype, int64_t n_rows, int64_t M, int32_t k);
 int32_t als_distill_rows(const void *scores, int32_t dtype, int64_t lds, int64_t n_rows, int64_t M, const int32_t *teacher_idx,
                          const float *teacher_val, int64_t ld_teacher, int32_t k, float temperature, const float *weight,

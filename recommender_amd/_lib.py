@@ -56,6 +56,9 @@ SIGNATURES = {
     "als_sample_rows": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp]),
     "als_distill_rows": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i32, c_f32, c_vp, c_vp, c_vp, c_i64, c_vp, c_sz,
                                  c_vp]),
+    "als_distill_topk_workspace_bytes": (c_sz, [c_i64, c_i64, c_i32, c_i32]),
+    "als_distill_topk_f32": (c_i32, [c_vp, c_i64, c_i64, c_vp, c_i64, c_vp, c_i64, c_i64, c_i32, c_vp, c_vp, c_i64, c_i32, c_f32,
+                                     c_vp, c_vp, c_vp, c_vp, c_vp, c_sz, c_vp]),
     "als_distill_rows_workspace_bytes": (c_sz, [c_i32, c_i64, c_i64, c_i32]),
     "als_predict_pairs_f32": (c_i32, [c_vp, c_i64, c_vp, c_i64, c_vp, c_vp, c_i64, c_i32, c_vp, c_vp]),
     "als_normalize_rows_f32": (c_i32, [c_vp, c_i64, c_i64, c_i32, c_vp, c_i64, c_vp]),

@@ -1,0 +1,721 @@
+// The distillation loss (als_distill.hip) straight from the factors: scores s_ui = <x_u, y_i>, loss and both gradients
+//     dX_u = sum_i slope_ui y_i,   dY_i = sum_u slope_ui x_u,   slope_ui = c_u (q_ui - t_ui),  c_u = weight_u / T
+// without a score matrix.  Two passes over the pairs (user, item), each a pair of chained matrix products on the fp16 matrix
+// cores with the exponential between them in registers:
+//   pass 1  users stationary, items streaming: s = x y^T, p = exp(s - running maximum), O += p y, Z += p; a user's O / Z is
+//           sum_i q_ui y_i.  Split over the items; the parts are joined afterwards.
+//   lists   per user: joins the parts, ln Z, the teacher's softmax, the loss, dX; and the list in item order.
+//   pass 2  items stationary, users streaming: s again, q = exp(s - ln Z_u), minus the listed t, dY += (q - t) (c_u x_u).
+// 8 n M f multiplications and additions, of which three products each: operands are two fp16 pieces of a value scaled by a
+// power of two (22 mantissa bits) and hi hi + hi lo + lo hi are accumulated in float32 - the accuracy of float32 products
+// at several times their rate.
+//
+// Layout.  v_mfma_f32_32x32x16_f16: operand A lane (h, i), h = lane / 32, holds row i, k = 8 h .. 8 h + 7; B lane (h, j)
+// column j, the same k; the result's register r in lane (h, j) is row 8 (r / 4) + 4 h + r % 4, column j.  A 32 x 32 tile of
+// scores [streaming row, stationary column] leaves a lane with 16 values of ONE column; taken as two k-steps of 8 they are
+// the B operand of the second product, if the other operand's k runs over the streaming rows in the same order.  So nothing
+// is exchanged between lanes, and both factors are laid out beforehand (prepare_kernel) as the lanes read them, per tile of
+// 32 rows: row form (KS = F / 16 k-steps x 2 pieces) and transposed form (F / 32 feature tiles x 2 k-steps x 2 pieces), each
+// 64 lanes x 16 bytes.  A stage is one tile: F / 4 KB, contiguous, copied to LDS by LDS-DMA.
+#include <hip/hip_runtime.h>
+
+#include <algorithm>
+#include <cstdint>
+
+#include "als_hip.h"
+
+int als_fail_(int code, const char *fmt, ...);  // defined in als_kernels.hip
+
+#define ALS_HIP_CHECK6(expr)                                                                      \
+    do {                                                                                          \
+        hipError_t e_ = (expr);                                                                   \
+        if (e_ != hipSuccess) return als_fail_(ALS_ERR_HIP, "%s: %s", #expr, hipGetErrorString(e_)); \
+    } while (0)
+
+namespace {
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+#include "als_fp16.inc"
+
+constexpr int LIST_MAX = 1024;
+constexpr int TILE = 32;                // rows per tile, of either factor
+constexpr int Y_MAX_BLOCKS = 256, X_MAX_BLOCKS = 64;
+constexpr float P_OFFSET = 8.f;         // pass 1: p 2^8, and at most 2^6 above the running maximum's: below 2^15
+constexpr float LAZY = 6.f;             // the running maximum follows when it lags by more than 2^6
+constexpr float Q_OFFSET = 14.f;        // pass 2: (q - t) 2^14
+constexpr float NEVER = 1e30f;          // bias of a padding user: q = 0
+constexpr int T_STRIDE = 36;            // floats per item column of the list tile: 16-byte aligned, columns on different banks
+
+struct FactorArgs {
+    const float *X, *Y;
+    int64_t ldx, ldy;
+    const int64_t *users;
+    int64_t n, M, x_rows;
+    int32_t f;
+    const int32_t *t_idx;
+    const float *t_val;
+    int64_t ldt;
+    int32_t k;
+    float inv_t;
+    const float *weight;
+    float *loss, *dX, *dY;
+    // workspace
+    float *maxima;        // Y_MAX_BLOCKS of |y|, X_MAX_BLOCKS of |x|, X_MAX_BLOCKS of |c x|
+    float *scales;        // {1 / (s_x s_y), 1 / s_y, 1 / (s_cx 2^Q_OFFSET)}
+    char *xt, *yt;        // the factors as tiles
+    float *o_part;        // [split, user, F]
+    float *stat_part;     // [split, user, 2]: running maximum (log2), sum
+    float *bias;          // log2 Z_u - Q_OFFSET, per user, NEVER for padding
+    int32_t *s_item;      // lists in item order [user, k]
+    float *s_t;           // t 2^Q_OFFSET
+    uint16_t *offs;       // [user, item blocks + 1] first list entry at or behind the block
+    float *dy_part;       // [split, item, F]
+    int64_t n_tiles, m_tiles;
+    int32_t splits1, splits2, item_blocks, block_items;
+};
+
+__device__ __forceinline__ float exp2_fast(const float x) { return __builtin_amdgcn_exp2f(x); }
+__device__ __forceinline__ float finite_abs(const float v) { const float a = fabsf(v); return a < 3e38f ? a : 0.f; }
+
+// The factor row of output row u, or NULL for a user id outside X.
+__device__ __forceinline__ const float *user_row(const FactorArgs &a, const int64_t u) {
+    const int64_t id = a.users ? a.users[u] : u;
+    return id >= 0 && id < a.x_rows ? a.X + id * a.ldx : nullptr;
+}
+
+__device__ __forceinline__ float block_max256(float v, float *red) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
+}
+__device__ __forceinline__ float block_sum256(float v, float *red) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    __syncthreads();
+    return (red[0] + red[1]) + (red[2] + red[3]);
+}
+
+// ----------------------------------------------------------------------------- laying the factors out
+// Largest |y|, |x| and |c x| (finite ones), one value per block: the reader takes the maximum over blocks.
+__global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
+    __shared__ float red[4];
+    const bool is_y = blockIdx.x < Y_MAX_BLOCKS;
+    const int b = is_y ? blockIdx.x : blockIdx.x - Y_MAX_BLOCKS, nb = is_y ? Y_MAX_BLOCKS : X_MAX_BLOCKS;
+    const int64_t rows = is_y ? a.M : a.n;
+    float m = 0.f, mc = 0.f;
+    // a wave takes a row at a time
+    for (int64_t r = (int64_t)b * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)nb * 4) {
+        const float *row = is_y ? a.Y + r * a.ldy : user_row(a, r);
+        if (!row) continue;
+        const float c = is_y || !a.weight ? 1.f : fabsf(a.weight[r]);
+        float mr = 0.f;
+        for (int k = threadIdx.x & 63; k < a.f; k += 64) mr = fmaxf(mr, finite_abs(row[k]));
+        m = fmaxf(m, mr);
+        mc = fmaxf(mc, finite_abs(mr * c * a.inv_t));
+    }
+    m = block_max256(m, red);
+    mc = block_max256(mc, red);
+    if (threadIdx.x == 0) {
+        a.maxima[blockIdx.x] = m;
+        if (!is_y) a.maxima[blockIdx.x + X_MAX_BLOCKS] = mc;
+    }
+}
+
+// hi and lo fp16 pieces of s x
+__device__ __forceinline__ void cut(const float x, const float s, _Float16 &hi, _Float16 &lo) {
+    const float v = x * s;
+    hi = (_Float16)v;
+    lo = (_Float16)(v - (float)hi);
+}
+
+// One tile of 32 rows per workgroup: through LDS, then both forms.  Tiles of Y first, then of X (whose row form carries
+// log2(e) / T and whose transposed form carries c_u).
+template <int F>
+__global__ __launch_bounds__(256) void prepare_kernel(const FactorArgs a) {
+    constexpr int KS = F / 16, FT = F / 32;
+    __shared__ float tile[TILE][F + 1];
+    __shared__ float red[4], cs[TILE];
+    const int tid = threadIdx.x;
+    const bool is_y = blockIdx.x < a.m_tiles;
+    const int64_t T = is_y ? blockIdx.x : blockIdx.x - a.m_tiles;
+    const int64_t rows = is_y ? a.M : a.n;
+    const float my = block_max256(tid < Y_MAX_BLOCKS ? a.maxima[tid] : 0.f, red);
+    const float mx = block_max256(tid < X_MAX_BLOCKS ? a.maxima[Y_MAX_BLOCKS + tid] : 0.f, red);
+    const float mc = block_max256(tid < X_MAX_BLOCKS ? a.maxima[Y_MAX_BLOCKS + X_MAX_BLOCKS + tid] : 0.f, red);
+    const float to_log2 = a.inv_t * 1.44269504f;
+    const float sy = op_scale(my).s, sx = op_scale(mx * to_log2).s, sc = op_scale(mc).s;
+    if (blockIdx.x == 0 && tid == 0) {
+        a.scales[0] = 1.f / (sx * sy);
+        a.scales[1] = 1.f / sy;
+        a.scales[2] = exp2f(-Q_OFFSET) / sc;
+    }
+    for (int q = tid; q < TILE * F; q += 256) {
+        const int i = q / F, k = q % F;
+        const int64_t r = T * TILE + i;
+        const float *row = r >= rows ? nullptr : is_y ? a.Y + r * a.ldy : user_row(a, r);
+        tile[i][k] = row && k < a.f ? row[k] : 0.f;
+    }
+    if (tid < TILE) {
+        const int64_t r = T * TILE + tid;
+        cs[tid] = is_y ? 1.f : r < rows ? (a.weight ? a.weight[r] : 1.f) * a.inv_t : 0.f;
+    }
+    __syncthreads();
+    char *out = (is_y ? a.yt : a.xt) + T * (F * 256);
+    const float s_row = is_y ? sy : sx, m_row = is_y ? 1.f : to_log2, s_tr = is_y ? sy : sc;
+    for (int q = tid; q < KS * 64; q += 256) {
+        const int ks = q >> 6, lane = q & 63, h = lane >> 5, i = lane & 31;
+        f16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            _Float16 x, y;
+            cut(tile[i][16 * ks + 8 * h + e] * m_row, s_row, x, y);
+            hi[e] = x; lo[e] = y;
+        }
+        *reinterpret_cast<f16x8 *>(out + (2 * ks) * 1024 + lane * 16) = hi;
+        *reinterpret_cast<f16x8 *>(out + (2 * ks + 1) * 1024 + lane * 16) = lo;
+    }
+    for (int q = tid; q < FT * 2 * 64; q += 256) {
+        const int fk = q >> 6, ft = fk >> 1, kk = fk & 1, lane = q & 63, h = lane >> 5, i = lane & 31;
+        f16x8 hi, lo;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+            const int row = 16 * kk + 8 * (e / 4) + 4 * h + e % 4;
+            _Float16 x, y;
+            cut(tile[row][32 * ft + i] * cs[row], s_tr, x, y);
+            hi[e] = x; lo[e] = y;
+        }
+        *reinterpret_cast<f16x8 *>(out + (2 * KS + 2 * fk) * 1024 + lane * 16) = hi;
+        *reinterpret_cast<f16x8 *>(out + (2 * KS + 2 * fk + 1) * 1024 + lane * 16) = lo;
+    }
+}
+
+// ----------------------------------------------------------------------------- the two passes
+#pragma clang diagnostic push
+#pragma clang diagnostic ignored "-Winline-asm"      // m0 is reserved, and written here on purpose: the LDS address of the DMA
+// 64 lanes x 16 bytes from g (per lane) to LDS bytes [lds, lds + 1024), lane l at 16 l
+__device__ __forceinline__ void dma16(const void *g, const unsigned lds) {
+    asm volatile("s_mov_b32 m0, %1\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, off"
+                 :: "v"(g), "s"(__builtin_amdgcn_readfirstlane((int)lds)) : "memory", "m0");
+}
+#pragma clang diagnostic pop
+__device__ __forceinline__ f32x16 mfma32(const u32x4 &a, const u32x4 &b, const f32x16 &c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+}
+// Two float32 values as fp16 pairs of both pieces.  Toward zero: the rest is exact and of one sign.
+__device__ __forceinline__ void cut_pair(const float p0, const float p1, unsigned &hi, unsigned &lo) {
+    const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
+    hi = __builtin_bit_cast(unsigned, h);
+    const auto l = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.f, p0), __builtin_fmaf((float)h[1], -1.f, p1));
+    lo = __builtin_bit_cast(unsigned, l);
+}
+
+// BACK = false: pass 1 (stationary X, streaming Y).  BACK = true: pass 2 (stationary Y, streaming X, lists).
+// A wave owns one stationary tile (32 rows: operands and result in registers); the WAVES waves of a workgroup share the
+// streaming tiles in LDS.  RING tiles are kept: the copy of tile t + RING - 1 starts while tile t is worked on.
+// TBUF list tiles are kept (one where LDS holds no second: F = 256).
+// Workgroup (split, block): the ids of one split go to one XCD, so that the blocks that stream the same tiles share its L2.
+template <int F, int WAVES, int RING, int TBUF, bool BACK>
+__global__ __launch_bounds__(WAVES * 64) void pass_kernel(const FactorArgs a) {
+    constexpr int KS = F / 16, FT = F / 32, CHUNKS = F / 4, PER_WAVE = CHUNKS / WAVES;
+    constexpr int LPR = WAVES * 2;                       // lanes that write one user's row of the list tile
+    static_assert(CHUNKS % WAVES == 0, "every wave copies the same number of chunks");
+    extern __shared__ char lds[];
+    u32x4 *ring = reinterpret_cast<u32x4 *>(lds);                                   // RING x CHUNKS x 64
+    float *t_tile = reinterpret_cast<float *>(lds + RING * CHUNKS * 1024);          // BACK: TBUF x WAVES * 32 x T_STRIDE
+    float *bias = t_tile + TBUF * WAVES * 32 * T_STRIDE;                            // BACK: TBUF x 32
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int h = lane >> 5, j = lane & 31;
+    const int splits = BACK ? a.splits2 : a.splits1;
+    const int64_t stat_tiles = BACK ? a.m_tiles : a.n_tiles, stream_tiles = BACK ? a.n_tiles : a.m_tiles;
+    const int64_t blocks = (stat_tiles + WAVES - 1) / WAVES;
+    const int64_t w = blockIdx.x;
+    const int group = splits >= 8 ? 8 : 1;               // splits is a multiple of 8 from 8 on
+    const int64_t block = (w / group) % blocks;
+    const int split = (int)(w / (group * blocks)) * group + (int)(w % group);
+    const int64_t per = (stream_tiles + splits - 1) / splits;
+    const int64_t t0 = split * per, t1 = t0 + per < stream_tiles ? t0 + per : stream_tiles;       // the host leaves no split empty
+    const char *stat = (BACK ? a.yt : a.xt);
+    const char *stream = (BACK ? a.xt : a.yt);
+    const int64_t tile = block * WAVES + wave;
+    const bool active = tile < stat_tiles;
+
+    const unsigned ring_base = (unsigned)(uintptr_t)(__attribute__((address_space(3))) char *)lds;
+    auto copy = [&](const int64_t t, const int slot) {
+        // past the range's end the last tile is copied again: every stage issues the same number of copies
+        const char *src = stream + (t < t1 ? t : t1 - 1) * (F * 256) + lane * 16;
+#pragma unroll
+        for (int q = 0; q < PER_WAVE; ++q) {
+            const int c = wave * PER_WAVE + q;
+            dma16(src + c * 1024, ring_base + (slot * CHUNKS + c) * 1024);
+        }
+    };
+
+    u32x4 BH[KS], BL[KS];
+    {
+        const u32x4 *src = reinterpret_cast<const u32x4 *>(stat + (active ? tile : 0) * (F * 256)) + lane;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) { BH[s] = src[(2 * s) * 64]; BL[s] = src[(2 * s + 1) * 64]; }
+    }
+    f32x16 O[FT];
+#pragma unroll
+    for (int q = 0; q < FT; ++q)
+#pragma unroll
+        for (int r = 0; r < 16; ++r) O[q][r] = 0.f;
+    const float k = a.scales[0];
+    float m = -__builtin_inff(), z = 0.f;
+
+    // ---- pass 2: the lists of the streaming users, as a dense tile [item of the block, user of the stage] that is zero but
+    // for the listed pairs.  LPR lanes of one wave own a user's row in both buffers: they clear what the stage before last
+    // wrote there and write the new entries, in order, without a barrier between.
+    const int row = BACK ? tid / LPR : 0, sub = BACK ? tid % LPR : 0;
+    const int64_t i_first = block * WAVES * 32;
+    struct Entries { int b, e, item; float t, bias; };
+    Entries now{0, 0, 0, 0.f, NEVER}, old[2] = {now, now};
+    int64_t old_user[2] = {0, 0};
+    auto fetch = [&](const int64_t t) {                  // the first LPR entries of the row's user in stage t
+        Entries x{0, 0, 0, 0.f, NEVER};
+        const int64_t u = t * TILE + row;
+        if (t < t1 && sub == 0) x.bias = a.bias[u];      // padding users have one too
+        if (t < t1 && u < a.n) {
+            const uint16_t *o = a.offs + u * (a.item_blocks + 1) + block;
+            x.b = o[0]; x.e = o[1];
+            if (x.b + sub < x.e) { x.item = a.s_item[u * a.k + x.b + sub]; x.t = a.s_t[u * a.k + x.b + sub]; }
+        }
+        return x;
+    };
+    auto place = [&](const int64_t t, const int parity) {   // writes `now`, the entries of stage t
+        const int buf = TBUF == 2 ? parity : 0;
+        float *tt = t_tile + buf * (WAVES * 32 * T_STRIDE);
+        const Entries o = TBUF == 2 && parity ? old[1] : old[0];
+        const int64_t ou = TBUF == 2 && parity ? old_user[1] : old_user[0];
+        if (o.b + sub < o.e) tt[(o.item - i_first) * T_STRIDE + row] = 0.f;
+        for (int q = o.b + sub + LPR; q < o.e; q += LPR)
+            tt[(a.s_item[ou * a.k + q] - i_first) * T_STRIDE + row] = 0.f;
+        const int64_t u = t * TILE + row;
+        if (now.b + sub < now.e) tt[(now.item - i_first) * T_STRIDE + row] = now.t;
+        for (int q = now.b + sub + LPR; q < now.e; q += LPR)
+            tt[(a.s_item[u * a.k + q] - i_first) * T_STRIDE + row] = a.s_t[u * a.k + q];
+        if (TBUF == 2 && parity) { old[1] = now; old_user[1] = u; }
+        else { old[0] = now; old_user[0] = u; }
+        if (sub == 0) bias[buf * 32 + row] = now.bias;
+    };
+
+    if constexpr (BACK) {
+        for (int q = tid; q < TBUF * WAVES * 32 * T_STRIDE; q += WAVES * 64) t_tile[q] = 0.f;
+        __syncthreads();
+        now = fetch(t0);
+        place(t0, 0);
+        now = fetch(t0 + 1);
+    }
+#pragma unroll
+    for (int q = 0; q < RING - 1; ++q) copy(t0 + q, q);
+    int slot = 0;
+    for (int64_t t = t0; t < t1; ++t) {
+        // this wave's copies of tile t have landed (behind them it issued RING - 2 further tiles, and maybe list loads, which
+        // only make the count stricter); after the barrier everyone's have, and everyone is done with tile t - 1
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"((RING - 2) * PER_WAVE) : "memory");
+        __syncthreads();
+        const int parity = (int)(t - t0) & 1, buf = TBUF == 2 ? parity : 0;
+        if constexpr (BACK && TBUF == 2) {
+            place(t + 1, parity ^ 1);
+            now = fetch(t + 2);
+        }
+        copy(t + RING - 1, slot == 0 ? RING - 1 : slot - 1);
+        const u32x4 *st = ring + slot * CHUNKS * 64 + lane;
+        slot = slot + 1 == RING ? 0 : slot + 1;
+        if (active) {
+        f32x16 S;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) S[r] = 0.f;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            const u32x4 ah = st[(2 * s) * 64], al = st[(2 * s + 1) * 64];
+            S = mfma32(al, BH[s], S);
+            S = mfma32(ah, BL[s], S);
+            S = mfma32(ah, BH[s], S);
+        }
+        unsigned PH[8], PL[8];
+        if constexpr (!BACK) {
+            if ((t + 1) * TILE > a.M) {                  // the last tile's padding rows
+#pragma unroll
+                for (int r = 0; r < 16; ++r)
+                    if (t * TILE + 8 * (r / 4) + 4 * h + r % 4 >= a.M) S[r] = -__builtin_inff();
+            }
+            float top = S[0];
+#pragma unroll
+            for (int r = 1; r < 16; ++r) top = fmaxf(top, S[r]);
+            top *= k;
+            if (__any(top > m + LAZY)) {
+                const float other = __shfl_xor(top, 32);
+                const float next = fmaxf(m, fmaxf(top, other));
+                const float scale = m == -__builtin_inff() ? 0.f : exp2_fast(m - next);
+                m = next;
+                z *= scale;
+#pragma unroll
+                for (int q = 0; q < FT; ++q)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) O[q][r] *= scale;
+            }
+            const float c = P_OFFSET - m;
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                const float p0 = exp2_fast(__builtin_fmaf(S[r], k, c)), p1 = exp2_fast(__builtin_fmaf(S[r + 1], k, c));
+                z += p0 + p1;
+                cut_pair(p0, p1, PH[r / 2], PL[r / 2]);
+            }
+        } else {
+            const f32x4 *tt = reinterpret_cast<const f32x4 *>(t_tile + buf * (WAVES * 32 * T_STRIDE) + (wave * 32 + j) * T_STRIDE) + h;
+            const f32x4 *bb = reinterpret_cast<const f32x4 *>(bias + buf * 32) + h;
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const f32x4 tv = tt[2 * g], bv = bb[2 * g];
+#pragma unroll
+                for (int e = 0; e < 4; e += 2) {
+                    const float p0 = exp2_fast(__builtin_fmaf(S[4 * g + e], k, -bv[e])) - tv[e];
+                    const float p1 = exp2_fast(__builtin_fmaf(S[4 * g + e + 1], k, -bv[e + 1])) - tv[e + 1];
+                    cut_pair(p0, p1, PH[2 * g + e / 2], PL[2 * g + e / 2]);
+                }
+            }
+        }
+#pragma unroll
+        for (int q = 0; q < FT; ++q)
+#pragma unroll
+            for (int kk = 0; kk < 2; ++kk) {
+                const u32x4 vh = st[(2 * KS + 4 * q + 2 * kk) * 64], vl = st[(2 * KS + 4 * q + 2 * kk + 1) * 64];
+                const u32x4 ph{PH[4 * kk], PH[4 * kk + 1], PH[4 * kk + 2], PH[4 * kk + 3]};
+                const u32x4 pl{PL[4 * kk], PL[4 * kk + 1], PL[4 * kk + 2], PL[4 * kk + 3]};
+                O[q] = mfma32(vl, ph, O[q]);
+                O[q] = mfma32(vh, pl, O[q]);
+                O[q] = mfma32(vh, ph, O[q]);
+            }
+        }
+        if constexpr (BACK && TBUF == 1) {               // one list tile: the next entries go in when everyone has read these
+            __syncthreads();
+            place(t + 1, 0);
+            now = fetch(t + 2);
+        }
+    }
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");     // no copy is left in flight
+    if (!active) return;
+    const int64_t r = tile * TILE + j;                   // this lane's stationary row
+    if constexpr (!BACK) {
+        z += __shfl_xor(z, 32);
+        if (r < a.n) {
+            const int64_t at = (int64_t)split * a.n + r;
+            if (h == 0) { a.stat_part[2 * at] = m; a.stat_part[2 * at + 1] = z; }
+#pragma unroll
+            for (int q = 0; q < FT; ++q)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4 *>(a.o_part + at * F + 32 * q + 8 * g + 4 * h) =
+                        f32x4{O[q][4 * g], O[q][4 * g + 1], O[q][4 * g + 2], O[q][4 * g + 3]};
+        }
+    } else if (r < a.M) {
+        if (splits == 1) {
+            const float inv = a.scales[2];
+#pragma unroll
+            for (int q = 0; q < FT; ++q)
+#pragma unroll
+                for (int e = 0; e < 16; ++e) {
+                    const int c = 32 * q + 8 * (e / 4) + 4 * h + e % 4;
+                    if (c < a.f) a.dY[r * a.f + c] = O[q][e] * inv;
+                }
+        } else {
+            const int64_t at = (int64_t)split * a.M + r;
+#pragma unroll
+            for (int q = 0; q < FT; ++q)
+#pragma unroll
+                for (int g = 0; g < 4; ++g)
+                    *reinterpret_cast<f32x4 *>(a.dy_part + at * F + 32 * q + 8 * g + 4 * h) =
+                        f32x4{O[q][4 * g], O[q][4 * g + 1], O[q][4 * g + 2], O[q][4 * g + 3]};
+        }
+    }
+}
+
+// dY from the parts of pass 2, in split order.
+__global__ __launch_bounds__(256) void join_items_kernel(const FactorArgs a, const int F) {
+    const float inv = a.scales[2];
+    const int64_t total = a.M * a.f;
+    for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
+        const int64_t i = q / a.f;
+        const int c = (int)(q - i * a.f);
+        float v = 0.f;
+        for (int s = 0; s < a.splits2; ++s) v += a.dy_part[((int64_t)s * a.M + i) * F + c];
+        a.dY[q] = v * inv;
+    }
+}
+
+// ----------------------------------------------------------------------------- lists
+// One workgroup per user (and per padding user of the last tile, which only gets its bias).
+__global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a, const int F) {
+    __shared__ uint64_t key[LIST_MAX];              // item << 32 | position, ~0 for padding
+    __shared__ float val[LIST_MAX], share[LIST_MAX];
+    __shared__ int32_t sorted[LIST_MAX];
+    __shared__ float x[256], part[4][256], red[4], stat[2];
+    __shared__ int32_t n_kept;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int64_t u = blockIdx.x;
+    if (u >= a.n) {
+        if (tid == 0) a.bias[u] = NEVER;
+        return;
+    }
+    const int f = a.f;
+    const float *xrow = user_row(a, u);
+    if (!xrow) {                                         // no such user: NaN for it, nothing for the items
+        if (tid == 0) { a.bias[u] = NEVER; a.loss[u] = __builtin_nanf(""); }
+        if (tid < f) a.dX[u * f + tid] = __builtin_nanf("");
+        for (int64_t b = tid; b <= a.item_blocks; b += 256) a.offs[u * (a.item_blocks + 1) + b] = 0;
+        return;
+    }
+    x[tid] = tid < f ? xrow[tid] : 0.f;
+    for (int p = tid; p < a.k; p += 256) {
+        const int32_t i = a.t_idx[u * a.ldt + p];
+        key[p] = i >= 0 && i < a.M ? (uint64_t)(uint32_t)i << 32 | (uint32_t)p : ~0ull;
+        val[p] = a.t_val[u * a.ldt + p];
+    }
+    if (tid == 0) n_kept = 0;
+    __syncthreads();
+    // of an item listed twice the first entry stands
+    float top = -__builtin_inff();
+    unsigned kept_mask = 0;
+    for (int p = tid, b = 0; p < a.k; p += 256, ++b) {
+        const uint64_t own = key[p];
+        bool keep = own != ~0ull;
+        for (int q = 0; q < a.k && keep; ++q) keep = !(key[q] >> 32 == own >> 32 && key[q] < own);
+        if (keep) { kept_mask |= 1u << b; top = fmaxf(top, val[p]); }
+    }
+    top = block_max256(top, red);
+    const bool any = top != -__builtin_inff();           // a list without weight asks for nothing
+    __syncthreads();
+    float sum = 0.f;
+    for (int p = tid, b = 0; p < a.k; p += 256, ++b) {
+        const bool keep = any && (kept_mask >> b & 1);
+        const float e = keep ? expf((val[p] - top) * a.inv_t) : 0.f;
+        share[p] = e;
+        sum += e;
+        if (!keep) key[p] = ~0ull;
+        else atomicAdd(&n_kept, 1);
+    }
+    sum = block_sum256(sum, red);
+    __syncthreads();
+    const int n_list = n_kept;
+    // item order, by rank among the kept
+    for (int p = tid; p < a.k; p += 256) {
+        const uint64_t own = key[p];
+        if (own == ~0ull) continue;
+        int rank = 0;
+        for (int q = 0; q < a.k; ++q) rank += key[q] < own;
+        sorted[rank] = (int32_t)(own >> 32);
+        const float t = share[p] / sum;
+        a.s_item[u * a.k + rank] = (int32_t)(own >> 32);
+        a.s_t[u * a.k + rank] = t * exp2f(Q_OFFSET);
+        share[p] = t;
+    }
+    __syncthreads();
+    for (int64_t b = tid; b <= a.item_blocks; b += 256) {
+        const int64_t first = b * a.block_items;
+        int lo = 0, hi = n_list;
+        while (lo < hi) {
+            const int mid = (lo + hi) >> 1;
+            if (sorted[mid] < first) lo = mid + 1;
+            else hi = mid;
+        }
+        a.offs[u * (a.item_blocks + 1) + b] = (uint16_t)lo;
+    }
+    // the parts of pass 1
+    {
+        float hi = -__builtin_inff();
+        for (int s = tid; s < a.splits1; s += 256) hi = fmaxf(hi, a.stat_part[2 * ((int64_t)s * a.n + u)]);
+        hi = block_max256(hi, red);
+        float zz = 0.f;
+        for (int s = tid; s < a.splits1; s += 256) {
+            const int64_t at = (int64_t)s * a.n + u;
+            zz += a.stat_part[2 * at + 1] * exp2_fast(a.stat_part[2 * at] - hi);
+        }
+        zz = block_sum256(zz, red);
+        if (tid == 0) {
+            stat[0] = hi; stat[1] = zz;
+            // a list without weight: c (q - t) must be 0 for all items, so its user's q is switched off
+            a.bias[u] = any ? hi + log2f(zz) - P_OFFSET - Q_OFFSET : NEVER;
+        }
+    }
+    __syncthreads();
+    const float m = stat[0], z = stat[1];
+    const float lse = (m + log2f(z) - P_OFFSET) * 0.69314718f;       // ln Z of s / T
+    // the listed items: t y summed, <x, y> for the loss; a wave takes an item at a time
+    float acc[4] = {0.f, 0.f, 0.f, 0.f}, loss = 0.f;
+    for (int p = wave; p < a.k; p += 4) {
+        const uint64_t own = key[p];
+        if (own == ~0ull) continue;
+        const float *y = a.Y + (int64_t)(own >> 32) * a.ldy;
+        const float t = share[p];
+        float dot = 0.f;
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int c = lane + 64 * q;
+            if (c < f) {
+                const float v = y[c];
+                dot = fmaf(v, x[c], dot);
+                acc[q] = fmaf(t, v, acc[q]);
+            }
+        }
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) dot += __shfl_xor(dot, o);
+        if (t != 0.f) loss += t * (logf(t) - (dot * a.inv_t - lse));
+    }
+#pragma unroll
+    for (int q = 0; q < 4; ++q) part[wave][lane + 64 * q] = acc[q];
+    if (lane == 0) red[wave] = loss;
+    __syncthreads();
+    if (tid == 0) a.loss[u] = any ? (red[0] + red[1]) + (red[2] + red[3]) : 0.f;
+    if (tid < f) {
+        float o = 0.f;
+        for (int s = 0; s < a.splits1; ++s) {
+            const int64_t at = (int64_t)s * a.n + u;
+            o += a.o_part[at * F + tid] * exp2_fast(a.stat_part[2 * at] - m);
+        }
+        const float listed = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
+        const float c = (a.weight ? a.weight[u] : 1.f) * a.inv_t;
+        a.dX[u * f + tid] = any ? c * (o / z * a.scales[1] - listed) : 0.f;
+    }
+}
+
+// ----------------------------------------------------------------------------- host
+int padded_factors(const int32_t f) { return f <= 32 ? 32 : f <= 64 ? 64 : f <= 128 ? 128 : 256; }
+int waves_of(const int F) { return F == 256 ? 4 : 8; }
+
+struct Plan {
+    int F, waves, splits1, splits2, item_blocks;
+    int64_t n_tiles, m_tiles;
+    size_t off_scales, off_xt, off_yt, off_o, off_stat, off_bias, off_item, off_t, off_offs, off_dy, total;
+};
+
+// Splits of a pass over `stream` tiles for `blocks` workgroups: enough workgroups for 512 (two per compute unit), at least
+// 8 tiles each, a multiple of 8 from 8 on (one XCD per split), none empty.
+int split_count(const int64_t blocks, const int64_t stream) {
+    int64_t s = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(blocks, 1), stream / 8));
+    if (s > 8) s = s / 8 * 8;
+    while (s > 1) {
+        const int64_t per = (stream + s - 1) / s;
+        if ((s - 1) * per < stream) break;
+        s = s > 8 ? s - 8 : s - 1;
+    }
+    return (int)s;
+}
+
+Plan make_plan(const int64_t n, const int64_t M, const int32_t f, const int32_t k) {
+    Plan p;
+    p.F = padded_factors(f);
+    p.waves = waves_of(p.F);
+    p.n_tiles = (n + TILE - 1) / TILE;
+    p.m_tiles = (M + TILE - 1) / TILE;
+    p.splits1 = split_count((p.n_tiles + p.waves - 1) / p.waves, p.m_tiles);
+    p.splits2 = split_count((p.m_tiles + p.waves - 1) / p.waves, p.n_tiles);
+    p.item_blocks = (int)((M + p.waves * TILE - 1) / (p.waves * TILE));
+    size_t at = 0;
+    auto take = [&](const size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
+    take((Y_MAX_BLOCKS + 2 * X_MAX_BLOCKS) * 4);
+    p.off_scales = take(16);
+    p.off_xt = take((size_t)p.n_tiles * p.F * 256);
+    p.off_yt = take((size_t)p.m_tiles * p.F * 256);
+    p.off_o = take((size_t)p.splits1 * n * p.F * 4);
+    p.off_stat = take((size_t)p.splits1 * n * 8);
+    p.off_bias = take((size_t)p.n_tiles * TILE * 4);
+    p.off_item = take((size_t)n * k * 4);
+    p.off_t = take((size_t)n * k * 4);
+    p.off_offs = take((size_t)n * (p.item_blocks + 1) * 2);
+    p.off_dy = take(p.splits2 > 1 ? (size_t)p.splits2 * M * p.F * 4 : 0);
+    p.total = at;
+    return p;
+}
+
+template <int F, int WAVES, int RING, int TBUF, bool BACK>
+int32_t launch_pass(const FactorArgs &a, hipStream_t st) {
+    const int64_t stat_tiles = BACK ? a.m_tiles : a.n_tiles;
+    const int64_t grid = (stat_tiles + WAVES - 1) / WAVES * (BACK ? a.splits2 : a.splits1);
+    if (grid > INT32_MAX) return als_fail_(ALS_ERR_UNSUPPORTED, "als_distill_topk_f32: too many workgroups");
+    constexpr int bytes = RING * (F / 4) * 1024 + (BACK ? TBUF * (WAVES * 32 * T_STRIDE + 32) * 4 : 0);
+    static_assert(bytes <= 160 * 1024, "LDS");
+    ALS_HIP_CHECK6(hipFuncSetAttribute((const void *)pass_kernel<F, WAVES, RING, TBUF, BACK>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
+    hipLaunchKernelGGL((pass_kernel<F, WAVES, RING, TBUF, BACK>), dim3((unsigned)grid), dim3(WAVES * 64), bytes, st, a);
+    ALS_HIP_CHECK6(hipGetLastError());
+    return ALS_OK;
+}
+
+template <int F, int WAVES, int RING1, int RING2, int TBUF>
+int32_t run(const FactorArgs &a, hipStream_t st) {
+    hipLaunchKernelGGL(maxima_kernel, dim3(Y_MAX_BLOCKS + X_MAX_BLOCKS), dim3(256), 0, st, a);
+    hipLaunchKernelGGL((prepare_kernel<F>), dim3((unsigned)(a.m_tiles + a.n_tiles)), dim3(256), 0, st, a);
+    ALS_HIP_CHECK6(hipGetLastError());
+    int32_t rc = launch_pass<F, WAVES, RING1, 1, false>(a, st);
+    if (rc) return rc;
+    hipLaunchKernelGGL(lists_kernel, dim3((unsigned)(a.n_tiles * TILE)), dim3(256), 0, st, a, F);
+    ALS_HIP_CHECK6(hipGetLastError());
+    rc = launch_pass<F, WAVES, RING2, TBUF, true>(a, st);
+    if (rc) return rc;
+    if (a.splits2 > 1) {
+        const int64_t blocks = std::min<int64_t>((a.M * a.f + 255) / 256, 4096);
+        hipLaunchKernelGGL(join_items_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a, F);
+        ALS_HIP_CHECK6(hipGetLastError());
+    }
+    return ALS_OK;
+}
+
+bool sizes_ok(const int64_t n, const int64_t M, const int32_t f, const int32_t k) {
+    return n >= 1 && M >= 1 && M <= INT32_MAX / 2 && n <= INT32_MAX / 2 && f >= 1 && f <= ALS_MAX_FACTORS && k >= 1 && k <= LIST_MAX;
+}
+
+}  // namespace
+
+extern "C" {
+
+size_t als_distill_topk_workspace_bytes(int64_t n_users, int64_t M, int32_t f, int32_t k) {
+    return sizes_ok(n_users, M, f, k) ? make_plan(n_users, M, f, k).total : 0;
+}
+
+int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const int64_t *user_ids, int64_t n_users, const float *Y,
+                             int64_t ldy, int64_t M, int32_t f, const int32_t *teacher_idx, const float *teacher_val, int64_t ld_teacher,
+                             int32_t k, float temperature, const float *weight, float *loss_out, float *dX_out, float *dY_out,
+                             void *workspace, size_t ws_bytes, void *stream) {
+    if (!X || !Y || !teacher_idx || !teacher_val || !loss_out || !dX_out || !dY_out || !workspace)
+        return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_topk_f32: null pointer");
+    if (f > ALS_MAX_FACTORS || k > LIST_MAX)
+        return als_fail_(ALS_ERR_UNSUPPORTED, "als_distill_topk_f32: f=%d (at most %d), k=%d (at most %d)", f, ALS_MAX_FACTORS, k, LIST_MAX);
+    if (!sizes_ok(n_users, M, f, k) || x_rows < 1 || (!user_ids && n_users > x_rows) || ldx < f || ldy < f || ld_teacher < k)
+        return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_topk_f32: bad sizes (n_users=%lld M=%lld f=%d k=%d)", (long long)n_users,
+                         (long long)M, f, k);
+    if (!(temperature >= 1e-6f && temperature <= 1e6f))
+        return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_topk_f32: temperature %g outside [1e-6, 1e6]", (double)temperature);
+    const Plan p = make_plan(n_users, M, f, k);
+    if (ws_bytes < p.total || (uintptr_t)workspace % 16)
+        return als_fail_(ALS_ERR_WORKSPACE, "als_distill_topk_f32: workspace too small or not 16-byte aligned: %zu < %zu", ws_bytes, p.total);
+    FactorArgs a;
+    a.X = X; a.Y = Y; a.ldx = ldx; a.ldy = ldy; a.users = user_ids; a.n = n_users; a.M = M; a.f = f; a.x_rows = x_rows;
+    a.t_idx = teacher_idx; a.t_val = teacher_val; a.ldt = ld_teacher; a.k = k; a.inv_t = 1.f / temperature; a.weight = weight;
+    a.loss = loss_out; a.dX = dX_out; a.dY = dY_out;
+    char *ws = (char *)workspace;
+    a.maxima = (float *)ws;
+    a.scales = (float *)(ws + p.off_scales);
+    a.xt = ws + p.off_xt; a.yt = ws + p.off_yt;
+    a.o_part = (float *)(ws + p.off_o); a.stat_part = (float *)(ws + p.off_stat); a.bias = (float *)(ws + p.off_bias);
+    a.s_item = (int32_t *)(ws + p.off_item); a.s_t = (float *)(ws + p.off_t); a.offs = (uint16_t *)(ws + p.off_offs);
+    a.dy_part = (float *)(ws + p.off_dy);
+    a.n_tiles = p.n_tiles; a.m_tiles = p.m_tiles; a.splits1 = p.splits1; a.splits2 = p.splits2; a.item_blocks = p.item_blocks;
+    a.block_items = p.waves * TILE;
+    hipStream_t st = (hipStream_t)stream;
+    switch (p.F) {
+        case 32: return run<32, 8, 4, 3, 2>(a, st);
+        case 64: return run<64, 8, 4, 3, 2>(a, st);
+        case 128: return run<128, 8, 3, 2, 2>(a, st);
+        default: return run<256, 4, 2, 2, 1>(a, st);
+    }
+}
+
+}  // extern "C"

@@ -749,6 +749,45 @@ def distill_rows(score_rows, teacher_idx, teacher_val, temperature=1.0, weight=N
     return loss, out
 
 
+def distill_topk(X, Y, users, teacher_idx, teacher_val, temperature=1.0, weight=None, M=None):
+    """distill_rows for the scores <X[users], Y[:M]> of two float32 factors, without the score matrix, and with the
+    gradients of the factors instead of the scores' (als_distill_topk_f32 in include/als_hip.h).  users: int64 device
+    tensor, or None for every row of X; an id outside X gives NaN for its own row and adds nothing to the items (the ids are
+    not looked at on the host: nothing here waits for the device).  The lists are one per user, as for distill_rows.
+    Returns (loss [n], dX [n, f], dY [M, f]): the unweighted losses and the gradients of sum(weight * loss) with respect
+    to the users' rows - a user listed twice has two - and to the first M (default: all) item rows."""
+    ldx = _factor_ld(X, "X"); ldy = _factor_ld(Y, "Y")
+    f = X.shape[1]
+    if Y.shape[1] != f or not (1 <= f <= _lib.MAX_FACTORS):
+        raise ValueError("factor counts differ or lie outside 1..%d" % _lib.MAX_FACTORS)
+    M = Y.shape[0] if M is None else int(M)
+    if not (1 <= M <= Y.shape[0]) or X.shape[0] < 1:
+        raise ValueError("M out of range, or X without rows")
+    if users is not None:
+        _index(users, torch.int64, "users")
+    n = X.shape[0] if users is None else users.shape[0]
+    k, ldt = _teacher_lists(teacher_idx, teacher_val, n, X)
+    T = _temperature(temperature)
+    if not (1e-6 <= T <= 1e6):
+        raise ValueError("temperature must lie in [1e-6, 1e6]")
+    if weight is not None:
+        _index(weight, torch.float32, "weight")
+        if weight.shape[0] != n:
+            raise ValueError("weight must have one value per user")
+    _same_device(X, Y, users, weight)
+    loss = torch.empty(n, dtype=torch.float32, device=X.device)
+    dX = torch.empty((n, f), dtype=torch.float32, device=X.device)
+    if n == 0:
+        return loss, dX, torch.zeros((M, f), dtype=torch.float32, device=X.device)
+    dY = torch.empty((M, f), dtype=torch.float32, device=X.device)
+    ws = torch.empty(lib.als_distill_topk_workspace_bytes(n, M, f, k), dtype=torch.uint8, device=X.device)
+    with torch.cuda.device(X.device):
+        check(lib.als_distill_topk_f32(_ptr(X), X.shape[0], ldx, _ptr(users), n, _ptr(Y), ldy, M, f, _ptr(teacher_idx),
+                                       _ptr(teacher_val), ldt, k, T, _ptr(weight), _ptr(loss), _ptr(dX), _ptr(dY), _ptr(ws), ws.numel(), _stream()),
+              "als_distill_topk_f32")
+    return loss, dX, dY
+
+
 def predict_pairs(X, Y, u, i):
     """out[p] = <X[u[p]], Y[i[p]]>: the ALS model's output for explicit (user, item) pairs
     (reclibwh/core/ALS.py:359-362)."""

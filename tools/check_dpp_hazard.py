@@ -19,7 +19,8 @@ import tempfile
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "recommender_amd", "csrc")
-SOURCES = ["als_kernels.hip", "als_cg.hip", "als_scoring.hip", "als_short_rows.hip", "als_sampling.hip", "als_distill.hip"]
+SOURCES = ["als_kernels.hip", "als_cg.hip", "als_scoring.hip", "als_short_rows.hip", "als_sampling.hip", "als_distill.hip",
+           "als_distill_factors.hip"]
 
 
 def makefile_flags():
