@@ -415,9 +415,11 @@ typedef struct {
     const float *top_p_rows;
     const float *min_p_rows;
 } als_sample_opts_t;
+size_t als_sample_rows_workspace_bytes(int32_t dtype, int64_t n_rows, int64_t M);
 int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows, int64_t M, const int64_t *ex_rowptr,
                         const int32_t *ex_col, const int64_t *ex_row_ids, const als_sample_opts_t *opts, const void *u,
-                        int32_t u_is_f64, int32_t n_draws, int32_t *idx_out, float *logp_out, void *stream);
+                        int32_t u_is_f64, int32_t n_draws, int32_t *idx_out, float *logp_out, void *workspace, size_t ws_bytes,
+                        void *stream);
 
 /* ------------------------------------------------------------------------------------
  * Following a teacher's ranked lists (no reference counterpart): how far a student's softmax over all items is from a

@@ -7,15 +7,20 @@
 //   4. with W the weight of what is left and u in [0, 1): the draw is the first item in rank order at which the running
 //      weight exceeds u W; its ln(w_i / W) is returned beside it.
 // Every step asks the same question - at which item, in rank order, does a running sum (of ones, or of weights) pass a
-// target - and the kernel has one answer to it (find): a histogram of the row over 2048 buckets of equal width in the
+// target - and the kernels have one answer to it (find): a histogram of the row over 2048 buckets of equal width in the
 // score gives the bucket, the bucket's few items are collected in LDS and ranked against each other.  Nothing is sorted.
 //
 // Weights are held as integers, round(w 2^Q) with Q = min(51, 62 - ceil(log2 M)): their sums are exact whatever the order,
-// so LDS atomics do not make the result depend on timing, and a draw differs from the definition's only where u W lies
+// so integer atomics do not make the result depend on timing, and a draw differs from the definition's only where u W lies
 // within the summed roundings of a border.  With M = 59 047 (Q = 46) that is a part in 10^11 of W; float32 sums would
 // decide one draw in a hundred wrongly on a catalogue of a million.  An item whose weight rounds to 0 (below 2^-47 of the
 // largest) counts as dropped.  exp is computed in float64 (which this chip multiplies at the float32 rate): x 256 / ln 2 =
 // k + r, 2^(k mod 256 / 256) from a table, a polynomial of degree 4 in r; error below 1e-15.
+//
+// Two forms.  sample_rows_kernel: one workgroup per row, one launch; the row is read from memory for its maximum and
+// then, mostly from the caches, once more (filtered rows) or twice more (rows of which much counts).  Few long rows are
+// cut into parts, one workgroup each, in four launches: maximum; histogram; items of the buckets the answers can lie in,
+// collected in a list; the answers from the list.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -37,10 +42,27 @@ namespace {
 
 typedef unsigned long long u64;
 
-constexpr int SR_THREADS = 1024;
-constexpr int SR_BUCKETS = 2048;      // 2 per thread
-constexpr int SR_LIST = 1024;         // items of one bucket that are ranked directly
-constexpr int SR_WAVES = SR_THREADS / 64;
+// A workgroup's size.  The steps between the passes are short and alike for all waves, so a workgroup has no more threads
+// than its row needs: 256 for rows its registers hold, else 512.
+template <int T, int B>
+struct Group {
+    static constexpr int THREADS = T, WAVES = T / 64, BUCKETS = B;
+    static constexpr int OWN = B / T;             // buckets per thread
+    static constexpr int RANKED = T / 4;          // items that are ranked against each other directly, four threads each
+};
+typedef Group<256, 512> Small;
+typedef Group<512, 2048> Large;
+constexpr int CUT_BUCKETS = Large::BUCKETS;
+constexpr int SR_LISTED = 16384;      // cut rows: items collected per row
+
+struct Found {            // an item collected by a workgroup of a cut row
+    float score;
+    int32_t index;
+};
+struct PartStat {
+    u64 best;             // rank key of the largest score << 32 | ~column: the best item of the part
+    float low, pad;       // smallest score that is no mask value
+};
 
 struct SampleArgs {
     void *scores;
@@ -53,107 +75,198 @@ struct SampleArgs {
     int32_t u_f64, n_draws, q_bits;
     int32_t *idx;
     float *logp;
+    // cut rows
+    int32_t n_parts, per_part;        // chunks per part
+    PartStat *stats;                  // [row, part]
+    u64 *wsum;                        // [row, bucket]
+    uint32_t *cnt;                    // [row, bucket]
+    uint32_t *n_found;                // [row]
+    Found *found;                     // [row, SR_LISTED]
 };
+
+// A value that is the same in all lanes of a wave, told to the compiler: it then lives in scalar registers.
+__device__ __forceinline__ uint32_t uniform(const uint32_t v) { return (uint32_t)__builtin_amdgcn_readfirstlane((int)v); }
+__device__ __forceinline__ int32_t uniform(const int32_t v) { return __builtin_amdgcn_readfirstlane(v); }
+__device__ __forceinline__ float uniform(const float v) { return __uint_as_float(uniform(__float_as_uint(v))); }
+__device__ __forceinline__ u64 uniform(const u64 v) { return (u64)uniform((uint32_t)(v >> 32)) << 32 | uniform((uint32_t)v); }
 
 // floats as unsigned keys of the same order
 __device__ __forceinline__ uint32_t rank_key(const float s) {
     const uint32_t b = __float_as_uint(s + 0.f);            // -0 and +0 are one score: -0 + 0 = +0
     return b & 0x80000000u ? ~b : b | 0x80000000u;
 }
+__device__ __forceinline__ float key_score(const uint32_t k) { return __uint_as_float(k & 0x80000000u ? k & 0x7fffffffu : ~k); }
 
 struct Picked {
     u64 before, weight;       // running weight in front of the item, its own
     int32_t index;
+    float score;
 };
 
+template <class G>
 struct SampleShared {
-    u64 wsum[SR_BUCKETS], wsub[SR_BUCKETS];
-    uint32_t cnt[SR_BUCKETS], csub[SR_BUCKETS];
-    u64 list[SR_LIST][2];           // (key << 32 | ~index, weight)
+    u64 wsum[G::BUCKETS];
+    uint32_t cnt[G::BUCKETS];
+    union {
+        struct { u64 wsub[G::BUCKETS]; uint32_t csub[G::BUCKETS]; };
+        u64 ranked[G::RANKED][2];           // (key << 32 | ~column, weight)
+    };
     double pow2[256];               // 2^(i / 256)
-    u64 wave_w[SR_WAVES];
-    uint32_t wave_c[SR_WAVES];
-    float wave_f[SR_WAVES], wave_g[SR_WAVES];
+    u64 wave_w[G::WAVES];
+    uint32_t wave_c[G::WAVES];
+    float wave_f[G::WAVES], wave_g[G::WAVES];
     Picked picked;
-    uint32_t bucket, n_list;
+    uint32_t bucket, n_list, k_lo, k_hi;
     u64 base_w;
     uint32_t base_c, in_bucket;
 };
 
-// What the steps of one row share.
-struct RowScale {
-    float top;          // the largest score
-    double inv_t;       // 1 / T
-    double cut;         // items with x < -cut have no weight
-    float min_p;
-    float per_score;    // buckets per unit of score
-    int q_bits;
+// A row's parameters.
+struct RowParams {
+    float T, top_p, min_p;
+    int32_t top_k;
 };
+__device__ __forceinline__ RowParams row_params(const SampleArgs &a, const int64_t r) {
+    RowParams p;
+    p.T = a.o.temperature_rows ? a.o.temperature_rows[r] : a.o.temperature;
+    p.top_k = a.o.top_k_rows ? a.o.top_k_rows[r] : a.o.top_k;
+    p.top_p = a.o.top_p_rows ? a.o.top_p_rows[r] : a.o.top_p;
+    const float m = a.o.min_p_rows ? a.o.min_p_rows[r] : a.o.min_p;
+    p.min_p = m > 0.f ? fminf(m, 1.f) : 0.f;                  // NaN: off
+    return p;
+}
 
-// exp(x) for x in [-cut, 0], and its integer weight
-__device__ __forceinline__ double exp_table(const double x, const double *pow2, int &k256) {
-    constexpr double C = 256.0 * 1.4426950408889634074, MAGIC = 6755399441055744.0;      // 1.5 2^52: adds, rounds to an integer
-    const double kd = fma(x, C, MAGIC);
+// Whether top-k can take part, and the histogram needs counts.
+__device__ __forceinline__ bool top_k_asked(const SampleArgs &a, const RowParams &p) { return p.top_k > 0 && p.top_k < a.M; }
+
+// How scores become weights and buckets.  (The largest score is finite here: rows with +inf are answered apart.)
+struct RowScale {
+    double top;         // the largest score
+    double steps;       // 256 / (T ln 2): a score's x in 256ths of a power of two
+    double cut;         // ... and how many of those below the top an item has no weight, or is below min_p
+    double min_w;       // min_p 2^Q
+    float top_f, per_score;    // buckets per unit of score
+    float reject;       // scores this many buckets or more below the top are beyond the cut
+};
+// low: the smallest score that is no mask value (+inf if there is none).  It only sets the buckets' width.
+__device__ __forceinline__ RowScale row_scale(const float top, const float low, const RowParams &p, const int q_bits, const int buckets) {
+    RowScale c;
+    double cut = 0.6931471805599453 * (q_bits + 1);           // beyond it a weight rounds to 0
+    if (p.min_p > 0.f) cut = fmin(cut, -log((double)p.min_p) + 1e-6);
+    c.top = (double)top;
+    c.steps = 256.0 * 1.4426950408889634074 / (double)p.T;
+    c.cut = cut * (256.0 * 1.4426950408889634074);
+    c.min_w = ldexp((double)p.min_p, q_bits);
+    const float reach = (float)fmin(cut * (double)p.T, 3e38);
+    const float width = fmaxf(low <= top ? fminf(reach, top - low) : reach, 1e-30f);
+    c.top_f = uniform(top);
+    c.per_score = uniform((float)buckets / width);
+    c.reject = uniform((float)buckets * fmaxf(1.f, reach / width) * 1.01f);
+    return c;
+}
+
+// pow2: 2^(Q + i / 256), i < 256.  2^(y / 256 + Q) for y <= 0, y = k + f with k an integer: table and a polynomial of degree 4.
+__device__ __forceinline__ double exp_table(const double y, const double *pow2) {
+    constexpr double MAGIC = 6755399441055744.0;              // 1.5 2^52: adds, rounds to an integer
+    const double kd = y + MAGIC;
     const int k = (int)(uint32_t)__double_as_longlong(kd);
-    const double r = fma(x, C, -(kd - MAGIC)) * (0.69314718055994530942 / 256.0);
+    const double r = (y - (kd - MAGIC)) * (0.69314718055994530942 / 256.0);
     const double p = fma(r, fma(r, fma(r, 1.0 / 24, 1.0 / 6), 0.5), 1.0);
-    k256 = k >> 8;
     const double t = pow2[k & 255];
-    return fma(t * r, p, t);
+    const double m = fma(t * r, p, t);
+    return __hiloint2double(__double2hiint(m) + ((k >> 8) << 20), __double2loint(m));
 }
+// The integer weight of a score; false if it has none.  Without branches: four at a time keep the float64 units busy.
 __device__ __forceinline__ bool weigh(const float s, const RowScale &c, const double *pow2, u64 &w) {
-    const double d = s == c.top ? 0.0 : (double)s - (double)c.top;
-    const double x = d * c.inv_t;
-    if (!(x >= -c.cut)) return false;                       // NaN scores and NaN products (inf x 0) among them
-    int e;
-    const double m = exp_table(x, pow2, e);                 // w = m 2^e, m in [1, 2)
-    const double w1 = __longlong_as_double(__double_as_longlong(m) + ((int64_t)e << 52));
-    if (!(w1 >= (double)c.min_p)) return false;
-    // w 2^Q + 2^52: the mantissa's low bits are the integer, rounded to nearest even
-    const double q = __longlong_as_double(__double_as_longlong(w1) + ((int64_t)c.q_bits << 52)) + 4503599627370496.0;
-    w = (u64)__double_as_longlong(q) & 0xfffffffffffffull;
-    return w != 0;
+    const double y = ((double)s - c.top) * c.steps;
+    const double m = exp_table(y, pow2);                      // w 2^Q
+    // + 2^52: the mantissa's low bits are the integer, rounded to nearest even
+    w = (u64)__double_as_longlong(m + 4503599627370496.0) & 0xfffffffffffffull;
+    return y >= -c.cut && m >= c.min_w && w != 0;             // not so for NaN scores and NaN products (-inf x 0)
 }
-// Bucket of a score: falls with the score (each operation is monotone), so buckets are runs of the rank order.
+// ln of a weight's integer: float32's logarithm of the mantissa and one Newton step with the exponential at hand (the
+// library's float64 logarithm would cost the kernels the registers of a second resident workgroup).
+__device__ __forceinline__ double log_of(const u64 w, const double *pow2, const int q_bits) {
+    const int e = 63 - __clzll((long long)w);
+    const double m = ldexp((double)w, -e);
+    const double y = (double)logf((float)m);
+    const double t = ldexp(exp_table(y * (-256.0 * 1.4426950408889634074), pow2), -q_bits);       // e^-y
+    return 0.69314718055994530942 * e + (y + fma(m, t, -1.0));
+}
+// Bucket of a score, B if it is certainly beyond the cut.  Falls with the score (every operation is monotone), so
+// buckets are runs of the rank order.  NaN scores get some bucket or none: they have no weight.
+template <int B>
 __device__ __forceinline__ uint32_t bucket_of(const float s, const RowScale &c) {
-    const float b = (c.top - s) * c.per_score;
-    return (uint32_t)(int)fminf(b, (float)(SR_BUCKETS - 1));
+    const float t = (c.top_f - s) * c.per_score;
+    return t <= c.reject ? (uint32_t)(int)fminf(t, (float)(B - 1)) : B;
 }
 
-__device__ __forceinline__ u64 shfl_up64(const u64 v, const int o) {
-    const uint32_t lo = (uint32_t)__shfl_up((int)(uint32_t)v, o), hi = (uint32_t)__shfl_up((int)(uint32_t)(v >> 32), o);
-    return (u64)hi << 32 | lo;
+// Inclusive running sums over a wave's lanes by DPP moves (rows of 16 lanes, then across rows).
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t moved(const uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xf, true);      // lanes without a source get 0
+}
+template <int CTRL, int ROWS>
+__device__ __forceinline__ u64 moved(const u64 v) {
+    return (u64)moved<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | moved<CTRL, ROWS>((uint32_t)v);
+}
+template <class V>
+__device__ __forceinline__ V wave_scan(V v) {
+    v += moved<0x111, 0xf>(v);        // row_shr:1
+    v += moved<0x112, 0xf>(v);        // row_shr:2
+    v += moved<0x114, 0xf>(v);        // row_shr:4
+    v += moved<0x118, 0xf>(v);        // row_shr:8
+    v += moved<0x142, 0xa>(v);        // row_bcast:15 into rows 1 and 3
+    v += moved<0x143, 0xc>(v);        // row_bcast:31 into rows 2 and 3
+    return v;
 }
 
-// Inclusive running sums over the 2048 buckets of (cnt, wsum), in place; every thread owns two.
-__device__ void scan_buckets(uint32_t *cnt, u64 *wsum, SampleShared &sh) {
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const uint32_t c0 = cnt[2 * tid], c1 = cnt[2 * tid + 1];
-    const u64 w0 = wsum[2 * tid], w1 = wsum[2 * tid + 1];
-    uint32_t c = c0 + c1;
-    u64 w = w0 + w1;
+// Sum of the first `n` of the per-wave values: a lane loads one each (a loop over them costs its unrolled registers).
+template <class G, class V>
+__device__ __forceinline__ V sum_of_first(const V *v, const int n) {
+    const int l = threadIdx.x & (G::WAVES - 1);
+    V s = l < n ? v[l] : 0;
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t cc = (uint32_t)__shfl_up((int)c, o);
-        const u64 ww = shfl_up64(w, o);
-        if (lane >= o) { c += cc; w += ww; }
+    for (int o = G::WAVES / 2; o >= 1; o >>= 1) {
+        if constexpr (sizeof(V) == 4) {
+            s += (V)__shfl_xor((int)s, o);
+        } else {
+            const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)s, o), hi = (uint32_t)__shfl_xor((int)(uint32_t)(s >> 32), o);
+            s += (u64)hi << 32 | lo;
+        }
     }
-    if (lane == 63) { sh.wave_c[wave] = c; sh.wave_w[wave] = w; }
+    return s;
+}
+
+// Inclusive running sums over the buckets of (cnt, wsum), in place; every thread has OWN neighbours.
+template <class G>
+__device__ __forceinline__ void scan_buckets(uint32_t *cnt, u64 *wsum, SampleShared<G> &sh) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    uint32_t c[G::OWN];
+    u64 w[G::OWN];
+#pragma unroll
+    for (int q = 0; q < G::OWN; ++q) {
+        c[q] = cnt[G::OWN * tid + q] + (q ? c[q - 1] : 0);
+        w[q] = wsum[G::OWN * tid + q] + (q ? w[q - 1] : 0);
+    }
+    uint32_t bc = wave_scan(c[G::OWN - 1]);
+    u64 bw = wave_scan(w[G::OWN - 1]);
+    if (lane == 63) { sh.wave_c[wave] = bc; sh.wave_w[wave] = bw; }
     __syncthreads();
-    uint32_t bc = 0;
-    u64 bw = 0;
-    for (int v = 0; v < wave; ++v) { bc += sh.wave_c[v]; bw += sh.wave_w[v]; }
-    cnt[2 * tid] = bc + c - c1; cnt[2 * tid + 1] = bc + c;
-    wsum[2 * tid] = bw + w - w1; wsum[2 * tid + 1] = bw + w;
+    bc += sum_of_first<G>(sh.wave_c, wave) - c[G::OWN - 1];          // in front of the thread's buckets
+    bw += sum_of_first<G>(sh.wave_w, wave) - w[G::OWN - 1];
+#pragma unroll
+    for (int q = 0; q < G::OWN; ++q) { cnt[G::OWN * tid + q] = bc + c[q]; wsum[G::OWN * tid + q] = bw + w[q]; }
     __syncthreads();
 }
 
 // The bucket at which the running sum (of ones or of weights) passes `target`; base sums in front of it.
+template <class G>
 __device__ void pick_bucket(const uint32_t *cnt, const u64 *wsum, const bool by_count, const u64 target, const uint32_t base_c,
-                            const u64 base_w, SampleShared &sh) {
+                            const u64 base_w, SampleShared<G> &sh) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-        const int b = 2 * threadIdx.x + h;
+    for (int q = 0; q < G::OWN; ++q) {
+        const int b = G::OWN * threadIdx.x + q;
         const uint32_t pc = b ? cnt[b - 1] : 0, cc = cnt[b];
         const u64 pw = b ? wsum[b - 1] : 0, cw = wsum[b];
         const u64 lo = by_count ? base_c + pc : base_w + pw, hi = by_count ? base_c + cc : base_w + cw;
@@ -164,66 +277,121 @@ __device__ void pick_bucket(const uint32_t *cnt, const u64 *wsum, const bool by_
     __syncthreads();
 }
 
-// The row, either held in registers (NV chunks per thread) or read from memory again at every pass (NV = 0).
-template <int TYPE, int NV>
-struct RowStore {
-    RowView<TYPE> view;
-    row_u32x4 held[NV ? NV : 1];
-    float extra;
-    int32_t extra_at;
+// ----------------------------------------------------------------------------- where a row's items come from
+// f(score, column) for the calling thread's share of the items; columns outside the row are never passed on, but scores
+// of -inf may stand for nothing.
 
-    __device__ __forceinline__ RowStore(const RowView<TYPE> &v) : view(v) {
-        if constexpr (NV > 0) {
+// Four items at a time, if any of them has a bucket: f(scores, column of the first, buckets), false to stop.
+template <int B, class F>
+__device__ __forceinline__ bool four_buckets(const float s0, const float s1, const float s2, const float s3, const int32_t i0,
+                                             const RowScale &c, F f) {
+    const float s[4] = {s0, s1, s2, s3};
+    const uint32_t b[4] = {bucket_of<B>(s0, c), bucket_of<B>(s1, c), bucket_of<B>(s2, c), bucket_of<B>(s3, c)};
+    return min(min(b[0], b[1]), min(b[2], b[3])) >= B || f(s, i0, b);
+}
+// Adds the four to the histogram.  Counts are only kept for rows that ask for them (top-k).
+template <int B>
+__device__ __forceinline__ void count_four(const float (&s)[4], const uint32_t (&b)[4], const RowScale &c, const double *pow2,
+                                           uint32_t *cnt, u64 *wsum, const bool counted) {
+    u64 w[4];
+    bool in[4];
 #pragma unroll
-            for (int q = 0; q < NV; ++q) {
-                held[q] = RowView<TYPE>::nothing();
-                if (q * SR_THREADS + (int)threadIdx.x < view.n_chunks) held[q] = view.load(q * SR_THREADS + threadIdx.x);
-            }
+    for (int q = 0; q < 4; ++q) in[q] = weigh(s[q], c, pow2, w[q]) && b[q] < B;
+#pragma unroll
+    for (int q = 0; q < 4; ++q)
+        if (in[q]) {
+            atomicAdd(&wsum[b[q]], w[q]);
+            if (counted) atomicAdd(&cnt[b[q]], 1u);
         }
-        extra_at = view.extra(threadIdx.x);
-        extra = extra_at >= 0 ? view.at(extra_at) : -__builtin_inff();
+}
+
+// Read from memory, four chunks in flight per thread: f(chunk, column of its first element), false to stop the wave's walk.
+template <class G, int TYPE, class F>
+__device__ __forceinline__ void each_chunk(const RowView<TYPE> &view, const int32_t q0, const int32_t q1, F f) {
+#pragma unroll 1
+    for (int32_t q = q0 + threadIdx.x; q < q1; q += 4 * G::THREADS) {
+        row_u32x4 v[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = RowView<TYPE>::nothing();
+            if (q + k * G::THREADS < q1) v[k] = view.load(q + k * G::THREADS);
+        }
+        bool go = true;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) go = f(v[k], view.index0(q + k * G::THREADS)) && go;
+        if (!__all(go)) break;
     }
-    // f(score, index) for this thread's elements; what lies outside the row comes as -inf
-    template <class F>
-    __device__ __forceinline__ void each(F f) const {
-        if constexpr (NV > 0) {
+}
+// The same, the four chunks together: f(chunks, column of the first one's first element); the others follow 4 THREADS
+// elements apart.
+template <class G, int TYPE, class F>
+__device__ __forceinline__ void each_quad(const RowView<TYPE> &view, const int32_t q0, const int32_t q1, F f) {
+#pragma unroll 1
+    for (int32_t q = q0 + threadIdx.x; q < q1; q += 4 * G::THREADS) {
+        row_u32x4 v[4];
 #pragma unroll
-            for (int q = 0; q < NV; ++q) {
-                const int32_t i0 = view.index0(q * SR_THREADS + threadIdx.x);
-#pragma unroll
-                for (int e = 0; e < RowView<TYPE>::VEC; ++e) f(RowView<TYPE>::value(held[q], e), i0 + e);
-            }
-        } else {
-            for (int32_t q = threadIdx.x; q < view.n_chunks; q += SR_THREADS) {
-                const row_u32x4 v = view.load(q);
-                const int32_t i0 = view.index0(q);
-#pragma unroll
-                for (int e = 0; e < RowView<TYPE>::VEC; ++e) f(RowView<TYPE>::value(v, e), i0 + e);
-            }
+        for (int k = 0; k < 4; ++k) {
+            v[k] = RowView<TYPE>::nothing();
+            if (q + k * G::THREADS < q1) v[k] = view.load(q + k * G::THREADS);
         }
-        if ((int)threadIdx.x < view.head + view.tail) f(extra, extra_at);
+        if (!f(v, view.index0(q))) break;
+    }
+}
+// The items that have a bucket, four at a time (see four_buckets).
+template <class G, int TYPE, class F>
+__device__ __forceinline__ void each_bucket(const RowView<TYPE> &view, const int32_t q0, const int32_t q1, const bool extra,
+                                            const RowScale &c, F f) {
+    each_chunk<G>(view, q0, q1, [&](const row_u32x4 &v, const int32_t i0) {
+        bool go = true;
+#pragma unroll
+        for (int e = 0; e < RowView<TYPE>::VEC; e += 4)
+            go = four_buckets<G::BUCKETS>(RowView<TYPE>::value(v, e), RowView<TYPE>::value(v, e + 1), RowView<TYPE>::value(v, e + 2),
+                                          RowView<TYPE>::value(v, e + 3), i0 + e, c, f) && go;
+        return go;
+    });
+    const int32_t x = extra ? view.extra(threadIdx.x) : -1;
+    if (x >= 0) four_buckets<G::BUCKETS>(view.at(x), -__builtin_inff(), -__builtin_inff(), -__builtin_inff(), x, c, f);
+}
+
+// The same for the rare passes over a whole row: not unrolled, it would take the registers of a resident workgroup.
+template <class G, int TYPE, class F>
+__device__ __forceinline__ void each_again(const RowView<TYPE> &view, F f) {
+#pragma unroll 1
+    for (int32_t i = threadIdx.x; i < view.M; i += G::THREADS) f(view.at(i), i);
+}
+
+// Collected in a list, or, where the list does not hold them, the whole row again.
+template <class G, int TYPE>
+struct ListedRow {
+    const RowView<TYPE> &view;
+    const Found *found;
+    uint32_t n;
+    bool whole;
+    template <class F>
+    __device__ __forceinline__ void each(F f) {
+        if (whole) each_again<G>(view, f);
+        else
+#pragma unroll 1
+            for (uint32_t q = threadIdx.x; q < n; q += G::THREADS) f(found[q].score, found[q].index);
     }
 };
 
-// Index of the m-th element (from 0, in index order) whose key is `key`; the rarest path: more than SR_LIST items of one
-// bucket share one score.  An element per thread and round.
-template <int TYPE>
-__device__ int32_t nth_of_key(const RowView<TYPE> &view, const uint32_t key, const u64 m, SampleShared &sh) {
+// Column of the m-th item (from 0, in column order) whose key is `key`; the rarest path: more than RANKED items of one
+// bucket share one score.  An item per thread and round.
+template <class G, int TYPE>
+__device__ int32_t nth_of_key(const RowView<TYPE> &view, const uint32_t key, const u64 m, SampleShared<G> &sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (tid == 0) sh.picked.index = -1;
     u64 seen = 0;
-    for (int64_t i0 = 0; i0 < view.M; i0 += SR_THREADS) {
+    for (int64_t i0 = 0; i0 < view.M; i0 += G::THREADS) {
         const int64_t i = i0 + tid;
         const bool hit = i < view.M && rank_key(view.at(i)) == key;
         const u64 mask = __ballot(hit);
         __syncthreads();                                     // the last round's wave sums have been read
         if (lane == 0) sh.wave_c[wave] = __popcll(mask);
         __syncthreads();
-        u64 before = seen + __popcll(mask & ((1ull << lane) - 1));
-        for (int x = 0; x < SR_WAVES; ++x) {
-            if (x < wave) before += sh.wave_c[x];
-            seen += sh.wave_c[x];
-        }
+        const u64 before = seen + __popcll(mask & ((1ull << lane) - 1)) + sum_of_first<G>(sh.wave_c, wave);
+        seen += sum_of_first<G>(sh.wave_c, G::WAVES);
         if (hit && before == m) sh.picked.index = (int32_t)i;
         if (m < seen) break;                                 // uniform: `seen` is the same in every thread
     }
@@ -231,199 +399,642 @@ __device__ int32_t nth_of_key(const RowView<TYPE> &view, const uint32_t key, con
     return sh.picked.index;
 }
 
+// ----------------------------------------------------------------------------- the question
 // The item, in rank order, at which the running sum of ones (by_count) or of weights passes `target`; the caller has
 // made sure that it does.  Every thread returns the same.
-template <int TYPE, int NV>
-__device__ Picked find(const RowStore<TYPE, NV> &row, const RowScale &c, const bool by_count, const u64 target,
-                       SampleShared &sh) {
+template <class G, int TYPE, class Row>
+__device__ Picked find(Row &row, const RowView<TYPE> &view, const RowScale &c, const bool by_count, const u64 target,
+                       const bool counted, SampleShared<G> &sh) {
     const int tid = threadIdx.x;
     pick_bucket(sh.cnt, sh.wsum, by_count, target, 0, 0, sh);
-    const uint32_t b = sh.bucket;
-    uint32_t n = sh.in_bucket, base_c = sh.base_c;
-    u64 base_w = sh.base_w;
-    // A bucket with more items than the list holds (many equal scores, or an outlier that stretches the buckets) is cut
-    // by its keys' digits, 11, 11 and 10 bits, until its part is short enough or a single key is left.
-    int shift = 32;
-    uint32_t prefix = 0;
-    while (n > SR_LIST && shift > 0) {
-        const int next = shift == 32 ? 21 : shift == 21 ? 10 : 0;
+    const uint32_t b = uniform(sh.bucket);
+    uint32_t n = counted ? uniform(sh.in_bucket) : 0, base_c = uniform(sh.base_c);      // 0: not known, tried
+    u64 base_w = uniform(sh.base_w);
+    // the bucket's keys [k_lo, k_hi] that are still in question; all of it to begin with
+    uint32_t k_lo = 0, k_hi = ~0u;
+    bool narrowed = false;
+    auto mine = [&](const float s, u64 &w) {                 // an item in question, and its weight
+        if (bucket_of<G::BUCKETS>(s, c) != b) return false;
+        const uint32_t key = rank_key(s);
+        return key >= k_lo && key <= k_hi && weigh(s, c, sh.pow2, w);
+    };
+    // More items than are ranked directly: first the keys they span, then, BUCKETS parts of that range a time, the part with
+    // the answer, until few are left (they are taken into LDS) or all that are left share one key.
+    int shift = 0;
+    for (;;) {
         __syncthreads();
-        sh.csub[2 * tid] = sh.csub[2 * tid + 1] = 0;
-        sh.wsub[2 * tid] = sh.wsub[2 * tid + 1] = 0;
+        const int act = n <= G::RANKED ? 2 : narrowed ? 1 : 0;
+        if (act == 1) {
+            if (k_lo == k_hi) {                              // one score, n items
+                const float s = key_score(k_lo);
+                u64 w = 1;
+                weigh(s, c, sh.pow2, w);
+                w = uniform(w);
+                const u64 m = by_count ? target - base_c : (target - base_w) / w;
+                const int32_t at = nth_of_key<G>(view, k_lo, m, sh);
+                __syncthreads();
+                return Picked{base_w + m * w, w, at, s};
+            }
+            const int bits = 32 - __clz(k_hi - k_lo), part_bits = 31 - __clz(G::BUCKETS);
+            shift = bits > part_bits ? bits - part_bits : 0;
+#pragma unroll
+            for (int q = 0; q < G::OWN; ++q) { sh.csub[G::OWN * tid + q] = 0; sh.wsub[G::OWN * tid + q] = 0; }
+        } else if (tid == 0) {
+            sh.k_lo = ~0u; sh.k_hi = 0;
+            sh.n_list = 0;
+        }
         __syncthreads();
-        row.each([&](const float s, const int32_t) {
-            if (bucket_of(s, c) != b) return;
-            const uint32_t key = rank_key(s);
-            if (shift < 32 && (key >> shift) != prefix) return;
+        row.each([&](const float s, const int32_t i) {
             u64 w;
-            if (!weigh(s, c, sh.pow2, w)) return;
-            const uint32_t d = SR_BUCKETS - 1 - ((key >> next) & (next ? 2047u : 1023u));     // large keys first
-            atomicAdd(&sh.csub[d], 1u);
-            atomicAdd(&sh.wsub[d], w);
+            if (!mine(s, w)) return;
+            const uint32_t key = rank_key(s);
+            if (act == 0) {
+                atomicMin(&sh.k_lo, key);
+                atomicMax(&sh.k_hi, key);
+            } else if (act == 1) {
+                const uint32_t d = (k_hi - key) >> shift;    // large keys first
+                atomicAdd(&sh.csub[d], 1u);
+                atomicAdd(&sh.wsub[d], w);
+            } else {
+                const uint32_t at = atomicAdd(&sh.n_list, 1u);
+                if (at < (uint32_t)G::RANKED) {
+                    sh.ranked[at][0] = (u64)key << 32 | (uint32_t)~(uint32_t)i;
+                    sh.ranked[at][1] = w;
+                }
+            }
         });
         __syncthreads();
+        if (act == 2) {
+            n = uniform(sh.n_list);
+            if (n <= G::RANKED) break;
+            continue;
+        }
+        if (act == 0) {
+            k_lo = uniform(sh.k_lo); k_hi = uniform(sh.k_hi);
+            narrowed = true;
+            continue;
+        }
         scan_buckets(sh.csub, sh.wsub, sh);
         pick_bucket(sh.csub, sh.wsub, by_count, target, base_c, base_w, sh);
-        const uint32_t digit = SR_BUCKETS - 1 - sh.bucket;
-        prefix = shift == 32 ? digit : next ? (prefix << 11 | digit) : (prefix << 10 | digit);
-        n = sh.in_bucket; base_c = sh.base_c; base_w = sh.base_w;
-        shift = next;
+        const uint32_t d = uniform(sh.bucket);
+        const uint64_t behind = (uint64_t)(d + 1) << shift;                // keys down to the part's end
+        k_lo = behind > k_hi - k_lo ? k_lo : k_hi - (uint32_t)behind + 1;
+        k_hi = k_hi - (d << shift);
+        n = uniform(sh.in_bucket); base_c = uniform(sh.base_c); base_w = uniform(sh.base_w);
+    }
+    // The few that are left are ranked against each other, four threads to an item.
+    const int e = tid >> 2;
+    const u64 own = e < (int)n ? sh.ranked[e][0] : 0, w = e < (int)n ? sh.ranked[e][1] : 0;
+    u64 before = 0;
+    uint32_t rank = 0;
+#pragma unroll 2
+    for (uint32_t q = tid & 3; q < n; q += 4)
+        if (sh.ranked[q][0] > own) { before += sh.ranked[q][1]; ++rank; }
+#pragma unroll
+    for (int o = 1; o <= 2; o <<= 1) {
+        const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)before, o), hi = (uint32_t)__shfl_xor((int)(uint32_t)(before >> 32), o);
+        before += (u64)hi << 32 | lo;
+        rank += (uint32_t)__shfl_xor((int)rank, o);
+    }
+    before += base_w;
+    rank += base_c;
+    if (e < (int)n && (by_count ? rank == target : (before <= target && target < before + w))) {
+        sh.picked.before = before; sh.picked.weight = w; sh.picked.index = (int32_t)~(uint32_t)own;
+        sh.picked.score = key_score((uint32_t)(own >> 32));
     }
     __syncthreads();
-    Picked out;
-    if (n > SR_LIST) {                                       // one score, n items
-        const float s = __uint_as_float(prefix & 0x80000000u ? prefix & 0x7fffffffu : ~prefix);
-        u64 w = 1;
-        weigh(s, c, sh.pow2, w);
-        const u64 m = by_count ? target - base_c : (target - base_w) / w;
-        out.index = nth_of_key<TYPE>(row.view, prefix, m, sh);
-        out.before = base_w + m * w;
-        out.weight = w;
-        __syncthreads();
-        return out;
-    }
-    if (tid == 0) sh.n_list = 0;
-    __syncthreads();
-    row.each([&](const float s, const int32_t i) {
-        if (bucket_of(s, c) != b) return;
-        const uint32_t key = rank_key(s);
-        if (shift < 32 && (key >> shift) != prefix) return;
-        u64 w;
-        if (!weigh(s, c, sh.pow2, w)) return;
-        const uint32_t at = atomicAdd(&sh.n_list, 1u);
-        if (at < SR_LIST) {
-            sh.list[at][0] = (u64)key << 32 | (uint32_t)~(uint32_t)i;
-            sh.list[at][1] = w;
-        }
-    });
-    __syncthreads();
-    if (tid < (int)n) {
-        const u64 mine = sh.list[tid][0], w = sh.list[tid][1];
-        u64 before = base_w;
-        uint32_t rank = base_c;
-        for (uint32_t q = 0; q < n; ++q)
-            if (sh.list[q][0] > mine) { before += sh.list[q][1]; ++rank; }
-        const bool here = by_count ? rank == target : (before <= target && target < before + w);
-        if (here) { sh.picked.before = before; sh.picked.weight = w; sh.picked.index = (int32_t)~(uint32_t)mine; }
-    }
-    __syncthreads();
-    out = sh.picked;
+    const Picked out{uniform(sh.picked.before), uniform(sh.picked.weight), uniform(sh.picked.index), uniform(sh.picked.score)};
     __syncthreads();
     return out;
 }
 
-// One workgroup per row.
-template <int TYPE, int NV>
-__global__ __launch_bounds__(SR_THREADS) void sample_rows_kernel(const SampleArgs a) {
-    __shared__ SampleShared sh;
+// Targets of the three steps (find passes a target: the first item whose running sum exceeds it).
+__device__ __forceinline__ u64 top_p_target(const float top_p, const u64 W) {
+    const double want = ceil((double)fmaxf(top_p, 0.f) * (double)W);
+    const u64 need = want < 1.0 ? 1 : want >= (double)W ? W : (u64)want;
+    return need - 1;
+}
+__device__ __forceinline__ double drawn_number(const SampleArgs &a, const int64_t at) {
+    const double u = a.u_f64 ? ((const double *)a.u)[at] : (double)((const float *)a.u)[at];
+    return u > 0.0 ? fmin(u, 1.0) : 0.0;                      // NaN: 0
+}
+__device__ __forceinline__ u64 draw_target(const double u, const u64 W) {
+    const double t = u * (double)W;
+    const u64 target = t >= (double)W ? W - 1 : (u64)t;
+    return target < W ? target : W - 1;
+}
+
+// First bucket whose running sum exceeds the target (the last one if none does).
+template <class G>
+__device__ __forceinline__ int bucket_passing(const u64 *sums, const u64 target) {
+    int lo = 0, hi = G::BUCKETS - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi) >> 1;
+        if (sums[mid] > target) hi = mid;
+        else lo = mid + 1;
+    }
+    return lo;
+}
+// The same for two targets, all threads together (every thread looks at its own buckets): a fifth of the search's time.
+template <class G, class V>
+__device__ __forceinline__ void buckets_passing(const V *sums, const u64 t0, const u64 t1, SampleShared<G> &sh, int &b0, int &b1) {
+    if (threadIdx.x == 0) { sh.k_lo = G::BUCKETS - 1; sh.k_hi = G::BUCKETS - 1; }
+    __syncthreads();
+    u64 before = threadIdx.x ? (u64)sums[G::OWN * threadIdx.x - 1] : 0;
+#pragma unroll
+    for (int q = 0; q < G::OWN; ++q) {
+        const int b = G::OWN * threadIdx.x + q;
+        const u64 last = (u64)sums[b];
+        if (before <= t0 && t0 < last) sh.k_lo = b;
+        if (before <= t1 && t1 < last) sh.k_hi = b;
+        before = last;
+    }
+    __syncthreads();
+    b0 = uniform((int32_t)sh.k_lo); b1 = uniform((int32_t)sh.k_hi);
+    __syncthreads();
+}
+// The buckets the answers can lie in, as bits: top-k's is known; what it leaves of the weight, and so top-p's target, is
+// known to within that bucket, and so on.
+template <class G>
+__device__ void wanted_buckets(const SampleArgs &a, const int64_t r, const RowParams &p, SampleShared<G> &sh,
+                                   uint32_t (&want)[G::BUCKETS / 32 + 1]) {
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    // ranges of buckets, +1 where one begins and -1 behind its end: the running sum is the number of ranges over a bucket
+    uint32_t *edge = sh.csub;
+#pragma unroll
+    for (int q = 0; q < G::OWN; ++q) edge[G::OWN * tid + q] = 0;
+    if (tid <= G::BUCKETS / 32) want[tid] = 0;              // one word more: "no bucket" is not wanted either
+    __syncthreads();
+    auto mark = [&](const int b0, const int b1) {
+        atomicAdd(&edge[b0], 1u);
+        if (b1 + 1 < G::BUCKETS) atomicAdd(&edge[b1 + 1], ~0u);
+    };
+    u64 w_lo = sh.wsum[G::BUCKETS - 1], w_hi = w_lo;
+    if (top_k_asked(a, p) && (uint32_t)p.top_k < sh.cnt[G::BUCKETS - 1]) {
+        int b, same;
+        buckets_passing(sh.cnt, (u64)p.top_k - 1, (u64)p.top_k - 1, sh, b, same);
+        if (tid == 0) mark(b, b);
+        w_lo = (b ? sh.wsum[b - 1] : 0) + 1; w_hi = sh.wsum[b];
+    }
+    if (p.top_p < 1.f) {
+        int b0, b1;
+        buckets_passing(sh.wsum, top_p_target(p.top_p, w_lo), top_p_target(p.top_p, w_hi), sh, b0, b1);
+        if (tid == 0) mark(b0, b1);
+        w_lo = (b0 ? sh.wsum[b0 - 1] : 0) + 1; w_hi = sh.wsum[b1];
+    }
+    if (a.n_draws <= 2) {
+        for (int d = 0; d < a.n_draws; ++d) {
+            const double u = drawn_number(a, r * a.n_draws + d);
+            int b0, b1;
+            buckets_passing(sh.wsum, draw_target(u, w_lo), draw_target(u, w_hi), sh, b0, b1);
+            if (tid == 0) mark(b0, b1);
+        }
+    } else for (int d = tid; d < a.n_draws; d += G::THREADS) {
+        const double u = drawn_number(a, r * a.n_draws + d);
+        mark(bucket_passing<G>(sh.wsum, draw_target(u, w_lo)), bucket_passing<G>(sh.wsum, draw_target(u, w_hi)));
+    }
+    __syncthreads();
+    uint32_t own[G::OWN], sum = 0;
+#pragma unroll
+    for (int q = 0; q < G::OWN; ++q) own[q] = sum += edge[G::OWN * tid + q];
+    uint32_t front = wave_scan(sum);
+    if (lane == 63) sh.wave_c[wave] = front;
+    __syncthreads();
+    front += sum_of_first<G>(sh.wave_c, wave) - sum;
+    uint32_t bits = 0;
+#pragma unroll
+    for (int q = 0; q < G::OWN; ++q)
+        if (front + own[q]) bits |= 1u << q;
+    if (bits) atomicOr(&want[G::OWN * tid / 32], bits << (G::OWN * tid & 31));
+    __syncthreads();
+}
+
+// Steps 2 to 4 from the running sums in sh.cnt / sh.wsum.
+template <class G, int TYPE, class Row>
+__device__ void answer(const SampleArgs &a, const int64_t r, Row &row, const RowView<TYPE> &view, const RowScale &c,
+                       const RowParams &p, SampleShared<G> &sh) {
+    u64 W = uniform(sh.wsum[G::BUCKETS - 1]);
+    // one call of find for all steps: it is long, and inlined
+    const bool by_k = top_k_asked(a, p) && (uint32_t)p.top_k < sh.cnt[G::BUCKETS - 1], by_p = p.top_p < 1.f;
+    for (int step = by_k ? -2 : by_p ? -1 : 0; step < a.n_draws; ++step) {
+        if (step == -1 && !by_p) continue;
+        const int64_t at = r * a.n_draws + step;
+        const u64 target = step == -2 ? (u64)p.top_k - 1 : step == -1 ? top_p_target(p.top_p, W) : draw_target(drawn_number(a, at), W);      // uniform
+        const Picked f = find<G>(row, view, c, step == -2, target, top_k_asked(a, p), sh);
+        if (step < 0) W = f.before + f.weight;
+        else if (threadIdx.x == 0) {                         // ln (w / W) = x - ln W
+            const double x = ((double)f.score - c.top) * c.steps * (0.69314718055994530942 / 256.0);
+            a.idx[at] = f.index;
+            a.logp[at] = (float)(x - (log_of(W, sh.pow2, a.q_bits) - 0.69314718055994530942 * a.q_bits));
+        }
+    }
+}
+__device__ void answer_all(const SampleArgs &a, const int64_t r, const int32_t index, const float logp) {
+    for (int d = threadIdx.x; d < a.n_draws; d += blockDim.x) { a.idx[r * a.n_draws + d] = index; a.logp[r * a.n_draws + d] = logp; }
+}
+
+// A row whose largest score is +inf: n items share everything, in column order.
+template <class G, int TYPE>
+__device__ void answer_infinite(const SampleArgs &a, const int64_t r, const RowView<TYPE> &view, const RowParams &p,
+                                SampleShared<G> &sh) {
+    if (threadIdx.x == 0) sh.n_list = 0;
+    __syncthreads();
+    each_again<G>(view, [&](const float s, const int32_t) { if (s == __builtin_inff()) atomicAdd(&sh.n_list, 1u); });
+    __syncthreads();
+    u64 n = sh.n_list;
+    if (p.top_k > 0 && (u64)p.top_k < n) n = (u64)p.top_k;
+    if (p.top_p < 1.f) n = top_p_target(p.top_p, n) + 1;
+    for (int d = 0; d < a.n_draws; ++d) {
+        const int64_t at = r * a.n_draws + d;
+        const int32_t i = nth_of_key<G>(view, rank_key(__builtin_inff()), draw_target(drawn_number(a, at), n), sh);
+        __syncthreads();
+        if (threadIdx.x == 0) { a.idx[at] = i; a.logp[at] = -logf((float)n); }
+    }
+}
+
+__device__ __forceinline__ u64 wave_max64(u64 v) {
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) {
+        const uint32_t lo = (uint32_t)__shfl_xor((int)(uint32_t)v, o), hi = (uint32_t)__shfl_xor((int)(uint32_t)(v >> 32), o);
+        const u64 x = (u64)hi << 32 | lo;
+        v = x > v ? x : v;
+    }
+    return v;
+}
+
+template <int TYPE>
+__device__ void exclude_items(const SampleArgs &a, const int64_t r, const RowView<TYPE> &view) {
+    const int64_t er = a.ex_rows ? a.ex_rows[r] : r;
+    for (int64_t q = a.ex_rowptr[er] + threadIdx.x; q < a.ex_rowptr[er + 1]; q += blockDim.x) {
+        const int32_t i = a.ex_col[q];
+        if (i >= 0 && i < a.M) RowView<TYPE>::put((char *)view.base, i, -__builtin_inff());
+    }
+}
+
+// ----------------------------------------------------------------------------- one workgroup per row
+template <class G, int TYPE>
+__global__ __launch_bounds__(G::THREADS) void sample_rows_kernel(const SampleArgs a) {
+    constexpr int LISTED = 2048;                            // items collected in LDS
+    __shared__ SampleShared<G> sh;
+    __shared__ Found found[LISTED];
+    __shared__ uint32_t want[G::BUCKETS / 32 + 1], n_found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t r = blockIdx.x;
     const RowView<TYPE> view(a.scores, r, a.lds, a.M);
     if (a.ex_rowptr) {
-        const int64_t er = a.ex_rows ? a.ex_rows[r] : r;
-        for (int64_t q = a.ex_rowptr[er] + tid; q < a.ex_rowptr[er + 1]; q += SR_THREADS) {
-            const int32_t i = a.ex_col[q];
-            if (i >= 0 && i < a.M) RowView<TYPE>::put((char *)view.base, i, -__builtin_inff());
+        exclude_items<TYPE>(a, r, view);
+        __syncthreads();
+    }
+    if (tid < 256) sh.pow2[tid] = exp2((double)tid / 256.0 + a.q_bits);
+#pragma unroll
+    for (int q = 0; q < G::OWN; ++q) { sh.cnt[q * G::THREADS + tid] = 0; sh.wsum[q * G::THREADS + tid] = 0; }
+    if (tid == 0) { sh.base_w = ~0ull; n_found = 0; }
+    const RowParams p = row_params(a, r);
+
+    float hi = -__builtin_inff(), low = __builtin_inff();
+    auto see = [&](const float s) {
+        hi = fmaxf(hi, s);
+        low = fminf(low, s > -1e30f ? s : __builtin_inff());
+    };
+    each_chunk<G>(view, 0, view.n_chunks, [&](const row_u32x4 &v, const int32_t) {
+#pragma unroll
+        for (int e = 0; e < RowView<TYPE>::VEC; ++e) see(RowView<TYPE>::value(v, e));
+        return true;
+    });
+    {
+        const int32_t x = view.extra(tid);
+        if (x >= 0) see(view.at(x));
+    }
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) { hi = fmaxf(hi, __shfl_xor(hi, o)); low = fminf(low, __shfl_xor(low, o)); }
+    if (lane == 0) { sh.wave_f[wave] = hi; sh.wave_g[wave] = low; }
+    __syncthreads();
+    hi = sh.wave_f[lane & (G::WAVES - 1)]; low = sh.wave_g[lane & (G::WAVES - 1)];
+#pragma unroll
+    for (int o = G::WAVES / 2; o >= 1; o >>= 1) { hi = fmaxf(hi, __shfl_xor(hi, o)); low = fminf(low, __shfl_xor(low, o)); }
+    __syncthreads();
+
+    if (hi == -__builtin_inff()) {                            // nothing to draw from
+        answer_all(a, r, -1, -__builtin_inff());
+        return;
+    }
+    if (!(p.T > 0.f)) {                                       // the best item: lowest column of the largest score
+        each_again<G>(view, [&](const float s, const int32_t i) { if (s == hi) atomicMin(&sh.base_w, (u64)i); });
+        __syncthreads();
+        answer_all(a, r, (int32_t)sh.base_w, 0.f);
+        return;
+    }
+    if (hi == __builtin_inff()) {
+        answer_infinite<G>(a, r, view, p, sh);
+        return;
+    }
+    const RowScale c = row_scale(hi, low, p, a.q_bits, G::BUCKETS);
+    const bool counted = top_k_asked(a, p);
+    // Items within the cut go to the list, unweighed, until it is full.  A filtered row (min-p, a low temperature) has a few
+    // per cent of them, spread over all waves: weighed where they are found they would cost a whole wave's weighing each.
+    constexpr int VEC = RowView<TYPE>::VEC, STEP = G::THREADS * VEC;
+    auto collect = [&](const row_u32x4 (&v)[4], const int32_t i0, auto wanted) {
+        bool go = true;
+#pragma unroll
+        for (int half = 0; half < (VEC == 4 ? 1 : 2); ++half) {                // 16 elements per lane, one counter step per wave
+            constexpr int CHUNKS = VEC == 4 ? 4 : 2;
+            u64 taken[16];
+            uint32_t total = 0;
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                taken[q] = __ballot(wanted(bucket_of<G::BUCKETS>(RowView<TYPE>::value(v[half * CHUNKS + q / VEC], q % VEC), c)));
+                total += (uint32_t)__popcll(taken[q]);
+            }
+            if (total == 0) continue;                        // uniform, as `total` is
+            uint32_t base = 0;
+            if (__builtin_amdgcn_mbcnt_hi(~0u, __builtin_amdgcn_mbcnt_lo(~0u, 0u)) == (uint32_t)__ffsll(__ballot(1)) - 1)
+                base = atomicAdd(&n_found, total);           // the first active lane, for the wave
+            base = uniform(base);
+            if (base >= (uint32_t)LISTED) return false;
+#pragma unroll
+            for (int q = 0; q < 16; ++q) {
+                const uint32_t at = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(taken[q] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)taken[q], 0u));
+                if ((taken[q] >> lane & 1) && at < (uint32_t)LISTED)
+                    found[at] = Found{RowView<TYPE>::value(v[half * CHUNKS + q / VEC], q % VEC), i0 + (half * CHUNKS + q / VEC) * STEP + q % VEC};
+                base += (uint32_t)__popcll(taken[q]);
+            }
+            go = go && base <= (uint32_t)LISTED;
+        }
+        return go;
+    };
+    auto collect_extra = [&](auto wanted) {
+        const int32_t x = view.extra(tid);
+        if (x < 0) return;
+        const float s = view.at(x);
+        if (!wanted(bucket_of<G::BUCKETS>(s, c))) return;
+        const uint32_t at = atomicAdd(&n_found, 1u);
+        if (at < (uint32_t)LISTED) found[at] = Found{s, x};
+    };
+    auto any_bucket = [](const uint32_t b) { return b < G::BUCKETS; };
+    each_quad<G>(view, 0, view.n_chunks, [&](const row_u32x4 (&v)[4], const int32_t i0) { return collect(v, i0, any_bucket); });
+    collect_extra(any_bucket);
+    __syncthreads();
+    if (n_found <= (uint32_t)LISTED) {
+        const uint32_t n = n_found;
+#pragma unroll 1
+        for (uint32_t q = tid; q < n; q += G::THREADS) {
+            const float s = found[q].score;
+            const uint32_t b = bucket_of<G::BUCKETS>(s, c);
+            u64 w;
+            if (weigh(s, c, sh.pow2, w)) {
+                atomicAdd(&sh.wsum[b], w);
+                if (counted) atomicAdd(&sh.cnt[b], 1u);
+            }
         }
         __syncthreads();
+        scan_buckets(sh.cnt, sh.wsum, sh);
+    } else {
+        // a row of which much counts: weighed as it is read; one more pass collects whatever the answers can be
+        each_bucket<G>(view, 0, view.n_chunks, true, c, [&](const float (&s)[4], const int32_t, const uint32_t (&b)[4]) {
+            count_four<G::BUCKETS>(s, b, c, sh.pow2, sh.cnt, sh.wsum, counted);
+            return true;
+        });
+        __syncthreads();
+        scan_buckets(sh.cnt, sh.wsum, sh);
+        wanted_buckets(a, r, p, sh, want);
+        if (tid == 0) n_found = 0;
+        __syncthreads();
+        auto in_wanted = [&](const uint32_t b) { return (want[b >> 5] >> (b & 31) & 1u) != 0; };
+        each_quad<G>(view, 0, view.n_chunks, [&](const row_u32x4 (&v)[4], const int32_t i0) { return collect(v, i0, in_wanted); });
+        collect_extra(in_wanted);
+        __syncthreads();
     }
-    if (tid < 256) sh.pow2[tid] = exp2((double)tid / 256.0);
-    sh.cnt[2 * tid] = sh.cnt[2 * tid + 1] = 0;
-    sh.wsum[2 * tid] = sh.wsum[2 * tid + 1] = 0;
-    const RowStore<TYPE, NV> row(view);
+    const bool whole = n_found > (uint32_t)LISTED;           // more than the list holds: the answers come from memory
+    ListedRow<G, TYPE> list{view, found, n_found, whole};
+    answer<G>(a, r, list, view, c, p, sh);
+}
 
-    // the largest score, and the smallest that is no mask value (it only sets the buckets' width)
-    float hi = -__builtin_inff(), lo = __builtin_inff();
-    row.each([&](const float s, const int32_t) {
-        hi = fmaxf(hi, s);
-        lo = s > -1e30f ? fminf(lo, s) : lo;
-    });
+// ----------------------------------------------------------------------------- cut rows
+typedef Large G;
+template <int TYPE>
+__global__ __launch_bounds__(256) void exclude_kernel(const SampleArgs a) {
+    const RowView<TYPE> view(a.scores, blockIdx.x, a.lds, a.M);
+    exclude_items<TYPE>(a, blockIdx.x, view);
+}
+
+// 1. Every part's best item and smallest scores; clears the row's histogram and list.
+template <int TYPE>
+__global__ __launch_bounds__(G::THREADS) void part_stats_kernel(const SampleArgs a) {
+    __shared__ u64 best_[G::WAVES];
+    __shared__ float low_[G::WAVES];
+    const int64_t r = blockIdx.x / a.n_parts;
+    const int part = blockIdx.x % a.n_parts, tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    for (int b = part * G::THREADS + tid; b < G::BUCKETS; b += a.n_parts * G::THREADS) { a.cnt[r * G::BUCKETS + b] = 0; a.wsum[r * G::BUCKETS + b] = 0; }
+    if (part == 0 && tid == 0) a.n_found[r] = 0;
+    const RowView<TYPE> view(a.scores, r, a.lds, a.M);
+    const int32_t q0 = part * a.per_part, q1 = min(q0 + a.per_part, view.n_chunks);
+    float hi = -__builtin_inff(), low = __builtin_inff();
+    int32_t at = 0x7fffffff;
+    auto see = [&](const float s, const int32_t i) {
+        if (s > hi || (s == hi && i < at)) { hi = s; at = i; }
+        low = fminf(low, s > -1e30f ? s : __builtin_inff());
+    };
+    each_chunk<G>(view, q0, q1, [&](const row_u32x4 &v, const int32_t i0) {
 #pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) { hi = fmaxf(hi, __shfl_xor(hi, o)); lo = fminf(lo, __shfl_xor(lo, o)); }
-    if (lane == 0) { sh.wave_f[wave] = hi; sh.wave_g[wave] = lo; }
-    __syncthreads();
-    for (int v = 0; v < SR_WAVES; ++v) { hi = fmaxf(hi, sh.wave_f[v]); lo = fminf(lo, sh.wave_g[v]); }
-
-    const float T = a.o.temperature_rows ? a.o.temperature_rows[r] : a.o.temperature;
-    const int32_t top_k = a.o.top_k_rows ? a.o.top_k_rows[r] : a.o.top_k;
-    const float top_p = a.o.top_p_rows ? a.o.top_p_rows[r] : a.o.top_p;
-    const float min_p = a.o.min_p_rows ? a.o.min_p_rows[r] : a.o.min_p;
-    int32_t *idx = a.idx + r * a.n_draws;
-    float *logp = a.logp + r * a.n_draws;
-    if (hi == -__builtin_inff()) {                            // nothing to draw from
-        for (int d = tid; d < a.n_draws; d += SR_THREADS) { idx[d] = -1; logp[d] = -__builtin_inff(); }
-        return;
-    }
-    if (!(T > 0.f)) {                                         // the best item: lowest column of the largest score
-        if (tid == 0) sh.base_w = ~0ull;
-        __syncthreads();
-        row.each([&](const float s, const int32_t i) { if (s == hi) atomicMin(&sh.base_w, (u64)i); });
-        __syncthreads();
-        for (int d = tid; d < a.n_draws; d += SR_THREADS) { idx[d] = (int32_t)sh.base_w; logp[d] = 0.f; }
-        return;
-    }
-    RowScale c;
-    c.top = hi;
-    c.inv_t = 1.0 / (double)T;
-    c.q_bits = a.q_bits;
-    c.min_p = min_p > 0.f ? fminf(min_p, 1.f) : 0.f;
-    c.cut = 0.6931471805599453 * (a.q_bits + 1);              // beyond it a weight rounds to 0
-    {
-        // buckets span the scores that can matter: down to the lowest, the cut, or min-p's threshold
-        double span = c.cut;
-        if (c.min_p > 0.f) span = fmin(span, -log((double)c.min_p) + 1e-6);
-        const float width = fminf((float)fmin(span * (double)T, 3e38), hi - lo);
-        c.per_score = (float)SR_BUCKETS / fmaxf(width, 1e-30f);
-    }
-    row.each([&](const float s, const int32_t) {
-        u64 w;
-        if (!weigh(s, c, sh.pow2, w)) return;
-        const uint32_t b = bucket_of(s, c);
-        atomicAdd(&sh.cnt[b], 1u);
-        atomicAdd(&sh.wsum[b], w);
+        for (int e = 0; e < RowView<TYPE>::VEC; ++e) see(RowView<TYPE>::value(v, e), i0 + e);
+        return true;
     });
+    {
+        const int32_t x = part == 0 ? view.extra(tid) : -1;
+        if (x >= 0) see(view.at(x), x);
+    }
+    u64 best = wave_max64((u64)rank_key(hi) << 32 | (uint32_t)~(uint32_t)at);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) low = fminf(low, __shfl_xor(low, o));
+    if (lane == 0) { best_[wave] = best; low_[wave] = low; }
+    __syncthreads();
+    if (tid == 0) {
+        for (int v = 1; v < G::WAVES; ++v) {
+            best = best_[v] > best ? best_[v] : best; low = fminf(low, low_[v]);
+        }
+        a.stats[blockIdx.x] = PartStat{best, low, 0.f};
+    }
+}
+// The row's, from its parts'.  Every wave computes it.
+__device__ __forceinline__ PartStat join_stats(const SampleArgs &a, const int64_t r) {
+    PartStat s{0, __builtin_inff(), 0.f};
+    for (int q = threadIdx.x & 63; q < a.n_parts; q += 64) {
+        const PartStat x = a.stats[r * a.n_parts + q];
+        s.best = x.best > s.best ? x.best : s.best;
+        s.low = fminf(s.low, x.low);
+    }
+    s.best = wave_max64(s.best);
+#pragma unroll
+    for (int o = 32; o >= 1; o >>= 1) s.low = fminf(s.low, __shfl_xor(s.low, o));
+    return s;
+}
+
+// 2. Every part's histogram, added to the row's by integer atomics.
+template <int TYPE>
+__global__ __launch_bounds__(G::THREADS) void part_histogram_kernel(const SampleArgs a) {
+    __shared__ u64 wsum[G::BUCKETS];
+    __shared__ uint32_t cnt[G::BUCKETS];
+    __shared__ double pow2[256];
+    const int64_t r = blockIdx.x / a.n_parts;
+    const int part = blockIdx.x % a.n_parts, tid = threadIdx.x;
+    const RowParams p = row_params(a, r);
+    const PartStat st = join_stats(a, r);
+    const float hi = key_score((uint32_t)(st.best >> 32));
+    if (!(fabsf(hi) < __builtin_inff()) || !(p.T > 0.f)) return;      // answered apart
+    if (tid < 256) pow2[tid] = exp2((double)tid / 256.0 + a.q_bits);
+    for (int b = tid; b < G::BUCKETS; b += G::THREADS) { cnt[b] = 0; wsum[b] = 0; }
+    const RowScale c = row_scale(hi, st.low, p, a.q_bits, G::BUCKETS);
+    __syncthreads();
+    const RowView<TYPE> view(a.scores, r, a.lds, a.M);
+    const int32_t q0 = part * a.per_part, q1 = min(q0 + a.per_part, view.n_chunks);
+    each_bucket<G>(view, q0, q1, part == 0, c, [&](const float (&s)[4], const int32_t, const uint32_t (&b)[4]) {
+        count_four<G::BUCKETS>(s, b, c, pow2, cnt, wsum, top_k_asked(a, p));
+        return true;
+    });
+    __syncthreads();
+    for (int b = tid; b < G::BUCKETS; b += G::THREADS)
+        if (wsum[b]) { atomicAdd(&a.cnt[r * G::BUCKETS + b], cnt[b]); atomicAdd(&a.wsum[r * G::BUCKETS + b], wsum[b]); }
+}
+
+// Loads the row's histogram and turns it into running sums.
+__device__ __forceinline__ void load_histogram(const SampleArgs &a, const int64_t r, SampleShared<G> &sh) {
+    const int tid = threadIdx.x;
+#pragma unroll
+    for (int h = 0; h < G::OWN; ++h) {
+        const int b = tid + h * G::THREADS;
+        sh.cnt[b] = a.cnt[r * G::BUCKETS + b];
+        sh.wsum[b] = a.wsum[r * G::BUCKETS + b];
+    }
     __syncthreads();
     scan_buckets(sh.cnt, sh.wsum, sh);
-    const uint32_t n = sh.cnt[SR_BUCKETS - 1];
-    u64 W = sh.wsum[SR_BUCKETS - 1];
-    if (top_k > 0 && (uint32_t)top_k < n) {
-        const Picked p = find<TYPE, NV>(row, c, true, (u64)top_k - 1, sh);
-        W = p.before + p.weight;
+}
+// 3. The items of those buckets.
+template <int TYPE>
+__global__ __launch_bounds__(G::THREADS) void part_collect_kernel(const SampleArgs a) {
+    __shared__ SampleShared<G> sh;
+    __shared__ uint32_t want[G::BUCKETS / 32 + 1];
+    const int64_t r = blockIdx.x / a.n_parts;
+    const int part = blockIdx.x % a.n_parts;
+    const RowParams p = row_params(a, r);
+    const PartStat st = join_stats(a, r);
+    const float hi = key_score((uint32_t)(st.best >> 32));
+    if (!(fabsf(hi) < __builtin_inff()) || !(p.T > 0.f)) return;      // answered apart
+    const RowScale c = row_scale(hi, st.low, p, a.q_bits, G::BUCKETS);
+    load_histogram(a, r, sh);
+    wanted_buckets(a, r, p, sh, want);
+    const RowView<TYPE> view(a.scores, r, a.lds, a.M);
+    const int32_t q0 = part * a.per_part, q1 = min(q0 + a.per_part, view.n_chunks);
+    each_bucket<G>(view, q0, q1, part == 0, c, [&](const float (&s)[4], const int32_t i, const uint32_t (&b)[4]) {
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            if (!(want[b[q] >> 5] >> (b[q] & 31) & 1u)) continue;
+            const uint32_t at = atomicAdd(&a.n_found[r], 1u);
+            if (at < SR_LISTED) a.found[r * SR_LISTED + at] = Found{s[q], i + q};
+        }
+        return true;
+    });
+}
+
+// 4. The answers.
+template <int TYPE>
+__global__ __launch_bounds__(G::THREADS) void part_answer_kernel(const SampleArgs a) {
+    __shared__ SampleShared<G> sh;
+    const int64_t r = blockIdx.x;
+    const RowParams p = row_params(a, r);
+    const PartStat st = join_stats(a, r);
+    const float hi = key_score((uint32_t)(st.best >> 32));
+    if (hi == -__builtin_inff()) {
+        answer_all(a, r, -1, -__builtin_inff());
+        return;
     }
-    if (top_p < 1.f) {
-        const double want = ceil((double)fmaxf(top_p, 0.f) * (double)W);
-        const u64 need = want < 1.0 ? 1 : (u64)want;
-        const Picked p = find<TYPE, NV>(row, c, false, (need < W ? need : W) - 1, sh);
-        W = p.before + p.weight;
+    if (!(p.T > 0.f)) {
+        answer_all(a, r, (int32_t)~(uint32_t)st.best, 0.f);
+        return;
     }
-    for (int d = 0; d < a.n_draws; ++d) {
-        const int64_t at = r * a.n_draws + d;
-        const double u = a.u_f64 ? ((const double *)a.u)[at] : (double)((const float *)a.u)[at];
-        const double t = u > 0.0 ? fmin(u, 1.0) * (double)W : 0.0;
-        const u64 target = t >= (double)W ? W - 1 : (u64)t;
-        const Picked p = find<TYPE, NV>(row, c, false, target < W ? target : W - 1, sh);
-        if (tid == 0) { idx[d] = p.index; logp[d] = (float)log((double)p.weight / (double)W); }
+    const RowView<TYPE> view(a.scores, r, a.lds, a.M);
+    if (hi == __builtin_inff()) {
+        answer_infinite<G>(a, r, view, p, sh);
+        return;
     }
+    if (threadIdx.x < 256) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x / 256.0 + a.q_bits);
+    const RowScale c = row_scale(hi, st.low, p, a.q_bits, G::BUCKETS);
+    load_histogram(a, r, sh);
+    const uint32_t n = a.n_found[r];
+    ListedRow<G, TYPE> row{view, a.found + r * SR_LISTED, n, n > SR_LISTED};       // more than the list holds: from memory
+    answer<G>(a, r, row, view, c, p, sh);
+}
+
+// ----------------------------------------------------------------------------- host
+constexpr int64_t SMALL_CHUNKS = 4096, CUT_CHUNKS = 16384, CUT_ROWS = 512;
+struct CutPlan {
+    int32_t n_parts, per_part;        // n_parts == 0: one workgroup per row
+    size_t off_wsum, off_cnt, off_nfound, off_found, total;
+};
+CutPlan cut_plan(const int32_t dtype, const int64_t n, const int64_t M) {
+    CutPlan p{0, 0, 0, 0, 0, 0, 16};
+    const int64_t chunks = M / (dtype == ALS_DTYPE_F32 ? 4 : 8);
+    if (chunks <= CUT_CHUNKS || n >= CUT_ROWS) return p;
+    // about 512 workgroups, of two chunks per thread or more each
+    const int64_t want = std::max<int64_t>((512 + n - 1) / n, 4);
+    p.n_parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 128), chunks / (4 * G::THREADS)));
+    p.per_part = (int32_t)((chunks + p.n_parts - 1) / p.n_parts + 1);        // + 1: the row's alignment may add none, but cover all
+    size_t at = 0;
+    auto take = [&](const size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
+    take((size_t)n * p.n_parts * sizeof(PartStat));
+    p.off_wsum = take((size_t)n * CUT_BUCKETS * 8);
+    p.off_cnt = take((size_t)n * CUT_BUCKETS * 4);
+    p.off_nfound = take((size_t)n * 4);
+    p.off_found = take((size_t)n * SR_LISTED * sizeof(Found));
+    p.total = at;
+    return p;
+}
+
+template <int TYPE>
+void launch(const SampleArgs &a, const int64_t n, hipStream_t st) {
+    const dim3 rows((unsigned)n), block(G::THREADS);
+    if (a.n_parts == 0) {
+        const int64_t chunks = a.M / RowView<TYPE>::VEC;
+        if (chunks <= SMALL_CHUNKS) hipLaunchKernelGGL((sample_rows_kernel<Small, TYPE>), rows, dim3(Small::THREADS), 0, st, a);
+        else hipLaunchKernelGGL((sample_rows_kernel<Large, TYPE>), rows, block, 0, st, a);
+        return;
+    }
+    const dim3 parts((unsigned)(n * a.n_parts));
+    if (a.ex_rowptr) hipLaunchKernelGGL((exclude_kernel<TYPE>), rows, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((part_stats_kernel<TYPE>), parts, block, 0, st, a);
+    hipLaunchKernelGGL((part_histogram_kernel<TYPE>), parts, block, 0, st, a);
+    hipLaunchKernelGGL((part_collect_kernel<TYPE>), parts, block, 0, st, a);
+    hipLaunchKernelGGL((part_answer_kernel<TYPE>), rows, block, 0, st, a);
 }
 
 }  // namespace
 
 extern "C" {
 
+size_t als_sample_rows_workspace_bytes(int32_t dtype, int64_t n_rows, int64_t M) {
+    if (dtype < ALS_DTYPE_F32 || dtype > ALS_DTYPE_BF16 || n_rows < 1 || M < 1 || M > INT32_MAX) return 0;
+    return cut_plan(dtype, n_rows, M).total;
+}
+
 int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows, int64_t M, const int64_t *ex_rowptr,
                         const int32_t *ex_col, const int64_t *ex_row_ids, const als_sample_opts_t *opts, const void *u,
-                        int32_t u_is_f64, int32_t n_draws, int32_t *idx_out, float *logp_out, void *stream) {
-    if (!scores || !opts || !u || !idx_out || !logp_out) return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: null pointer");
+                        int32_t u_is_f64, int32_t n_draws, int32_t *idx_out, float *logp_out, void *workspace, size_t ws_bytes,
+                        void *stream) {
+    if (!scores || !opts || !u || !idx_out || !logp_out || !workspace)
+        return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: null pointer");
     if (n_rows < 1 || M < 1 || lds < M || M > INT32_MAX || n_draws < 1)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: bad sizes (n_rows=%lld M=%lld lds=%lld n_draws=%d)", (long long)n_rows,
                          (long long)M, (long long)lds, n_draws);
-    if (n_rows > INT32_MAX) return als_fail_(ALS_ERR_UNSUPPORTED, "als_sample_rows: more than 2^31 - 1 rows per call");
     if (dtype < ALS_DTYPE_F32 || dtype > ALS_DTYPE_BF16)
         return als_fail_(ALS_ERR_UNSUPPORTED, "als_sample_rows: dtype %d (0 float32, 1 float16, 2 bfloat16)", dtype);
     if ((uintptr_t)scores % (dtype == ALS_DTYPE_F32 ? 4 : 2))
         return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: scores are not aligned to their type");
     if ((ex_rowptr == nullptr) != (ex_col == nullptr))
         return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: pass both exclusion arrays or neither");
+    const CutPlan plan = cut_plan(dtype, n_rows, M);
+    if (n_rows * std::max<int64_t>(plan.n_parts, 1) > INT32_MAX)
+        return als_fail_(ALS_ERR_UNSUPPORTED, "als_sample_rows: too many rows for one launch");
+    if (ws_bytes < plan.total || (uintptr_t)workspace % 16)
+        return als_fail_(ALS_ERR_WORKSPACE, "als_sample_rows: workspace too small or not 16-byte aligned: %zu < %zu", ws_bytes, plan.total);
     SampleArgs a;
     a.scores = scores; a.lds = lds; a.M = M;
     a.ex_rowptr = ex_rowptr; a.ex_col = ex_col; a.ex_rows = ex_rowptr ? ex_row_ids : nullptr;
@@ -433,13 +1044,14 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
     while ((1LL << bits) < M) ++bits;
     a.q_bits = std::min(51, 62 - bits);
     a.idx = idx_out; a.logp = logp_out;
-    const dim3 grid((unsigned)n_rows), block(SR_THREADS);
+    char *ws = (char *)workspace;
+    a.n_parts = plan.n_parts; a.per_part = plan.per_part;
+    a.stats = (PartStat *)ws; a.wsum = (u64 *)(ws + plan.off_wsum); a.cnt = (uint32_t *)(ws + plan.off_cnt);
+    a.n_found = (uint32_t *)(ws + plan.off_nfound); a.found = (Found *)(ws + plan.off_found);
     hipStream_t st = (hipStream_t)stream;
-    switch (dtype) {
-        case ALS_DTYPE_F32: hipLaunchKernelGGL((sample_rows_kernel<ROW_F32, 0>), grid, block, 0, st, a); break;
-        case ALS_DTYPE_F16: hipLaunchKernelGGL((sample_rows_kernel<ROW_F16, 0>), grid, block, 0, st, a); break;
-        default: hipLaunchKernelGGL((sample_rows_kernel<ROW_BF16, 0>), grid, block, 0, st, a); break;
-    }
+    if (dtype == ALS_DTYPE_F32) launch<ROW_F32>(a, n_rows, st);
+    else if (dtype == ALS_DTYPE_F16) launch<ROW_F16>(a, n_rows, st);
+    else launch<ROW_BF16>(a, n_rows, st);
     ALS_HIP_CHECK4(hipGetLastError());
     return ALS_OK;
 }

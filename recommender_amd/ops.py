@@ -674,11 +674,12 @@ def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, e
     logp = torch.empty(u.shape, dtype=torch.float32, device=score_rows.device)
     if n == 0:
         return idx, logp
+    ws = torch.empty(lib.als_sample_rows_workspace_bytes(dtype, n, M), dtype=torch.uint8, device=score_rows.device)
     opts = _lib.SampleOpts(t, k, p, m, *(x.data_ptr() if x is not None else None for x in (t_rows, k_rows, p_rows, m_rows)))
     with torch.cuda.device(score_rows.device):
         check(lib.als_sample_rows(_ptr(score_rows), dtype, ld, n, M, _ptr(ex_ptr), _ptr(ex_col), _ptr(exclude_rows),
                                   ctypes.byref(opts), _ptr(u), int(u.dtype == torch.float64), u.numel() // n, _ptr(idx),
-                                  _ptr(logp), _stream()), "als_sample_rows")
+                                  _ptr(logp), _ptr(ws), ws.numel(), _stream()), "als_sample_rows")
     return idx, logp
 
 
