@@ -18,7 +18,7 @@
 // k + r, 2^(k mod 256 / 256) from a table, a polynomial of degree 4 in r; error below 1e-15.
 //
 // Two forms.  sample_rows_kernel: one workgroup per row, one launch; the row is read from memory for its maximum and
-// then, mostly from the caches, once more (filtered rows) or twice more (rows of which much counts).  Few long rows are
+// for the items that can matter, in one pass if they are few (filtered rows), and otherwise, mostly from the caches, twice more.  Few long rows are
 // cut into parts, one workgroup each, in four launches: maximum; histogram; items of the buckets the answers can lie in,
 // collected in a list; the answers from the list.
 #include <hip/hip_runtime.h>
@@ -148,17 +148,26 @@ struct RowScale {
     float top_f, per_score;    // buckets per unit of score
     float reject;       // scores this many buckets or more below the top are beyond the cut
 };
-// low: the smallest score that is no mask value (+inf if there is none).  It only sets the buckets' width.
-__device__ __forceinline__ RowScale row_scale(const float top, const float low, const RowParams &p, const int q_bits, const int buckets) {
+// How far below the largest x an item can be and count: beyond it a weight rounds to 0, or is below min_p.
+__device__ __forceinline__ double item_cut(const RowParams &p, const int q_bits) {
+    const double cut = 0.6931471805599453 * (q_bits + 1);
+    return p.min_p > 0.f ? fmin(cut, -log((double)p.min_p) + 1e-6) : cut;
+}
+// The same in scores; +inf where that exceeds what scores can differ by.
+__device__ __forceinline__ float score_reach(const double cut, const float T) {
+    const double reach = cut * (double)T;
+    return reach < 1e38 ? (float)reach : __builtin_inff();
+}
+// low: a low score of the row that is no mask value (+inf if there is none).  It only sets the buckets' width.
+__device__ __forceinline__ RowScale row_scale(const float top, const float low, const double cut, const RowParams &p, const int q_bits,
+                                              const int buckets) {
     RowScale c;
-    double cut = 0.6931471805599453 * (q_bits + 1);           // beyond it a weight rounds to 0
-    if (p.min_p > 0.f) cut = fmin(cut, -log((double)p.min_p) + 1e-6);
     c.top = (double)top;
     c.steps = 256.0 * 1.4426950408889634074 / (double)p.T;
     c.cut = cut * (256.0 * 1.4426950408889634074);
     c.min_w = ldexp((double)p.min_p, q_bits);
-    const float reach = (float)fmin(cut * (double)p.T, 3e38);
-    const float width = fmaxf(low <= top ? fminf(reach, top - low) : reach, 1e-30f);
+    const float reach = score_reach(cut, p.T);
+    const float width = fminf(fmaxf(low <= top ? fminf(reach, top - low) : reach, 1e-30f), 3e38f);
     c.top_f = uniform(top);
     c.per_score = uniform((float)buckets / width);
     c.reject = uniform((float)buckets * fmaxf(1.f, reach / width) * 1.01f);
@@ -673,7 +682,7 @@ __device__ void exclude_items(const SampleArgs &a, const int64_t r, const RowVie
 
 // ----------------------------------------------------------------------------- one workgroup per row
 template <class G, int TYPE>
-__global__ __launch_bounds__(G::THREADS) void sample_rows_kernel(const SampleArgs a) {
+__global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const SampleArgs a) {
     constexpr int LISTED = 2048;                            // items collected in LDS
     __shared__ SampleShared<G> sh;
     __shared__ Found found[LISTED];
@@ -691,47 +700,10 @@ __global__ __launch_bounds__(G::THREADS) void sample_rows_kernel(const SampleArg
     if (tid == 0) { sh.base_w = ~0ull; n_found = 0; }
     const RowParams p = row_params(a, r);
 
-    float hi = -__builtin_inff(), low = __builtin_inff();
-    auto see = [&](const float s) {
-        hi = fmaxf(hi, s);
-        low = fminf(low, s > -1e30f ? s : __builtin_inff());
-    };
-    each_chunk<G>(view, 0, view.n_chunks, [&](const row_u32x4 &v, const int32_t) {
-#pragma unroll
-        for (int e = 0; e < RowView<TYPE>::VEC; ++e) see(RowView<TYPE>::value(v, e));
-        return true;
-    });
-    {
-        const int32_t x = view.extra(tid);
-        if (x >= 0) see(view.at(x));
-    }
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) { hi = fmaxf(hi, __shfl_xor(hi, o)); low = fminf(low, __shfl_xor(low, o)); }
-    if (lane == 0) { sh.wave_f[wave] = hi; sh.wave_g[wave] = low; }
-    __syncthreads();
-    hi = sh.wave_f[lane & (G::WAVES - 1)]; low = sh.wave_g[lane & (G::WAVES - 1)];
-#pragma unroll
-    for (int o = G::WAVES / 2; o >= 1; o >>= 1) { hi = fmaxf(hi, __shfl_xor(hi, o)); low = fminf(low, __shfl_xor(low, o)); }
-    __syncthreads();
-
-    if (hi == -__builtin_inff()) {                            // nothing to draw from
-        answer_all(a, r, -1, -__builtin_inff());
-        return;
-    }
-    if (!(p.T > 0.f)) {                                       // the best item: lowest column of the largest score
-        each_again<G>(view, [&](const float s, const int32_t i) { if (s == hi) atomicMin(&sh.base_w, (u64)i); });
-        __syncthreads();
-        answer_all(a, r, (int32_t)sh.base_w, 0.f);
-        return;
-    }
-    if (hi == __builtin_inff()) {
-        answer_infinite<G>(a, r, view, p, sh);
-        return;
-    }
-    const RowScale c = row_scale(hi, low, p, a.q_bits, G::BUCKETS);
-    const bool counted = top_k_asked(a, p);
-    // Items within the cut go to the list, unweighed, until it is full.  A filtered row (min-p, a low temperature) has a few
-    // per cent of them, spread over all waves: weighed where they are found they would cost a whole wave's weighing each.
+    // One pass over the row finds its maximum and, on the way, collects the items that can matter, unweighed: those within
+    // the cut below the maximum so far, and at or above a score that some more than top_k items are likely to reach.  (A
+    // filtered row has a few per cent of them, spread over all waves: weighed where they are found they would cost a whole
+    // wave's weighing each.)  A row whose items do not fit the list is read again, see below.
     constexpr int VEC = RowView<TYPE>::VEC, STEP = G::THREADS * VEC;
     auto collect = [&](const row_u32x4 (&v)[4], const int32_t i0, auto wanted) {
         bool go = true;
@@ -742,7 +714,7 @@ __global__ __launch_bounds__(G::THREADS) void sample_rows_kernel(const SampleArg
             uint32_t total = 0;
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
-                taken[q] = __ballot(wanted(bucket_of<G::BUCKETS>(RowView<TYPE>::value(v[half * CHUNKS + q / VEC], q % VEC), c)));
+                taken[q] = __ballot(wanted(RowView<TYPE>::value(v[half * CHUNKS + q / VEC], q % VEC)));
                 total += (uint32_t)__popcll(taken[q]);
             }
             if (total == 0) continue;                        // uniform, as `total` is
@@ -753,28 +725,124 @@ __global__ __launch_bounds__(G::THREADS) void sample_rows_kernel(const SampleArg
             if (base >= (uint32_t)LISTED) return false;
 #pragma unroll
             for (int q = 0; q < 16; ++q) {
+                if (taken[q] == 0) continue;                 // uniform: most of them in a filtered row
+                const float s = RowView<TYPE>::value(v[half * CHUNKS + q / VEC], q % VEC);
                 const uint32_t at = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(taken[q] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)taken[q], 0u));
-                if ((taken[q] >> lane & 1) && at < (uint32_t)LISTED)
-                    found[at] = Found{RowView<TYPE>::value(v[half * CHUNKS + q / VEC], q % VEC), i0 + (half * CHUNKS + q / VEC) * STEP + q % VEC};
+                if (wanted(s) && at < (uint32_t)LISTED) found[at] = Found{s, i0 + (half * CHUNKS + q / VEC) * STEP + q % VEC};
                 base += (uint32_t)__popcll(taken[q]);
             }
             go = go && base <= (uint32_t)LISTED;
         }
         return go;
     };
-    auto collect_extra = [&](auto wanted) {
-        const int32_t x = view.extra(tid);
-        if (x < 0) return;
-        const float s = view.at(x);
-        if (!wanted(bucket_of<G::BUCKETS>(s, c))) return;
+    auto collect_one = [&](const float s, const int32_t i) {
         const uint32_t at = atomicAdd(&n_found, 1u);
-        if (at < (uint32_t)LISTED) found[at] = Found{s, x};
+        if (at < (uint32_t)LISTED) found[at] = Found{s, i};
     };
-    auto any_bucket = [](const uint32_t b) { return b < G::BUCKETS; };
-    each_quad<G>(view, 0, view.n_chunks, [&](const row_u32x4 (&v)[4], const int32_t i0) { return collect(v, i0, any_bucket); });
-    collect_extra(any_bucket);
-    __syncthreads();
-    if (n_found <= (uint32_t)LISTED) {
+    float hi = -__builtin_inff(), low = __builtin_inff();     // low: of the first chunks, it only sets the buckets' width
+    auto top_of = [&](const row_u32x4 (&v)[4]) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) hi = fmaxf(hi, RowView<TYPE>::value(v[k], e));
+    };
+    auto load_quad = [&](row_u32x4 (&v)[4], const int32_t q) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = RowView<TYPE>::nothing();
+            if (q + k * G::THREADS < view.n_chunks) v[k] = view.load(q + k * G::THREADS);
+        }
+    };
+    // over the workgroup
+    auto join_seen = [&]() {
+#pragma unroll
+        for (int o = 32; o >= 1; o >>= 1) { hi = fmaxf(hi, __shfl_xor(hi, o)); low = fminf(low, __shfl_xor(low, o)); }
+        if (lane == 0) { sh.wave_f[wave] = hi; sh.wave_g[wave] = low; }
+        __syncthreads();
+        hi = sh.wave_f[lane & (G::WAVES - 1)]; low = sh.wave_g[lane & (G::WAVES - 1)];
+#pragma unroll
+        for (int o = G::WAVES / 2; o >= 1; o >>= 1) { hi = fmaxf(hi, __shfl_xor(hi, o)); low = fminf(low, __shfl_xor(low, o)); }
+        __syncthreads();
+    };
+    const double cut = item_cut(p, a.q_bits);
+    const float reach = score_reach(cut, p.T) * 1.0001f;        // items further below the top do not count
+    float at_least = -__builtin_inff();                                        // top-k: a score to start from
+    const bool counted = top_k_asked(a, p), drawn = p.T > 0.f;
+    {
+        row_u32x4 v[4], next[4];
+        load_quad(v, tid);
+        const int32_t x = view.extra(tid);
+        const float x_score = x >= 0 ? view.at(x) : -__builtin_inff();
+        load_quad(next, tid + 4 * G::THREADS);
+        top_of(v);
+        hi = fmaxf(hi, x_score);
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int e = 0; e < VEC; ++e) {
+                const float s = RowView<TYPE>::value(v[k], e);
+                low = fminf(low, s > -1e30f ? s : __builtin_inff());
+            }
+        join_seen();
+        const float seen = fminf(2.f * STEP, (float)a.M), share = seen / (float)a.M, expect = share * (float)p.top_k;
+        const float enough = 1.5f * expect + 4.f * sqrtf(expect) + 8.f;        // of the first two chunks' items
+        if (counted && drawn && fabsf(hi) < __builtin_inff() && enough < 0.8f * share * (float)LISTED && hi > low) {
+            const float per = (float)G::BUCKETS / (hi - low), top = hi;
+            auto count = [&](const float s) {
+                const float t = (top - s) * per;
+                if (t < (float)G::BUCKETS) atomicAdd(&sh.cnt[(int)t], 1u);
+            };
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int e = 0; e < VEC; ++e) count(RowView<TYPE>::value(v[k], e));
+            __syncthreads();
+            scan_buckets(sh.cnt, sh.wsum, sh);
+            int b, same;
+            buckets_passing(sh.cnt, (u64)enough, (u64)enough, sh, b, same);
+            at_least = uniform(hi - (float)(b + 1) / per);
+#pragma unroll
+            for (int q = 0; q < G::OWN; ++q) sh.cnt[q * G::THREADS + tid] = 0;
+            __syncthreads();
+        }
+        bool collecting = drawn && hi < __builtin_inff();
+        float floor = fmaxf(fmaxf(hi - reach, at_least), -3.402823466e38f);    // at the least everything but -inf
+        auto wanted = [&](const float s) { return s >= floor; };
+        if (collecting) {
+            if (wanted(x_score)) collect_one(x_score, x);
+            collecting = __all(collect(v, view.index0(tid), wanted));
+        }
+#pragma unroll 1
+        for (int32_t q = tid + 4 * G::THREADS; q - tid < view.n_chunks; q += 4 * G::THREADS) {
+#pragma unroll
+            for (int k = 0; k < 4; ++k) v[k] = next[k];
+            load_quad(next, q + 4 * G::THREADS);
+            top_of(v);
+            if (collecting) {                                // per wave
+                floor = fmaxf(floor, hi - reach);            // the lane's own maximum: never above the row's
+                collecting = __all(collect(v, view.index0(q), wanted));
+            }
+        }
+        join_seen();
+    }
+
+    if (hi == -__builtin_inff()) {                            // nothing to draw from
+        answer_all(a, r, -1, -__builtin_inff());
+        return;
+    }
+    if (!drawn) {                                             // the best item: lowest column of the largest score
+        each_again<G>(view, [&](const float s, const int32_t i) { if (s == hi) atomicMin(&sh.base_w, (u64)i); });
+        __syncthreads();
+        answer_all(a, r, (int32_t)sh.base_w, 0.f);
+        return;
+    }
+    if (hi == __builtin_inff()) {
+        answer_infinite<G>(a, r, view, p, sh);
+        return;
+    }
+    const RowScale c = row_scale(hi, low, cut, p, a.q_bits, G::BUCKETS);
+    bool fits = n_found <= (uint32_t)LISTED;
+    if (fits) {
         const uint32_t n = n_found;
 #pragma unroll 1
         for (uint32_t q = tid; q < n; q += G::THREADS) {
@@ -788,7 +856,16 @@ __global__ __launch_bounds__(G::THREADS) void sample_rows_kernel(const SampleArg
         }
         __syncthreads();
         scan_buckets(sh.cnt, sh.wsum, sh);
-    } else {
+        // started from a score that fewer than top_k reach, although items below it count
+        if (counted && at_least > hi - reach && sh.cnt[G::BUCKETS - 1] < (uint32_t)p.top_k) {
+            fits = false;
+            __syncthreads();
+#pragma unroll
+            for (int q = 0; q < G::OWN; ++q) { sh.cnt[q * G::THREADS + tid] = 0; sh.wsum[q * G::THREADS + tid] = 0; }
+            __syncthreads();
+        }
+    }
+    if (!fits) {
         // a row of which much counts: weighed as it is read; one more pass collects whatever the answers can be
         each_bucket<G>(view, 0, view.n_chunks, true, c, [&](const float (&s)[4], const int32_t, const uint32_t (&b)[4]) {
             count_four<G::BUCKETS>(s, b, c, sh.pow2, sh.cnt, sh.wsum, counted);
@@ -799,9 +876,13 @@ __global__ __launch_bounds__(G::THREADS) void sample_rows_kernel(const SampleArg
         wanted_buckets(a, r, p, sh, want);
         if (tid == 0) n_found = 0;
         __syncthreads();
-        auto in_wanted = [&](const uint32_t b) { return (want[b >> 5] >> (b & 31) & 1u) != 0; };
-        each_quad<G>(view, 0, view.n_chunks, [&](const row_u32x4 (&v)[4], const int32_t i0) { return collect(v, i0, in_wanted); });
-        collect_extra(in_wanted);
+        auto wanted = [&](const float s) {
+            const uint32_t b = bucket_of<G::BUCKETS>(s, c);
+            return (want[b >> 5] >> (b & 31) & 1u) != 0;
+        };
+        each_quad<G>(view, 0, view.n_chunks, [&](const row_u32x4 (&v)[4], const int32_t i0) { return collect(v, i0, wanted); });
+        const int32_t x = view.extra(tid);
+        if (x >= 0 && wanted(view.at(x))) collect_one(view.at(x), x);
         __syncthreads();
     }
     const bool whole = n_found > (uint32_t)LISTED;           // more than the list holds: the answers come from memory
@@ -883,7 +964,7 @@ __global__ __launch_bounds__(G::THREADS) void part_histogram_kernel(const Sample
     if (!(fabsf(hi) < __builtin_inff()) || !(p.T > 0.f)) return;      // answered apart
     if (tid < 256) pow2[tid] = exp2((double)tid / 256.0 + a.q_bits);
     for (int b = tid; b < G::BUCKETS; b += G::THREADS) { cnt[b] = 0; wsum[b] = 0; }
-    const RowScale c = row_scale(hi, st.low, p, a.q_bits, G::BUCKETS);
+    const RowScale c = row_scale(hi, st.low, item_cut(p, a.q_bits), p, a.q_bits, G::BUCKETS);
     __syncthreads();
     const RowView<TYPE> view(a.scores, r, a.lds, a.M);
     const int32_t q0 = part * a.per_part, q1 = min(q0 + a.per_part, view.n_chunks);
@@ -919,7 +1000,7 @@ __global__ __launch_bounds__(G::THREADS) void part_collect_kernel(const SampleAr
     const PartStat st = join_stats(a, r);
     const float hi = key_score((uint32_t)(st.best >> 32));
     if (!(fabsf(hi) < __builtin_inff()) || !(p.T > 0.f)) return;      // answered apart
-    const RowScale c = row_scale(hi, st.low, p, a.q_bits, G::BUCKETS);
+    const RowScale c = row_scale(hi, st.low, item_cut(p, a.q_bits), p, a.q_bits, G::BUCKETS);
     load_histogram(a, r, sh);
     wanted_buckets(a, r, p, sh, want);
     const RowView<TYPE> view(a.scores, r, a.lds, a.M);
@@ -957,7 +1038,7 @@ __global__ __launch_bounds__(G::THREADS) void part_answer_kernel(const SampleArg
         return;
     }
     if (threadIdx.x < 256) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x / 256.0 + a.q_bits);
-    const RowScale c = row_scale(hi, st.low, p, a.q_bits, G::BUCKETS);
+    const RowScale c = row_scale(hi, st.low, item_cut(p, a.q_bits), p, a.q_bits, G::BUCKETS);
     load_histogram(a, r, sh);
     const uint32_t n = a.n_found[r];
     ListedRow<G, TYPE> row{view, a.found + r * SR_LISTED, n, n > SR_LISTED};       // more than the list holds: from memory
