@@ -7,6 +7,10 @@
                                           (reclibwh/core/ALS.py:160-233)
   half_sweep_cg  the same half-sweep with a fixed number of conjugate-gradient steps per row
                  instead of the exact solve (no reference counterpart; the path for f > 128)
+  sample_rows / recommend_sample   random draws from the softmax of score rows / of the factors' scores, with
+                 temperature, min-p, top-k and top-p (no reference counterpart)
+  distill_rows / distill_topk      loss and gradient of following a teacher's ranked lists, on score rows /
+                 straight from the factors (no reference counterpart)
 
 torch is used for device memory and streams only; every computation is a HIP kernel
 in libals_hip.so.  Arguments are validated here (dtype, contiguity, device, index
@@ -905,3 +909,40 @@ def recommend_topk(X, Y, users, k, M=None, exclude_csr=None, block_users=4096, f
         else:
             idx[pos] = i_; val[pos] = v_
     return idx, val
+
+
+def recommend_sample(X, Y, users, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, M=None, exclude_csr=None, block_users=4096):
+    """Random items for `users` (int64 device tensor) by sample_rows of their scores, block_users users at a time: the
+    exploring counterpart of recommend_topk, with the same X, Y (or its PreparedItems), M and exclude_csr.  u and the
+    parameters as for sample_rows, one row per user.  Returns (idx int32, logp float32), shaped like u.
+
+    A single top_k of 1 to 1024 draws from recommend_topk's list (no score matrix): the kept items are the same, being the
+    first in rank order either way.  Otherwise the scores of a block are materialised, at most 4 GiB at a time."""
+    M = Y.shape[0] if M is None else int(M)
+    _index(users, torch.int64, "users")
+    nu = users.shape[0]
+    if not isinstance(u, torch.Tensor) or u.dim() not in (1, 2) or u.shape[0] != nu:
+        raise ValueError("u must be [n_users] or [n_users, n_draws]")
+    _same_device(X, users, u)
+    idx = torch.empty(u.shape, dtype=torch.int32, device=X.device)
+    logp = torch.empty(u.shape, dtype=torch.float32, device=X.device)
+    part = lambda v, s, e: v[s:e] if torch.is_tensor(v) and v.dim() else v  # noqa: E731
+    if not (torch.is_tensor(top_k) and top_k.dim()) and 1 <= int(top_k) <= min(1024, M):
+        items, val = recommend_topk(X, Y, users, int(top_k), M, exclude_csr, block_users)
+        at, logp = sample_rows(val, u, temperature, 0, top_p, min_p)
+        got = torch.gather(items, 1, at.reshape(nu, -1).clamp(min=0).long()).reshape(u.shape)
+        return torch.where(at < 0, at, got), logp
+    ex = None
+    if exclude_csr is not None:
+        ex = device_exclusions(exclude_csr, X.device)
+    rows_per = max(1, min(block_users, max(nu, 1), (1 << 30) // max(M, 1)))
+    buf = None
+    for s in range(0, nu, rows_per):
+        e = min(nu, s + rows_per)
+        if buf is None:
+            buf = torch.empty((min(rows_per, nu), M), dtype=torch.float32, device=X.device)
+        sc = scores(X, Y, users[s:e], M, out=buf)
+        i_, l_ = sample_rows(sc, u[s:e], part(temperature, s, e), part(top_k, s, e), part(top_p, s, e), part(min_p, s, e), ex,
+                             users[s:e] if ex else None)
+        idx[s:e] = i_; logp[s:e] = l_
+    return idx, logp

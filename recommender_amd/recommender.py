@@ -233,19 +233,83 @@ class RecommenderALS:
         k = min(int(k), self.n_items)
         ex = None
         if filter_rated and self.Utrain is not None:
-            # the training matrix as the engine already holds it on the device; otherwise uploaded once and kept
-            if self.engine is not None:
-                ex = self.engine.csr_users
-            else:
-                if self._exclusions is None:
-                    self._exclusions = ops.device_exclusions((self.Utrain.indptr, self.Utrain.indices), self.device)
-                ex = self._exclusions
+            ex = self._rated()
         if ex is not None:
             u = np.asarray(users, dtype=np.int64).reshape(-1)
             if u.size and (u.min() < 0 or u.max() >= self.Utrain.shape[0]):
                 raise ValueError("filter_rated: user id outside the training matrix (%d users)" % self.Utrain.shape[0])
         idx, val = ops.recommend_topk(self.X, self._items_for_scoring(), self._idx(users), k, M=self.n_items, exclude_csr=ex)
         return idx.cpu().numpy().astype(np.int64), val.cpu().numpy()
+
+    def sample(self, users, n=1, temperature=1.0, top_k=200, top_p=1.0, min_p=0.0, filter_rated=False, u=None, seed=None):
+        """n random items for each of `users`, drawn with replacement from the softmax of their scores at `temperature`
+        cut by min_p, top_k and top_p (ops.sample_rows; the parameters may be arrays with one value per user): exploration
+        around the ranked list of recommend(), with the probability a logged policy needs.  u: the random numbers in
+        [0, 1), [nu, n]; drawn with torch's generator (seeded by `seed` if given) when left out.  filter_rated drops items
+        the user rated in the training data.  Returns (idx [nu, n], logp [nu, n]); a user with nothing to draw gets -1
+        and -inf.  No reference counterpart."""
+        users = np.asarray(users, dtype=np.int64).reshape(-1)
+        n = int(n)
+        if n < 1:
+            raise ValueError("n must be >= 1")
+        ex = None
+        if filter_rated and self.Utrain is not None:
+            if users.size and (users.min() < 0 or users.max() >= self.Utrain.shape[0]):
+                raise ValueError("filter_rated: user id outside the training matrix (%d users)" % self.Utrain.shape[0])
+            ex = self._rated()
+        if u is None:
+            gen = None
+            if seed is not None:
+                gen = torch.Generator(device=self.device)
+                gen.manual_seed(int(seed))
+            u = torch.rand((len(users), n), dtype=torch.float64, device=self.device, generator=gen)
+        else:
+            u = torch.as_tensor(np.ascontiguousarray(u, dtype=np.float64).reshape(len(users), n), device=self.device)
+        par = [v if np.ndim(v) == 0 else torch.as_tensor(np.ascontiguousarray(v, dtype=t), device=self.device)
+               for v, t in ((temperature, np.float32), (top_k, np.int32), (top_p, np.float32), (min_p, np.float32))]
+        if np.ndim(top_k) == 0:
+            par[1] = 0 if int(top_k) >= self.n_items else int(top_k)
+        idx, logp = ops.recommend_sample(self.X, self._items_for_scoring(), self._idx(users), u, *par, M=self.n_items, exclude_csr=ex)
+        return idx.cpu().numpy().astype(np.int64), logp.cpu().numpy()
+
+    def distill(self, teacher_idx, teacher_scores, users, lr, temperature=1.0):
+        """One gradient step of this model towards a teacher's ranked lists: for the given users (each once), the mean of
+        KL(softmax(teacher_scores / T) over the list || softmax(own scores / T) over all items) (ops.distill_topk) is
+        lowered by plain gradient descent with step `lr` on the users' rows and the whole item factor.  teacher_idx /
+        teacher_scores: [nu, k] arrays as recommend() of another model returns them (an index outside the items is
+        padding).  Returns the mean loss before the step.  Fits a small model's ranking to a large one's; no reference
+        counterpart."""
+        if self.mode != "train":
+            raise RuntimeError("cannot call distill() when mode is not 'train'")
+        if self.X is None:
+            self._ensure_factors()
+        users = np.asarray(users, dtype=np.int64).reshape(-1)
+        if len(users) == 0:
+            return float("nan")
+        if len(np.unique(users)) != len(users):
+            raise ValueError("a user listed twice: every user's list counts once per step")
+        if users.min() < 0 or users.max() >= self.n_users:
+            raise ValueError("user id outside the model")
+        ti = teacher_idx.cpu().numpy() if torch.is_tensor(teacher_idx) else np.asarray(teacher_idx)
+        tv = teacher_scores.cpu().numpy() if torch.is_tensor(teacher_scores) else np.asarray(teacher_scores)
+        ti = torch.as_tensor(np.where((ti >= 0) & (ti < self.n_items), ti, -1).astype(np.int32), device=self.device)
+        tv = torch.as_tensor(np.ascontiguousarray(tv, dtype=np.float32), device=self.device)
+        uid = self._idx(users)
+        w = torch.full((len(users),), 1.0 / len(users), dtype=torch.float32, device=self.device)
+        loss, dX, dY = ops.distill_topk(self.X, self.Y, uid, ti, tv, temperature=temperature, weight=w, M=self.n_items)
+        self.X.index_add_(0, uid, dX, alpha=-float(lr))
+        self.Y[: self.n_items].add_(dY, alpha=-float(lr))
+        self._prepared = None                             # the item factor has changed
+        self._foldin_cache = None
+        return float(loss.double().mean().item())
+
+    def _rated(self):
+        """The training matrix as exclusions: as the engine already holds it on the device, otherwise uploaded once and kept."""
+        if self.engine is not None:
+            return self.engine.csr_users
+        if self._exclusions is None:
+            self._exclusions = ops.device_exclusions((self.Utrain.indptr, self.Utrain.indices), self.device)
+        return self._exclusions
 
     def _items_for_scoring(self):
         """The item factor as recommend() hands it to the top-k: converted once per trained / loaded model into the
