@@ -222,7 +222,7 @@ __device__ __forceinline__ void cut_pair(const float p0, const float p1, unsigne
 // TBUF list tiles are kept (one where LDS holds no second: F = 256).
 // Workgroup (split, block): the ids of one split go to one XCD, so that the blocks that stream the same tiles share its L2.
 template <int F, int WAVES, int RING, int TBUF, bool BACK>
-__global__ __launch_bounds__(WAVES * 64) void pass_kernel(const FactorArgs a) {
+__global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const FactorArgs a) {
     constexpr int KS = F / 16, FT = F / 32, CHUNKS = F / 4, PER_WAVE = CHUNKS / WAVES;
     constexpr int LPR = WAVES * 2;                       // lanes that write one user's row of the list tile
     static_assert(CHUNKS % WAVES == 0, "every wave copies the same number of chunks");
@@ -277,8 +277,10 @@ __global__ __launch_bounds__(WAVES * 64) void pass_kernel(const FactorArgs a) {
     const int row = BACK ? tid / LPR : 0, sub = BACK ? tid % LPR : 0;
     const int64_t i_first = block * WAVES * 32;
     struct Entries { int b, e, item; float t, bias; };
-    Entries now{0, 0, 0, 0.f, NEVER}, old[2] = {now, now};
-    int64_t old_user[2] = {0, 0};
+    Entries now{0, 0, 0, 0.f, NEVER}, old[TBUF];
+    int64_t old_user[TBUF];
+#pragma unroll
+    for (int q = 0; q < TBUF; ++q) { old[q] = now; old_user[q] = 0; }
     auto fetch = [&](const int64_t t) {                  // the first LPR entries of the row's user in stage t
         Entries x{0, 0, 0, 0.f, NEVER};
         const int64_t u = t * TILE + row;
@@ -293,8 +295,8 @@ __global__ __launch_bounds__(WAVES * 64) void pass_kernel(const FactorArgs a) {
     auto place = [&](const int64_t t, const int parity) {   // writes `now`, the entries of stage t
         const int buf = TBUF == 2 ? parity : 0;
         float *tt = t_tile + buf * (WAVES * 32 * T_STRIDE);
-        const Entries o = TBUF == 2 && parity ? old[1] : old[0];
-        const int64_t ou = TBUF == 2 && parity ? old_user[1] : old_user[0];
+        const Entries o = TBUF == 2 && parity ? old[TBUF - 1] : old[0];
+        const int64_t ou = TBUF == 2 && parity ? old_user[TBUF - 1] : old_user[0];
         if (o.b + sub < o.e) tt[(o.item - i_first) * T_STRIDE + row] = 0.f;
         for (int q = o.b + sub + LPR; q < o.e; q += LPR)
             tt[(a.s_item[ou * a.k + q] - i_first) * T_STRIDE + row] = 0.f;
@@ -302,7 +304,7 @@ __global__ __launch_bounds__(WAVES * 64) void pass_kernel(const FactorArgs a) {
         if (now.b + sub < now.e) tt[(now.item - i_first) * T_STRIDE + row] = now.t;
         for (int q = now.b + sub + LPR; q < now.e; q += LPR)
             tt[(a.s_item[u * a.k + q] - i_first) * T_STRIDE + row] = a.s_t[u * a.k + q];
-        if (TBUF == 2 && parity) { old[1] = now; old_user[1] = u; }
+        if (TBUF == 2 && parity) { old[TBUF - 1] = now; old_user[TBUF - 1] = u; }
         else { old[0] = now; old_user[0] = u; }
         if (sub == 0) bias[buf * 32 + row] = now.bias;
     };
@@ -711,8 +713,8 @@ int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const 
     a.block_items = p.waves * TILE;
     hipStream_t st = (hipStream_t)stream;
     switch (p.F) {
-        case 32: return run<32, 8, 4, 3, 2>(a, st);
-        case 64: return run<64, 8, 4, 3, 2>(a, st);
+        case 32: return run<32, 8, 4, 2, 1>(a, st);
+        case 64: return run<64, 8, 4, 2, 1>(a, st);
         case 128: return run<128, 8, 3, 2, 2>(a, st);
         default: return run<256, 4, 2, 2, 1>(a, st);
     }
