@@ -40,8 +40,9 @@ typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
 #include "als_fp16.inc"
 
 constexpr int LIST_MAX = 1024;
+constexpr int MAX_SPLITS = 512;
 constexpr int TILE = 32;                // rows per tile, of either factor
-constexpr int Y_MAX_BLOCKS = 256, X_MAX_BLOCKS = 64;
+constexpr int Y_MAX_BLOCKS = 1024, X_MAX_BLOCKS = 256;
 constexpr float P_OFFSET = 8.f;         // pass 1: p 2^8, and at most 2^6 above the running maximum's: below 2^15
 constexpr float LAZY = 6.f;             // the running maximum follows when it lags by more than 2^6
 constexpr float Q_OFFSET = 14.f;        // pass 2: (q - t) 2^14
@@ -85,6 +86,15 @@ __device__ __forceinline__ const float *user_row(const FactorArgs &a, const int6
     return id >= 0 && id < a.x_rows ? a.X + id * a.ldx : nullptr;
 }
 
+// Four factors of a row, zero beyond f.  VEC: one 16-byte load.
+template <bool VEC>
+__device__ __forceinline__ f32x4 load4(const float *row, const int c, const int f) {
+    if constexpr (VEC) return c < f ? *reinterpret_cast<const f32x4 *>(row + c) : f32x4{0.f, 0.f, 0.f, 0.f};
+    f32x4 v;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = c + e < f ? row[c + e] : 0.f;
+    return v;
+}
 __device__ __forceinline__ float block_max256(float v, float *red) {
 #pragma unroll
     for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
@@ -104,19 +114,24 @@ __device__ __forceinline__ float block_sum256(float v, float *red) {
 
 // ----------------------------------------------------------------------------- laying the factors out
 // Largest |y|, |x| and |c x| (finite ones), one value per block: the reader takes the maximum over blocks.
+template <bool VEC>
 __global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
     __shared__ float red[4];
     const bool is_y = blockIdx.x < Y_MAX_BLOCKS;
     const int b = is_y ? blockIdx.x : blockIdx.x - Y_MAX_BLOCKS, nb = is_y ? Y_MAX_BLOCKS : X_MAX_BLOCKS;
     const int64_t rows = is_y ? a.M : a.n;
     float m = 0.f, mc = 0.f;
-    // a wave takes a row at a time
-    for (int64_t r = (int64_t)b * 4 + (threadIdx.x >> 6); r < rows; r += (int64_t)nb * 4) {
+    // sixteen lanes take a row at a time
+    for (int64_t r = (int64_t)b * 16 + (threadIdx.x >> 4); r < rows; r += (int64_t)nb * 16) {
         const float *row = is_y ? a.Y + r * a.ldy : user_row(a, r);
         if (!row) continue;
         const float c = is_y || !a.weight ? 1.f : fabsf(a.weight[r]);
         float mr = 0.f;
-        for (int k = threadIdx.x & 63; k < a.f; k += 64) mr = fmaxf(mr, finite_abs(row[k]));
+        for (int k = 4 * (threadIdx.x & 15); k < a.f; k += 64) {
+            const f32x4 v = load4<VEC>(row, k, a.f);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) mr = fmaxf(mr, finite_abs(v[e]));
+        }
         m = fmaxf(m, mr);
         mc = fmaxf(mc, finite_abs(mr * c * a.inv_t));
     }
@@ -146,9 +161,11 @@ __global__ __launch_bounds__(256) void prepare_kernel(const FactorArgs a) {
     const bool is_y = blockIdx.x < a.m_tiles;
     const int64_t T = is_y ? blockIdx.x : blockIdx.x - a.m_tiles;
     const int64_t rows = is_y ? a.M : a.n;
-    const float my = block_max256(tid < Y_MAX_BLOCKS ? a.maxima[tid] : 0.f, red);
-    const float mx = block_max256(tid < X_MAX_BLOCKS ? a.maxima[Y_MAX_BLOCKS + tid] : 0.f, red);
-    const float mc = block_max256(tid < X_MAX_BLOCKS ? a.maxima[Y_MAX_BLOCKS + X_MAX_BLOCKS + tid] : 0.f, red);
+    float my = 0.f;
+    for (int q = tid; q < Y_MAX_BLOCKS; q += 256) my = fmaxf(my, a.maxima[q]);
+    my = block_max256(my, red);
+    const float mx = block_max256(a.maxima[Y_MAX_BLOCKS + tid], red);             // X_MAX_BLOCKS = 256
+    const float mc = block_max256(a.maxima[Y_MAX_BLOCKS + X_MAX_BLOCKS + tid], red);
     const float to_log2 = a.inv_t * 1.44269504f;
     const float sy = op_scale(my).s, sx = op_scale(mx * to_log2).s, sc = op_scale(mc).s;
     if (blockIdx.x == 0 && tid == 0) {
@@ -455,14 +472,27 @@ __global__ __launch_bounds__(256) void join_items_kernel(const FactorArgs a, con
 }
 
 // ----------------------------------------------------------------------------- lists
-// One workgroup per user (and per padding user of the last tile, which only gets its bias).
-__global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a, const int F) {
-    __shared__ uint64_t key[LIST_MAX];              // item << 32 | position, ~0 for padding
-    __shared__ float val[LIST_MAX], share[LIST_MAX];
-    __shared__ int32_t sorted[LIST_MAX];
-    __shared__ float x[256], part[4][256], red[4], stat[2];
+// One workgroup per user (and per padding user of the last tile, which only gets its bias).  Sixteen lanes work on one
+// listed item, sixteen items at a time, four floats per lane and 64 factors; VEC: the rows allow 16-byte loads.  K_MAX: lists of up to
+// 256 items leave room for eight workgroups per compute unit.
+__device__ __forceinline__ float sum16(float v) {
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    return v;
+}
+
+template <int F, bool VEC, int K_MAX>
+__global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
+    constexpr int NC = F <= 64 ? 1 : F / 64;        // float4 per lane and item
+    constexpr int QUADS = F / 4, GROUPS = 256 / QUADS;
+    __shared__ uint64_t key[K_MAX];              // item << 32 | position, ~0 for padding
+    __shared__ float val[K_MAX], share[K_MAX];
+    __shared__ int32_t sorted[K_MAX];
+    __shared__ float sorted_t[K_MAX];
+    __shared__ f32x4 part[16][QUADS], o_sum[GROUPS][QUADS];
+    __shared__ float x[F], red[4], loss_part[16], scale[MAX_SPLITS];
     __shared__ int32_t n_kept;
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int tid = threadIdx.x;
     const int64_t u = blockIdx.x;
     if (u >= a.n) {
         if (tid == 0) a.bias[u] = NEVER;
@@ -476,21 +506,32 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a, const in
         for (int64_t b = tid; b <= a.item_blocks; b += 256) a.offs[u * (a.item_blocks + 1) + b] = 0;
         return;
     }
-    x[tid] = tid < f ? xrow[tid] : 0.f;
+    if (tid < F) x[tid] = tid < f ? xrow[tid] : 0.f;
     for (int p = tid; p < a.k; p += 256) {
         const int32_t i = a.t_idx[u * a.ldt + p];
         key[p] = i >= 0 && i < a.M ? (uint64_t)(uint32_t)i << 32 | (uint32_t)p : ~0ull;
         val[p] = a.t_val[u * a.ldt + p];
     }
     if (tid == 0) n_kept = 0;
-    __syncthreads();
+    // the parts of pass 1
+    float hi = -__builtin_inff();
+    for (int s = tid; s < a.splits1; s += 256) hi = fmaxf(hi, a.stat_part[2 * ((int64_t)s * a.n + u)]);
+    hi = block_max256(hi, red);
+    float z = 0.f;
+    for (int s = tid; s < a.splits1; s += 256) {
+        const int64_t at = (int64_t)s * a.n + u;
+        const float c = exp2_fast(a.stat_part[2 * at] - hi);
+        scale[s] = c;
+        z += a.stat_part[2 * at + 1] * c;
+    }
+    z = block_sum256(z, red);
     // of an item listed twice the first entry stands
     float top = -__builtin_inff();
     unsigned kept_mask = 0;
     for (int p = tid, b = 0; p < a.k; p += 256, ++b) {
         const uint64_t own = key[p];
         bool keep = own != ~0ull;
-        for (int q = 0; q < a.k && keep; ++q) keep = !(key[q] >> 32 == own >> 32 && key[q] < own);
+        for (int q = 0; q < a.k; ++q) keep = keep && !(key[q] >> 32 == own >> 32 && key[q] < own);
         if (keep) { kept_mask |= 1u << b; top = fmaxf(top, val[p]); }
     }
     top = block_max256(top, red);
@@ -511,81 +552,81 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a, const in
     // item order, by rank among the kept
     for (int p = tid; p < a.k; p += 256) {
         const uint64_t own = key[p];
-        if (own == ~0ull) continue;
         int rank = 0;
+#pragma unroll 4
         for (int q = 0; q < a.k; ++q) rank += key[q] < own;
-        sorted[rank] = (int32_t)(own >> 32);
+        if (own == ~0ull) continue;
         const float t = share[p] / sum;
+        sorted[rank] = (int32_t)(own >> 32);
+        sorted_t[rank] = t;
         a.s_item[u * a.k + rank] = (int32_t)(own >> 32);
         a.s_t[u * a.k + rank] = t * exp2f(Q_OFFSET);
-        share[p] = t;
     }
     __syncthreads();
     for (int64_t b = tid; b <= a.item_blocks; b += 256) {
         const int64_t first = b * a.block_items;
-        int lo = 0, hi = n_list;
-        while (lo < hi) {
-            const int mid = (lo + hi) >> 1;
+        int lo = 0, end = n_list;
+        while (lo < end) {
+            const int mid = (lo + end) >> 1;
             if (sorted[mid] < first) lo = mid + 1;
-            else hi = mid;
+            else end = mid;
         }
         a.offs[u * (a.item_blocks + 1) + b] = (uint16_t)lo;
     }
-    // the parts of pass 1
-    {
-        float hi = -__builtin_inff();
-        for (int s = tid; s < a.splits1; s += 256) hi = fmaxf(hi, a.stat_part[2 * ((int64_t)s * a.n + u)]);
-        hi = block_max256(hi, red);
-        float zz = 0.f;
-        for (int s = tid; s < a.splits1; s += 256) {
-            const int64_t at = (int64_t)s * a.n + u;
-            zz += a.stat_part[2 * at + 1] * exp2_fast(a.stat_part[2 * at] - hi);
-        }
-        zz = block_sum256(zz, red);
-        if (tid == 0) {
-            stat[0] = hi; stat[1] = zz;
-            // a list without weight: c (q - t) must be 0 for all items, so its user's q is switched off
-            a.bias[u] = any ? hi + log2f(zz) - P_OFFSET - Q_OFFSET : NEVER;
-        }
-    }
-    __syncthreads();
-    const float m = stat[0], z = stat[1];
-    const float lse = (m + log2f(z) - P_OFFSET) * 0.69314718f;       // ln Z of s / T
-    // the listed items: t y summed, <x, y> for the loss; a wave takes an item at a time
-    float acc[4] = {0.f, 0.f, 0.f, 0.f}, loss = 0.f;
-    for (int p = wave; p < a.k; p += 4) {
-        const uint64_t own = key[p];
-        if (own == ~0ull) continue;
-        const float *y = a.Y + (int64_t)(own >> 32) * a.ldy;
-        const float t = share[p];
+    // a list without weight: c (q - t) must be 0 for all items, so its user's q is switched off
+    if (tid == 0) a.bias[u] = any ? hi + log2f(z) - P_OFFSET - Q_OFFSET : NEVER;
+    const float lse = (hi + log2f(z) - P_OFFSET) * 0.69314718f;      // ln Z of s / T
+    // the listed items: t y summed, <x, y> for the loss
+    const int group = tid >> 4, l = tid & 15;
+    f32x4 acc[NC];
+    float loss = 0.f;
+#pragma unroll
+    for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int p = group; p < n_list; p += 16) {
+        const float *y = a.Y + (int64_t)sorted[p] * a.ldy;
+        const float t = sorted_t[p];
         float dot = 0.f;
 #pragma unroll
-        for (int q = 0; q < 4; ++q) {
-            const int c = lane + 64 * q;
-            if (c < f) {
-                const float v = y[c];
-                dot = fmaf(v, x[c], dot);
-                acc[q] = fmaf(t, v, acc[q]);
+        for (int c = 0; c < NC; ++c) {
+            const int k0 = 64 * c + 4 * l;
+            const f32x4 v = k0 < F ? load4<VEC>(y, k0, f) : f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                dot = fmaf(v[e], k0 < F ? x[k0 + e] : 0.f, dot);
+                acc[c][e] = fmaf(t, v[e], acc[c][e]);
             }
         }
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) dot += __shfl_xor(dot, o);
+        dot = sum16(dot);
         if (t != 0.f) loss += t * (logf(t) - (dot * a.inv_t - lse));
     }
 #pragma unroll
-    for (int q = 0; q < 4; ++q) part[wave][lane + 64 * q] = acc[q];
-    if (lane == 0) red[wave] = loss;
+    for (int c = 0; c < NC; ++c)
+        if (64 * c + 4 * l < F) part[group][16 * c + l] = acc[c];
+    if (l == 0) loss_part[group] = loss;
+    // O, its parts dealt out over the threads by four factors and split
+    {
+        const int quad = tid % QUADS, g = tid / QUADS;
+        f32x4 o{0.f, 0.f, 0.f, 0.f};
+        const float *src = a.o_part + u * F + 4 * quad;
+#pragma unroll 4
+        for (int s = g; s < a.splits1; s += GROUPS) o += *reinterpret_cast<const f32x4 *>(src + (int64_t)s * a.n * F) * scale[s];
+        o_sum[g][quad] = o;
+    }
     __syncthreads();
-    if (tid == 0) a.loss[u] = any ? (red[0] + red[1]) + (red[2] + red[3]) : 0.f;
-    if (tid < f) {
-        float o = 0.f;
-        for (int s = 0; s < a.splits1; ++s) {
-            const int64_t at = (int64_t)s * a.n + u;
-            o += a.o_part[at * F + tid] * exp2_fast(a.stat_part[2 * at] - m);
-        }
-        const float listed = (part[0][tid] + part[1][tid]) + (part[2][tid] + part[3][tid]);
-        const float c = (a.weight ? a.weight[u] : 1.f) * a.inv_t;
-        a.dX[u * f + tid] = any ? c * (o / z * a.scales[1] - listed) : 0.f;
+    if (tid < 16) {
+        const float all = sum16(loss_part[tid]);
+        if (tid == 0) a.loss[u] = any ? all : 0.f;
+    }
+    if (tid < QUADS && 4 * tid < f) {
+        f32x4 o = o_sum[0][tid], listed = part[0][tid];
+#pragma unroll 3
+        for (int g = 1; g < GROUPS; ++g) o += o_sum[g][tid];
+#pragma unroll 3
+        for (int g = 1; g < 16; ++g) listed += part[g][tid];
+        const float c = (a.weight ? a.weight[u] : 1.f) * a.inv_t, inv = a.scales[1] / z;
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+            if (4 * tid + e < f) a.dX[u * f + 4 * tid + e] = any ? c * (o[e] * inv - listed[e]) : 0.f;
     }
 }
 
@@ -602,7 +643,7 @@ struct Plan {
 // Splits of a pass over `stream` tiles for `blocks` workgroups: enough workgroups for 512 (two per compute unit), at least
 // 8 tiles each, a multiple of 8 from 8 on (one XCD per split), none empty.
 int split_count(const int64_t blocks, const int64_t stream) {
-    int64_t s = std::max<int64_t>(1, std::min<int64_t>(512 / std::max<int64_t>(blocks, 1), stream / 8));
+    int64_t s = std::max<int64_t>(1, std::min<int64_t>(MAX_SPLITS / std::max<int64_t>(blocks, 1), stream / 8));
     if (s > 8) s = s / 8 * 8;
     while (s > 1) {
         const int64_t per = (stream + s - 1) / s;
@@ -653,18 +694,28 @@ int32_t launch_pass(const FactorArgs &a, hipStream_t st) {
 
 template <int F, int WAVES, int RING1, int RING2, int TBUF>
 int32_t run(const FactorArgs &a, hipStream_t st) {
-    hipLaunchKernelGGL(maxima_kernel, dim3(Y_MAX_BLOCKS + X_MAX_BLOCKS), dim3(256), 0, st, a);
+    const bool vec = a.f % 4 == 0 && a.ldy % 4 == 0 && a.ldx % 4 == 0 && ((uintptr_t)a.Y | (uintptr_t)a.X) % 16 == 0;
+    const dim3 blocks(Y_MAX_BLOCKS + X_MAX_BLOCKS);
+    if (vec) hipLaunchKernelGGL((maxima_kernel<true>), blocks, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((maxima_kernel<false>), blocks, dim3(256), 0, st, a);
     hipLaunchKernelGGL((prepare_kernel<F>), dim3((unsigned)(a.m_tiles + a.n_tiles)), dim3(256), 0, st, a);
     ALS_HIP_CHECK6(hipGetLastError());
     int32_t rc = launch_pass<F, WAVES, RING1, 1, false>(a, st);
     if (rc) return rc;
-    hipLaunchKernelGGL(lists_kernel, dim3((unsigned)(a.n_tiles * TILE)), dim3(256), 0, st, a, F);
+    const dim3 users((unsigned)(a.n_tiles * TILE));
+    if (a.k <= 256) {
+        if (vec) hipLaunchKernelGGL((lists_kernel<F, true, 256>), users, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((lists_kernel<F, false, 256>), users, dim3(256), 0, st, a);
+    } else {
+        if (vec) hipLaunchKernelGGL((lists_kernel<F, true, LIST_MAX>), users, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((lists_kernel<F, false, LIST_MAX>), users, dim3(256), 0, st, a);
+    }
     ALS_HIP_CHECK6(hipGetLastError());
     rc = launch_pass<F, WAVES, RING2, TBUF, true>(a, st);
     if (rc) return rc;
     if (a.splits2 > 1) {
-        const int64_t blocks = std::min<int64_t>((a.M * a.f + 255) / 256, 4096);
-        hipLaunchKernelGGL(join_items_kernel, dim3((unsigned)blocks), dim3(256), 0, st, a, F);
+        const int64_t n_blocks = std::min<int64_t>((a.M * a.f + 255) / 256, 4096);
+        hipLaunchKernelGGL(join_items_kernel, dim3((unsigned)n_blocks), dim3(256), 0, st, a, F);
         ALS_HIP_CHECK6(hipGetLastError());
     }
     return ALS_OK;
