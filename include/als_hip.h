@@ -400,7 +400,8 @@ int32_t als_recommend_topk_prepared_f32(const float *X, int64_t ldx, const int64
  * parameters alone.
  * opts      [host] one value for all rows, or a [device] array with one per row where the pointer is not NULL.
  * ex_*      as als_topk_rows_f32: those columns are set to -inf first, in place; columns outside [0, M) are ignored.
- * All other pointers are [device].
+ * All other pointers are [device].  Few long rows need a workspace of als_sample_rows_workspace_bytes bytes (0: none, the
+ * pointer may be NULL).
  * ------------------------------------------------------------------------------------ */
 #define ALS_DTYPE_F32 0
 #define ALS_DTYPE_F16 1
@@ -435,6 +436,7 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  * als_distill_rows   the scores are given, [n_rows, lds] row major in float32, float16 or bfloat16; grad_out [n_rows, ldg]
  *                    of the same type receives slope and may be `scores` itself (same ld).  Sums are float32 in runs of 4
  *                    or 8 items, float64 above, in an order set by M and the row's address modulo 16 alone.
+ *                    Long rows need a workspace of als_distill_rows_workspace_bytes bytes (0: none, may be NULL).
  * als_distill_topk_f32   the scores are those of the factors, s_ui = <X[user_ids[u]], Y[i]> for i < M (user_ids NULL: rows
  *                    0..n_users-1), and never stored: loss_out [n_users], and the gradients of sum_u weight_u loss_u
  *                        dX_out [n_users, f]: sum_i slope_ui Y[i]    (a user listed twice has two rows),

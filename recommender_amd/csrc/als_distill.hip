@@ -335,14 +335,14 @@ extern "C" {
 size_t als_distill_rows_workspace_bytes(int32_t dtype, int64_t n_rows, int64_t M, int32_t k) {
     if (dtype < ALS_DTYPE_F32 || dtype > ALS_DTYPE_BF16 || n_rows < 1 || M < 1 || M > INT32_MAX || k < 1 || k > LIST_MAX) return 0;
     const int64_t chunks = M / (dtype == ALS_DTYPE_F32 ? 4 : 8);
-    if (chunks <= 16 * DR_THREADS) return 16;                 // held by one workgroup: nothing is kept between launches
+    if (chunks <= 16 * DR_THREADS) return 0;                  // held by one workgroup: nothing is kept between launches
     return (size_t)n_rows * ((size_t)row_parts(dtype, M) * sizeof(PartStat) + (size_t)k * 4) + 16;
 }
 
 int32_t als_distill_rows(const void *scores, int32_t dtype, int64_t lds, int64_t n_rows, int64_t M, const int32_t *teacher_idx,
                          const float *teacher_val, int64_t ld_teacher, int32_t k, float temperature, const float *weight,
                          float *loss_out, void *grad_out, int64_t ldg, void *workspace, size_t ws_bytes, void *stream) {
-    if (!scores || !teacher_idx || !teacher_val || !loss_out || !grad_out || !workspace)
+    if (!scores || !teacher_idx || !teacher_val || !loss_out || !grad_out)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_rows: null pointer");
     if (n_rows < 1 || M < 1 || lds < M || ldg < M || M > INT32_MAX || n_rows > INT32_MAX || ld_teacher < k)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_rows: bad sizes (n_rows=%lld M=%lld lds=%lld ldg=%lld)", (long long)n_rows,
@@ -355,7 +355,7 @@ int32_t als_distill_rows(const void *scores, int32_t dtype, int64_t lds, int64_t
     if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || !(1.f / temperature < 3e38f))
         return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_rows: temperature %g", (double)temperature);
     const size_t need = als_distill_rows_workspace_bytes(dtype, n_rows, M, k);
-    if (ws_bytes < need || (uintptr_t)workspace % 8)
+    if (need && (!workspace || ws_bytes < need || (uintptr_t)workspace % 8))
         return als_fail_(ALS_ERR_WORKSPACE, "als_distill_rows: workspace too small or not 8-byte aligned: %zu < %zu", ws_bytes, need);
     if (n_rows * row_parts(dtype, M) > INT32_MAX)
         return als_fail_(ALS_ERR_UNSUPPORTED, "als_distill_rows: too many rows of this length for one launch");

@@ -243,7 +243,9 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
     constexpr int KS = F / 16, FT = F / 32, CHUNKS = F / 4, PER_WAVE = CHUNKS / WAVES;
     constexpr int LPR = WAVES * 2;                       // lanes that write one user's row of the list tile
     static_assert(CHUNKS % WAVES == 0, "every wave copies the same number of chunks");
-    extern __shared__ char lds[];
+    constexpr int LDS_BYTES = RING * CHUNKS * 1024 + (BACK ? TBUF * (WAVES * 32 * T_STRIDE + 32) * 4 : 0);
+    static_assert(LDS_BYTES <= 160 * 1024, "LDS");
+    __shared__ __attribute__((aligned(16))) char lds[LDS_BYTES];
     u32x4 *ring = reinterpret_cast<u32x4 *>(lds);                                   // RING x CHUNKS x 64
     float *t_tile = reinterpret_cast<float *>(lds + RING * CHUNKS * 1024);          // BACK: TBUF x WAVES * 32 x T_STRIDE
     float *bias = t_tile + TBUF * WAVES * 32 * T_STRIDE;                            // BACK: TBUF x 32
@@ -293,6 +295,7 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
     // wrote there and write the new entries, in order, without a barrier between.
     const int row = BACK ? tid / LPR : 0, sub = BACK ? tid % LPR : 0;
     const int64_t i_first = block * WAVES * 32;
+    const uint16_t *offs = BACK ? a.offs + block : nullptr;
     struct Entries { int b, e, item; float t, bias; };
     Entries now{0, 0, 0, 0.f, NEVER}, old[TBUF];
     int64_t old_user[TBUF];
@@ -303,9 +306,10 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         const int64_t u = t * TILE + row;
         if (t < t1 && sub == 0) x.bias = a.bias[u];      // padding users have one too
         if (t < t1 && u < a.n) {
-            const uint16_t *o = a.offs + u * (a.item_blocks + 1) + block;
+            const uint16_t *o = offs + (uint64_t)(uint32_t)u * (uint32_t)(a.item_blocks + 1);
             x.b = o[0]; x.e = o[1];
-            if (x.b + sub < x.e) { x.item = a.s_item[u * a.k + x.b + sub]; x.t = a.s_t[u * a.k + x.b + sub]; }
+            const uint64_t at = (uint64_t)(uint32_t)u * (uint32_t)a.k + (uint32_t)(x.b + sub);
+            if (x.b + sub < x.e) { x.item = a.s_item[at]; x.t = a.s_t[at]; }
         }
         return x;
     };
@@ -641,7 +645,8 @@ struct Plan {
 };
 
 // Splits of a pass over `stream` tiles for `blocks` workgroups: enough workgroups for 512 (two per compute unit), at least
-// 8 tiles each, a multiple of 8 from 8 on (one XCD per split), none empty.
+// 8 tiles each (fewer do not end sooner: a workgroup's start takes as long as 8 tiles), a multiple of 8 from 8 on (one XCD
+// per split), none empty.
 int split_count(const int64_t blocks, const int64_t stream) {
     int64_t s = std::max<int64_t>(1, std::min<int64_t>(MAX_SPLITS / std::max<int64_t>(blocks, 1), stream / 8));
     if (s > 8) s = s / 8 * 8;
@@ -684,10 +689,7 @@ int32_t launch_pass(const FactorArgs &a, hipStream_t st) {
     const int64_t stat_tiles = BACK ? a.m_tiles : a.n_tiles;
     const int64_t grid = (stat_tiles + WAVES - 1) / WAVES * (BACK ? a.splits2 : a.splits1);
     if (grid > INT32_MAX) return als_fail_(ALS_ERR_UNSUPPORTED, "als_distill_topk_f32: too many workgroups");
-    constexpr int bytes = RING * (F / 4) * 1024 + (BACK ? TBUF * (WAVES * 32 * T_STRIDE + 32) * 4 : 0);
-    static_assert(bytes <= 160 * 1024, "LDS");
-    ALS_HIP_CHECK6(hipFuncSetAttribute((const void *)pass_kernel<F, WAVES, RING, TBUF, BACK>, hipFuncAttributeMaxDynamicSharedMemorySize, bytes));
-    hipLaunchKernelGGL((pass_kernel<F, WAVES, RING, TBUF, BACK>), dim3((unsigned)grid), dim3(WAVES * 64), bytes, st, a);
+    hipLaunchKernelGGL((pass_kernel<F, WAVES, RING, TBUF, BACK>), dim3((unsigned)grid), dim3(WAVES * 64), 0, st, a);
     ALS_HIP_CHECK6(hipGetLastError());
     return ALS_OK;
 }

@@ -1052,7 +1052,7 @@ struct CutPlan {
     size_t off_wsum, off_cnt, off_nfound, off_found, total;
 };
 CutPlan cut_plan(const int32_t dtype, const int64_t n, const int64_t M) {
-    CutPlan p{0, 0, 0, 0, 0, 0, 16};
+    CutPlan p{0, 0, 0, 0, 0, 0, 0};
     const int64_t chunks = M / (dtype == ALS_DTYPE_F32 ? 4 : 8);
     if (chunks <= CUT_CHUNKS || n >= CUT_ROWS) return p;
     // about 512 workgroups, of two chunks per thread or more each
@@ -1100,7 +1100,7 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
                         const int32_t *ex_col, const int64_t *ex_row_ids, const als_sample_opts_t *opts, const void *u,
                         int32_t u_is_f64, int32_t n_draws, int32_t *idx_out, float *logp_out, void *workspace, size_t ws_bytes,
                         void *stream) {
-    if (!scores || !opts || !u || !idx_out || !logp_out || !workspace)
+    if (!scores || !opts || !u || !idx_out || !logp_out)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: null pointer");
     if (n_rows < 1 || M < 1 || lds < M || M > INT32_MAX || n_draws < 1)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: bad sizes (n_rows=%lld M=%lld lds=%lld n_draws=%d)", (long long)n_rows,
@@ -1114,7 +1114,7 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
     const CutPlan plan = cut_plan(dtype, n_rows, M);
     if (n_rows * std::max<int64_t>(plan.n_parts, 1) > INT32_MAX)
         return als_fail_(ALS_ERR_UNSUPPORTED, "als_sample_rows: too many rows for one launch");
-    if (ws_bytes < plan.total || (uintptr_t)workspace % 16)
+    if (plan.total && (!workspace || ws_bytes < plan.total || (uintptr_t)workspace % 16))
         return als_fail_(ALS_ERR_WORKSPACE, "als_sample_rows: workspace too small or not 16-byte aligned: %zu < %zu", ws_bytes, plan.total);
     SampleArgs a;
     a.scores = scores; a.lds = lds; a.M = M;

@@ -33,6 +33,18 @@ def _stream():
     return ctypes.c_void_p(torch.cuda.current_stream().cuda_stream)
 
 
+def _addr(t):
+    """A tensor's address as the binding takes it (an int costs a fraction of a c_void_p: these calls can be a few
+    microseconds of GPU work)."""
+    return None if t is None else t.data_ptr()
+
+
+def _enqueue(name, device, *args):
+    """Calls the library's `name` with args and the current stream of `device`, the device of the call's tensors."""
+    with torch.cuda.device(device.index):
+        check(getattr(lib, name)(*args, _stream()), name)
+
+
 def _need(t, dtype, name, dim=None):
     if not isinstance(t, torch.Tensor) or not t.is_cuda:
         raise ValueError("%s must be a CUDA/HIP tensor" % name)
@@ -678,12 +690,12 @@ def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, e
     logp = torch.empty(u.shape, dtype=torch.float32, device=score_rows.device)
     if n == 0:
         return idx, logp
-    ws = torch.empty(lib.als_sample_rows_workspace_bytes(dtype, n, M), dtype=torch.uint8, device=score_rows.device)
-    opts = _lib.SampleOpts(t, k, p, m, *(x.data_ptr() if x is not None else None for x in (t_rows, k_rows, p_rows, m_rows)))
-    with torch.cuda.device(score_rows.device):
-        check(lib.als_sample_rows(_ptr(score_rows), dtype, ld, n, M, _ptr(ex_ptr), _ptr(ex_col), _ptr(exclude_rows),
-                                  ctypes.byref(opts), _ptr(u), int(u.dtype == torch.float64), u.numel() // n, _ptr(idx),
-                                  _ptr(logp), _ptr(ws), ws.numel(), _stream()), "als_sample_rows")
+    need = lib.als_sample_rows_workspace_bytes(dtype, n, M)
+    ws = torch.empty(need, dtype=torch.uint8, device=score_rows.device) if need else None
+    opts = _lib.SampleOpts(t, k, p, m, _addr(t_rows), _addr(k_rows), _addr(p_rows), _addr(m_rows))
+    _enqueue("als_sample_rows", score_rows.device, _addr(score_rows), dtype, ld, n, M, _addr(ex_ptr), _addr(ex_col),
+             _addr(exclude_rows), ctypes.byref(opts), _addr(u), int(u.dtype == torch.float64), u.numel() // n, _addr(idx),
+             _addr(logp), _addr(ws), need)
     return idx, logp
 
 
@@ -747,10 +759,10 @@ def distill_rows(score_rows, teacher_idx, teacher_val, temperature=1.0, weight=N
     loss = torch.empty(n, dtype=torch.float32, device=score_rows.device)
     if n == 0:
         return loss, out
-    ws = torch.empty(lib.als_distill_rows_workspace_bytes(dtype, n, M, k), dtype=torch.uint8, device=score_rows.device)
-    with torch.cuda.device(score_rows.device):
-        check(lib.als_distill_rows(_ptr(score_rows), dtype, ld, n, M, _ptr(teacher_idx), _ptr(teacher_val), ldt, k, T, _ptr(weight),
-                                   _ptr(loss), _ptr(out), ldo, _ptr(ws), ws.numel(), _stream()), "als_distill_rows")
+    need = lib.als_distill_rows_workspace_bytes(dtype, n, M, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=score_rows.device) if need else None
+    _enqueue("als_distill_rows", score_rows.device, _addr(score_rows), dtype, ld, n, M, _addr(teacher_idx), _addr(teacher_val), ldt,
+             k, T, _addr(weight), _addr(loss), _addr(out), ldo, _addr(ws), need)
     return loss, out
 
 
@@ -785,11 +797,10 @@ def distill_topk(X, Y, users, teacher_idx, teacher_val, temperature=1.0, weight=
     if n == 0:
         return loss, dX, torch.zeros((M, f), dtype=torch.float32, device=X.device)
     dY = torch.empty((M, f), dtype=torch.float32, device=X.device)
-    ws = torch.empty(lib.als_distill_topk_workspace_bytes(n, M, f, k), dtype=torch.uint8, device=X.device)
-    with torch.cuda.device(X.device):
-        check(lib.als_distill_topk_f32(_ptr(X), X.shape[0], ldx, _ptr(users), n, _ptr(Y), ldy, M, f, _ptr(teacher_idx),
-                                       _ptr(teacher_val), ldt, k, T, _ptr(weight), _ptr(loss), _ptr(dX), _ptr(dY), _ptr(ws), ws.numel(), _stream()),
-              "als_distill_topk_f32")
+    need = lib.als_distill_topk_workspace_bytes(n, M, f, k)
+    ws = torch.empty(need, dtype=torch.uint8, device=X.device)
+    _enqueue("als_distill_topk_f32", X.device, _addr(X), X.shape[0], ldx, _addr(users), n, _addr(Y), ldy, M, f, _addr(teacher_idx),
+             _addr(teacher_val), ldt, k, T, _addr(weight), _addr(loss), _addr(dX), _addr(dY), _addr(ws), need)
     return loss, dX, dY
 
 
