@@ -443,12 +443,21 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
     } else if (r < a.M) {
         if (splits == 1) {
             const float inv = a.scales[2];
+            const bool quads = a.f % 4 == 0 && (uintptr_t)a.dY % 16 == 0;
 #pragma unroll
             for (int q = 0; q < FT; ++q)
 #pragma unroll
-                for (int e = 0; e < 16; ++e) {
-                    const int c = 32 * q + 8 * (e / 4) + 4 * h + e % 4;
-                    if (c < a.f) a.dY[r * a.f + c] = O[q][e] * inv;
+                for (int g = 0; g < 4; ++g) {
+                    const int c = 32 * q + 8 * g + 4 * h;
+                    const f32x4 v{O[q][4 * g] * inv, O[q][4 * g + 1] * inv, O[q][4 * g + 2] * inv, O[q][4 * g + 3] * inv};
+                    float *dst = a.dY + r * a.f + c;
+                    if (quads) {
+                        if (c < a.f) *reinterpret_cast<f32x4 *>(dst) = v;
+                    } else {
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (c + e < a.f) dst[e] = v[e];
+                    }
                 }
         } else {
             const int64_t at = (int64_t)split * a.M + r;
@@ -768,7 +777,7 @@ int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const 
     switch (p.F) {
         case 32: return run<32, 8, 4, 2, 1>(a, st);
         case 64: return run<64, 8, 4, 2, 1>(a, st);
-        case 128: return run<128, 8, 3, 2, 2>(a, st);
+        case 128: return run<128, 8, 3, 2, 1>(a, st);
         default: return run<256, 4, 2, 2, 1>(a, st);
     }
 }
