@@ -398,6 +398,7 @@ int32_t als_recommend_topk_prepared_f32(const float *X, int64_t ldx, const int64
  * column -1 and logp -inf.  +inf scores share all the weight.  Weights are summed as integers of 2^-Q of the largest,
  * Q = min(51, 62 - ceil(log2 M)); an item below half of that counts as dropped.  The answer depends on the row and its
  * parameters alone.
+ * Rows of at most 2^31 - 2^16 columns, at most 2^20 draws per row (they are made one after the other).
  * opts      [host] one value for all rows, or a [device] array with one per row where the pointer is not NULL.
  * ex_*      as als_topk_rows_f32: those columns are set to -inf first, in place; columns outside [0, M) are ignored.
  * All other pointers are [device].  Few long rows need a workspace of als_sample_rows_workspace_bytes bytes (0: none, the
@@ -436,14 +437,15 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  * als_distill_rows   the scores are given, [n_rows, lds] row major in float32, float16 or bfloat16; grad_out [n_rows, ldg]
  *                    of the same type receives slope and may be `scores` itself (same ld).  Sums are float32 in runs of 4
  *                    or 8 items, float64 above, in an order set by M and the row's address modulo 16 alone.
- *                    Long rows need a workspace of als_distill_rows_workspace_bytes bytes (0: none, may be NULL).
+ *                    M <= 2^31 - 2^16.  Long rows need a workspace of als_distill_rows_workspace_bytes bytes (0: none,
+ *                    may be NULL).
  * als_distill_topk_f32   the scores are those of the factors, s_ui = <X[user_ids[u]], Y[i]> for i < M (user_ids NULL: rows
  *                    0..n_users-1), and never stored: loss_out [n_users], and the gradients of sum_u weight_u loss_u
  *                        dX_out [n_users, f]: sum_i slope_ui Y[i]    (a user listed twice has two rows),
  *                        dY_out [M, f]:       sum_u slope_ui X[user_ids[u]],
  *                    both dense row major.  A user id outside [0, x_rows) gives NaN for its loss and dX row and adds nothing
- *                    to dY.  Any f <= ALS_MAX_FACTORS and alignment; temperature in [1e-6, 1e6]; the
- *                    factors must be finite.  Products of 22-bit operands (two fp16 pieces of a value scaled by one power
+ *                    to dY.  Any f <= ALS_MAX_FACTORS and alignment; temperature in [1e-6, 1e6];
+ *                    n_users, M <= 2^27; the factors must be finite.  Products of 22-bit operands (two fp16 pieces of a value scaled by one power
  *                    of two per factor; values below 2^-18 of the factor's largest lose bits) accumulated in float32.
  *                    8 n M f operations, three products each.  Workspace: about 8 (n + M) F bytes, F = f rounded up to 32,
  *                    64, 128 or 256, plus the parts of split sums.

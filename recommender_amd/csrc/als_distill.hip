@@ -37,7 +37,7 @@ __device__ __forceinline__ float exp2_fast(const float x) { return __builtin_amd
 
 struct RowsArgs {
     const void *scores;
-    int64_t lds, M;
+    int64_t lds, n, M;
     const int32_t *t_idx;
     const float *t_val;
     int64_t ldt;
@@ -223,7 +223,8 @@ __device__ __forceinline__ RowScale row_scale(const RowsArgs &a, const int64_t r
 template <int TYPE, int NV>
 __global__ __launch_bounds__(DR_THREADS, NV <= 8 ? 8 : 4) void distill_rows_kernel(const RowsArgs a) {
     __shared__ ListShared sh;
-    const int64_t r = blockIdx.x;
+    const int64_t r = row_of_block();
+    if (r >= a.n) return;
     const RowView<TYPE> view(a.scores, r, a.lds, a.M);
     RowPart<TYPE, NV> part;
     part.load(view, 0, true);
@@ -316,9 +317,9 @@ template <int TYPE>
 void launch_rows(const RowsArgs &a, const int64_t n, void *ws, hipStream_t st) {
     const int64_t chunks = a.M / RowView<TYPE>::VEC;
     const dim3 block(DR_THREADS);
-    if (chunks <= 4 * DR_THREADS) hipLaunchKernelGGL((distill_rows_kernel<TYPE, 4>), dim3((unsigned)n), block, 0, st, a);
-    else if (chunks <= 8 * DR_THREADS) hipLaunchKernelGGL((distill_rows_kernel<TYPE, 8>), dim3((unsigned)n), block, 0, st, a);
-    else if (chunks <= 16 * DR_THREADS) hipLaunchKernelGGL((distill_rows_kernel<TYPE, 16>), dim3((unsigned)n), block, 0, st, a);
+    if (chunks <= 4 * DR_THREADS) hipLaunchKernelGGL((distill_rows_kernel<TYPE, 4>), grid_of_rows(n), block, 0, st, a);
+    else if (chunks <= 8 * DR_THREADS) hipLaunchKernelGGL((distill_rows_kernel<TYPE, 8>), grid_of_rows(n), block, 0, st, a);
+    else if (chunks <= 16 * DR_THREADS) hipLaunchKernelGGL((distill_rows_kernel<TYPE, 16>), grid_of_rows(n), block, 0, st, a);
     else {
         const int parts = (int)row_parts(TYPE, a.M);
         PartStat *stats = (PartStat *)ws;
@@ -333,7 +334,7 @@ void launch_rows(const RowsArgs &a, const int64_t n, void *ws, hipStream_t st) {
 extern "C" {
 
 size_t als_distill_rows_workspace_bytes(int32_t dtype, int64_t n_rows, int64_t M, int32_t k) {
-    if (dtype < ALS_DTYPE_F32 || dtype > ALS_DTYPE_BF16 || n_rows < 1 || M < 1 || M > INT32_MAX || k < 1 || k > LIST_MAX) return 0;
+    if (dtype < ALS_DTYPE_F32 || dtype > ALS_DTYPE_BF16 || n_rows < 1 || M < 1 || M > ROW_MAX || k < 1 || k > LIST_MAX) return 0;
     const int64_t chunks = M / (dtype == ALS_DTYPE_F32 ? 4 : 8);
     if (chunks <= 16 * DR_THREADS) return 0;                  // held by one workgroup: nothing is kept between launches
     return (size_t)n_rows * ((size_t)row_parts(dtype, M) * sizeof(PartStat) + (size_t)k * 4) + 16;
@@ -344,7 +345,7 @@ int32_t als_distill_rows(const void *scores, int32_t dtype, int64_t lds, int64_t
                          float *loss_out, void *grad_out, int64_t ldg, void *workspace, size_t ws_bytes, void *stream) {
     if (!scores || !teacher_idx || !teacher_val || !loss_out || !grad_out)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_rows: null pointer");
-    if (n_rows < 1 || M < 1 || lds < M || ldg < M || M > INT32_MAX || n_rows > INT32_MAX || ld_teacher < k)
+    if (n_rows < 1 || M < 1 || lds < M || ldg < M || M > ROW_MAX || n_rows > INT32_MAX || ld_teacher < k)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_rows: bad sizes (n_rows=%lld M=%lld lds=%lld ldg=%lld)", (long long)n_rows,
                          (long long)M, (long long)lds, (long long)ldg);
     if (k < 1 || k > LIST_MAX) return als_fail_(ALS_ERR_UNSUPPORTED, "als_distill_rows: k=%d outside [1, %d]", k, LIST_MAX);
@@ -357,10 +358,10 @@ int32_t als_distill_rows(const void *scores, int32_t dtype, int64_t lds, int64_t
     const size_t need = als_distill_rows_workspace_bytes(dtype, n_rows, M, k);
     if (need && (!workspace || ws_bytes < need || (uintptr_t)workspace % 8))
         return als_fail_(ALS_ERR_WORKSPACE, "als_distill_rows: workspace too small or not 8-byte aligned: %zu < %zu", ws_bytes, need);
-    if (n_rows * row_parts(dtype, M) > INT32_MAX)
+    if (need && n_rows * row_parts(dtype, M) > GRID_X)
         return als_fail_(ALS_ERR_UNSUPPORTED, "als_distill_rows: too many rows of this length for one launch");
     RowsArgs a;
-    a.scores = scores; a.lds = lds; a.M = M; a.t_idx = teacher_idx; a.t_val = teacher_val; a.ldt = ld_teacher; a.k = k;
+    a.scores = scores; a.lds = lds; a.n = n_rows; a.M = M; a.t_idx = teacher_idx; a.t_val = teacher_val; a.ldt = ld_teacher; a.k = k;
     a.inv_t = 1.f / temperature; a.weight = weight; a.loss = loss_out; a.grad = grad_out; a.ldg = ldg;
     hipStream_t st = (hipStream_t)stream;
     if (dtype == ALS_DTYPE_F32) launch_rows<ROW_F32>(a, n_rows, workspace, st);

@@ -43,6 +43,8 @@ constexpr int LIST_MAX = 1024;
 constexpr int MAX_SPLITS = 512;
 constexpr int TILE = 32;                // rows per tile, of either factor
 constexpr int Y_MAX_BLOCKS = 1024, X_MAX_BLOCKS = 256;
+constexpr int64_t ROWS_MAX = 1 << 27;   // of either factor: a launch takes fewer than 2^32 threads along x, here 256 per tile
+constexpr int64_t GRID_X = 1 << 21;     // a workgroup per user: beyond that along y
 constexpr float P_OFFSET = 8.f;         // pass 1: p 2^8, and at most 2^6 above the running maximum's: below 2^15
 constexpr float LAZY = 6.f;             // the running maximum follows when it lags by more than 2^6
 constexpr float Q_OFFSET = 14.f;        // pass 2: (q - t) 2^14
@@ -143,6 +145,18 @@ __global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
     }
 }
 
+// Whether a user's list has an entry that counts: of an item listed twice the first stands.  (For the few whose weight is
+// not finite, by one thread.)
+__device__ bool list_has_weight(const FactorArgs &a, const int64_t u) {
+    const int32_t *idx = a.t_idx + u * a.ldt;
+    for (int p = 0; p < a.k; ++p) {
+        if (idx[p] < 0 || idx[p] >= a.M || !(a.t_val[u * a.ldt + p] > -__builtin_inff())) continue;
+        bool first = true;
+        for (int q = 0; q < p && first; ++q) first = idx[q] != idx[p];
+        if (first) return true;
+    }
+    return false;
+}
 // hi and lo fp16 pieces of s x
 __device__ __forceinline__ void cut(const float x, const float s, _Float16 &hi, _Float16 &lo) {
     const float v = x * s;
@@ -181,7 +195,13 @@ __global__ __launch_bounds__(256) void prepare_kernel(const FactorArgs a) {
     }
     if (tid < TILE) {
         const int64_t r = T * TILE + tid;
-        cs[tid] = is_y ? 1.f : r < rows ? (a.weight ? a.weight[r] : 1.f) * a.inv_t : 0.f;
+        float c = is_y ? 1.f : 0.f;
+        if (!is_y && r < rows) {
+            c = (a.weight ? a.weight[r] : 1.f) * a.inv_t;
+            // a mean over the list's own length weights an empty list by infinity: it asks for nothing all the same
+            if (!(fabsf(c) < 3e38f) && !(user_row(a, r) && list_has_weight(a, r))) c = 0.f;
+        }
+        cs[tid] = c;
     }
     __syncthreads();
     char *out = (is_y ? a.yt : a.xt) + T * (F * 256);
@@ -506,9 +526,9 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
     __shared__ float x[F], red[4], loss_part[16], scale[MAX_SPLITS];
     __shared__ int32_t n_kept;
     const int tid = threadIdx.x;
-    const int64_t u = blockIdx.x;
+    const int64_t u = (int64_t)blockIdx.y * GRID_X + blockIdx.x;
     if (u >= a.n) {
-        if (tid == 0) a.bias[u] = NEVER;
+        if (tid == 0 && u < a.n_tiles * TILE) a.bias[u] = NEVER;
         return;
     }
     const int f = a.f;
@@ -713,7 +733,8 @@ int32_t run(const FactorArgs &a, hipStream_t st) {
     ALS_HIP_CHECK6(hipGetLastError());
     int32_t rc = launch_pass<F, WAVES, RING1, 1, false>(a, st);
     if (rc) return rc;
-    const dim3 users((unsigned)(a.n_tiles * TILE));
+    const int64_t n_users = a.n_tiles * TILE;
+    const dim3 users((unsigned)std::min(n_users, GRID_X), (unsigned)((n_users + GRID_X - 1) / GRID_X));
     if (a.k <= 256) {
         if (vec) hipLaunchKernelGGL((lists_kernel<F, true, 256>), users, dim3(256), 0, st, a);
         else hipLaunchKernelGGL((lists_kernel<F, false, 256>), users, dim3(256), 0, st, a);
@@ -733,7 +754,7 @@ int32_t run(const FactorArgs &a, hipStream_t st) {
 }
 
 bool sizes_ok(const int64_t n, const int64_t M, const int32_t f, const int32_t k) {
-    return n >= 1 && M >= 1 && M <= INT32_MAX / 2 && n <= INT32_MAX / 2 && f >= 1 && f <= ALS_MAX_FACTORS && k >= 1 && k <= LIST_MAX;
+    return n >= 1 && M >= 1 && M <= ROWS_MAX && n <= ROWS_MAX && f >= 1 && f <= ALS_MAX_FACTORS && k >= 1 && k <= LIST_MAX;
 }
 
 }  // namespace
@@ -748,7 +769,7 @@ int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const 
                              int64_t ldy, int64_t M, int32_t f, const int32_t *teacher_idx, const float *teacher_val, int64_t ld_teacher,
                              int32_t k, float temperature, const float *weight, float *loss_out, float *dX_out, float *dY_out,
                              void *workspace, size_t ws_bytes, void *stream) {
-    if (!X || !Y || !teacher_idx || !teacher_val || !loss_out || !dX_out || !dY_out || !workspace)
+    if (!X || !Y || !teacher_idx || !teacher_val || !loss_out || !dX_out || !dY_out)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_topk_f32: null pointer");
     if (f > ALS_MAX_FACTORS || k > LIST_MAX)
         return als_fail_(ALS_ERR_UNSUPPORTED, "als_distill_topk_f32: f=%d (at most %d), k=%d (at most %d)", f, ALS_MAX_FACTORS, k, LIST_MAX);
@@ -758,7 +779,7 @@ int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const 
     if (!(temperature >= 1e-6f && temperature <= 1e6f))
         return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_topk_f32: temperature %g outside [1e-6, 1e6]", (double)temperature);
     const Plan p = make_plan(n_users, M, f, k);
-    if (ws_bytes < p.total || (uintptr_t)workspace % 16)
+    if (!workspace || ws_bytes < p.total || (uintptr_t)workspace % 16)
         return als_fail_(ALS_ERR_WORKSPACE, "als_distill_topk_f32: workspace too small or not 16-byte aligned: %zu < %zu", ws_bytes, p.total);
     FactorArgs a;
     a.X = X; a.Y = Y; a.ldx = ldx; a.ldy = ldy; a.users = user_ids; a.n = n_users; a.M = M; a.f = f; a.x_rows = x_rows;

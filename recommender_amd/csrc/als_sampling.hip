@@ -54,6 +54,7 @@ typedef Group<256, 512> Small;
 typedef Group<512, 2048> Large;
 constexpr int CUT_BUCKETS = Large::BUCKETS;
 constexpr int SR_LISTED = 16384;      // cut rows: items collected per row
+constexpr int32_t DRAWS_MAX = 1 << 20;      // a row's draws are made one after the other: some microseconds each
 
 struct Found {            // an item collected by a workgroup of a cut row
     float score;
@@ -66,7 +67,7 @@ struct PartStat {
 
 struct SampleArgs {
     void *scores;
-    int64_t lds, M;
+    int64_t lds, n, M;
     const int64_t *ex_rowptr;
     const int32_t *ex_col;
     const int64_t *ex_rows;
@@ -688,7 +689,8 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
     __shared__ Found found[LISTED];
     __shared__ uint32_t want[G::BUCKETS / 32 + 1], n_found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int64_t r = blockIdx.x;
+    const int64_t r = row_of_block();
+    if (r >= a.n) return;
     const RowView<TYPE> view(a.scores, r, a.lds, a.M);
     if (a.ex_rowptr) {
         exclude_items<TYPE>(a, r, view);
@@ -1072,7 +1074,7 @@ CutPlan cut_plan(const int32_t dtype, const int64_t n, const int64_t M) {
 
 template <int TYPE>
 void launch(const SampleArgs &a, const int64_t n, hipStream_t st) {
-    const dim3 rows((unsigned)n), block(G::THREADS);
+    const dim3 rows = grid_of_rows(n), block(G::THREADS);
     if (a.n_parts == 0) {
         const int64_t chunks = a.M / RowView<TYPE>::VEC;
         if (chunks <= SMALL_CHUNKS) hipLaunchKernelGGL((sample_rows_kernel<Small, TYPE>), rows, dim3(Small::THREADS), 0, st, a);
@@ -1092,7 +1094,7 @@ void launch(const SampleArgs &a, const int64_t n, hipStream_t st) {
 extern "C" {
 
 size_t als_sample_rows_workspace_bytes(int32_t dtype, int64_t n_rows, int64_t M) {
-    if (dtype < ALS_DTYPE_F32 || dtype > ALS_DTYPE_BF16 || n_rows < 1 || M < 1 || M > INT32_MAX) return 0;
+    if (dtype < ALS_DTYPE_F32 || dtype > ALS_DTYPE_BF16 || n_rows < 1 || M < 1 || M > ROW_MAX) return 0;
     return cut_plan(dtype, n_rows, M).total;
 }
 
@@ -1102,7 +1104,7 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
                         void *stream) {
     if (!scores || !opts || !u || !idx_out || !logp_out)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: null pointer");
-    if (n_rows < 1 || M < 1 || lds < M || M > INT32_MAX || n_draws < 1)
+    if (n_rows < 1 || M < 1 || lds < M || M > ROW_MAX || n_rows > INT32_MAX || n_draws < 1 || n_draws > DRAWS_MAX)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: bad sizes (n_rows=%lld M=%lld lds=%lld n_draws=%d)", (long long)n_rows,
                          (long long)M, (long long)lds, n_draws);
     if (dtype < ALS_DTYPE_F32 || dtype > ALS_DTYPE_BF16)
@@ -1112,12 +1114,10 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
     if ((ex_rowptr == nullptr) != (ex_col == nullptr))
         return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: pass both exclusion arrays or neither");
     const CutPlan plan = cut_plan(dtype, n_rows, M);
-    if (n_rows * std::max<int64_t>(plan.n_parts, 1) > INT32_MAX)
-        return als_fail_(ALS_ERR_UNSUPPORTED, "als_sample_rows: too many rows for one launch");
     if (plan.total && (!workspace || ws_bytes < plan.total || (uintptr_t)workspace % 16))
         return als_fail_(ALS_ERR_WORKSPACE, "als_sample_rows: workspace too small or not 16-byte aligned: %zu < %zu", ws_bytes, plan.total);
     SampleArgs a;
-    a.scores = scores; a.lds = lds; a.M = M;
+    a.scores = scores; a.lds = lds; a.n = n_rows; a.M = M;
     a.ex_rowptr = ex_rowptr; a.ex_col = ex_col; a.ex_rows = ex_rowptr ? ex_row_ids : nullptr;
     a.o = *opts;
     a.u = u; a.u_f64 = u_is_f64 != 0; a.n_draws = n_draws;

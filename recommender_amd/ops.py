@@ -658,6 +658,8 @@ def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, e
         raise ValueError("u must be a float32 or float64 tensor")
     if u.dim() not in (1, 2) or u.shape[0] != n or (u.dim() == 2 and u.shape[1] < 1):
         raise ValueError("u must be [n_rows] or [n_rows, n_draws]")
+    if u.dim() == 2 and u.shape[1] > 1 << 20:
+        raise ValueError("at most 2^20 draws per row, got %d" % u.shape[1])
     if not u.is_cuda or not u.is_contiguous():
         raise ValueError("u must be a contiguous CUDA/HIP tensor")
     t, t_rows = _row_param(temperature, n, torch.float32, "temperature", score_rows)
@@ -937,6 +939,8 @@ def recommend_sample(X, Y, users, u, temperature=1.0, top_k=0, top_p=1.0, min_p=
     _same_device(X, users, u)
     idx = torch.empty(u.shape, dtype=torch.int32, device=X.device)
     logp = torch.empty(u.shape, dtype=torch.float32, device=X.device)
+    if nu == 0:
+        return idx, logp
     part = lambda v, s, e: v[s:e] if torch.is_tensor(v) and v.dim() else v  # noqa: E731
     if not (torch.is_tensor(top_k) and top_k.dim()) and 1 <= int(top_k) <= min(1024, M):
         items, val = recommend_topk(X, Y, users, int(top_k), M, exclude_csr, block_users)

@@ -241,3 +241,26 @@ def test_no_rows_and_refusals(ops):
                 lambda: ops.distill_rows(S[:1].expand(4, 10), idx, val)]:
         with pytest.raises(ValueError):
             bad()
+
+
+def test_more_rows_than_one_axis_of_a_launch_takes(ops):
+    rng = np.random.default_rng(41)
+    n = (1 << 21) + 21
+    S = torch.from_numpy(rng.normal(size=(n, 7)).astype(np.float32)).cuda()
+    idx = torch.from_numpy(rng.integers(0, 7, (n, 2)).astype(np.int32)).cuda()
+    val = torch.from_numpy(rng.normal(size=(n, 2)).astype(np.float32)).cuda()
+    loss, grad = ops.distill_rows(S, idx, val)
+    for part in (slice(0, 64), slice(n - 64, n)):
+        # one alignment modulo 16 bytes for every fourth row: the order of the sums is the same
+        rows = torch.arange(n, device="cuda")[part]
+        l, g = ops.distill_rows(S[part], idx[part].contiguous(), val[part].contiguous())
+        assert torch.equal(l, loss[rows]) and torch.equal(g, grad[rows])
+
+
+def test_an_empty_list_weighted_by_infinity(ops):
+    rng = np.random.default_rng(42)
+    S = torch.from_numpy(rng.normal(size=(3, 500)).astype(np.float32)).cuda()
+    idx, val = lists(rng, 3, 500, 20)
+    idx[1] = -1
+    loss, grad = ops.distill_rows(S, idx, val, weight=torch.tensor([1.0, float("inf"), 1.0], device="cuda"))
+    assert torch.isfinite(loss).all() and torch.isfinite(grad).all() and not grad[1].any()

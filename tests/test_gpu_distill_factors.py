@@ -236,3 +236,49 @@ def test_no_users_and_refusals(ops):
                 lambda: ops.distill_topk(X.t(), Y, u, idx, val), lambda: ops.distill_topk(wide, wide, u, idx, val)]:
         with pytest.raises(ValueError):
             bad()
+
+
+def test_an_empty_list_weighted_by_infinity(ops):
+    """1 / (length of the list) as a weight: an empty list asks for nothing, and the items' gradients stay finite."""
+    rng = np.random.default_rng(51)
+    X, Y, u, idx, val = inputs(rng, 70, 300, 20, 9)
+    idx[3] = -1; idx[40] = 300; val[41] = -np.inf
+    idx[42] = 5; val[42, 0] = -np.inf                    # an item listed again: its first entry stands, and has no weight
+    w = torch.rand(70, device="cuda") + 0.5
+    none = [3, 40, 41, 42]
+    w[none] = 0.0
+    want = ops.distill_topk(X, Y, u, idx, val, weight=w)
+    for bad in (np.inf, -np.inf, np.nan):
+        w[none] = bad
+        got = ops.distill_topk(X, Y, u, idx, val, weight=w)
+        for g, v in zip(got, want):
+            assert torch.equal(g, v)
+    w[none] = 1.0
+    check(ops, X, Y, u, idx, val, w=w)
+
+
+def test_more_users_than_one_axis_of_a_launch_takes(ops):
+    rng = np.random.default_rng(52)
+    n, M, f, k = (1 << 21) + 45, 40, 8, 3
+    X = torch.from_numpy(rng.uniform(-0.99, 0.99, size=(n, f)).astype(np.float32)).cuda()
+    X[-1, 0] = 1.0                                       # the largest value, which sets the operands' scale, in the part looked at
+    Y = torch.from_numpy(rng.uniform(-1, 1, size=(M, f)).astype(np.float32)).cuda()
+    idx = torch.from_numpy((rng.integers(0, M - k, (n, 1)) + np.arange(k)).astype(np.int32)).cuda()
+    val = torch.from_numpy(rng.normal(size=(n, k)).astype(np.float32)).cuda()
+    loss, dX, dY = ops.distill_topk(X, Y, None, idx, val)
+    part = slice(n - 80, n)
+    wl, wx, _, tl, tx, _ = definition(X[part].cpu().numpy(), Y.cpu().numpy(), idx[part].cpu().numpy(), val[part].cpu().numpy(), 1.0,
+                                      np.ones(80))
+    assert np.all(np.abs(loss[part].double().cpu().numpy() - wl) <= tl)
+    assert np.all(np.abs(dX[part].double().cpu().numpy() - wx) <= tx)
+    # every user's share of dY, in float64
+    Xd, Yd = X.double(), Y.double()
+    slope = torch.softmax(Xd @ Yd.T.contiguous(), 1)
+    mag = slope.clone()
+    t = torch.softmax(val.double(), 1)
+    slope.scatter_add_(1, idx.long(), -t)
+    mag.scatter_add_(1, idx.long(), t)
+    want = slope.T.contiguous() @ Xd
+    e = 2.0 ** -18 * f + 2.0 ** -19                      # scores: 2 d with |x|, |y| <= 1
+    tol = (e + 2.0 ** -19 + 3 * n / 16 * 2.0 ** -24) * (mag.T.contiguous() @ Xd.abs())
+    assert ((dY.double() - want).abs() <= tol).all()

@@ -283,3 +283,26 @@ def test_refusals(ops):
                                                        torch.zeros(1, dtype=torch.int32, device="cuda")))]:
         with pytest.raises(ValueError):
             bad()
+
+
+def test_more_rows_than_one_axis_of_a_launch_takes(ops):
+    rng = np.random.default_rng(31)
+    n = (1 << 21) + 37
+    S = torch.from_numpy(rng.normal(size=(n, 6)).astype(np.float16)).cuda()
+    u = torch.from_numpy(rng.random(n).astype(np.float32)).cuda()
+    idx, logp = ops.sample_rows(S, u)
+    assert int(idx.min()) >= 0 and int(idx.max()) < 6
+    for part in (slice(0, 100), slice(n - 100, n)):
+        i, l = ops.sample_rows(S[part].clone(), u[part])
+        assert torch.equal(i, idx[part]) and torch.equal(l, logp[part])
+
+
+def test_more_draws_than_are_taken(ops):
+    S = torch.zeros((1, 10), device="cuda")
+    with pytest.raises(ValueError, match="draws"):
+        ops.sample_rows(S, torch.zeros((1, (1 << 20) + 1), device="cuda"))
+
+
+def test_a_thousand_draws_of_a_row(ops):
+    rng = np.random.default_rng(32)
+    check(ops, scores(rng, 2, 5000, "f32"), torch.from_numpy(rng.random((2, 1000))).cuda(), T=2.0, p=0.95)

@@ -113,3 +113,70 @@ def test_distill_step_and_the_run_of_all_three(ra):
         student.distill(ti[:2], tv[:2], [1, 80], lr=0.1)
     with pytest.raises(ValueError):
         student.distill(ti[:2], tv[:1], [1, 2], lr=0.1)
+
+
+def test_no_users(ra):
+    from recommender_amd import ops
+    X = torch.randn(5, 8, device="cuda"); Y = torch.randn(30, 8, device="cuda")
+    none = torch.empty(0, dtype=torch.int64, device="cuda")
+    for kw in (dict(top_k=3), dict(top_k=0), dict(top_k=0, top_p=0.5)):
+        idx, logp = ops.recommend_sample(X, Y, none, torch.empty((0, 4), device="cuda"), **kw)
+        assert idx.shape == (0, 4) and logp.shape == (0, 4)
+
+
+def work(ops, rng):
+    """One call of every operator, of the forms with a workspace: few long rows, rows in parts, split passes."""
+    long_rows = torch.from_numpy(rng.normal(size=(2, 100001)).astype(np.float32)).cuda()
+    u = torch.from_numpy(rng.random((2, 3))).cuda()
+    idx = torch.from_numpy(rng.integers(0, 100001, (2, 50)).astype(np.int32)).cuda()
+    val = torch.from_numpy(rng.normal(size=(2, 50)).astype(np.float32)).cuda()
+    X = torch.from_numpy(rng.normal(size=(40, 24)).astype(np.float32)).cuda()
+    Y = torch.from_numpy(rng.normal(size=(5000, 24)).astype(np.float32)).cuda()
+    li = torch.from_numpy(rng.integers(0, 5000, (40, 30)).astype(np.int32)).cuda()
+    lv = torch.from_numpy(rng.normal(size=(40, 30)).astype(np.float32)).cuda()
+    torch.cuda.synchronize()
+
+    def call():
+        return [*ops.sample_rows(long_rows, u, top_k=500, top_p=0.9), *ops.distill_rows(long_rows, idx, val),
+                *ops.distill_topk(X, Y, None, li, lv)]
+    return call
+
+
+def test_two_streams_at_once(ra):
+    from recommender_amd import ops
+    rng = np.random.default_rng(7)
+    a, b = work(ops, rng), work(ops, rng)
+    want_a, want_b = a(), b()
+    sa, sb = torch.cuda.Stream(), torch.cuda.Stream()
+    torch.cuda.synchronize()
+    got = []
+    for _ in range(5):
+        with torch.cuda.stream(sa):
+            got.append((a(), want_a))
+        with torch.cuda.stream(sb):
+            got.append((b(), want_b))
+    torch.cuda.synchronize()
+    for g, w in got:
+        assert all(torch.equal(x, y) for x, y in zip(g, w))
+
+
+def test_two_graphs_of_one_pool(ra):
+    from recommender_amd import ops
+    rng = np.random.default_rng(8)
+    a, b = work(ops, rng), work(ops, rng)
+    want_a, want_b = a(), b()
+    torch.cuda.synchronize()
+    ga, gb = torch.cuda.CUDAGraph(), torch.cuda.CUDAGraph()
+    with torch.cuda.graph(ga):
+        out_a = a()
+    with torch.cuda.graph(gb, pool=ga.pool()):
+        out_b = b()
+    for _ in range(4):
+        for g in (ga, gb, gb, ga):
+            g.replay()
+        (torch.randn(1000, 1000, device="cuda") * 2).sum()
+        torch.cuda.synchronize()
+        assert all(torch.equal(x, y) for x, y in zip(out_a, want_a))
+        assert all(torch.equal(x, y) for x, y in zip(out_b, want_b))
+        for o in out_a + out_b:
+            o.zero_()
