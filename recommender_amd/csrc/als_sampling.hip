@@ -49,6 +49,7 @@ struct Group {
     static constexpr int THREADS = T, WAVES = T / 64, BUCKETS = B;
     static constexpr int OWN = B / T;             // buckets per thread
     static constexpr int RANKED = T / 4;          // items that are ranked against each other directly, four threads each
+    static constexpr int WAVE_ITEMS = T / 4;      // ... by one wave
 };
 typedef Group<256, 512> Small;
 typedef Group<512, 2048> Large;
@@ -111,6 +112,7 @@ struct SampleShared {
     union {
         struct { u64 wsub[G::BUCKETS]; uint32_t csub[G::BUCKETS]; };
         u64 ranked[G::RANKED][2];           // (key << 32 | ~column, weight)
+        u64 wave_ranked[G::WAVES][G::WAVE_ITEMS][2];
     };
     double pow2[256];               // 2^(i / 256)
     u64 wave_w[G::WAVES];
@@ -118,7 +120,7 @@ struct SampleShared {
     float wave_f[G::WAVES], wave_g[G::WAVES];
     Picked picked;
     uint32_t bucket, n_list, k_lo, k_hi;
-    u64 base_w;
+    u64 base_w, kept;
     uint32_t base_c, in_bucket;
 };
 
@@ -386,8 +388,7 @@ struct ListedRow {
     }
 };
 
-// Column of the m-th item (from 0, in column order) whose key is `key`; the rarest path: more than RANKED items of one
-// bucket share one score.  An item per thread and round.
+// Column of the m-th item (from 0, in column order) whose key is `key`, an item per thread and round: for the +inf of a row.
 template <class G, int TYPE>
 __device__ int32_t nth_of_key(const RowView<TYPE> &view, const uint32_t key, const u64 m, SampleShared<G> &sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -420,49 +421,39 @@ __device__ Picked find(Row &row, const RowView<TYPE> &view, const RowScale &c, c
     const uint32_t b = uniform(sh.bucket);
     uint32_t n = counted ? uniform(sh.in_bucket) : 0, base_c = uniform(sh.base_c);      // 0: not known, tried
     u64 base_w = uniform(sh.base_w);
-    // the bucket's keys [k_lo, k_hi] that are still in question; all of it to begin with
-    uint32_t k_lo = 0, k_hi = ~0u;
-    bool narrowed = false;
-    auto mine = [&](const float s, u64 &w) {                 // an item in question, and its weight
+    // the bucket's keys [k_lo, k_hi] that are still in question: to begin with its scores and a bucket's width more on either
+    // side, for roundings (the last bucket is open downwards)
+    const float width = 1.f / c.per_score;
+    uint32_t k_hi = rank_key(fminf(c.top_f - (float)((int)b - 1) * width, c.top_f));
+    uint32_t k_lo = b == G::BUCKETS - 1 ? 0 : rank_key(c.top_f - (float)(b + 2) * width);
+    k_lo = uniform(k_lo); k_hi = uniform(k_hi);
+    uint32_t i_lo = 0, i_hi = (uint32_t)view.M - 1;          // once they share one key: their columns
+    auto mine = [&](const float s, const uint32_t i, u64 &w) {           // an item in question, and its weight
         if (bucket_of<G::BUCKETS>(s, c) != b) return false;
         const uint32_t key = rank_key(s);
-        return key >= k_lo && key <= k_hi && weigh(s, c, sh.pow2, w);
+        return key >= k_lo && key <= k_hi && i >= i_lo && i <= i_hi && weigh(s, c, sh.pow2, w);
     };
-    // More items than are ranked directly: first the keys they span, then, BUCKETS parts of that range a time, the part with
-    // the answer, until few are left (they are taken into LDS) or all that are left share one key.
+    // More items than are ranked directly: of BUCKETS parts of the range the part with the answer, and of one key's columns
+    // likewise, until few are left (they are taken into LDS).
     int shift = 0;
     for (;;) {
         __syncthreads();
-        const int act = n <= G::RANKED ? 2 : narrowed ? 1 : 0;
-        if (act == 1) {
-            if (k_lo == k_hi) {                              // one score, n items
-                const float s = key_score(k_lo);
-                u64 w = 1;
-                weigh(s, c, sh.pow2, w);
-                w = uniform(w);
-                const u64 m = by_count ? target - base_c : (target - base_w) / w;
-                const int32_t at = nth_of_key<G>(view, k_lo, m, sh);
-                __syncthreads();
-                return Picked{base_w + m * w, w, at, s};
-            }
-            const int bits = 32 - __clz(k_hi - k_lo), part_bits = 31 - __clz(G::BUCKETS);
+        const bool rank_them = n <= G::RANKED, by_column = k_lo == k_hi;
+        if (!rank_them) {
+            const int bits = 32 - __clz(by_column ? i_hi - i_lo : k_hi - k_lo), part_bits = 31 - __clz(G::BUCKETS);
             shift = bits > part_bits ? bits - part_bits : 0;
 #pragma unroll
             for (int q = 0; q < G::OWN; ++q) { sh.csub[G::OWN * tid + q] = 0; sh.wsub[G::OWN * tid + q] = 0; }
         } else if (tid == 0) {
-            sh.k_lo = ~0u; sh.k_hi = 0;
             sh.n_list = 0;
         }
         __syncthreads();
         row.each([&](const float s, const int32_t i) {
             u64 w;
-            if (!mine(s, w)) return;
+            if (!mine(s, (uint32_t)i, w)) return;
             const uint32_t key = rank_key(s);
-            if (act == 0) {
-                atomicMin(&sh.k_lo, key);
-                atomicMax(&sh.k_hi, key);
-            } else if (act == 1) {
-                const uint32_t d = (k_hi - key) >> shift;    // large keys first
+            if (!rank_them) {
+                const uint32_t d = (by_column ? (uint32_t)i - i_lo : k_hi - key) >> shift;       // in rank order
                 atomicAdd(&sh.csub[d], 1u);
                 atomicAdd(&sh.wsub[d], w);
             } else {
@@ -474,22 +465,22 @@ __device__ Picked find(Row &row, const RowView<TYPE> &view, const RowScale &c, c
             }
         });
         __syncthreads();
-        if (act == 2) {
+        if (rank_them) {
             n = uniform(sh.n_list);
             if (n <= G::RANKED) break;
-            continue;
-        }
-        if (act == 0) {
-            k_lo = uniform(sh.k_lo); k_hi = uniform(sh.k_hi);
-            narrowed = true;
             continue;
         }
         scan_buckets(sh.csub, sh.wsub, sh);
         pick_bucket(sh.csub, sh.wsub, by_count, target, base_c, base_w, sh);
         const uint32_t d = uniform(sh.bucket);
         const uint64_t behind = (uint64_t)(d + 1) << shift;                // keys down to the part's end
-        k_lo = behind > k_hi - k_lo ? k_lo : k_hi - (uint32_t)behind + 1;
-        k_hi = k_hi - (d << shift);
+        if (by_column) {
+            i_hi = behind > i_hi - i_lo ? i_hi : i_lo + (uint32_t)behind - 1;
+            i_lo += d << shift;
+        } else {
+            k_lo = behind > k_hi - k_lo ? k_lo : k_hi - (uint32_t)behind + 1;
+            k_hi = k_hi - (d << shift);
+        }
         n = uniform(sh.in_bucket); base_c = uniform(sh.base_c); base_w = uniform(sh.base_w);
     }
     // The few that are left are ranked against each other, four threads to an item.
@@ -516,6 +507,61 @@ __device__ Picked find(Row &row, const RowView<TYPE> &view, const RowScale &c, c
     const Picked out{uniform(sh.picked.before), uniform(sh.picked.weight), uniform(sh.picked.index), uniform(sh.picked.score)};
     __syncthreads();
     return out;
+}
+
+// The same by one wave, from a list in LDS: without barriers, so that draws are made side by side.  False if the bucket has
+// more items than a wave ranks.
+template <class G>
+__device__ __forceinline__ bool wave_find(const Found *list, const uint32_t n, const RowScale &c, const bool by_count, const u64 target,
+                                          SampleShared<G> &sh, Picked &out) {
+    constexpr int SEGMENT = G::BUCKETS / 64;
+    const int lane = threadIdx.x & 63;
+    u64(*items)[2] = sh.wave_ranked[threadIdx.x >> 6];
+    auto sum_at = [&](const int b) { return by_count ? (u64)sh.cnt[b] : sh.wsum[b]; };
+    const int seg = __ffsll(__ballot(sum_at(SEGMENT * lane + SEGMENT - 1) > target)) - 1;
+    const int b = SEGMENT * seg + __ffsll(__ballot(sum_at(SEGMENT * seg + (lane & (SEGMENT - 1))) > target)) - 1;
+    const u64 base_w = b ? sh.wsum[b - 1] : 0;
+    const uint32_t base_c = b ? sh.cnt[b - 1] : 0;
+    uint32_t m = 0;
+    for (uint32_t q0 = 0; q0 < n; q0 += 64) {
+        const uint32_t q = q0 + lane;
+        const Found f = list[q < n ? q : n - 1];
+        bool hit = q < n && bucket_of<G::BUCKETS>(f.score, c) == (uint32_t)b;
+        if (__ballot(hit) == 0) continue;
+        u64 w;
+        hit = weigh(f.score, c, sh.pow2, w) && hit;
+        const u64 mask = __ballot(hit);
+        const uint32_t at = m + __builtin_amdgcn_mbcnt_hi((uint32_t)(mask >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask, 0u));
+        if (hit && at < (uint32_t)G::WAVE_ITEMS) {
+            items[at][0] = (u64)rank_key(f.score) << 32 | (uint32_t)~(uint32_t)f.index;
+            items[at][1] = w;
+        }
+        m += (uint32_t)__popcll(mask);
+    }
+    if (m > (uint32_t)G::WAVE_ITEMS) return false;
+    __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+#pragma unroll 1
+    for (uint32_t e0 = 0; e0 < m; e0 += 64) {
+        const uint32_t e = e0 + lane < m ? e0 + lane : m - 1;
+        const u64 own = items[e][0], w = items[e][1];
+        u64 before = base_w;
+        uint32_t rank = base_c;
+#pragma unroll 4
+        for (uint32_t q = 0; q < m; ++q)
+            if (items[q][0] > own) { before += items[q][1]; ++rank; }
+        const u64 found = __ballot(by_count ? rank == target : before <= target && target < before + w);
+        if (found == 0) continue;
+        const int from = __ffsll(found) - 1;
+        auto lane64 = [&](const u64 v) {
+            return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), from) << 32 |
+                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, from);
+        };
+        const u64 key = lane64(own);
+        out = Picked{lane64(before), lane64(w), (int32_t)~(uint32_t)key, key_score((uint32_t)(key >> 32))};
+        return true;
+    }
+    return false;
 }
 
 // Targets of the three steps (find passes a target: the first item whose running sum exceeds it).
@@ -619,24 +665,56 @@ __device__ void wanted_buckets(const SampleArgs &a, const int64_t r, const RowPa
     __syncthreads();
 }
 
-// Steps 2 to 4 from the running sums in sh.cnt / sh.wsum.
+// Steps 2 to 4 from the running sums in sh.cnt / sh.wsum.  in_lds: the row's items are a list in LDS; then of several draws a
+// wave makes one each, and the workgroup together those that a wave does not (one alone takes a wave as long: 19.7 and 20.2 us
+// for a row of 59 047 at n = 1, but 36 against 31 for 300 rows of 9 724).
 template <class G, int TYPE, class Row>
-__device__ void answer(const SampleArgs &a, const int64_t r, Row &row, const RowView<TYPE> &view, const RowScale &c,
+__device__ void answer(const SampleArgs &a, const int64_t r, Row &row, const bool in_lds, const bool counted, const RowView<TYPE> &view, const RowScale &c,
                        const RowParams &p, SampleShared<G> &sh) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u64 W = uniform(sh.wsum[G::BUCKETS - 1]);
-    // one call of find for all steps: it is long, and inlined
     const bool by_k = top_k_asked(a, p) && (uint32_t)p.top_k < sh.cnt[G::BUCKETS - 1], by_p = p.top_p < 1.f;
-    for (int step = by_k ? -2 : by_p ? -1 : 0; step < a.n_draws; ++step) {
-        if (step == -1 && !by_p) continue;
-        const int64_t at = r * a.n_draws + step;
-        const u64 target = step == -2 ? (u64)p.top_k - 1 : step == -1 ? top_p_target(p.top_p, W) : draw_target(drawn_number(a, at), W);      // uniform
-        const Picked f = find<G>(row, view, c, step == -2, target, top_k_asked(a, p), sh);
-        if (step < 0) W = f.before + f.weight;
-        else if (threadIdx.x == 0) {                         // ln (w / W) = x - ln W
-            const double x = ((double)f.score - c.top) * c.steps * (0.69314718055994530942 / 256.0);
-            a.idx[at] = f.index;
-            a.logp[at] = (float)(x - (log_of(W, sh.pow2, a.q_bits) - 0.69314718055994530942 * a.q_bits));
+    auto target_of = [&](const int step) {
+        return step == -2 ? (u64)p.top_k - 1 : step == -1 ? top_p_target(p.top_p, W) : draw_target(drawn_number(a, r * a.n_draws + step), W);
+    };
+    auto finish = [&](const int step, const Picked &f) {     // one thread
+        if (step < 0) {
+            sh.kept = f.before + f.weight;
+            return;
         }
+        const int64_t at = r * a.n_draws + step;             // ln (w / W) = x - ln W
+        const double x = ((double)f.score - c.top) * c.steps * (0.69314718055994530942 / 256.0);
+        a.idx[at] = f.index;
+        a.logp[at] = (float)(x - (log_of(W, sh.pow2, a.q_bits) - 0.69314718055994530942 * a.q_bits));
+    };
+    int step = by_k ? -2 : by_p ? -1 : 0;
+    while (step < a.n_draws) {                               // uniform
+        if (step == -1 && !by_p) {
+            step = 0;
+            continue;
+        }
+        const int many = step < 0 ? 1 : min(G::WAVES, a.n_draws - step);
+        uint32_t open = (1u << many) - 1;
+        if (in_lds && many > 1) {
+            bool done = true;
+            if (wave < many) {
+                Picked f;
+                done = wave_find<G>(row.found, row.n, c, step == -2, target_of(step + wave), sh, f);
+                if (done && lane == 0) finish(step + wave, f);
+            }
+            if (lane == 0) sh.wave_c[wave] = !done;
+            __syncthreads();
+            open = (uint32_t)__ballot(lane < G::WAVES && sh.wave_c[lane & (G::WAVES - 1)]);
+        }
+        while (open) {
+            const int mine = step + __ffs(open) - 1;
+            open &= open - 1;
+            const Picked f = find<G>(row, view, c, step == -2, target_of(mine), counted, sh);
+            if (threadIdx.x == 0) finish(mine, f);
+        }
+        __syncthreads();
+        if (step < 0) W = uniform(sh.kept);
+        step += many;
     }
 }
 __device__ void answer_all(const SampleArgs &a, const int64_t r, const int32_t index, const float logp) {
@@ -889,7 +967,7 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
     }
     const bool whole = n_found > (uint32_t)LISTED;           // more than the list holds: the answers come from memory
     ListedRow<G, TYPE> list{view, found, n_found, whole};
-    answer<G>(a, r, list, view, c, p, sh);
+    answer<G>(a, r, list, !whole, counted, view, c, p, sh);
 }
 
 // ----------------------------------------------------------------------------- cut rows
@@ -971,7 +1049,7 @@ __global__ __launch_bounds__(G::THREADS) void part_histogram_kernel(const Sample
     const RowView<TYPE> view(a.scores, r, a.lds, a.M);
     const int32_t q0 = part * a.per_part, q1 = min(q0 + a.per_part, view.n_chunks);
     each_bucket<G>(view, q0, q1, part == 0, c, [&](const float (&s)[4], const int32_t, const uint32_t (&b)[4]) {
-        count_four<G::BUCKETS>(s, b, c, pow2, cnt, wsum, top_k_asked(a, p));
+        count_four<G::BUCKETS>(s, b, c, pow2, cnt, wsum, true);
         return true;
     });
     __syncthreads();
@@ -1043,8 +1121,15 @@ __global__ __launch_bounds__(G::THREADS) void part_answer_kernel(const SampleArg
     const RowScale c = row_scale(hi, st.low, item_cut(p, a.q_bits), p, a.q_bits, G::BUCKETS);
     load_histogram(a, r, sh);
     const uint32_t n = a.n_found[r];
-    ListedRow<G, TYPE> row{view, a.found + r * SR_LISTED, n, n > SR_LISTED};       // more than the list holds: from memory
-    answer<G>(a, r, row, view, c, p, sh);
+    constexpr uint32_t IN_LDS = 2048;                        // (read once per step and round)
+    __shared__ Found found[IN_LDS];
+    const bool in_lds = n <= IN_LDS;
+    if (in_lds) {
+        for (uint32_t q = threadIdx.x; q < n; q += G::THREADS) found[q] = a.found[r * SR_LISTED + q];
+        __syncthreads();
+    }
+    ListedRow<G, TYPE> row{view, in_lds ? found : a.found + r * SR_LISTED, n, n > SR_LISTED};      // more than the list holds: from memory
+    answer<G>(a, r, row, in_lds, true, view, c, p, sh);
 }
 
 // ----------------------------------------------------------------------------- host
