@@ -97,19 +97,34 @@ __device__ __forceinline__ f32x4 load4(const float *row, const int c, const int 
     for (int e = 0; e < 4; ++e) v[e] = c + e < f ? row[c + e] : 0.f;
     return v;
 }
+// v of another lane of the wave by a DPP move; lanes without a source get `none`
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(const float v, const float none) {
+    return __uint_as_float((unsigned)__builtin_amdgcn_update_dpp((int)__float_as_uint(none), (int)__float_as_uint(v), CTRL, ROWS, 0xf, false));
+}
+// Over the workgroup's 256 threads.  In a wave: towards lane 63 (a row's 16 lanes, then across rows).
 __device__ __forceinline__ float block_max256(float v, float *red) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    const float none = -__builtin_inff();
+    v = fmaxf(v, moved<0x111, 0xf>(v, none));
+    v = fmaxf(v, moved<0x112, 0xf>(v, none));
+    v = fmaxf(v, moved<0x114, 0xf>(v, none));
+    v = fmaxf(v, moved<0x118, 0xf>(v, none));
+    v = fmaxf(v, moved<0x142, 0xa>(v, none));
+    v = fmaxf(v, moved<0x143, 0xc>(v, none));
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
     __syncthreads();
     return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 __device__ __forceinline__ float block_sum256(float v, float *red) {
-#pragma unroll
-    for (int o = 32; o >= 1; o >>= 1) v += __shfl_xor(v, o);
+    v += moved<0x111, 0xf>(v, 0.f);
+    v += moved<0x112, 0xf>(v, 0.f);
+    v += moved<0x114, 0xf>(v, 0.f);
+    v += moved<0x118, 0xf>(v, 0.f);
+    v += moved<0x142, 0xa>(v, 0.f);
+    v += moved<0x143, 0xc>(v, 0.f);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) red[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 63) red[threadIdx.x >> 6] = v;
     __syncthreads();
     return (red[0] + red[1]) + (red[2] + red[3]);
 }
@@ -519,12 +534,11 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
     constexpr int NC = F <= 64 ? 1 : F / 64;        // float4 per lane and item
     constexpr int QUADS = F / 4, GROUPS = 256 / QUADS;
     __shared__ uint64_t key[K_MAX];              // item << 32 | position, ~0 for padding
-    __shared__ float val[K_MAX], share[K_MAX];
     __shared__ int32_t sorted[K_MAX];
     __shared__ float sorted_t[K_MAX];
     __shared__ f32x4 part[16][QUADS], o_sum[GROUPS][QUADS];
     __shared__ float x[F], red[4], loss_part[16], scale[MAX_SPLITS];
-    __shared__ int32_t n_kept;
+    __shared__ int32_t n_kept, n_again;
     const int tid = threadIdx.x;
     const int64_t u = (int64_t)blockIdx.y * GRID_X + blockIdx.x;
     if (u >= a.n) {
@@ -539,61 +553,92 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
         for (int64_t b = tid; b <= a.item_blocks; b += 256) a.offs[u * (a.item_blocks + 1) + b] = 0;
         return;
     }
-    if (tid < F) x[tid] = tid < f ? xrow[tid] : 0.f;
-    for (int p = tid; p < a.k; p += 256) {
-        const int32_t i = a.t_idx[u * a.ldt + p];
-        key[p] = i >= 0 && i < a.M ? (uint64_t)(uint32_t)i << 32 | (uint32_t)p : ~0ull;
-        val[p] = a.t_val[u * a.ldt + p];
+    // everything that is read whatever the list holds, at once
+    constexpr int OWN = K_MAX / 256, S_OWN = MAX_SPLITS / 256;
+    const int quad = tid % QUADS, o_first = tid / QUADS;
+    const float *o_src = a.o_part + u * F + 4 * quad;
+    const float x_own = tid < f ? xrow[tid] : 0.f;
+    uint64_t own[OWN];
+    float own_val[OWN], m_own[S_OWN], z_own[S_OWN];
+#pragma unroll
+    for (int b = 0; b < OWN; ++b) {
+        const int p = tid + 256 * b;
+        const int32_t i = p < a.k ? a.t_idx[u * a.ldt + p] : -1;
+        own_val[b] = p < a.k ? a.t_val[u * a.ldt + p] : 0.f;
+        own[b] = i >= 0 && i < a.M ? (uint64_t)(uint32_t)i << 32 | (uint32_t)p : ~0ull;
     }
-    if (tid == 0) n_kept = 0;
+#pragma unroll
+    for (int b = 0; b < S_OWN; ++b) {
+        const int64_t at = (int64_t)(tid + 256 * b) * a.n + u;
+        m_own[b] = tid + 256 * b < a.splits1 ? a.stat_part[2 * at] : -__builtin_inff();
+        z_own[b] = tid + 256 * b < a.splits1 ? a.stat_part[2 * at + 1] : 0.f;
+    }
+    f32x4 o{0.f, 0.f, 0.f, 0.f};
+    if (o_first < a.splits1) o = *reinterpret_cast<const f32x4 *>(o_src + (int64_t)o_first * a.n * F);
+    if (tid < F) x[tid] = x_own;
+#pragma unroll
+    for (int b = 0; b < OWN; ++b)
+        if (tid + 256 * b < a.k) key[tid + 256 * b] = own[b];
+    if (tid == 0) { n_kept = 0; n_again = 0; }
     // the parts of pass 1
-    float hi = -__builtin_inff();
-    for (int s = tid; s < a.splits1; s += 256) hi = fmaxf(hi, a.stat_part[2 * ((int64_t)s * a.n + u)]);
+    float hi = fmaxf(m_own[0], m_own[S_OWN - 1]);
     hi = block_max256(hi, red);
     float z = 0.f;
-    for (int s = tid; s < a.splits1; s += 256) {
-        const int64_t at = (int64_t)s * a.n + u;
-        const float c = exp2_fast(a.stat_part[2 * at] - hi);
-        scale[s] = c;
-        z += a.stat_part[2 * at + 1] * c;
+#pragma unroll
+    for (int b = 0; b < S_OWN; ++b) {
+        const float c = exp2_fast(m_own[b] - hi);
+        if (tid + 256 * b < a.splits1) {
+            scale[tid + 256 * b] = c;
+            z += z_own[b] * c;
+        }
     }
     z = block_sum256(z, red);
     // of an item listed twice the first entry stands
     float top = -__builtin_inff();
-    unsigned kept_mask = 0;
-    for (int p = tid, b = 0; p < a.k; p += 256, ++b) {
-        const uint64_t own = key[p];
-        bool keep = own != ~0ull;
-        for (int q = 0; q < a.k; ++q) keep = keep && !(key[q] >> 32 == own >> 32 && key[q] < own);
-        if (keep) { kept_mask |= 1u << b; top = fmaxf(top, val[p]); }
+    int rank[OWN];                                       // entries in front of the own one in item order
+    bool keep[OWN];
+#pragma unroll
+    for (int b = 0; b < OWN; ++b) {
+        rank[b] = 0; keep[b] = false;
+        if (tid + 256 * b >= a.k || own[b] == ~0ull) continue;
+        bool again = false;
+#pragma unroll 8
+        for (int q = 0; q < a.k; ++q) {
+            const uint64_t other = key[q];
+            const bool before = other < own[b];
+            rank[b] += before;
+            again |= before & ((other ^ own[b]) >> 32 == 0);
+        }
+        keep[b] = !again;
+        if (again) n_again = 1;
+        else top = fmaxf(top, own_val[b]);
     }
     top = block_max256(top, red);
     const bool any = top != -__builtin_inff();           // a list without weight asks for nothing
-    __syncthreads();
-    float sum = 0.f;
-    for (int p = tid, b = 0; p < a.k; p += 256, ++b) {
-        const bool keep = any && (kept_mask >> b & 1);
-        const float e = keep ? expf((val[p] - top) * a.inv_t) : 0.f;
-        share[p] = e;
-        sum += e;
-        if (!keep) key[p] = ~0ull;
-        else atomicAdd(&n_kept, 1);
+    float sum = 0.f, share[OWN];
+#pragma unroll
+    for (int b = 0; b < OWN; ++b) {
+        keep[b] = keep[b] && any;
+        share[b] = keep[b] ? expf((own_val[b] - top) * a.inv_t) : 0.f;
+        sum += share[b];
+        if (keep[b]) atomicAdd(&n_kept, 1);
+        else if (tid + 256 * b < a.k) key[tid + 256 * b] = ~0ull;
     }
     sum = block_sum256(sum, red);
-    __syncthreads();
     const int n_list = n_kept;
     // item order, by rank among the kept
-    for (int p = tid; p < a.k; p += 256) {
-        const uint64_t own = key[p];
-        int rank = 0;
-#pragma unroll 4
-        for (int q = 0; q < a.k; ++q) rank += key[q] < own;
-        if (own == ~0ull) continue;
-        const float t = share[p] / sum;
-        sorted[rank] = (int32_t)(own >> 32);
-        sorted_t[rank] = t;
-        a.s_item[u * a.k + rank] = (int32_t)(own >> 32);
-        a.s_t[u * a.k + rank] = t * exp2f(Q_OFFSET);
+#pragma unroll
+    for (int b = 0; b < OWN; ++b) {
+        if (!keep[b]) continue;
+        if (n_again) {
+            rank[b] = 0;
+            for (int q = 0; q < a.k; ++q) rank[b] += key[q] < own[b];
+        }
+        const float t = share[b] / sum;
+        sorted[rank[b]] = (int32_t)(own[b] >> 32);
+        sorted_t[rank[b]] = t;
+        a.s_item[u * a.k + rank[b]] = (int32_t)(own[b] >> 32);
+        a.s_t[u * a.k + rank[b]] = t * exp2f(Q_OFFSET);
     }
     __syncthreads();
     for (int64_t b = tid; b <= a.item_blocks; b += 256) {
@@ -615,22 +660,34 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
     float loss = 0.f;
 #pragma unroll
     for (int c = 0; c < NC; ++c) acc[c] = f32x4{0.f, 0.f, 0.f, 0.f};
-    for (int p = group; p < n_list; p += 16) {
-        const float *y = a.Y + (int64_t)sorted[p] * a.ldy;
-        const float t = sorted_t[p];
-        float dot = 0.f;
+    constexpr int AHEAD = NC == 1 ? 4 : 2;               // items whose rows are under way together
+    for (int p0 = group; p0 < n_list; p0 += 16 * AHEAD) {
+        f32x4 v[AHEAD][NC];
+        float ts[AHEAD];
 #pragma unroll
-        for (int c = 0; c < NC; ++c) {
-            const int k0 = 64 * c + 4 * l;
-            const f32x4 v = k0 < F ? load4<VEC>(y, k0, f) : f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int i = 0; i < AHEAD; ++i) {
+            const int p = p0 + 16 * i < n_list ? p0 + 16 * i : p0;
+            const float *y = a.Y + (int64_t)sorted[p] * a.ldy;
+            ts[i] = p0 + 16 * i < n_list ? sorted_t[p] : 0.f;
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                dot = fmaf(v[e], k0 < F ? x[k0 + e] : 0.f, dot);
-                acc[c][e] = fmaf(t, v[e], acc[c][e]);
-            }
+            for (int c = 0; c < NC; ++c) v[i][c] = 64 * c + 4 * l < F ? load4<VEC>(y, 64 * c + 4 * l, f) : f32x4{0.f, 0.f, 0.f, 0.f};
         }
-        dot = sum16(dot);
-        if (t != 0.f) loss += t * (logf(t) - (dot * a.inv_t - lse));
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+            const float t = ts[i];
+            float dot = 0.f;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const int k0 = 64 * c + 4 * l;
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    dot = fmaf(v[i][c][e], k0 < F ? x[k0 + e] : 0.f, dot);
+                    acc[c][e] = fmaf(t, v[i][c][e], acc[c][e]);
+                }
+            }
+            dot = sum16(dot);
+            if (t != 0.f) loss += t * (logf(t) - (dot * a.inv_t - lse));
+        }
     }
 #pragma unroll
     for (int c = 0; c < NC; ++c)
@@ -638,12 +695,11 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
     if (l == 0) loss_part[group] = loss;
     // O, its parts dealt out over the threads by four factors and split
     {
-        const int quad = tid % QUADS, g = tid / QUADS;
-        f32x4 o{0.f, 0.f, 0.f, 0.f};
-        const float *src = a.o_part + u * F + 4 * quad;
+        if (o_first < a.splits1) o *= scale[o_first];
 #pragma unroll 4
-        for (int s = g; s < a.splits1; s += GROUPS) o += *reinterpret_cast<const f32x4 *>(src + (int64_t)s * a.n * F) * scale[s];
-        o_sum[g][quad] = o;
+        for (int s = o_first + GROUPS; s < a.splits1; s += GROUPS)
+            o += *reinterpret_cast<const f32x4 *>(o_src + (int64_t)s * a.n * F) * scale[s];
+        o_sum[o_first][quad] = o;
     }
     __syncthreads();
     if (tid < 16) {
