@@ -48,12 +48,14 @@ template <int T, int B>
 struct Group {
     static constexpr int THREADS = T, WAVES = T / 64, BUCKETS = B;
     static constexpr int OWN = B / T;             // buckets per thread
+    static constexpr bool BY_VALUE = T > 256;     // 16-bit rows: see count_values
     static constexpr int RANKED = T / 4;          // items that are ranked against each other directly, four threads each
     static constexpr int WAVE_ITEMS = T / 4;      // ... by one wave
 };
 typedef Group<256, 512> Small;
 typedef Group<512, 2048> Large;
 constexpr int CUT_BUCKETS = Large::BUCKETS;
+constexpr int LISTED = 2048;          // items collected in LDS
 constexpr int SR_LISTED = 16384;      // cut rows: items collected per row
 constexpr int32_t DRAWS_MAX = 1 << 20;      // a row's draws are made one after the other: some microseconds each
 
@@ -109,10 +111,17 @@ template <class G>
 struct SampleShared {
     u64 wsum[G::BUCKETS];
     uint32_t cnt[G::BUCKETS];
+    static constexpr int VALUES = G::BY_VALUE ? (G::BUCKETS * 12 + LISTED * 8) / 4 : 1;
     union {
-        struct { u64 wsub[G::BUCKETS]; uint32_t csub[G::BUCKETS]; };
-        u64 ranked[G::RANKED][2];           // (key << 32 | ~column, weight)
-        u64 wave_ranked[G::WAVES][G::WAVE_ITEMS][2];
+        struct {
+            union {
+                struct { u64 wsub[G::BUCKETS]; uint32_t csub[G::BUCKETS]; };
+                u64 ranked[G::RANKED][2];           // (key << 32 | ~column, weight)
+                u64 wave_ranked[G::WAVES][G::WAVE_ITEMS][2];
+            };
+            Found found[LISTED];
+        };
+        uint32_t values[VALUES];                    // how often a 16-bit value and its negative occur
     };
     double pow2[256];               // 2^(i / 256)
     u64 wave_w[G::WAVES];
@@ -274,7 +283,7 @@ __device__ __forceinline__ void scan_buckets(uint32_t *cnt, u64 *wsum, SampleSha
 
 // The bucket at which the running sum (of ones or of weights) passes `target`; base sums in front of it.
 template <class G>
-__device__ void pick_bucket(const uint32_t *cnt, const u64 *wsum, const bool by_count, const u64 target, const uint32_t base_c,
+__device__ __forceinline__ void pick_bucket(const uint32_t *cnt, const u64 *wsum, const bool by_count, const u64 target, const uint32_t base_c,
                             const u64 base_w, SampleShared<G> &sh) {
 #pragma unroll
     for (int q = 0; q < G::OWN; ++q) {
@@ -390,7 +399,7 @@ struct ListedRow {
 
 // Column of the m-th item (from 0, in column order) whose key is `key`, an item per thread and round: for the +inf of a row.
 template <class G, int TYPE>
-__device__ int32_t nth_of_key(const RowView<TYPE> &view, const uint32_t key, const u64 m, SampleShared<G> &sh) {
+__device__ __forceinline__ int32_t nth_of_key(const RowView<TYPE> &view, const uint32_t key, const u64 m, SampleShared<G> &sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     if (tid == 0) sh.picked.index = -1;
     u64 seen = 0;
@@ -414,7 +423,7 @@ __device__ int32_t nth_of_key(const RowView<TYPE> &view, const uint32_t key, con
 // The item, in rank order, at which the running sum of ones (by_count) or of weights passes `target`; the caller has
 // made sure that it does.  Every thread returns the same.
 template <class G, int TYPE, class Row>
-__device__ Picked find(Row &row, const RowView<TYPE> &view, const RowScale &c, const bool by_count, const u64 target,
+__device__ __forceinline__ Picked find(Row &row, const RowView<TYPE> &view, const RowScale &c, const bool by_count, const u64 target,
                        const bool counted, SampleShared<G> &sh) {
     const int tid = threadIdx.x;
     pick_bucket(sh.cnt, sh.wsum, by_count, target, 0, 0, sh);
@@ -612,7 +621,7 @@ __device__ __forceinline__ void buckets_passing(const V *sums, const u64 t0, con
 // The buckets the answers can lie in, as bits: top-k's is known; what it leaves of the weight, and so top-p's target, is
 // known to within that bucket, and so on.
 template <class G>
-__device__ void wanted_buckets(const SampleArgs &a, const int64_t r, const RowParams &p, SampleShared<G> &sh,
+__device__ __forceinline__ void wanted_buckets(const SampleArgs &a, const int64_t r, const RowParams &p, SampleShared<G> &sh,
                                    uint32_t (&want)[G::BUCKETS / 32 + 1]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // ranges of buckets, +1 where one begins and -1 behind its end: the running sum is the number of ranges over a bucket
@@ -669,7 +678,7 @@ __device__ void wanted_buckets(const SampleArgs &a, const int64_t r, const RowPa
 // wave makes one each, and the workgroup together those that a wave does not (one alone takes a wave as long: 19.7 and 20.2 us
 // for a row of 59 047 at n = 1, but 36 against 31 for 300 rows of 9 724).
 template <class G, int TYPE, class Row>
-__device__ void answer(const SampleArgs &a, const int64_t r, Row &row, const bool in_lds, const bool counted, const RowView<TYPE> &view, const RowScale &c,
+__device__ __forceinline__ void answer(const SampleArgs &a, const int64_t r, Row &row, const bool in_lds, const bool counted, const RowView<TYPE> &view, const RowScale &c,
                        const RowParams &p, SampleShared<G> &sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u64 W = uniform(sh.wsum[G::BUCKETS - 1]);
@@ -717,13 +726,13 @@ __device__ void answer(const SampleArgs &a, const int64_t r, Row &row, const boo
         step += many;
     }
 }
-__device__ void answer_all(const SampleArgs &a, const int64_t r, const int32_t index, const float logp) {
+__device__ __forceinline__ void answer_all(const SampleArgs &a, const int64_t r, const int32_t index, const float logp) {
     for (int d = threadIdx.x; d < a.n_draws; d += blockDim.x) { a.idx[r * a.n_draws + d] = index; a.logp[r * a.n_draws + d] = logp; }
 }
 
 // A row whose largest score is +inf: n items share everything, in column order.
 template <class G, int TYPE>
-__device__ void answer_infinite(const SampleArgs &a, const int64_t r, const RowView<TYPE> &view, const RowParams &p,
+__device__ __forceinline__ void answer_infinite(const SampleArgs &a, const int64_t r, const RowView<TYPE> &view, const RowParams &p,
                                 SampleShared<G> &sh) {
     if (threadIdx.x == 0) sh.n_list = 0;
     __syncthreads();
@@ -751,7 +760,7 @@ __device__ __forceinline__ u64 wave_max64(u64 v) {
 }
 
 template <int TYPE>
-__device__ void exclude_items(const SampleArgs &a, const int64_t r, const RowView<TYPE> &view) {
+__device__ __forceinline__ void exclude_items(const SampleArgs &a, const int64_t r, const RowView<TYPE> &view) {
     const int64_t er = a.ex_rows ? a.ex_rows[r] : r;
     for (int64_t q = a.ex_rowptr[er] + threadIdx.x; q < a.ex_rowptr[er + 1]; q += blockDim.x) {
         const int32_t i = a.ex_col[q];
@@ -759,12 +768,123 @@ __device__ void exclude_items(const SampleArgs &a, const int64_t r, const RowVie
     }
 }
 
+// ----------------------------------------------------------------------------- 16-bit rows
+// The histogram of a row by its values: 16-bit scores have few (a few thousand where a catalogue has 10^5 items), so they are
+// counted, 16 bits for a value and 16 for its negative in one word of LDS, and weighed once each - eight instructions and an
+// LDS atomic per item instead of forty and two.  A word per magnitude from the largest that can count downwards; the few
+// items of smaller magnitude are listed.  False, with sh.wsum and sh.cnt in disorder, if their list or a count overflows
+// (a row of equal scores, or most scores 2^-8 of the largest or less): the caller weighs item by item.
+template <class G, int TYPE>
+__device__ __forceinline__ bool count_values(const RowView<TYPE> &view, const RowScale &c, const float reach, const bool counted,
+                                             SampleShared<G> &sh) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    constexpr int FEW = 2048;
+    __shared__ unsigned short few[FEW];
+    __shared__ uint32_t n_few;
+    constexpr uint32_t INF = TYPE == ROW_F16 ? 0x7c00u : 0x7f80u;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    auto bits_above = [](const float v) {                    // of a 16-bit value above v >= 0
+        if constexpr (TYPE == ROW_BF16) return (__float_as_uint(v) >> 16) + 1;
+        return v < 65504.f ? (uint32_t)__builtin_bit_cast(unsigned short, (_Float16)v) + 1 : INF;
+    };
+    auto value_of = [](const uint32_t bits) { return RowView<TYPE>::value(row_u32x4{bits, 0, 0, 0}, 0); };
+    const float floor = c.top_f - reach;
+    const uint32_t most = min(INF - 1, max(bits_above(fabsf(c.top_f)), floor < 0.f ? bits_above(-floor) : 0u));
+    const uint32_t cap = min((uint32_t)SampleShared<G>::VALUES - 1, most + 1), first = most + 1 - cap;       // word t: magnitude first + t
+    for (uint32_t t = tid; t < cap; t += G::THREADS) sh.values[t] = 0;
+    if (tid == 0) n_few = 0;
+    __syncthreads();
+    const u16x2 first2{(unsigned short)first, (unsigned short)first}, cap2{(unsigned short)cap, (unsigned short)cap};
+    uint32_t n_in = 0, zeros = 0;                            // n_in: of the wave; its first lane has all of it
+    auto add = [&](const uint32_t t4, const uint32_t sign) {
+        const bool in = t4 < 4 * cap;
+        n_in += (uint32_t)__popcll(__ballot(in));
+        if (in) atomicAdd((uint32_t *)((char *)sh.values + t4), sign ? 0x10000u : 1u);
+    };
+    auto add_few = [&](const uint32_t bits) {
+        if ((bits & 0x7fff) == 0) ++zeros;
+        else {
+            const uint32_t at = atomicAdd(&n_few, 1u);
+            if (at < (uint32_t)FEW) few[at] = (unsigned short)bits;
+        }
+    };
+    each_quad<G>(view, 0, view.n_chunks, [&](const row_u32x4 (&v)[4], const int32_t) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            u16x2 least = cap2;
+#pragma unroll
+            for (int d = 0; d < 4; ++d) {
+                const uint32_t w = v[k][d];
+                const u16x2 t = __builtin_elementwise_min(
+                    __builtin_elementwise_sub_sat(__builtin_bit_cast(u16x2, w & 0x7fff7fffu), first2), cap2);
+                least = __builtin_elementwise_min(least, t);
+                const uint32_t t4 = __builtin_bit_cast(uint32_t, (u16x2)(t << (unsigned short)2));
+                add(t4 & 0xffffu, w & 0x8000u);
+                add(t4 >> 16, w & 0x80000000u);
+            }
+            if (first != 0 && (least[0] == 0 || least[1] == 0)) {
+#pragma unroll
+                for (int d = 0; d < 4; ++d) {
+                    const uint32_t w = v[k][d];
+                    if ((w & 0x7fffu) <= first) add_few(w & 0xffffu);
+                    if ((w >> 16 & 0x7fffu) <= first) add_few(w >> 16);
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        return true;
+    });
+    __syncthreads();
+    auto put = [&](const float s, const uint32_t n) {        // n items of score s
+        const uint32_t b = bucket_of<G::BUCKETS>(s, c);
+        u64 w;
+        if (weigh(s, c, sh.pow2, w) && b < (uint32_t)G::BUCKETS) {
+            atomicAdd(&sh.wsum[b], w * n);
+            if (counted) atomicAdd(&sh.cnt[b], n);
+        }
+    };
+    uint32_t sum = lane == 0 ? 0u - n_in : 0u;
+#pragma unroll 1
+    for (uint32_t t = tid; t < cap; t += 2 * G::THREADS) {   // two words, four values, at a time
+        const uint32_t t1 = t + G::THREADS;
+        uint32_t n0 = sh.values[t], n1 = t1 < cap ? sh.values[t1] : 0;
+        sum += (n0 & 0xffffu) + (n0 >> 16) + (n1 & 0xffffu) + (n1 >> 16);
+        if (t == 0 && first != 0) n0 = 0;
+        if ((n0 | n1) == 0) continue;
+        const float s0 = value_of(first + t), s1 = value_of(first + t1);
+        const float s[4] = {s0, -s0, s1, -s1};
+        const uint32_t n[4] = {n0 & 0xffffu, n0 >> 16, n1 & 0xffffu, n1 >> 16};
+        u64 w[4];
+        bool in[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) in[q] = weigh(s[q], c, sh.pow2, w[q]);
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const uint32_t b = bucket_of<G::BUCKETS>(s[q], c);
+            if (in[q] && n[q] && b < (uint32_t)G::BUCKETS) {
+                atomicAdd(&sh.wsum[b], w[q] * n[q]);
+                if (counted) atomicAdd(&sh.cnt[b], n[q]);
+            }
+        }
+    }
+    if (zeros) put(0.f, zeros);
+    const uint32_t n = n_few;
+    for (uint32_t q = tid; q < min(n, (uint32_t)FEW); q += G::THREADS) put(value_of(few[q]), 1);
+    {
+        const int32_t x = view.extra(tid);
+        if (x >= 0) put(view.at(x), 1);
+    }
+    sum = wave_scan(sum);
+    __syncthreads();
+    if (lane == 63) sh.wave_c[wave] = sum;
+    __syncthreads();
+    return sum_of_first<G>(sh.wave_c, G::WAVES) == 0 && n <= (uint32_t)FEW;
+}
+
 // ----------------------------------------------------------------------------- one workgroup per row
 template <class G, int TYPE>
 __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const SampleArgs a) {
-    constexpr int LISTED = 2048;                            // items collected in LDS
     __shared__ SampleShared<G> sh;
-    __shared__ Found found[LISTED];
     __shared__ uint32_t want[G::BUCKETS / 32 + 1], n_found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t r = row_of_block();
@@ -808,7 +928,7 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
                 if (taken[q] == 0) continue;                 // uniform: most of them in a filtered row
                 const float s = RowView<TYPE>::value(v[half * CHUNKS + q / VEC], q % VEC);
                 const uint32_t at = base + __builtin_amdgcn_mbcnt_hi((uint32_t)(taken[q] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)taken[q], 0u));
-                if (wanted(s) && at < (uint32_t)LISTED) found[at] = Found{s, i0 + (half * CHUNKS + q / VEC) * STEP + q % VEC};
+                if (wanted(s) && at < (uint32_t)LISTED) sh.found[at] = Found{s, i0 + (half * CHUNKS + q / VEC) * STEP + q % VEC};
                 base += (uint32_t)__popcll(taken[q]);
             }
             go = go && base <= (uint32_t)LISTED;
@@ -817,7 +937,7 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
     };
     auto collect_one = [&](const float s, const int32_t i) {
         const uint32_t at = atomicAdd(&n_found, 1u);
-        if (at < (uint32_t)LISTED) found[at] = Found{s, i};
+        if (at < (uint32_t)LISTED) sh.found[at] = Found{s, i};
     };
     float hi = -__builtin_inff(), low = __builtin_inff();     // low: of the first chunks, it only sets the buckets' width
     auto top_of = [&](const row_u32x4 (&v)[4]) {
@@ -926,7 +1046,7 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
         const uint32_t n = n_found;
 #pragma unroll 1
         for (uint32_t q = tid; q < n; q += G::THREADS) {
-            const float s = found[q].score;
+            const float s = sh.found[q].score;
             const uint32_t b = bucket_of<G::BUCKETS>(s, c);
             u64 w;
             if (weigh(s, c, sh.pow2, w)) {
@@ -947,10 +1067,24 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
     }
     if (!fits) {
         // a row of which much counts: weighed as it is read; one more pass collects whatever the answers can be
-        each_bucket<G>(view, 0, view.n_chunks, true, c, [&](const float (&s)[4], const int32_t, const uint32_t (&b)[4]) {
-            count_four<G::BUCKETS>(s, b, c, sh.pow2, sh.cnt, sh.wsum, counted);
-            return true;
-        });
+        bool weighed = false;
+        if constexpr (TYPE != ROW_F32 && G::BY_VALUE) {
+            // bfloat16 has few values in any row of this group (161 against 182 us at 33 001 items); float16 eight times as
+            // many, worth it from about 80 000 items on (257 against 279 us at 131 071, but 292 against 276 at 65 535)
+            const bool by_value = TYPE == ROW_BF16 || view.M >= 81920;
+            if (by_value) weighed = count_values<G>(view, c, reach, counted, sh);
+            if (by_value && !weighed) {
+                __syncthreads();
+#pragma unroll
+                for (int q = 0; q < G::OWN; ++q) { sh.cnt[q * G::THREADS + tid] = 0; sh.wsum[q * G::THREADS + tid] = 0; }
+                __syncthreads();
+            }
+        }
+        if (!weighed)
+            each_bucket<G>(view, 0, view.n_chunks, true, c, [&](const float (&s)[4], const int32_t, const uint32_t (&b)[4]) {
+                count_four<G::BUCKETS>(s, b, c, sh.pow2, sh.cnt, sh.wsum, counted);
+                return true;
+            });
         __syncthreads();
         scan_buckets(sh.cnt, sh.wsum, sh);
         wanted_buckets(a, r, p, sh, want);
@@ -966,7 +1100,7 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
         __syncthreads();
     }
     const bool whole = n_found > (uint32_t)LISTED;           // more than the list holds: the answers come from memory
-    ListedRow<G, TYPE> list{view, found, n_found, whole};
+    ListedRow<G, TYPE> list{view, sh.found, n_found, whole};
     answer<G>(a, r, list, !whole, counted, view, c, p, sh);
 }
 
@@ -1121,14 +1255,12 @@ __global__ __launch_bounds__(G::THREADS) void part_answer_kernel(const SampleArg
     const RowScale c = row_scale(hi, st.low, item_cut(p, a.q_bits), p, a.q_bits, G::BUCKETS);
     load_histogram(a, r, sh);
     const uint32_t n = a.n_found[r];
-    constexpr uint32_t IN_LDS = 2048;                        // (read once per step and round)
-    __shared__ Found found[IN_LDS];
-    const bool in_lds = n <= IN_LDS;
+    const bool in_lds = n <= (uint32_t)LISTED;                // it is read once per step and round
     if (in_lds) {
-        for (uint32_t q = threadIdx.x; q < n; q += G::THREADS) found[q] = a.found[r * SR_LISTED + q];
+        for (uint32_t q = threadIdx.x; q < n; q += G::THREADS) sh.found[q] = a.found[r * SR_LISTED + q];
         __syncthreads();
     }
-    ListedRow<G, TYPE> row{view, in_lds ? found : a.found + r * SR_LISTED, n, n > SR_LISTED};      // more than the list holds: from memory
+    ListedRow<G, TYPE> row{view, in_lds ? sh.found : a.found + r * SR_LISTED, n, n > SR_LISTED};      // more than the list holds: from memory
     answer<G>(a, r, row, in_lds, true, view, c, p, sh);
 }
 

@@ -306,3 +306,21 @@ def test_more_draws_than_are_taken(ops):
 def test_a_thousand_draws_of_a_row(ops):
     rng = np.random.default_rng(32)
     check(ops, scores(rng, 2, 5000, "f32"), torch.from_numpy(rng.random((2, 1000))).cuda(), T=2.0, p=0.95)
+
+
+@pytest.mark.parametrize("dtype", ["f16", "bf16"])
+@pytest.mark.parametrize("M", [30011, 131071])
+def test_16_bit_rows_counted_by_value(ops, dtype, M):
+    """Rows of which much counts: few values, one value more often than 16 bits count, zeros of both signs, magnitudes too
+    small for the table of values, more of them than their list takes, masks, only negative scores, one binade."""
+    rng = np.random.default_rng(M)
+    base = rng.normal(size=M).astype(np.float32)
+    rows = [base, np.where(rng.random(M) < 0.7, 1.0, base), np.where(rng.random(M) < 0.5, -np.inf, base),
+            np.where(rng.random(M) < 0.02, np.where(rng.random(M) < 0.5, 0.0, -0.0), base),
+            np.where(rng.random(M) < 0.005, base * 2.0 ** -12, base), np.where(rng.random(M) < 0.3, base * 2.0 ** -12, base),
+            -np.abs(base) - 0.25, 1.0 + rng.random(M) * 0.5, np.where(rng.random(M) < 0.6, 0.0, base),
+            np.where(rng.random(M) < 0.3, -65504.0, base), np.full(M, 0.5), base * 1000.0, base * 2.0 ** -14]
+    S = torch.from_numpy(np.stack(rows).astype(np.float32)).cuda().to(TYPES[dtype])
+    u = torch.from_numpy(rng.random((len(rows), 5))).cuda()
+    for kw in (dict(T=0.5), dict(T=3.0, p=0.7), dict(T=0.5, k=M // 2), dict(T=1e30), dict(T=0.01, p=0.999)):
+        check(ops, S, u, **kw)
