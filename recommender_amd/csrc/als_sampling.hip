@@ -48,9 +48,10 @@ template <int T, int B>
 struct Group {
     static constexpr int THREADS = T, WAVES = T / 64, BUCKETS = B;
     static constexpr int OWN = B / T;             // buckets per thread
+    static constexpr int EDGE = B / 100 + 1;      // bucket_of takes scores 1 % beyond the last bucket's width into it
     static constexpr bool BY_VALUE = T > 256;     // 16-bit rows: see count_values
     static constexpr int RANKED = T / 4;          // items that are ranked against each other directly, four threads each
-    static constexpr int WAVE_ITEMS = T / 4;      // ... by one wave
+    static constexpr int WAVE_ITEMS = T > 256 ? 192 : 64;      // ... by one wave
 };
 typedef Group<256, 512> Small;
 typedef Group<512, 2048> Large;
@@ -550,9 +551,15 @@ __device__ __forceinline__ bool wave_find(const Found *list, const uint32_t n, c
     if (m > (uint32_t)G::WAVE_ITEMS) return false;
     __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
     __builtin_amdgcn_wave_barrier();
-#pragma unroll 1
-    for (uint32_t e0 = 0; e0 < m; e0 += 64) {
-        const uint32_t e = e0 + lane < m ? e0 + lane : m - 1;
+    auto of_lane = [&](const u64 v, const int from) {
+        return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), from) << 32 |
+               (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, from);
+    };
+    auto picked = [&](const u64 before, const u64 w, const u64 key) {
+        return Picked{before, w, (int32_t)~(uint32_t)key, key_score((uint32_t)(key >> 32))};
+    };
+    if (m <= 64) {                                           // each against all
+        const uint32_t e = (uint32_t)lane < m ? (uint32_t)lane : m - 1;
         const u64 own = items[e][0], w = items[e][1];
         u64 before = base_w;
         uint32_t rank = base_c;
@@ -560,15 +567,62 @@ __device__ __forceinline__ bool wave_find(const Found *list, const uint32_t n, c
         for (uint32_t q = 0; q < m; ++q)
             if (items[q][0] > own) { before += items[q][1]; ++rank; }
         const u64 found = __ballot(by_count ? rank == target : before <= target && target < before + w);
-        if (found == 0) continue;
+        if (found == 0) return false;
         const int from = __ffsll(found) - 1;
-        auto lane64 = [&](const u64 v) {
-            return (u64)(uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(v >> 32), from) << 32 |
-                   (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)v, from);
-        };
-        const u64 key = lane64(own);
-        out = Picked{lane64(before), lane64(w), (int32_t)~(uint32_t)key, key_score((uint32_t)(key >> 32))};
+        out = picked(of_lane(before, from), of_lane(w, from), of_lane(own, from));
         return true;
+    }
+    if constexpr (G::WAVE_ITEMS > 64) {                      // halving what is in question by one of its items, about ten times
+        constexpr int SLOTS = G::WAVE_ITEMS / 64;
+        u64 key[SLOTS], w[SLOTS];
+        bool in[SLOTS];
+#pragma unroll
+        for (int k = 0; k < SLOTS; ++k) {
+            const uint32_t e = lane + 64 * k;
+            in[k] = e < m;
+            key[k] = items[in[k] ? e : 0][0]; w[k] = items[in[k] ? e : 0][1];
+        }
+        u64 before = base_w;
+        uint32_t rank = base_c;
+        for (uint32_t round = 1; round <= m; ++round) {      // a round takes one item out at least
+            u64 pivot = 0, pivot_w = 0;
+            bool have = false;
+#pragma unroll
+            for (int k = 0; k < SLOTS; ++k) {                // any item: the list is in no order that matters, but not shuffled
+                const u64 mask = __ballot(in[k]);
+                if (mask == 0 || (have && (round + k) % 2)) continue;
+                const uint32_t turn = 37 * round & 63;
+                const u64 turned = mask >> turn | mask << (64 - turn & 63);
+                const int from = (int)((__ffsll(turned) - 1 + turn) & 63);
+                pivot = of_lane(key[k], from); pivot_w = of_lane(w[k], from);
+                have = true;
+            }
+            if (!have) return false;
+            u64 front_w = 0;
+            uint32_t front_c = 0;
+#pragma unroll
+            for (int k = 0; k < SLOTS; ++k) {
+                const bool front = in[k] && key[k] > pivot;
+                front_w += front ? w[k] : 0;
+                front_c += (uint32_t)__popcll(__ballot(front));
+            }
+            front_w = of_lane(wave_scan(front_w), 63);
+            if (by_count ? target < rank + front_c : target < before + front_w) {
+#pragma unroll
+                for (int k = 0; k < SLOTS; ++k) in[k] = in[k] && key[k] > pivot;
+                continue;
+            }
+            before += front_w;
+            rank += front_c;
+            if (by_count ? target == rank : target < before + pivot_w) {
+                out = picked(before, pivot_w, pivot);
+                return true;
+            }
+            before += pivot_w;
+            rank += 1;
+#pragma unroll
+            for (int k = 0; k < SLOTS; ++k) in[k] = in[k] && key[k] < pivot;
+        }
     }
     return false;
 }
@@ -618,17 +672,16 @@ __device__ __forceinline__ void buckets_passing(const V *sums, const u64 t0, con
     b0 = uniform((int32_t)sh.k_lo); b1 = uniform((int32_t)sh.k_hi);
     __syncthreads();
 }
-// The buckets the answers can lie in, as bits: top-k's is known; what it leaves of the weight, and so top-p's target, is
+// The buckets the answers can lie in, a byte each: top-k's is known; what it leaves of the weight, and so top-p's target, is
 // known to within that bucket, and so on.
 template <class G>
-__device__ __forceinline__ void wanted_buckets(const SampleArgs &a, const int64_t r, const RowParams &p, SampleShared<G> &sh,
-                                   uint32_t (&want)[G::BUCKETS / 32 + 1]) {
+__device__ __forceinline__ void wanted_buckets(const SampleArgs &a, const int64_t r, const RowParams &p, const bool open_end, SampleShared<G> &sh,
+                                               unsigned char (&want)[G::BUCKETS + G::EDGE + 1]) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     // ranges of buckets, +1 where one begins and -1 behind its end: the running sum is the number of ranges over a bucket
     uint32_t *edge = sh.csub;
 #pragma unroll
     for (int q = 0; q < G::OWN; ++q) edge[G::OWN * tid + q] = 0;
-    if (tid <= G::BUCKETS / 32) want[tid] = 0;              // one word more: "no bucket" is not wanted either
     __syncthreads();
     auto mark = [&](const int b0, const int b1) {
         atomicAdd(&edge[b0], 1u);
@@ -666,11 +719,11 @@ __device__ __forceinline__ void wanted_buckets(const SampleArgs &a, const int64_
     if (lane == 63) sh.wave_c[wave] = front;
     __syncthreads();
     front += sum_of_first<G>(sh.wave_c, wave) - sum;
-    uint32_t bits = 0;
 #pragma unroll
-    for (int q = 0; q < G::OWN; ++q)
-        if (front + own[q]) bits |= 1u << q;
-    if (bits) atomicOr(&want[G::OWN * tid / 32], bits << (G::OWN * tid & 31));
+    for (int q = 0; q < G::OWN; ++q) want[G::OWN * tid + q] = front + own[q] != 0;
+    // behind them scores beyond the last bucket's width, which bucket_of may take into it: EDGE widths, and all the rest
+    if (tid == G::THREADS - 1)
+        for (int q = 0; q <= G::EDGE; ++q) want[G::BUCKETS + q] = front + own[G::OWN - 1] != 0 && (q < G::EDGE || open_end);
     __syncthreads();
 }
 
@@ -885,7 +938,8 @@ __device__ __forceinline__ bool count_values(const RowView<TYPE> &view, const Ro
 template <class G, int TYPE>
 __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const SampleArgs a) {
     __shared__ SampleShared<G> sh;
-    __shared__ uint32_t want[G::BUCKETS / 32 + 1], n_found;
+    __shared__ unsigned char want[G::BUCKETS + G::EDGE + 1];
+    __shared__ uint32_t n_found;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int64_t r = row_of_block();
     if (r >= a.n) return;
@@ -968,12 +1022,14 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
     const float reach = score_reach(cut, p.T) * 1.0001f;        // items further below the top do not count
     float at_least = -__builtin_inff();                                        // top-k: a score to start from
     const bool counted = top_k_asked(a, p), drawn = p.T > 0.f;
+    constexpr int AHEAD = TYPE == ROW_F32 ? 2 : 1;           // quads under way (4096 x 59047 f32: 234 us, 238 with one; 16-bit: spills)
     {
-        row_u32x4 v[4], next[4];
+        row_u32x4 v[4], next[AHEAD][4];
         load_quad(v, tid);
         const int32_t x = view.extra(tid);
         const float x_score = x >= 0 ? view.at(x) : -__builtin_inff();
-        load_quad(next, tid + 4 * G::THREADS);
+#pragma unroll
+        for (int d = 0; d < AHEAD; ++d) load_quad(next[d], tid + 4 * (d + 1) * G::THREADS);
         top_of(v);
         hi = fmaxf(hi, x_score);
 #pragma unroll
@@ -1015,8 +1071,12 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
 #pragma unroll 1
         for (int32_t q = tid + 4 * G::THREADS; q - tid < view.n_chunks; q += 4 * G::THREADS) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) v[k] = next[k];
-            load_quad(next, q + 4 * G::THREADS);
+            for (int k = 0; k < 4; ++k) {
+                v[k] = next[0][k];
+#pragma unroll
+                for (int d = 0; d + 1 < AHEAD; ++d) next[d][k] = next[d + 1][k];
+            }
+            load_quad(next[AHEAD - 1], q + 4 * AHEAD * G::THREADS);
             top_of(v);
             if (collecting) {                                // per wave
                 floor = fmaxf(floor, hi - reach);            // the lane's own maximum: never above the row's
@@ -1087,12 +1147,12 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
             });
         __syncthreads();
         scan_buckets(sh.cnt, sh.wsum, sh);
-        wanted_buckets(a, r, p, sh, want);
+        wanted_buckets(a, r, p, c.reject > (float)G::BUCKETS * 1.02f, sh, want);
         if (tid == 0) n_found = 0;
         __syncthreads();
         auto wanted = [&](const float s) {
-            const uint32_t b = bucket_of<G::BUCKETS>(s, c);
-            return (want[b >> 5] >> (b & 31) & 1u) != 0;
+            // bucket_of without the cut: an item beyond it is in the list for nothing
+            return want[(uint32_t)fminf((c.top_f - s) * c.per_score, (float)(G::BUCKETS + G::EDGE))] != 0;
         };
         each_quad<G>(view, 0, view.n_chunks, [&](const row_u32x4 (&v)[4], const int32_t i0) { return collect(v, i0, wanted); });
         const int32_t x = view.extra(tid);
@@ -1207,7 +1267,7 @@ __device__ __forceinline__ void load_histogram(const SampleArgs &a, const int64_
 template <int TYPE>
 __global__ __launch_bounds__(G::THREADS) void part_collect_kernel(const SampleArgs a) {
     __shared__ SampleShared<G> sh;
-    __shared__ uint32_t want[G::BUCKETS / 32 + 1];
+    __shared__ unsigned char want[G::BUCKETS + G::EDGE + 1];
     const int64_t r = blockIdx.x / a.n_parts;
     const int part = blockIdx.x % a.n_parts;
     const RowParams p = row_params(a, r);
@@ -1216,13 +1276,13 @@ __global__ __launch_bounds__(G::THREADS) void part_collect_kernel(const SampleAr
     if (!(fabsf(hi) < __builtin_inff()) || !(p.T > 0.f)) return;      // answered apart
     const RowScale c = row_scale(hi, st.low, item_cut(p, a.q_bits), p, a.q_bits, G::BUCKETS);
     load_histogram(a, r, sh);
-    wanted_buckets(a, r, p, sh, want);
+    wanted_buckets(a, r, p, false, sh, want);
     const RowView<TYPE> view(a.scores, r, a.lds, a.M);
     const int32_t q0 = part * a.per_part, q1 = min(q0 + a.per_part, view.n_chunks);
     each_bucket<G>(view, q0, q1, part == 0, c, [&](const float (&s)[4], const int32_t i, const uint32_t (&b)[4]) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
-            if (!(want[b[q] >> 5] >> (b[q] & 31) & 1u)) continue;
+            if (b[q] >= (uint32_t)G::BUCKETS || !want[b[q]]) continue;
             const uint32_t at = atomicAdd(&a.n_found[r], 1u);
             if (at < SR_LISTED) a.found[r * SR_LISTED + at] = Found{s[q], i + q};
         }
