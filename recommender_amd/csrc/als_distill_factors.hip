@@ -311,6 +311,11 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         }
     };
 
+    // under way while the rest is set up (F = 128: 365 us, 420 with the copies below; pass 2 gets slower by as much, 430 and 474)
+    if constexpr (!BACK) {
+#pragma unroll
+        for (int q = 0; q < RING - 1; ++q) copy(t0 + q, q);
+    }
     u32x4 BH[KS], BL[KS];
     {
         const u32x4 *src = reinterpret_cast<const u32x4 *>(stat + (active ? tile : 0) * (F * 256)) + lane;
@@ -366,14 +371,16 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
     };
 
     if constexpr (BACK) {
-        for (int q = tid; q < TBUF * WAVES * 32 * T_STRIDE; q += WAVES * 64) t_tile[q] = 0.f;
+        for (int q = tid; q < TBUF * WAVES * 32 * T_STRIDE / 4; q += WAVES * 64) reinterpret_cast<f32x4 *>(t_tile)[q] = f32x4{0.f, 0.f, 0.f, 0.f};
         __syncthreads();
         now = fetch(t0);
         place(t0, 0);
         now = fetch(t0 + 1);
     }
+    if constexpr (BACK) {
 #pragma unroll
-    for (int q = 0; q < RING - 1; ++q) copy(t0 + q, q);
+        for (int q = 0; q < RING - 1; ++q) copy(t0 + q, q);
+    }
     int slot = 0;
     for (int64_t t = t0; t < t1; ++t) {
         // this wave's copies of tile t have landed (behind them it issued RING - 2 further tiles, and maybe list loads, which
