@@ -261,10 +261,11 @@ __device__ __forceinline__ f32x16 mfma32(const u32x4 &a, const u32x4 &b, const f
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
 // Two float32 values as fp16 pairs of both pieces.  Toward zero: the rest is exact and of one sign.
-__device__ __forceinline__ void cut_pair(const float p0, const float p1, unsigned &hi, unsigned &lo) {
+// minus_one: -1 in a register that the compiler does not look into, so that p - h is one instruction which reads h as it lies.
+__device__ __forceinline__ void cut_pair(const float p0, const float p1, const float minus_one, unsigned &hi, unsigned &lo) {
     const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
     hi = __builtin_bit_cast(unsigned, h);
-    const auto l = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], -1.f, p0), __builtin_fmaf((float)h[1], -1.f, p1));
+    const auto l = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], minus_one, p0), __builtin_fmaf((float)h[1], minus_one, p1));
     lo = __builtin_bit_cast(unsigned, l);
 }
 
@@ -321,6 +322,9 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         const u32x4 *src = reinterpret_cast<const u32x4 *>(stat + (active ? tile : 0) * (F * 256)) + lane;
 #pragma unroll
         for (int s = 0; s < KS; ++s) { BH[s] = src[(2 * s) * 64]; BL[s] = src[(2 * s + 1) * 64]; }
+        // waited for here: in the loop their waits would also wait, every time, for the copies under way
+#pragma unroll
+        for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(BH[s]), "+v"(BL[s]));
     }
     f32x16 O[FT];
 #pragma unroll
@@ -329,6 +333,8 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         for (int r = 0; r < 16; ++r) O[q][r] = 0.f;
     const float k = a.scales[0];
     float m = -__builtin_inff(), z = 0.f;
+    float minus_one = -1.f;
+    asm volatile("" : "+s"(minus_one));
 
     // ---- pass 2: the lists of the streaming users, as a dense tile [item of the block, user of the stage] that is zero but
     // for the listed pairs.  LPR lanes of one wave own a user's row in both buffers: they clear what the stage before last
@@ -409,9 +415,11 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         unsigned PH[8], PL[8];
         if constexpr (!BACK) {
             if ((t + 1) * TILE > a.M) {                  // the last tile's padding rows
+                const int rows = (int)(a.M - t * TILE) - 4 * h;
+                asm volatile("" ::: "memory");           // stays a branch: taken into the loop, it is 48 instructions a tile
 #pragma unroll
                 for (int r = 0; r < 16; ++r)
-                    if (t * TILE + 8 * (r / 4) + 4 * h + r % 4 >= a.M) S[r] = -__builtin_inff();
+                    if (8 * (r / 4) + r % 4 >= rows) S[r] = -__builtin_inff();
             }
             float top = S[0];
 #pragma unroll
@@ -433,7 +441,7 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
             for (int r = 0; r < 16; r += 2) {
                 const float p0 = exp2_fast(__builtin_fmaf(S[r], k, c)), p1 = exp2_fast(__builtin_fmaf(S[r + 1], k, c));
                 z += p0 + p1;
-                cut_pair(p0, p1, PH[r / 2], PL[r / 2]);
+                cut_pair(p0, p1, minus_one, PH[r / 2], PL[r / 2]);
             }
         } else {
             const f32x4 *tt = reinterpret_cast<const f32x4 *>(t_tile + buf * (WAVES * 32 * T_STRIDE) + (wave * 32 + j) * T_STRIDE) + h;
@@ -445,7 +453,7 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
                 for (int e = 0; e < 4; e += 2) {
                     const float p0 = exp2_fast(__builtin_fmaf(S[4 * g + e], k, -bv[e])) - tv[e];
                     const float p1 = exp2_fast(__builtin_fmaf(S[4 * g + e + 1], k, -bv[e + 1])) - tv[e + 1];
-                    cut_pair(p0, p1, PH[2 * g + e / 2], PL[2 * g + e / 2]);
+                    cut_pair(p0, p1, minus_one, PH[2 * g + e / 2], PL[2 * g + e / 2]);
                 }
             }
         }
