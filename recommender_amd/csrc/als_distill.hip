@@ -123,8 +123,10 @@ __device__ __forceinline__ float loss_term(const float t, const float s, const f
 }
 
 // Chunk q of the gradient row.  Its address has the alignment of the type only where scores and gradient lie differently.
+// STREAM: past the caches, which keep the scores instead.
 struct __attribute__((packed, aligned(2))) Chunk16 { row_u32x4 v; };
-template <int TYPE>
+typedef unsigned loose_u32x4 __attribute__((ext_vector_type(4), aligned(2)));
+template <int TYPE, bool STREAM>
 __device__ __forceinline__ void put_chunk(char *out, const RowView<TYPE> &view, const int32_t q, const float (&g)[8]) {
     Chunk16 c;
 #pragma unroll
@@ -132,7 +134,9 @@ __device__ __forceinline__ void put_chunk(char *out, const RowView<TYPE> &view, 
         if constexpr (TYPE == ROW_F32) c.v[e] = __float_as_uint(g[e]);
         else c.v[e] = RowView<TYPE>::narrow(g[2 * e]) | RowView<TYPE>::narrow(g[2 * e + 1]) << 16;
     }
-    *reinterpret_cast<Chunk16 *>(out + (int64_t)view.index0(q) * RowView<TYPE>::BYTES) = c;
+    char *at = out + (int64_t)view.index0(q) * RowView<TYPE>::BYTES;
+    if constexpr (STREAM) __builtin_nontemporal_store((loose_u32x4)c.v, reinterpret_cast<loose_u32x4 *>(at));
+    else *reinterpret_cast<Chunk16 *>(at) = c;
 }
 
 // A part of a row - NV chunks per thread from chunk q0 on, in registers - and this thread's element outside the body.
@@ -187,6 +191,7 @@ struct RowPart {
         }
         return z;
     }
+    template <bool STREAM>
     __device__ __forceinline__ void put_slopes(char *out, const RowView<TYPE> &view, const int32_t q0, const float m, const float c2,
                                                const float cq, const bool any) {
         pin();
@@ -197,7 +202,7 @@ struct RowPart {
                 float g[8];
 #pragma unroll
                 for (int e = 0; e < VEC; ++e) g[e] = any ? cq * exp2_fast((RowView<TYPE>::value(held[q], e) - m) * c2) : 0.f;
-                put_chunk<TYPE>(out, view, at, g);
+                put_chunk<TYPE, STREAM>(out, view, at, g);
             }
             __builtin_amdgcn_sched_barrier(0);
         }
@@ -239,7 +244,7 @@ __global__ __launch_bounds__(DR_THREADS, NV <= 8 ? 8 : 4) void distill_rows_kern
     const RowScale c = row_scale(a, r, z, block_max(item >= 0 ? 1.f : 0.f, sh) > 0.f);
     if (threadIdx.x == 0) a.loss[r] = c.any ? (float)loss : 0.f;
     char *out = (char *)a.grad + r * a.ldg * RowView<TYPE>::BYTES;
-    part.put_slopes(out, view, 0, top, c2, c.cq, c.any);
+    part.template put_slopes<false>(out, view, 0, top, c2, c.cq, c.any);
     __syncthreads();
     if (item >= 0) RowView<TYPE>::put(out, item, c.scale * (exp2_fast((s_item - top) * c2) * c.inv_z - t));
 }
@@ -270,8 +275,12 @@ __global__ __launch_bounds__(DR_THREADS, 8) void distill_slopes_kernel(const Row
                                                                     const PartStat *__restrict__ stats,
                                                                     const float *__restrict__ listed) {
     __shared__ ListShared sh;
-    const int64_t r = blockIdx.x / n_parts;
-    const int part_no = blockIdx.x % n_parts;
+    // Backwards, and the gradient past the caches: what the launch before read last may be in the last-level cache still
+    // (61 x 1000003 float32: 124 us, 150 without the second, 153 without either; in the form of one launch, which reads
+    // nothing twice, streaming stores cost float32 rows 3 %).
+    const unsigned w = gridDim.x - 1 - blockIdx.x;
+    const int64_t r = w / n_parts;
+    const int part_no = w % n_parts;
     const RowView<TYPE> view(a.scores, r, a.lds, a.M);
     RowPart<TYPE, DR_PART_NV> part;
     const int32_t q0 = part_no * DR_PART_NV * DR_THREADS;
@@ -297,7 +306,7 @@ __global__ __launch_bounds__(DR_THREADS, 8) void distill_slopes_kernel(const Row
     }
     char *out = (char *)a.grad + r * a.ldg * RowView<TYPE>::BYTES;
     part.load(view, q0, part_no == 0);          // not earlier: two workgroups per unit overlap, and their registers do not spill
-    part.put_slopes(out, view, q0, top, c2, c.cq, c.any);
+    part.template put_slopes<true>(out, view, q0, top, c2, c.cq, c.any);
     __syncthreads();
     // the listed items of this part
     if (item >= 0) {
