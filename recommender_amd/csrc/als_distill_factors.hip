@@ -190,18 +190,9 @@ __global__ __launch_bounds__(256) void prepare_kernel(const FactorArgs a) {
     const bool is_y = blockIdx.x < a.m_tiles;
     const int64_t T = is_y ? blockIdx.x : blockIdx.x - a.m_tiles;
     const int64_t rows = is_y ? a.M : a.n;
-    float my = 0.f;
-    for (int q = tid; q < Y_MAX_BLOCKS; q += 256) my = fmaxf(my, a.maxima[q]);
-    my = block_max256(my, red);
-    const float mx = block_max256(a.maxima[Y_MAX_BLOCKS + tid], red);             // X_MAX_BLOCKS = 256
-    const float mc = block_max256(a.maxima[Y_MAX_BLOCKS + X_MAX_BLOCKS + tid], red);
-    const float to_log2 = a.inv_t * 1.44269504f;
-    const float sy = op_scale(my).s, sx = op_scale(mx * to_log2).s, sc = op_scale(mc).s;
-    if (blockIdx.x == 0 && tid == 0) {
-        a.scales[0] = 1.f / (sx * sy);
-        a.scales[1] = 1.f / sy;
-        a.scales[2] = exp2f(-Q_OFFSET) / sc;
-    }
+    float my = 0.f, mx = a.maxima[Y_MAX_BLOCKS + tid], mc = a.maxima[Y_MAX_BLOCKS + X_MAX_BLOCKS + tid];      // X_MAX_BLOCKS = 256
+#pragma unroll
+    for (int q = 0; q < Y_MAX_BLOCKS; q += 256) my = fmaxf(my, a.maxima[q + tid]);
     for (int q = tid; q < TILE * F; q += 256) {
         const int i = q / F, k = q % F;
         const int64_t r = T * TILE + i;
@@ -218,7 +209,16 @@ __global__ __launch_bounds__(256) void prepare_kernel(const FactorArgs a) {
         }
         cs[tid] = c;
     }
-    __syncthreads();
+    my = block_max256(my, red);                          // the first of them waits for the tile as well
+    mx = block_max256(mx, red);
+    mc = block_max256(mc, red);
+    const float to_log2 = a.inv_t * 1.44269504f;
+    const float sy = op_scale(my).s, sx = op_scale(mx * to_log2).s, sc = op_scale(mc).s;
+    if (blockIdx.x == 0 && tid == 0) {
+        a.scales[0] = 1.f / (sx * sy);
+        a.scales[1] = 1.f / sy;
+        a.scales[2] = exp2f(-Q_OFFSET) / sc;
+    }
     char *out = (is_y ? a.yt : a.xt) + T * (F * 256);
     const float s_row = is_y ? sy : sx, m_row = is_y ? 1.f : to_log2, s_tr = is_y ? sy : sc;
     for (int q = tid; q < KS * 64; q += 256) {

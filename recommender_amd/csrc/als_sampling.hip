@@ -243,6 +243,22 @@ __device__ __forceinline__ V wave_scan(V v) {
     return v;
 }
 
+// The wave's largest `hi` (returned) and smallest `low`, in lane 63.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ float moved(const float v, const float none) {
+    return __uint_as_float((uint32_t)__builtin_amdgcn_update_dpp((int)__float_as_uint(none), (int)__float_as_uint(v), CTRL, ROWS, 0xf, false));
+}
+__device__ __forceinline__ float wave_ends(float hi, float &low) {
+    const float inf = __builtin_inff();
+    hi = fmaxf(hi, moved<0x111, 0xf>(hi, -inf)); low = fminf(low, moved<0x111, 0xf>(low, inf));
+    hi = fmaxf(hi, moved<0x112, 0xf>(hi, -inf)); low = fminf(low, moved<0x112, 0xf>(low, inf));
+    hi = fmaxf(hi, moved<0x114, 0xf>(hi, -inf)); low = fminf(low, moved<0x114, 0xf>(low, inf));
+    hi = fmaxf(hi, moved<0x118, 0xf>(hi, -inf)); low = fminf(low, moved<0x118, 0xf>(low, inf));
+    hi = fmaxf(hi, moved<0x142, 0xa>(hi, -inf)); low = fminf(low, moved<0x142, 0xa>(low, inf));
+    hi = fmaxf(hi, moved<0x143, 0xc>(hi, -inf)); low = fminf(low, moved<0x143, 0xc>(low, inf));
+    return hi;
+}
+
 // Sum of the first `n` of the per-wave values: a lane loads one each (a loop over them costs its unrolled registers).
 template <class G, class V>
 __device__ __forceinline__ V sum_of_first(const V *v, const int n) {
@@ -328,20 +344,25 @@ __device__ __forceinline__ void count_four(const float (&s)[4], const uint32_t (
 }
 
 // Read from memory, four chunks in flight per thread: f(chunk, column of its first element), false to stop the wave's walk.
-template <class G, int TYPE, class F>
-__device__ __forceinline__ void each_chunk(const RowView<TYPE> &view, const int32_t q0, const int32_t q1, F f) {
-#pragma unroll 1
-    for (int32_t q = q0 + threadIdx.x; q < q1; q += 4 * G::THREADS) {
-        row_u32x4 v[4];
+// v: the thread's first four, which the caller has loaded (load_four).
+template <class G, int TYPE>
+__device__ __forceinline__ void load_four(const RowView<TYPE> &view, const int32_t q, const int32_t q1, row_u32x4 (&v)[4]) {
 #pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            v[k] = RowView<TYPE>::nothing();
-            if (q + k * G::THREADS < q1) v[k] = view.load(q + k * G::THREADS);
-        }
+    for (int k = 0; k < 4; ++k) {
+        v[k] = RowView<TYPE>::nothing();
+        if (q + k * G::THREADS < q1) v[k] = view.load(q + k * G::THREADS);
+    }
+}
+template <class G, int TYPE, class F>
+__device__ __forceinline__ void each_chunk(const RowView<TYPE> &view, const int32_t q0, const int32_t q1, row_u32x4 (&v)[4], F f) {
+#pragma unroll 1
+    for (int32_t q = q0 + threadIdx.x; q < q1;) {
         bool go = true;
 #pragma unroll
         for (int k = 0; k < 4; ++k) go = f(v[k], view.index0(q + k * G::THREADS)) && go;
         if (!__all(go)) break;
+        q += 4 * G::THREADS;
+        load_four<G>(view, q, q1, v);
     }
 }
 // The same, the four chunks together: f(chunks, column of the first one's first element); the others follow 4 THREADS
@@ -362,8 +383,8 @@ __device__ __forceinline__ void each_quad(const RowView<TYPE> &view, const int32
 // The items that have a bucket, four at a time (see four_buckets).
 template <class G, int TYPE, class F>
 __device__ __forceinline__ void each_bucket(const RowView<TYPE> &view, const int32_t q0, const int32_t q1, const bool extra,
-                                            const RowScale &c, F f) {
-    each_chunk<G>(view, q0, q1, [&](const row_u32x4 &v, const int32_t i0) {
+                                            row_u32x4 (&first)[4], const RowScale &c, F f) {
+    each_chunk<G>(view, q0, q1, first, [&](const row_u32x4 &v, const int32_t i0) {
         bool go = true;
 #pragma unroll
         for (int e = 0; e < RowView<TYPE>::VEC; e += 4)
@@ -948,17 +969,29 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
         exclude_items<TYPE>(a, r, view);
         __syncthreads();
     }
+    constexpr int VEC = RowView<TYPE>::VEC, STEP = G::THREADS * VEC;
+    constexpr int AHEAD = TYPE == ROW_F32 ? 2 : 1;           // quads under way (4096 x 59047 f32: 234 us, 238 with one; 16-bit: spills)
+    auto load_quad = [&](row_u32x4 (&v)[4], const int32_t q) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            v[k] = RowView<TYPE>::nothing();
+            if (q + k * G::THREADS < view.n_chunks) v[k] = view.load(q + k * G::THREADS);
+        }
+    };
+    row_u32x4 v[4], next[AHEAD][4];
+    load_quad(v, tid);                                       // under way while the tables are made
+    const int32_t x = view.extra(tid);
+    const float x_score = x >= 0 ? view.at(x) : -__builtin_inff();
+    const RowParams p = row_params(a, r);
     if (tid < 256) sh.pow2[tid] = exp2((double)tid / 256.0 + a.q_bits);
 #pragma unroll
     for (int q = 0; q < G::OWN; ++q) { sh.cnt[q * G::THREADS + tid] = 0; sh.wsum[q * G::THREADS + tid] = 0; }
     if (tid == 0) { sh.base_w = ~0ull; n_found = 0; }
-    const RowParams p = row_params(a, r);
 
     // One pass over the row finds its maximum and, on the way, collects the items that can matter, unweighed: those within
     // the cut below the maximum so far, and at or above a score that some more than top_k items are likely to reach.  (A
     // filtered row has a few per cent of them, spread over all waves: weighed where they are found they would cost a whole
     // wave's weighing each.)  A row whose items do not fit the list is read again, see below.
-    constexpr int VEC = RowView<TYPE>::VEC, STEP = G::THREADS * VEC;
     auto collect = [&](const row_u32x4 (&v)[4], const int32_t i0, auto wanted) {
         bool go = true;
 #pragma unroll
@@ -1000,34 +1033,21 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
 #pragma unroll
             for (int e = 0; e < VEC; ++e) hi = fmaxf(hi, RowView<TYPE>::value(v[k], e));
     };
-    auto load_quad = [&](row_u32x4 (&v)[4], const int32_t q) {
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            v[k] = RowView<TYPE>::nothing();
-            if (q + k * G::THREADS < view.n_chunks) v[k] = view.load(q + k * G::THREADS);
-        }
-    };
     // over the workgroup
     auto join_seen = [&]() {
-#pragma unroll
-        for (int o = 32; o >= 1; o >>= 1) { hi = fmaxf(hi, __shfl_xor(hi, o)); low = fminf(low, __shfl_xor(low, o)); }
-        if (lane == 0) { sh.wave_f[wave] = hi; sh.wave_g[wave] = low; }
+        hi = wave_ends(hi, low);
+        if (lane == 63) { sh.wave_f[wave] = hi; sh.wave_g[wave] = low; }
         __syncthreads();
-        hi = sh.wave_f[lane & (G::WAVES - 1)]; low = sh.wave_g[lane & (G::WAVES - 1)];
+        hi = sh.wave_f[0]; low = sh.wave_g[0];
 #pragma unroll
-        for (int o = G::WAVES / 2; o >= 1; o >>= 1) { hi = fmaxf(hi, __shfl_xor(hi, o)); low = fminf(low, __shfl_xor(low, o)); }
+        for (int q = 1; q < G::WAVES; ++q) { hi = fmaxf(hi, sh.wave_f[q]); low = fminf(low, sh.wave_g[q]); }
         __syncthreads();
     };
     const double cut = item_cut(p, a.q_bits);
     const float reach = score_reach(cut, p.T) * 1.0001f;        // items further below the top do not count
     float at_least = -__builtin_inff();                                        // top-k: a score to start from
     const bool counted = top_k_asked(a, p), drawn = p.T > 0.f;
-    constexpr int AHEAD = TYPE == ROW_F32 ? 2 : 1;           // quads under way (4096 x 59047 f32: 234 us, 238 with one; 16-bit: spills)
     {
-        row_u32x4 v[4], next[AHEAD][4];
-        load_quad(v, tid);
-        const int32_t x = view.extra(tid);
-        const float x_score = x >= 0 ? view.at(x) : -__builtin_inff();
 #pragma unroll
         for (int d = 0; d < AHEAD; ++d) load_quad(next[d], tid + 4 * (d + 1) * G::THREADS);
         top_of(v);
@@ -1140,11 +1160,13 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
                 __syncthreads();
             }
         }
-        if (!weighed)
-            each_bucket<G>(view, 0, view.n_chunks, true, c, [&](const float (&s)[4], const int32_t, const uint32_t (&b)[4]) {
+        if (!weighed) {
+            load_quad(v, tid);
+            each_bucket<G>(view, 0, view.n_chunks, true, v, c, [&](const float (&s)[4], const int32_t, const uint32_t (&b)[4]) {
                 count_four<G::BUCKETS>(s, b, c, sh.pow2, sh.cnt, sh.wsum, counted);
                 return true;
             });
+        }
         __syncthreads();
         scan_buckets(sh.cnt, sh.wsum, sh);
         wanted_buckets(a, r, p, c.reject > (float)G::BUCKETS * 1.02f, sh, want);
@@ -1189,7 +1211,9 @@ __global__ __launch_bounds__(G::THREADS) void part_stats_kernel(const SampleArgs
         if (s > hi || (s == hi && i < at)) { hi = s; at = i; }
         low = fminf(low, s > -1e30f ? s : __builtin_inff());
     };
-    each_chunk<G>(view, q0, q1, [&](const row_u32x4 &v, const int32_t i0) {
+    row_u32x4 first[4];
+    load_four<G>(view, q0 + tid, q1, first);
+    each_chunk<G>(view, q0, q1, first, [&](const row_u32x4 &v, const int32_t i0) {
 #pragma unroll
         for (int e = 0; e < RowView<TYPE>::VEC; ++e) see(RowView<TYPE>::value(v, e), i0 + e);
         return true;
@@ -1232,6 +1256,10 @@ __global__ __launch_bounds__(G::THREADS) void part_histogram_kernel(const Sample
     __shared__ double pow2[256];
     const int64_t r = blockIdx.x / a.n_parts;
     const int part = blockIdx.x % a.n_parts, tid = threadIdx.x;
+    const RowView<TYPE> view(a.scores, r, a.lds, a.M);
+    const int32_t q0 = part * a.per_part, q1 = min(q0 + a.per_part, view.n_chunks);
+    row_u32x4 first[4];
+    load_four<G>(view, q0 + tid, q1, first);                  // under way while the parts' maxima are joined
     const RowParams p = row_params(a, r);
     const PartStat st = join_stats(a, r);
     const float hi = key_score((uint32_t)(st.best >> 32));
@@ -1240,9 +1268,7 @@ __global__ __launch_bounds__(G::THREADS) void part_histogram_kernel(const Sample
     for (int b = tid; b < G::BUCKETS; b += G::THREADS) { cnt[b] = 0; wsum[b] = 0; }
     const RowScale c = row_scale(hi, st.low, item_cut(p, a.q_bits), p, a.q_bits, G::BUCKETS);
     __syncthreads();
-    const RowView<TYPE> view(a.scores, r, a.lds, a.M);
-    const int32_t q0 = part * a.per_part, q1 = min(q0 + a.per_part, view.n_chunks);
-    each_bucket<G>(view, q0, q1, part == 0, c, [&](const float (&s)[4], const int32_t, const uint32_t (&b)[4]) {
+    each_bucket<G>(view, q0, q1, part == 0, first, c, [&](const float (&s)[4], const int32_t, const uint32_t (&b)[4]) {
         count_four<G::BUCKETS>(s, b, c, pow2, cnt, wsum, true);
         return true;
     });
@@ -1251,18 +1277,25 @@ __global__ __launch_bounds__(G::THREADS) void part_histogram_kernel(const Sample
         if (wsum[b]) { atomicAdd(&a.cnt[r * G::BUCKETS + b], cnt[b]); atomicAdd(&a.wsum[r * G::BUCKETS + b], wsum[b]); }
 }
 
-// Loads the row's histogram and turns it into running sums.
-__device__ __forceinline__ void load_histogram(const SampleArgs &a, const int64_t r, SampleShared<G> &sh) {
-    const int tid = threadIdx.x;
+// The row's histogram, loaded early and turned into running sums.
+struct Histogram {
+    uint32_t cnt[G::OWN];
+    u64 wsum[G::OWN];
+    __device__ __forceinline__ void load(const SampleArgs &a, const int64_t r) {
 #pragma unroll
-    for (int h = 0; h < G::OWN; ++h) {
-        const int b = tid + h * G::THREADS;
-        sh.cnt[b] = a.cnt[r * G::BUCKETS + b];
-        sh.wsum[b] = a.wsum[r * G::BUCKETS + b];
+        for (int h = 0; h < G::OWN; ++h) {
+            const int b = threadIdx.x + h * G::THREADS;
+            cnt[h] = a.cnt[r * G::BUCKETS + b];
+            wsum[h] = a.wsum[r * G::BUCKETS + b];
+        }
     }
-    __syncthreads();
-    scan_buckets(sh.cnt, sh.wsum, sh);
-}
+    __device__ __forceinline__ void scan(SampleShared<G> &sh) const {
+#pragma unroll
+        for (int h = 0; h < G::OWN; ++h) { sh.cnt[threadIdx.x + h * G::THREADS] = cnt[h]; sh.wsum[threadIdx.x + h * G::THREADS] = wsum[h]; }
+        __syncthreads();
+        scan_buckets(sh.cnt, sh.wsum, sh);
+    }
+};
 // 3. The items of those buckets.
 template <int TYPE>
 __global__ __launch_bounds__(G::THREADS) void part_collect_kernel(const SampleArgs a) {
@@ -1270,16 +1303,20 @@ __global__ __launch_bounds__(G::THREADS) void part_collect_kernel(const SampleAr
     __shared__ unsigned char want[G::BUCKETS + G::EDGE + 1];
     const int64_t r = blockIdx.x / a.n_parts;
     const int part = blockIdx.x % a.n_parts;
+    const RowView<TYPE> view(a.scores, r, a.lds, a.M);
+    const int32_t q0 = part * a.per_part, q1 = min(q0 + a.per_part, view.n_chunks);
+    row_u32x4 first[4];
+    load_four<G>(view, q0 + threadIdx.x, q1, first);
+    Histogram h;
+    h.load(a, r);
     const RowParams p = row_params(a, r);
     const PartStat st = join_stats(a, r);
     const float hi = key_score((uint32_t)(st.best >> 32));
     if (!(fabsf(hi) < __builtin_inff()) || !(p.T > 0.f)) return;      // answered apart
     const RowScale c = row_scale(hi, st.low, item_cut(p, a.q_bits), p, a.q_bits, G::BUCKETS);
-    load_histogram(a, r, sh);
+    h.scan(sh);
     wanted_buckets(a, r, p, false, sh, want);
-    const RowView<TYPE> view(a.scores, r, a.lds, a.M);
-    const int32_t q0 = part * a.per_part, q1 = min(q0 + a.per_part, view.n_chunks);
-    each_bucket<G>(view, q0, q1, part == 0, c, [&](const float (&s)[4], const int32_t i, const uint32_t (&b)[4]) {
+    each_bucket<G>(view, q0, q1, part == 0, first, c, [&](const float (&s)[4], const int32_t i, const uint32_t (&b)[4]) {
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             if (b[q] >= (uint32_t)G::BUCKETS || !want[b[q]]) continue;
@@ -1295,6 +1332,9 @@ template <int TYPE>
 __global__ __launch_bounds__(G::THREADS) void part_answer_kernel(const SampleArgs a) {
     __shared__ SampleShared<G> sh;
     const int64_t r = blockIdx.x;
+    Histogram h;
+    h.load(a, r);
+    const uint32_t n = a.n_found[r];
     const RowParams p = row_params(a, r);
     const PartStat st = join_stats(a, r);
     const float hi = key_score((uint32_t)(st.best >> 32));
@@ -1313,8 +1353,7 @@ __global__ __launch_bounds__(G::THREADS) void part_answer_kernel(const SampleArg
     }
     if (threadIdx.x < 256) sh.pow2[threadIdx.x] = exp2((double)threadIdx.x / 256.0 + a.q_bits);
     const RowScale c = row_scale(hi, st.low, item_cut(p, a.q_bits), p, a.q_bits, G::BUCKETS);
-    load_histogram(a, r, sh);
-    const uint32_t n = a.n_found[r];
+    h.scan(sh);
     const bool in_lds = n <= (uint32_t)LISTED;                // it is read once per step and round
     if (in_lds) {
         for (uint32_t q = threadIdx.x; q < n; q += G::THREADS) sh.found[q] = a.found[r * SR_LISTED + q];
