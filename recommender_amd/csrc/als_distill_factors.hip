@@ -272,19 +272,18 @@ __device__ __forceinline__ void cut_pair(const float p0, const float p1, const f
 // BACK = false: pass 1 (stationary X, streaming Y).  BACK = true: pass 2 (stationary Y, streaming X, lists).
 // A wave owns one stationary tile (32 rows: operands and result in registers); the WAVES waves of a workgroup share the
 // streaming tiles in LDS.  RING tiles are kept: the copy of tile t + RING - 1 starts while tile t is worked on.
-// TBUF list tiles are kept (one where LDS holds no second: F = 256).
 // Workgroup (split, block): the ids of one split go to one XCD, so that the blocks that stream the same tiles share its L2.
-template <int F, int WAVES, int RING, int TBUF, bool BACK>
+template <int F, int WAVES, int RING, bool BACK>
 __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const FactorArgs a) {
     constexpr int KS = F / 16, FT = F / 32, CHUNKS = F / 4, PER_WAVE = CHUNKS / WAVES;
     constexpr int LPR = WAVES * 2;                       // lanes that write one user's row of the list tile
     static_assert(CHUNKS % WAVES == 0, "every wave copies the same number of chunks");
-    constexpr int LDS_BYTES = RING * CHUNKS * 1024 + (BACK ? TBUF * (WAVES * 32 * T_STRIDE + 32) * 4 : 0);
+    constexpr int LDS_BYTES = RING * CHUNKS * 1024 + (BACK ? (WAVES * T_STRIDE + 1) * 32 * 4 : 0);
     static_assert(LDS_BYTES <= 160 * 1024, "LDS");
     __shared__ __attribute__((aligned(16))) char lds[LDS_BYTES];
     u32x4 *ring = reinterpret_cast<u32x4 *>(lds);                                   // RING x CHUNKS x 64
-    float *t_tile = reinterpret_cast<float *>(lds + RING * CHUNKS * 1024);          // BACK: TBUF x WAVES * 32 x T_STRIDE
-    float *bias = t_tile + TBUF * WAVES * 32 * T_STRIDE;                            // BACK: TBUF x 32
+    float *t_tile = reinterpret_cast<float *>(lds + RING * CHUNKS * 1024);          // BACK: WAVES * 32 x T_STRIDE
+    float *bias = t_tile + WAVES * 32 * T_STRIDE;                                   // BACK: 32
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int h = lane >> 5, j = lane & 31;
     const int splits = BACK ? a.splits2 : a.splits1;
@@ -337,16 +336,16 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
     asm volatile("" : "+s"(minus_one));
 
     // ---- pass 2: the lists of the streaming users, as a dense tile [item of the block, user of the stage] that is zero but
-    // for the listed pairs.  LPR lanes of one wave own a user's row in both buffers: they clear what the stage before last
-    // wrote there and write the new entries, in order, without a barrier between.
+    // for the listed pairs.  LPR lanes of a wave own a user's row: between two barriers they clear what they wrote there for
+    // the last stage and write the new entries, which they loaded a stage ahead.  A second tile in place of the second barrier
+    // leaves room for one workgroup per compute unit (f = 64: 276 us, 237 with one tile).  Also measured there: each wave on
+    // its own 32 items without that barrier 254-270, entries loaded a stage after their ranges 246, 32-bit addresses 258.
     const int row = BACK ? tid / LPR : 0, sub = BACK ? tid % LPR : 0;
     const int64_t i_first = block * WAVES * 32;
     const uint16_t *offs = BACK ? a.offs + block : nullptr;
     struct Entries { int b, e, item; float t, bias; };
-    Entries now{0, 0, 0, 0.f, NEVER}, old[TBUF];
-    int64_t old_user[TBUF];
-#pragma unroll
-    for (int q = 0; q < TBUF; ++q) { old[q] = now; old_user[q] = 0; }
+    Entries now{0, 0, 0, 0.f, NEVER}, old = now;
+    int64_t old_user = 0;
     auto fetch = [&](const int64_t t) {                  // the first LPR entries of the row's user in stage t
         Entries x{0, 0, 0, 0.f, NEVER};
         const int64_t u = t * TILE + row;
@@ -359,28 +358,23 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         }
         return x;
     };
-    auto place = [&](const int64_t t, const int parity) {   // writes `now`, the entries of stage t
-        const int buf = TBUF == 2 ? parity : 0;
-        float *tt = t_tile + buf * (WAVES * 32 * T_STRIDE);
-        const Entries o = TBUF == 2 && parity ? old[TBUF - 1] : old[0];
-        const int64_t ou = TBUF == 2 && parity ? old_user[TBUF - 1] : old_user[0];
-        if (o.b + sub < o.e) tt[(o.item - i_first) * T_STRIDE + row] = 0.f;
-        for (int q = o.b + sub + LPR; q < o.e; q += LPR)
-            tt[(a.s_item[ou * a.k + q] - i_first) * T_STRIDE + row] = 0.f;
+    auto place = [&](const int64_t t) {                  // writes `now`, the entries of stage t
+        if (old.b + sub < old.e) t_tile[(old.item - i_first) * T_STRIDE + row] = 0.f;
+        for (int q = old.b + sub + LPR; q < old.e; q += LPR) t_tile[(a.s_item[old_user * a.k + q] - i_first) * T_STRIDE + row] = 0.f;
         const int64_t u = t * TILE + row;
-        if (now.b + sub < now.e) tt[(now.item - i_first) * T_STRIDE + row] = now.t;
+        if (now.b + sub < now.e) t_tile[(now.item - i_first) * T_STRIDE + row] = now.t;
         for (int q = now.b + sub + LPR; q < now.e; q += LPR)
-            tt[(a.s_item[u * a.k + q] - i_first) * T_STRIDE + row] = a.s_t[u * a.k + q];
-        if (TBUF == 2 && parity) { old[TBUF - 1] = now; old_user[TBUF - 1] = u; }
-        else { old[0] = now; old_user[0] = u; }
-        if (sub == 0) bias[buf * 32 + row] = now.bias;
+            t_tile[(a.s_item[u * a.k + q] - i_first) * T_STRIDE + row] = a.s_t[u * a.k + q];
+        old = now;
+        old_user = u;
+        if (sub == 0) bias[row] = now.bias;
     };
 
     if constexpr (BACK) {
-        for (int q = tid; q < TBUF * WAVES * 32 * T_STRIDE / 4; q += WAVES * 64) reinterpret_cast<f32x4 *>(t_tile)[q] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int q = tid; q < WAVES * 32 * T_STRIDE / 4; q += WAVES * 64) reinterpret_cast<f32x4 *>(t_tile)[q] = f32x4{0.f, 0.f, 0.f, 0.f};
         __syncthreads();
         now = fetch(t0);
-        place(t0, 0);
+        place(t0);
         now = fetch(t0 + 1);
     }
     if constexpr (BACK) {
@@ -393,11 +387,6 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         // only make the count stricter); after the barrier everyone's have, and everyone is done with tile t - 1
         asm volatile("s_waitcnt vmcnt(%0)" :: "n"((RING - 2) * PER_WAVE) : "memory");
         __syncthreads();
-        const int parity = (int)(t - t0) & 1, buf = TBUF == 2 ? parity : 0;
-        if constexpr (BACK && TBUF == 2) {
-            place(t + 1, parity ^ 1);
-            now = fetch(t + 2);
-        }
         copy(t + RING - 1, slot == 0 ? RING - 1 : slot - 1);
         const u32x4 *st = ring + slot * CHUNKS * 64 + lane;
         slot = slot + 1 == RING ? 0 : slot + 1;
@@ -444,8 +433,8 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
                 cut_pair(p0, p1, minus_one, PH[r / 2], PL[r / 2]);
             }
         } else {
-            const f32x4 *tt = reinterpret_cast<const f32x4 *>(t_tile + buf * (WAVES * 32 * T_STRIDE) + (wave * 32 + j) * T_STRIDE) + h;
-            const f32x4 *bb = reinterpret_cast<const f32x4 *>(bias + buf * 32) + h;
+            const f32x4 *tt = reinterpret_cast<const f32x4 *>(t_tile + (wave * 32 + j) * T_STRIDE) + h;
+            const f32x4 *bb = reinterpret_cast<const f32x4 *>(bias) + h;
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const f32x4 tv = tt[2 * g], bv = bb[2 * g];
@@ -469,9 +458,9 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
                 O[q] = mfma32(vh, ph, O[q]);
             }
         }
-        if constexpr (BACK && TBUF == 1) {               // one list tile: the next entries go in when everyone has read these
+        if constexpr (BACK) {                            // the next entries go in when everyone has read these
             __syncthreads();
-            place(t + 1, 0);
+            place(t + 1);
             now = fetch(t + 2);
         }
     }
@@ -784,17 +773,17 @@ Plan make_plan(const int64_t n, const int64_t M, const int32_t f, const int32_t 
     return p;
 }
 
-template <int F, int WAVES, int RING, int TBUF, bool BACK>
+template <int F, int WAVES, int RING, bool BACK>
 int32_t launch_pass(const FactorArgs &a, hipStream_t st) {
     const int64_t stat_tiles = BACK ? a.m_tiles : a.n_tiles;
     const int64_t grid = (stat_tiles + WAVES - 1) / WAVES * (BACK ? a.splits2 : a.splits1);
     if (grid > INT32_MAX) return als_fail_(ALS_ERR_UNSUPPORTED, "als_distill_topk_f32: too many workgroups");
-    hipLaunchKernelGGL((pass_kernel<F, WAVES, RING, TBUF, BACK>), dim3((unsigned)grid), dim3(WAVES * 64), 0, st, a);
+    hipLaunchKernelGGL((pass_kernel<F, WAVES, RING, BACK>), dim3((unsigned)grid), dim3(WAVES * 64), 0, st, a);
     ALS_HIP_CHECK6(hipGetLastError());
     return ALS_OK;
 }
 
-template <int F, int WAVES, int RING1, int RING2, int TBUF>
+template <int F, int WAVES, int RING1, int RING2>
 int32_t run(const FactorArgs &a, hipStream_t st) {
     const bool vec = a.f % 4 == 0 && a.ldy % 4 == 0 && a.ldx % 4 == 0 && ((uintptr_t)a.Y | (uintptr_t)a.X) % 16 == 0;
     const dim3 blocks(Y_MAX_BLOCKS + X_MAX_BLOCKS);
@@ -802,7 +791,7 @@ int32_t run(const FactorArgs &a, hipStream_t st) {
     else hipLaunchKernelGGL((maxima_kernel<false>), blocks, dim3(256), 0, st, a);
     hipLaunchKernelGGL((prepare_kernel<F>), dim3((unsigned)(a.m_tiles + a.n_tiles)), dim3(256), 0, st, a);
     ALS_HIP_CHECK6(hipGetLastError());
-    int32_t rc = launch_pass<F, WAVES, RING1, 1, false>(a, st);
+    int32_t rc = launch_pass<F, WAVES, RING1, false>(a, st);
     if (rc) return rc;
     const int64_t n_users = a.n_tiles * TILE;
     const dim3 users((unsigned)std::min(n_users, GRID_X), (unsigned)((n_users + GRID_X - 1) / GRID_X));
@@ -814,7 +803,7 @@ int32_t run(const FactorArgs &a, hipStream_t st) {
         else hipLaunchKernelGGL((lists_kernel<F, false, LIST_MAX>), users, dim3(256), 0, st, a);
     }
     ALS_HIP_CHECK6(hipGetLastError());
-    rc = launch_pass<F, WAVES, RING2, TBUF, true>(a, st);
+    rc = launch_pass<F, WAVES, RING2, true>(a, st);
     if (rc) return rc;
     if (a.splits2 > 1) {
         const int64_t n_blocks = std::min<int64_t>((a.M * a.f + 255) / 256, 4096);
@@ -867,10 +856,10 @@ int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const 
     a.block_items = p.waves * TILE;
     hipStream_t st = (hipStream_t)stream;
     switch (p.F) {
-        case 32: return run<32, 8, 4, 2, 1>(a, st);
-        case 64: return run<64, 8, 4, 2, 1>(a, st);
-        case 128: return run<128, 8, 3, 2, 1>(a, st);
-        default: return run<256, 4, 2, 2, 1>(a, st);
+        case 32: return run<32, 8, 4, 2>(a, st);
+        case 64: return run<64, 8, 4, 2>(a, st);
+        case 128: return run<128, 8, 3, 2>(a, st);
+        default: return run<256, 4, 2, 2>(a, st);
     }
 }
 
