@@ -526,7 +526,8 @@ __global__ __launch_bounds__(256) void join_items_kernel(const FactorArgs a, con
 // ----------------------------------------------------------------------------- lists
 // One workgroup per user (and per padding user of the last tile, which only gets its bias).  Sixteen lanes work on one
 // listed item, sixteen items at a time, four floats per lane and 64 factors; VEC: the rows allow 16-byte loads.  K_MAX: lists of up to
-// 256 items leave room for eight workgroups per compute unit.
+// 256 items leave room for eight workgroups per compute unit (4096 x 59047, f = 64, k = 100: 439 us for all of distill_topk, 448
+// with room for 1024).
 __device__ __forceinline__ float sum16(float v) {
 #pragma unroll
     for (int o = 8; o >= 1; o >>= 1) v += __shfl_xor(v, o);

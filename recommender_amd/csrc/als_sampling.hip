@@ -1377,7 +1377,16 @@ __global__ __launch_bounds__(G::THREADS) void part_answer_kernel(const SampleArg
 }
 
 // ----------------------------------------------------------------------------- host
-constexpr int64_t SMALL_CHUNKS = 4096, CUT_CHUNKS = 16384, CUT_ROWS = 512;
+// Rows of 65 536 items and more (32-bit; 131 072 of 16 bits) are cut while they are few: 64 at 131 072 items, 128 from 262 144 on.
+// Cut or not, in us (float32, top-p): 1 x 131071 31 / 75, 64 x 131071 54 / 82, 256 x 131071 120 / 98; 1 x 1000003 37 / 470,
+// 128 x 1000003 398 / 658.  Filtered rows need one pass: 28 / 28, 48 / 32 at 64 x 131071, 319 / 441 at 128 x 1000003.
+constexpr int64_t CUT_CHUNKS = 16384;
+int64_t cut_rows(const int64_t M) { return std::min<int64_t>(128, M / 2048); }
+// The small workgroup, of which four are resident per compute unit instead of two: for short rows, and for longer ones if
+// there are more of them than the large workgroups that are resident.  Small / large in us (float32, all filters; none):
+// 2000 x 9724 38 / 72; 57 / 80, 2000 x 32768 61 / 86; 136 / 145, 4096 x 59047 190 / 218; 461 / 476, 1000 x 100003 87 / 92; 225 / 217,
+// 300 x 24576 21 / 24; 37 / 32.
+constexpr int64_t SMALL_CHUNKS = 4096, SMALL_ITEMS = 65536, LARGE_RESIDENT = 512;
 struct CutPlan {
     int32_t n_parts, per_part;        // n_parts == 0: one workgroup per row
     size_t off_wsum, off_cnt, off_nfound, off_found, total;
@@ -1385,7 +1394,7 @@ struct CutPlan {
 CutPlan cut_plan(const int32_t dtype, const int64_t n, const int64_t M) {
     CutPlan p{0, 0, 0, 0, 0, 0, 0};
     const int64_t chunks = M / (dtype == ALS_DTYPE_F32 ? 4 : 8);
-    if (chunks <= CUT_CHUNKS || n >= CUT_ROWS) return p;
+    if (chunks <= CUT_CHUNKS || n > cut_rows(M)) return p;
     // about 512 workgroups, of two chunks per thread or more each
     const int64_t want = std::max<int64_t>((512 + n - 1) / n, 4);
     p.n_parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>(std::min<int64_t>(want, 128), chunks / (4 * G::THREADS)));
@@ -1406,7 +1415,7 @@ void launch(const SampleArgs &a, const int64_t n, hipStream_t st) {
     const dim3 rows = grid_of_rows(n), block(G::THREADS);
     if (a.n_parts == 0) {
         const int64_t chunks = a.M / RowView<TYPE>::VEC;
-        if (chunks <= SMALL_CHUNKS) hipLaunchKernelGGL((sample_rows_kernel<Small, TYPE>), rows, dim3(Small::THREADS), 0, st, a);
+        if (chunks <= SMALL_CHUNKS || (n > LARGE_RESIDENT && a.M <= SMALL_ITEMS)) hipLaunchKernelGGL((sample_rows_kernel<Small, TYPE>), rows, dim3(Small::THREADS), 0, st, a);
         else hipLaunchKernelGGL((sample_rows_kernel<Large, TYPE>), rows, block, 0, st, a);
         return;
     }
