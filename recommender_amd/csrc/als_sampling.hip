@@ -1415,7 +1415,8 @@ int64_t cut_rows(const int64_t M) { return std::min<int64_t>(128, M / 2048); }
 // The small workgroup, of which four are resident per compute unit instead of two: for short rows, and for longer ones if
 // there are more of them than the large workgroups that are resident.  Small / large in us (float32, all filters; none):
 // 2000 x 9724 38 / 72; 57 / 80, 2000 x 32768 61 / 86; 136 / 145, 4096 x 59047 190 / 218; 461 / 476, 1000 x 100003 87 / 92; 225 / 217,
-// 300 x 24576 21 / 24; 37 / 32.
+// 300 x 24576 21 / 24; 37 / 32.  With more draws per row the wider buckets of the small one overflow the list: 8 draws of
+// 600 x 65000, all filters 44 / 53, none 146 / 116, every row its own 301 / 126.
 constexpr int64_t SMALL_CHUNKS = 4096, SMALL_ITEMS = 65536, LARGE_RESIDENT = 512;
 struct CutPlan {
     int32_t n_parts, per_part;        // n_parts == 0: one workgroup per row
@@ -1445,7 +1446,7 @@ void launch(const SampleArgs &a, const int64_t n, hipStream_t st) {
     const dim3 rows = grid_of_rows(n), block(G::THREADS);
     if (a.n_parts == 0) {
         const int64_t chunks = a.M / RowView<TYPE>::VEC;
-        if (chunks <= SMALL_CHUNKS || (n > LARGE_RESIDENT && a.M <= SMALL_ITEMS)) hipLaunchKernelGGL((sample_rows_kernel<Small, TYPE>), rows, dim3(Small::THREADS), 0, st, a);
+        if (chunks <= SMALL_CHUNKS || (n > LARGE_RESIDENT && a.M <= SMALL_ITEMS && a.n_draws <= 2)) hipLaunchKernelGGL((sample_rows_kernel<Small, TYPE>), rows, dim3(Small::THREADS), 0, st, a);
         else hipLaunchKernelGGL((sample_rows_kernel<Large, TYPE>), rows, block, 0, st, a);
         return;
     }
