@@ -17,6 +17,14 @@
 // is exchanged between lanes, and both factors are laid out beforehand (prepare_kernel) as the lanes read them, per tile of
 // 32 rows: row form (KS = F / 16 k-steps x 2 pieces) and transposed form (F / 32 feature tiles x 2 k-steps x 2 pieces), each
 // 64 lanes x 16 bytes.  A stage is one tile: F / 4 KB, contiguous, copied to LDS by LDS-DMA.
+//
+// What bounds it (one MI355X).  24 n M f operations at the 1.18 PFLOP/s a large fp16 library product reaches here (at 1.6 GHz:
+// power) are 315 us at 4096 x 59047, f = 64, and 666 us at 1023 x 250001, f = 128; whole calls take 418 and 873.  Of these the
+// passes are 180 + 240 and 365 + 440 us: the matrix pipe is busy 68 and 46 % of their cycles at f = 64, 58 and 45 % at 128, and
+// vector instructions take the rest (per tile and wave at f = 64: 24 matrix instructions of 32 cycles, 16 exponentials of 16,
+// some 90 others of 4, which do not overlap them).  Pass 2 has the lists on top, and 231 blocks of items for 256 compute units.
+// The other launches are memory: laying out 14 and 86 us, lists 40 and 23, the maxima 5 and 32.  Small calls are launches
+// and latency: 64 x 9724, f = 20, 34 us in five launches.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -777,8 +785,7 @@ Plan make_plan(const int64_t n, const int64_t M, const int32_t f, const int32_t 
 template <int F, int WAVES, int RING, bool BACK>
 int32_t launch_pass(const FactorArgs &a, hipStream_t st) {
     const int64_t stat_tiles = BACK ? a.m_tiles : a.n_tiles;
-    const int64_t grid = (stat_tiles + WAVES - 1) / WAVES * (BACK ? a.splits2 : a.splits1);
-    if (grid > INT32_MAX) return als_fail_(ALS_ERR_UNSUPPORTED, "als_distill_topk_f32: too many workgroups");
+    const int64_t grid = (stat_tiles + WAVES - 1) / WAVES * (BACK ? a.splits2 : a.splits1);      // below 2^23 (ROWS_MAX)
     hipLaunchKernelGGL((pass_kernel<F, WAVES, RING, BACK>), dim3((unsigned)grid), dim3(WAVES * 64), 0, st, a);
     ALS_HIP_CHECK6(hipGetLastError());
     return ALS_OK;
