@@ -113,6 +113,7 @@ __device__ __forceinline__ float moved(const float v, const float none) {
 // Over the workgroup's 256 threads.  In a wave: towards lane 63 (a row's 16 lanes, then across rows).
 __device__ __forceinline__ float block_max256(float v, float *red) {
     const float none = -__builtin_inff();
+    asm volatile("s_nop 1" : "+v"(v));      // a DPP move reads its register two states after the write, wherever that was
     v = fmaxf(v, moved<0x111, 0xf>(v, none));
     v = fmaxf(v, moved<0x112, 0xf>(v, none));
     v = fmaxf(v, moved<0x114, 0xf>(v, none));
@@ -125,6 +126,7 @@ __device__ __forceinline__ float block_max256(float v, float *red) {
     return fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
 }
 __device__ __forceinline__ float block_sum256(float v, float *red) {
+    asm volatile("s_nop 1" : "+v"(v));
     v += moved<0x111, 0xf>(v, 0.f);
     v += moved<0x112, 0xf>(v, 0.f);
     v += moved<0x114, 0xf>(v, 0.f);

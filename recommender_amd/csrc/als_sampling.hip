@@ -240,6 +240,7 @@ __device__ __forceinline__ u64 moved(const u64 v) {
 }
 template <class V>
 __device__ __forceinline__ V wave_scan(V v) {
+    asm volatile("s_nop 1" : "+v"(v));      // a DPP move reads its register two states after the write, wherever that was
     v += moved<0x111, 0xf>(v);        // row_shr:1
     v += moved<0x112, 0xf>(v);        // row_shr:2
     v += moved<0x114, 0xf>(v);        // row_shr:4
@@ -256,6 +257,7 @@ __device__ __forceinline__ float moved(const float v, const float none) {
 }
 __device__ __forceinline__ float wave_ends(float hi, float &low) {
     const float inf = __builtin_inff();
+    asm volatile("s_nop 1" : "+v"(hi), "+v"(low));
     hi = fmaxf(hi, moved<0x111, 0xf>(hi, -inf)); low = fminf(low, moved<0x111, 0xf>(low, inf));
     hi = fmaxf(hi, moved<0x112, 0xf>(hi, -inf)); low = fminf(low, moved<0x112, 0xf>(low, inf));
     hi = fmaxf(hi, moved<0x114, 0xf>(hi, -inf)); low = fminf(low, moved<0x114, 0xf>(low, inf));
