@@ -663,8 +663,8 @@ def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, e
         raise ValueError("u must be a float32 or float64 tensor")
     if u.dim() not in (1, 2) or u.shape[0] != n or (u.dim() == 2 and u.shape[1] < 1):
         raise ValueError("u must be [n_rows] or [n_rows, n_draws]")
-    if u.dim() == 2 and u.shape[1] > 1 << 20:
-        raise ValueError("at most 2^20 draws per row, got %d" % u.shape[1])
+    if u.dim() == 2 and u.shape[1] > 1 << 16:
+        raise ValueError("at most 2^16 draws per row, got %d" % u.shape[1])
     if not u.is_cuda or not u.is_contiguous():
         raise ValueError("u must be a contiguous CUDA/HIP tensor")
     t, t_rows = _row_param(temperature, n, torch.float32, "temperature", score_rows)

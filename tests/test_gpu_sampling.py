@@ -300,7 +300,7 @@ def test_more_rows_than_one_axis_of_a_launch_takes(ops):
 def test_more_draws_than_are_taken(ops):
     S = torch.zeros((1, 10), device="cuda")
     with pytest.raises(ValueError, match="draws"):
-        ops.sample_rows(S, torch.zeros((1, (1 << 20) + 1), device="cuda"))
+        ops.sample_rows(S, torch.zeros((1, (1 << 16) + 1), device="cuda"))
 
 
 def test_a_thousand_draws_of_a_row(ops):
@@ -324,3 +324,24 @@ def test_16_bit_rows_counted_by_value(ops, dtype, M):
     u = torch.from_numpy(rng.random((len(rows), 5))).cuda()
     for kw in (dict(T=0.5), dict(T=3.0, p=0.7), dict(T=0.5, k=M // 2), dict(T=1e30), dict(T=0.01, p=0.999)):
         check(ops, S, u, **kw)
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("M", [700, 40001, 70003])
+def test_best_item_at_temperature_zero(ops, dtype, M):
+    """Many equal best items (more than a list holds), an infinite one at the start, the end and late, masks, NaN: the lowest
+    column of the largest score, whatever the filters say."""
+    rng = np.random.default_rng(M)
+    base = rng.normal(size=M).astype(np.float32)
+    rows = [base, np.zeros(M), np.where(rng.random(M) < 0.5, 7.0, base), np.where(np.arange(M) == M - 3, np.inf, base),
+            np.where(np.arange(M) == 1, np.inf, base), np.where(np.arange(M) >= M // 2, np.inf, base), np.full(M, -np.inf),
+            np.where(np.arange(M) % 2 == 0, np.nan, base), np.arange(M) / 64.0, -np.arange(M) / 64.0, np.full(M, -65504.0)]
+    S = torch.from_numpy(np.stack(rows).astype(np.float32)).cuda().to(TYPES[dtype])
+    s = S.float().cpu().numpy()
+    s = np.where(np.isnan(s), -np.inf, s)
+    want = np.where(s.max(1) == -np.inf, -1, s.argmax(1))
+    u = torch.from_numpy(rng.random((len(rows), 2))).cuda()
+    for kw in (dict(), dict(top_k=5, top_p=0.5), dict(min_p=0.5)):
+        idx, logp = ops.sample_rows(S, u, temperature=0.0, **kw)
+        assert np.array_equal(idx.cpu().numpy(), np.stack([want, want], 1))
+        assert torch.equal(logp, torch.where(idx < 0, -torch.inf, 0.0).float())

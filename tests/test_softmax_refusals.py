@@ -35,7 +35,7 @@ def sample(**over):
     (dict(scores=None), "INVALID_ARG", "null"), (dict(opts=None), "INVALID_ARG", "null"), (dict(u=None), "INVALID_ARG", "null"),
     (dict(idx=None), "INVALID_ARG", "null"), (dict(logp=None), "INVALID_ARG", "null"),
     (dict(n=0), "INVALID_ARG", "sizes"), (dict(n=-1), "INVALID_ARG", "sizes"), (dict(M=0), "INVALID_ARG", "sizes"),
-    (dict(lds=99), "INVALID_ARG", "sizes"), (dict(draws=0), "INVALID_ARG", "sizes"), (dict(draws=(1 << 20) + 1), "INVALID_ARG", "sizes"),
+    (dict(lds=99), "INVALID_ARG", "sizes"), (dict(draws=0), "INVALID_ARG", "sizes"), (dict(draws=(1 << 16) + 1), "INVALID_ARG", "sizes"),
     (dict(n=1 << 31), "INVALID_ARG", "sizes"),
     # a thread's next index behind the row would pass 32 bits
     (dict(M=(1 << 31) - 1, lds=1 << 31), "INVALID_ARG", "sizes"), (dict(M=(1 << 31) - 65535, lds=1 << 31), "INVALID_ARG", "sizes"),
