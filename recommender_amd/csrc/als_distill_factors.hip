@@ -148,8 +148,20 @@ __global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
     const int b = is_y ? blockIdx.x : blockIdx.x - Y_MAX_BLOCKS, nb = is_y ? Y_MAX_BLOCKS : X_MAX_BLOCKS;
     const int64_t rows = is_y ? a.M : a.n;
     float m = 0.f, mc = 0.f;
-    // sixteen lanes take a row at a time
-    for (int64_t r = (int64_t)b * 16 + (threadIdx.x >> 4); r < rows; r += (int64_t)nb * 16) {
+    // rows without gaps are one long row (500 000 x 33: 36 us otherwise); of others sixteen lanes take a row at a time
+    const bool flat = is_y && a.ldy == a.f && (uintptr_t)a.Y % 16 == 0;
+    if (flat) {
+        const int64_t quads = a.M * a.f / 4, rest = 4 * quads + threadIdx.x;
+        const f32x4 *y = reinterpret_cast<const f32x4 *>(a.Y);
+#pragma unroll 4
+        for (int64_t q = (int64_t)b * 256 + threadIdx.x; q < quads; q += (int64_t)nb * 256) {
+            const f32x4 v = y[q];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) m = fmaxf(m, finite_abs(v[e]));
+        }
+        if (b == 0 && rest < a.M * a.f) m = fmaxf(m, finite_abs(a.Y[rest]));
+    }
+    if (!flat) for (int64_t r = (int64_t)b * 16 + (threadIdx.x >> 4); r < rows; r += (int64_t)nb * 16) {
         const float *row = is_y ? a.Y + r * a.ldy : user_row(a, r);
         if (!row) continue;
         const float c = is_y || !a.weight ? 1.f : fabsf(a.weight[r]);
@@ -321,8 +333,10 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         }
     };
 
-    // under way while the rest is set up (F = 128: 365 us, 420 with the copies below; pass 2 gets slower by as much, 430 and 474)
-    if constexpr (!BACK) {
+    // under way while the rest is set up (F = 128: 365 us, 420 with the copies behind that; in pass 2, where they are less of the
+    // work, 474 and 430)
+    constexpr bool EARLY = !BACK || F <= 64;
+    if constexpr (EARLY) {
 #pragma unroll
         for (int q = 0; q < RING - 1; ++q) copy(t0 + q, q);
     }
@@ -331,10 +345,12 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         const u32x4 *src = reinterpret_cast<const u32x4 *>(stat + (active ? tile : 0) * (F * 256)) + lane;
 #pragma unroll
         for (int s = 0; s < KS; ++s) { BH[s] = src[(2 * s) * 64]; BL[s] = src[(2 * s + 1) * 64]; }
-        // waited for here: in the loop their waits would also wait, every time, for the copies under way
+    }
+    // waited for before the loop (pin): in it, their waits would also wait, every time, for the copies under way
+    auto pin = [&]() {
 #pragma unroll
         for (int s = 0; s < KS; ++s) asm volatile("" : "+v"(BH[s]), "+v"(BL[s]));
-    }
+    };
     f32x16 O[FT];
 #pragma unroll
     for (int q = 0; q < FT; ++q)
@@ -382,12 +398,15 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
 
     if constexpr (BACK) {
         for (int q = tid; q < WAVES * 32 * T_STRIDE / 4; q += WAVES * 64) reinterpret_cast<f32x4 *>(t_tile)[q] = f32x4{0.f, 0.f, 0.f, 0.f};
-        __syncthreads();
         now = fetch(t0);
+        pin();
+        __syncthreads();
         place(t0);
         now = fetch(t0 + 1);
+    } else {
+        pin();
     }
-    if constexpr (BACK) {
+    if constexpr (!EARLY) {
 #pragma unroll
         for (int q = 0; q < RING - 1; ++q) copy(t0 + q, q);
     }
