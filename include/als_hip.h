@@ -448,7 +448,8 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  *                    n_users, M <= 2^27; the factors must be finite.  Products of 22-bit operands (two fp16 pieces of a value scaled by one power
  *                    of two per factor; values below 2^-18 of the factor's largest lose bits) accumulated in float32.
  *                    8 n M f operations, three products each.  Workspace: about 8 (n + M) F bytes, F = f rounded up to 32,
- *                    64, 128 or 256, plus the parts of split sums.
+ *                    64, 128 or 256, plus the parts of split sums.  Up to 4 users (8 where M >= 65536 and f <= 128) are
+ *                    computed in float32 products from one read of the item factor, with 4 n M bytes of workspace.
  * ------------------------------------------------------------------------------------ */
 size_t als_distill_topk_workspace_bytes(int64_t n_users, int64_t M, int32_t f, int32_t k);
 int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const int64_t *user_ids, int64_t n_users, const float *Y,

@@ -10,6 +10,8 @@
 // power of two (22 mantissa bits) and hi hi + hi lo + lo hi are accumulated in float32 - the accuracy of float32 products
 // at several times their rate.
 //
+// A handful of users leaves such tiles mostly empty: they take als_distill_few.inc's vector kernels instead.
+//
 // Layout.  v_mfma_f32_32x32x16_f16: operand A lane (h, i), h = lane / 32, holds row i, k = 8 h .. 8 h + 7; B lane (h, j)
 // column j, the same k; the result's register r in lane (h, j) is row 8 (r / 4) + 4 h + r % 4, column j.  A 32 x 32 tile of
 // scores [streaming row, stationary column] leaves a lane with 16 values of ONE column; taken as two k-steps of 8 they are
@@ -753,12 +755,19 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
     }
 }
 
+#include "als_distill_few.inc"
+
 // ----------------------------------------------------------------------------- host
 int padded_factors(const int32_t f) { return f <= 32 ? 32 : f <= 64 ? 64 : f <= 128 ? 128 : 256; }
+// Up to how many users take als_distill_few's kernels, which hold their rows and O in registers.  Few / tiles in us: 1 x 9724,
+// f = 20, 22 / 31, four users 29 / 31, eight 40 / 32; 8 x 59047, f = 64, 47 / 50; 8 x 1000003, f = 20, 201 / 249, f = 128, 389 / 1007;
+// 4 x 1000003, f = 256, 515 / 2269.
+int few_users(const int F, const int64_t M) { return F == 256 || M < 65536 ? 4 : 8; }
 int waves_of(const int F) { return F == 256 ? 4 : 8; }
 
 struct Plan {
     int F, waves, splits1, splits2, item_blocks;
+    bool few;
     int64_t n_tiles, m_tiles;
     size_t off_scales, off_xt, off_yt, off_o, off_stat, off_bias, off_item, off_t, off_offs, off_dy, total;
 };
@@ -783,15 +792,21 @@ Plan make_plan(const int64_t n, const int64_t M, const int32_t f, const int32_t 
     p.waves = waves_of(p.F);
     p.n_tiles = (n + TILE - 1) / TILE;
     p.m_tiles = (M + TILE - 1) / TILE;
+    p.few = n <= few_users(p.F, M);
     p.splits1 = split_count((p.n_tiles + p.waves - 1) / p.waves, p.m_tiles);
     p.splits2 = split_count((p.m_tiles + p.waves - 1) / p.waves, p.n_tiles);
     p.item_blocks = (int)((M + p.waves * TILE - 1) / (p.waves * TILE));
+    if (p.few) {                                         // eight items per row of lanes or more, none without items
+        const int64_t s = std::min<int64_t>(MAX_SPLITS, (M + 255) / 256), per = (M + s - 1) / s;
+        p.splits1 = (int)((M + per - 1) / per);
+        p.splits2 = 1;
+    }
     size_t at = 0;
     auto take = [&](const size_t bytes) { const size_t here = at; at += (bytes + 255) / 256 * 256; return here; };
     take((Y_MAX_BLOCKS + 2 * X_MAX_BLOCKS) * 4);
     p.off_scales = take(16);
-    p.off_xt = take((size_t)p.n_tiles * p.F * 256);
-    p.off_yt = take((size_t)p.m_tiles * p.F * 256);
+    p.off_xt = take(p.few ? 0 : (size_t)p.n_tiles * p.F * 256);
+    p.off_yt = take(p.few ? (size_t)n * M * 4 : (size_t)p.m_tiles * p.F * 256);       // few: the scores
     p.off_o = take((size_t)p.splits1 * n * p.F * 4);
     p.off_stat = take((size_t)p.splits1 * n * 8);
     p.off_bias = take((size_t)p.n_tiles * TILE * 4);
@@ -812,16 +827,8 @@ int32_t launch_pass(const FactorArgs &a, hipStream_t st) {
     return ALS_OK;
 }
 
-template <int F, int WAVES, int RING1, int RING2>
-int32_t run(const FactorArgs &a, hipStream_t st) {
-    const bool vec = a.f % 4 == 0 && a.ldy % 4 == 0 && a.ldx % 4 == 0 && ((uintptr_t)a.Y | (uintptr_t)a.X) % 16 == 0;
-    const dim3 blocks(Y_MAX_BLOCKS + X_MAX_BLOCKS);
-    if (vec) hipLaunchKernelGGL((maxima_kernel<true>), blocks, dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((maxima_kernel<false>), blocks, dim3(256), 0, st, a);
-    hipLaunchKernelGGL((prepare_kernel<F>), dim3((unsigned)(a.m_tiles + a.n_tiles)), dim3(256), 0, st, a);
-    ALS_HIP_CHECK6(hipGetLastError());
-    int32_t rc = launch_pass<F, WAVES, RING1, false>(a, st);
-    if (rc) return rc;
+template <int F>
+void launch_lists(const FactorArgs &a, const bool vec, hipStream_t st) {
     const int64_t n_users = a.n_tiles * TILE;
     const dim3 users((unsigned)std::min(n_users, GRID_X), (unsigned)((n_users + GRID_X - 1) / GRID_X));
     if (a.k <= 256) {
@@ -831,6 +838,43 @@ int32_t run(const FactorArgs &a, hipStream_t st) {
         if (vec) hipLaunchKernelGGL((lists_kernel<F, true, LIST_MAX>), users, dim3(256), 0, st, a);
         else hipLaunchKernelGGL((lists_kernel<F, false, LIST_MAX>), users, dim3(256), 0, st, a);
     }
+}
+bool vector_rows(const FactorArgs &a) {
+    return a.f % 4 == 0 && a.ldy % 4 == 0 && a.ldx % 4 == 0 && ((uintptr_t)a.Y | (uintptr_t)a.X) % 16 == 0;
+}
+
+template <int F, int NU, bool VEC>
+int32_t run_few(const FactorArgs &a, hipStream_t st) {
+    float *scores = (float *)a.yt;
+    hipLaunchKernelGGL((few_scan_kernel<F, NU, VEC>), dim3((unsigned)a.splits1), dim3(512), 0, st, a, scores);
+    launch_lists<F>(a, VEC, st);
+    const int64_t blocks = std::min<int64_t>((a.M + 63) / 64, 2048);      // four items per row of lanes or more
+    hipLaunchKernelGGL((few_back_kernel<F, NU, VEC>), dim3((unsigned)blocks), dim3(256), 0, st, a, scores);
+    hipLaunchKernelGGL((few_listed_kernel<NU>), dim3((unsigned)(a.n * a.k)), dim3(64), 0, st, a, scores);
+    ALS_HIP_CHECK6(hipGetLastError());
+    return ALS_OK;
+}
+template <int F>
+int32_t run_few(const FactorArgs &a, hipStream_t st) {
+    const bool vec = vector_rows(a);
+    if (a.n <= 2) return vec ? run_few<F, 2, true>(a, st) : run_few<F, 2, false>(a, st);
+    if (F == 256 || a.n <= 4) return vec ? run_few<F, 4, true>(a, st) : run_few<F, 4, false>(a, st);
+    if constexpr (F < 256) return vec ? run_few<F, 8, true>(a, st) : run_few<F, 8, false>(a, st);
+    return ALS_OK;
+}
+
+template <int F, int WAVES, int RING1, int RING2>
+int32_t run(const FactorArgs &a, const bool few, hipStream_t st) {
+    if (few) return run_few<F>(a, st);
+    const bool vec = vector_rows(a);
+    const dim3 blocks(Y_MAX_BLOCKS + X_MAX_BLOCKS);
+    if (vec) hipLaunchKernelGGL((maxima_kernel<true>), blocks, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((maxima_kernel<false>), blocks, dim3(256), 0, st, a);
+    hipLaunchKernelGGL((prepare_kernel<F>), dim3((unsigned)(a.m_tiles + a.n_tiles)), dim3(256), 0, st, a);
+    ALS_HIP_CHECK6(hipGetLastError());
+    int32_t rc = launch_pass<F, WAVES, RING1, false>(a, st);
+    if (rc) return rc;
+    launch_lists<F>(a, vec, st);
     ALS_HIP_CHECK6(hipGetLastError());
     rc = launch_pass<F, WAVES, RING2, true>(a, st);
     if (rc) return rc;
@@ -885,10 +929,10 @@ int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const 
     a.block_items = p.waves * TILE;
     hipStream_t st = (hipStream_t)stream;
     switch (p.F) {
-        case 32: return run<32, 8, 4, 2>(a, st);
-        case 64: return run<64, 8, 4, 2>(a, st);
-        case 128: return run<128, 8, 3, 2>(a, st);
-        default: return run<256, 4, 2, 2>(a, st);
+        case 32: return run<32, 8, 4, 2>(a, p.few, st);
+        case 64: return run<64, 8, 4, 2>(a, p.few, st);
+        case 128: return run<128, 8, 3, 2>(a, p.few, st);
+        default: return run<256, 4, 2, 2>(a, p.few, st);
     }
 }
 

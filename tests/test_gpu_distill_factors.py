@@ -282,3 +282,51 @@ def test_more_users_than_one_axis_of_a_launch_takes(ops):
     e = 2.0 ** -18 * f + 2.0 ** -19                      # scores: 2 d with |x|, |y| <= 1
     tol = (e + 2.0 ** -19 + 3 * n / 16 * 2.0 ** -24) * (mag.T.contiguous() @ Xd.abs())
     assert ((dY.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.parametrize("n", [1, 2, 3, 4, 5, 8, 9])
+@pytest.mark.parametrize("M, f", [(700, 20), (9000, 33), (70001, 64), (66000, 100), (70000, 256)])
+def test_few_users(ops, n, M, f):
+    """Up to four users, eight of a large catalogue: lists that share items, repeat them, or are empty; a user listed twice and
+    an unknown one; lists of more than 64 items; both alignments of the factors' rows."""
+    rng = np.random.default_rng(100 * n + f)
+    X, Y, u, idx, val = inputs(rng, n, M, f, 150)
+    idx[:, :40] = idx[0, :40].clone()                    # shared by all
+    idx[:, 50] = idx[:, 3]                               # repeated
+    if n > 2:
+        idx[1] = -1
+        u[2] = u[0]
+    w = torch.from_numpy(rng.uniform(0.2, 2, n).astype(np.float32)).cuda()
+    check(ops, X, Y, u, idx, val, T=0.7, w=w)
+    if n > 3:
+        loss, dX, dY = ops.distill_topk(X, Y, u, idx, val, weight=w)
+        lost = u.clone(); lost[3] = 10 ** 9              # the others' rows and the items as if it were not there
+        l2, a2, d2 = ops.distill_topk(X, Y, lost, idx, val, weight=w)
+        keep = [i for i in range(n) if i != 3]
+        assert torch.isnan(l2[3]) and torch.isnan(a2[3]).all() and torch.isfinite(d2).all()
+        assert torch.equal(l2[keep], loss[keep]) and torch.equal(a2[keep], dX[keep])
+        _, _, d3 = ops.distill_topk(X, Y, u[keep].contiguous(), idx[keep].contiguous(), val[keep].contiguous(), weight=w[keep].contiguous())
+        assert torch.allclose(d2, d3, rtol=1e-5, atol=1e-6)
+    bad = w.clone()
+    if n > 2:
+        bad[1] = np.inf                                  # its list is empty
+        want = ops.distill_topk(X, Y, u, idx, val, weight=w)
+        got = ops.distill_topk(X, Y, u, idx, val, weight=bad)
+        assert all(torch.equal(g, v) for g, v in zip(got, want))
+
+
+def test_few_users_in_a_graph(ops):
+    rng = np.random.default_rng(61)
+    X, Y, u, idx, val = inputs(rng, 3, 30001, 48, 70)
+    want = ops.distill_topk(X, Y, u, idx, val)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = ops.distill_topk(X, Y, u, idx, val)
+    for _ in range(4):
+        g.replay()
+        (torch.randn(500, 500, device="cuda") * 2).sum()
+        torch.cuda.synchronize()
+        assert all(torch.equal(o, v) for o, v in zip(out, want))
+        for o in out:
+            o.zero_()
