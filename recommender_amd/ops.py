@@ -631,14 +631,15 @@ def _score_rows(t, name):
     n, M = t.shape
     if M < 1:
         raise ValueError("%s have no columns" % name)
-    if (M > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < M):
+    ld, inner = t.stride()
+    if (M > 1 and inner != 1) or (n > 1 and ld < M):
         raise ValueError("%s must be row-major with unit inner stride (rows that overlap are not)" % name)
-    return _lib.DTYPES[t.dtype], (t.stride(0) if n > 1 else M)
+    return _lib.DTYPES[t.dtype], (ld if n > 1 else M)
 
 
 def _row_param(v, n, dtype, name, like):
     """A parameter of the sampling: (scalar, None), or (0, tensor) with one value per row."""
-    if torch.is_tensor(v) and v.dim():
+    if isinstance(v, torch.Tensor) and v.dim():
         _index(v, dtype, name)
         if v.shape[0] != n:
             raise ValueError("%s must have one value per row" % name)
@@ -693,8 +694,8 @@ def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, e
     elif exclude_rows is not None:
         raise ValueError("exclude_rows without exclude")
     _same_device(score_rows, u, ex_ptr, ex_col, exclude_rows)
-    idx = torch.empty(u.shape, dtype=torch.int32, device=score_rows.device)
-    logp = torch.empty(u.shape, dtype=torch.float32, device=score_rows.device)
+    idx = u.new_empty(u.shape, dtype=torch.int32)
+    logp = u.new_empty(u.shape, dtype=torch.float32)
     if n == 0:
         return idx, logp
     need = lib.als_sample_rows_workspace_bytes(dtype, n, M)
@@ -715,15 +716,13 @@ def _teacher_lists(idx, val, n, like):
     k = idx.shape[1]
     if not (1 <= k <= 1024):
         raise ValueError("lists of 1 to 1024 items, got %d" % k)
-    lds = []
-    for t in (idx, val):
-        if (k > 1 and t.stride(1) != 1) or (n > 1 and t.stride(0) < k):
-            raise ValueError("teacher lists must be row-major with unit inner stride")
-        lds.append(t.stride(0) if n > 1 else k)
-    if lds[0] != lds[1]:
+    (ld, inner), (ld_val, inner_val) = idx.stride(), val.stride()
+    if (k > 1 and (inner != 1 or inner_val != 1)) or (n > 1 and (ld < k or ld_val < k)):
+        raise ValueError("teacher lists must be row-major with unit inner stride")
+    if n > 1 and ld != ld_val:
         raise ValueError("teacher_idx and teacher_val must have the same row stride")
     _same_device(like, idx, val)
-    return k, lds[0]
+    return k, (ld if n > 1 else k)
 
 
 def _temperature(t):
@@ -750,10 +749,11 @@ def distill_rows(score_rows, teacher_idx, teacher_val, temperature=1.0, weight=N
         if weight.shape[0] != n:
             raise ValueError("weight must have one value per row")
     if out is None:
-        out = torch.empty((n, M), dtype=score_rows.dtype, device=score_rows.device)
-    odt, ldo = _score_rows(out, "out")
-    if odt != dtype or out.shape != score_rows.shape:
-        raise ValueError("out must have the scores' shape and type")
+        out, ldo = score_rows.new_empty((n, M)), M
+    else:
+        odt, ldo = _score_rows(out, "out")
+        if odt != dtype or out.shape != score_rows.shape:
+            raise ValueError("out must have the scores' shape and type")
     if out.data_ptr() == score_rows.data_ptr():
         if ldo != ld:
             raise ValueError("out is laid over score_rows with another row stride")
@@ -763,7 +763,7 @@ def distill_rows(score_rows, teacher_idx, teacher_val, temperature=1.0, weight=N
         if a < b + ((n - 1) * ldo + M) * size and b < a + ((n - 1) * ld + M) * size:
             raise ValueError("out overlaps score_rows without being it")
     _same_device(score_rows, weight, out)
-    loss = torch.empty(n, dtype=torch.float32, device=score_rows.device)
+    loss = teacher_val.new_empty(n)
     if n == 0:
         return loss, out
     need = lib.als_distill_rows_workspace_bytes(dtype, n, M, k)
@@ -799,11 +799,10 @@ def distill_topk(X, Y, users, teacher_idx, teacher_val, temperature=1.0, weight=
         if weight.shape[0] != n:
             raise ValueError("weight must have one value per user")
     _same_device(X, Y, users, weight)
-    loss = torch.empty(n, dtype=torch.float32, device=X.device)
-    dX = torch.empty((n, f), dtype=torch.float32, device=X.device)
+    loss, dX = X.new_empty(n), X.new_empty((n, f))
     if n == 0:
-        return loss, dX, torch.zeros((M, f), dtype=torch.float32, device=X.device)
-    dY = torch.empty((M, f), dtype=torch.float32, device=X.device)
+        return loss, dX, X.new_zeros((M, f))
+    dY = X.new_empty((M, f))
     need = lib.als_distill_topk_workspace_bytes(n, M, f, k)
     ws = torch.empty(need, dtype=torch.uint8, device=X.device)
     _enqueue("als_distill_topk_f32", X.device, _addr(X), X.shape[0], ldx, _addr(users), n, _addr(Y), ldy, M, f, _addr(teacher_idx),
