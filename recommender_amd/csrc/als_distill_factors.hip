@@ -21,12 +21,12 @@
 // 64 lanes x 16 bytes.  A stage is one tile: F / 4 KB, contiguous, copied to LDS by LDS-DMA.
 //
 // What bounds it (one MI355X).  24 n M f operations at the 1.18 PFLOP/s a large fp16 library product reaches here (at 1.6 GHz:
-// power) are 315 us at 4096 x 59047, f = 64, and 666 us at 1023 x 250001, f = 128; whole calls take 417 and 861.  Under a
+// power) are 315 us at 4096 x 59047, f = 64, and 666 us at 1023 x 250001, f = 128; whole calls take 411 and 853.  Under a
 // profiler, which makes them 490 and 1020, the passes are 181 + 238 and 401 + 478 us: the matrix pipe is busy 68 and 46 % of their cycles at f = 64, 58 and 45 % at 128, and
 // vector instructions take the rest (per tile and wave at f = 64: 24 matrix instructions of 32 cycles, 16 exponentials of 16,
 // some 90 others of 4, which do not overlap them).  Pass 2 has the lists on top, and 231 blocks of items for 256 compute units.
 // The other launches are memory: laying out 14 and 86 us, lists 40 and 23, the maxima 5 and 32.  Small calls are launches
-// and latency: 64 x 9724, f = 20, 34 us in five launches.
+// and latency: 64 x 9724, f = 20, 33 us in five launches.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -24,9 +24,9 @@
 //
 // What bounds it (whole calls on one MI355X).  Filtered rows: the read, 4096 x 59047 float32 in 181 us = 5.3 TB/s (a plain
 // sum over them reads 4.0).  Rows of which much counts: vector instructions and LDS atomics; 1021 x 131071 bfloat16 with
-// 8 draws each takes 195 us, 185 000 cycles a row with two rows on a compute unit: about 40 000 for the maximum, 55 000 for
+// 8 draws each takes 192 us, 185 000 cycles a row with two rows on a compute unit: about 40 000 for the maximum, 55 000 for
 // counting the values, 40 000 for collecting, 40 000 for the draws.  Single rows: a chain of memory round trips and some
-// forty barriers, 20 us for 59 047 items; 10^6 items in four launches 38 us (5 + 10 + 11 + 12 and their gaps).
+// forty barriers, 19 us for 59 047 items; 10^6 items in four launches 37 us (5 + 9 + 11 + 13 and their gaps).
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
