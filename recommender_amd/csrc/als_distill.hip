@@ -298,8 +298,9 @@ __global__ __launch_bounds__(DR_THREADS, 8) void distill_slopes_kernel(const Row
     const float top = hi == -__builtin_inff() ? 0.f : hi;
     double z = 0.0;
     for (int p = threadIdx.x; p < n_parts; p += DR_THREADS) {
+        // a part of nothing but -inf has no weight: its stand-in maximum 0 may lie any distance above the row's (0 x inf)
         const PartStat s = stats[r * n_parts + p];
-        z += s.z * (double)exp2_fast(((s.top == -__builtin_inff() ? 0.f : s.top) - top) * c2);
+        if (s.z != 0.0) z += s.z * (double)exp2_fast(((s.top == -__builtin_inff() ? 0.f : s.top) - top) * c2);
     }
     z = block_sum(z, sh);
     const RowScale c = row_scale(a, r, z, block_max(item >= 0 ? 1.f : 0.f, sh) > 0.f);
