@@ -432,7 +432,8 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  * teacher_idx / teacher_val [n_rows, ld_teacher] int32 / float32, the first k (<= 1024) of a row; an index outside [0, M)
  * is padding, of an item listed twice the first entry stands.  A list without entries (or whose values are all -inf)
  * gives loss 0 and gradient 0.  weight: float32 per row, or NULL for 1.  A student score of -inf has q = 0 (and makes the
- * loss +inf if the teacher lists it with t > 0); NaN or +inf scores make their row NaN.
+ * loss +inf if the teacher lists it with t > 0); NaN or +inf scores make their row NaN, and NaN or +inf in a list its loss and
+ * the listed items' slopes.
  *
  * als_distill_rows   the scores are given, [n_rows, lds] row major in float32, float16 or bfloat16; grad_out [n_rows, ldg]
  *                    of the same type receives slope and may be `scores` itself (same ld).  Sums are float32 in runs of 4

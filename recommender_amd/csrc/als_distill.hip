@@ -110,7 +110,8 @@ __device__ void teacher_entry(const RowsArgs &a, const int64_t r, ListShared &sh
     }
     __syncthreads();
     if (item >= 0 && sh.first[slot] != tid) item = -1;
-    const float top = block_max(item >= 0 ? z : -__builtin_inff(), sh);
+    // a NaN counts as the largest: the list is not an empty one, and its sum and shares become NaN
+    const float top = block_max(item < 0 ? -__builtin_inff() : z == z ? z : __builtin_inff(), sh);
     float e = 0.f;
     if (item >= 0 && top != -__builtin_inff()) e = expf((z - top) * a.inv_t);
     const double sum = block_sum((double)e, sh);

@@ -189,7 +189,7 @@ __global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
 __device__ bool list_has_weight(const FactorArgs &a, const int64_t u) {
     const int32_t *idx = a.t_idx + u * a.ldt;
     for (int p = 0; p < a.k; ++p) {
-        if (idx[p] < 0 || idx[p] >= a.M || !(a.t_val[u * a.ldt + p] > -__builtin_inff())) continue;
+        if (idx[p] < 0 || idx[p] >= a.M || a.t_val[u * a.ldt + p] == -__builtin_inff()) continue;
         bool first = true;
         for (int q = 0; q < p && first; ++q) first = idx[q] != idx[p];
         if (first) return true;
@@ -647,7 +647,7 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
         }
         keep[b] = !again;
         if (again) n_again = 1;
-        else top = fmaxf(top, own_val[b]);
+        else top = fmaxf(top, own_val[b] == own_val[b] ? own_val[b] : __builtin_inff());      // NaN: not an empty list
     }
     top = block_max256(top, red);
     const bool any = top != -__builtin_inff();           // a list without weight asks for nothing

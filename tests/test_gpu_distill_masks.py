@@ -43,3 +43,41 @@ def test_a_masked_stretch_of_a_row_far_from_zero(ops, M, level, T):
     assert ((grad.double() - want).abs() <= tol * mag).all()
     assert ((loss.double() - terms.sum(1)).abs() <= tol * terms.abs().sum(1) + tol).all()
     assert not grad[:, : M * 7 // 10].any()
+
+
+@pytest.mark.parametrize("M", [700, 200003])
+def test_lists_with_nan_are_not_empty_lists(ops, M):
+    """softmax of a list that holds a NaN or +inf is NaN, also where it holds nothing else; the items off the list keep their
+    slopes, and a list of -inf alone is the empty one."""
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    S = torch.randn(5, M, generator=g, device="cuda")
+    idx = torch.arange(5, 15, device="cuda", dtype=torch.int32).repeat(5, 1)
+    val = torch.randn(5, 10, generator=g, device="cuda")
+    val[0] = float("nan")
+    val[1, 3] = float("nan")
+    val[2] = float("inf")
+    val[3] = float("-inf")
+    loss, grad = ops.distill_rows(S, idx, val)
+    want, slopes = ops.distill_rows(S, idx, torch.zeros_like(val))
+    assert torch.isnan(loss[:3]).all() and torch.isnan(grad[:3, 5:15]).all()
+    assert float(loss[3]) == 0.0 and not grad[3].any() and torch.isfinite(loss[4])
+    off = torch.ones(M, dtype=torch.bool, device="cuda")
+    off[5:15] = False
+    assert torch.equal(grad[[0, 1, 2, 4]][:, off], slopes[[0, 1, 2, 4]][:, off])
+
+
+@pytest.mark.parametrize("n, M", [(4, 700), (40, 700), (8, 70001)])
+def test_factor_form_lists_with_nan_are_not_empty_lists(ops, n, M):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(2)
+    X, Y = torch.randn(n, 20, generator=g, device="cuda"), torch.randn(M, 20, generator=g, device="cuda")
+    idx = torch.arange(5, 15, device="cuda", dtype=torch.int32).repeat(n, 1)
+    val = torch.randn(n, 10, generator=g, device="cuda")
+    val[0] = float("nan")
+    val[1] = float("-inf")
+    loss, dX, dY = ops.distill_topk(X, Y, None, idx, val)
+    assert torch.isnan(loss[0]) and torch.isnan(dX[0]).all() and torch.isnan(dY[5:15]).all()
+    assert float(loss[1]) == 0.0 and not dX[1].any()
+    rest = torch.cat([dY[:5], dY[15:]])
+    assert torch.isfinite(rest).all() and torch.isfinite(loss[1:]).all() and torch.isfinite(dX[1:]).all()
