@@ -447,8 +447,9 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  *                    both dense row major.  A user id outside [0, x_rows) gives NaN for its loss and dX row and adds nothing
  *                    to dY.  Any f <= ALS_MAX_FACTORS and alignment; temperature in [1e-6, 1e6];
  *                    n_users, M <= 2^27; the factors must be finite.  Products of 22-bit operands (two fp16 pieces of a value scaled by one power
- *                    of two per factor; values below 2^-18 of the factor's largest lose bits; q - t of dY is held to
- *                    2^-39) accumulated in float32.
+ *                    of two per factor; values below 2^-18 of the factor's largest lose bits; q - t of dY by one per item, so
+ *                    those below 2^-10 of the item's largest over the users lose bits, and none more than 2^-33 of that)
+ *                    accumulated in float32.
  *                    8 n M f operations, three products each.  Workspace: about 8 (n + M) F bytes, F = f rounded up to 32,
  *                    64, 128 or 256, plus the parts of split sums.  Up to 4 users (8 where M >= 65536 and f <= 128) are
  *                    computed in float32 products from one read of the item factor, with 4 n M bytes of workspace.

@@ -57,7 +57,8 @@ constexpr int64_t ROWS_MAX = 1 << 27;   // of either factor: a launch takes fewe
 constexpr int64_t GRID_X = 1 << 21;     // a workgroup per user: beyond that along y
 constexpr float P_OFFSET = 8.f;         // pass 1: p 2^8, and at most 2^6 above the running maximum's: below 2^15
 constexpr float LAZY = 6.f;             // the running maximum follows when it lags by more than 2^6
-constexpr float Q_OFFSET = 14.f;        // pass 2: (q - t) 2^14
+constexpr int Q_TOP = 15, Q_ROOM = 6;   // pass 2: an item's q - t times a power of two that keeps them below 2^Q_TOP; when one passes
+                                        // that, the power is set so that Q_ROOM bits are free above it
 constexpr float NEVER = 1e30f;          // bias of a padding user: q = 0
 constexpr int T_STRIDE = 36;            // floats per item column of the list tile: 16-byte aligned, columns on different banks
 
@@ -76,13 +77,13 @@ struct FactorArgs {
     float *loss, *dX, *dY;
     // workspace
     float *maxima;        // Y_MAX_BLOCKS of |y|, X_MAX_BLOCKS of |x|, X_MAX_BLOCKS of |c x|
-    float *scales;        // {1 / (s_x s_y), 1 / s_y, 1 / (s_cx 2^Q_OFFSET)}
+    float *scales;        // {1 / (s_x s_y), 1 / s_y, 1 / s_cx}
     char *xt, *yt;        // the factors as tiles
     float *o_part;        // [split, user, F]
     float *stat_part;     // [split, user, 2]: running maximum (log2), sum
-    float *bias;          // log2 Z_u - Q_OFFSET, per user, NEVER for padding
+    float *bias;          // log2 Z_u, per user, NEVER for padding
     int32_t *s_item;      // lists in item order [user, k]
-    float *s_t;           // t 2^Q_OFFSET
+    float *s_t;           // t
     uint16_t *offs;       // [user, item blocks + 1] first list entry at or behind the block
     float *dy_part;       // [split, item, F]
     int64_t n_tiles, m_tiles;
@@ -241,7 +242,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const FactorArgs a) {
     if (blockIdx.x == 0 && tid == 0) {
         a.scales[0] = 1.f / (sx * sy);
         a.scales[1] = 1.f / sy;
-        a.scales[2] = exp2f(-Q_OFFSET) / sc;
+        a.scales[2] = 1.f / sc;
     }
     char *out = (is_y ? a.yt : a.xt) + T * (F * 256);
     const float s_row = is_y ? sy : sx, m_row = is_y ? 1.f : to_log2, s_tr = is_y ? sy : sc;
@@ -292,6 +293,15 @@ __device__ __forceinline__ void cut_pair(const float p0, const float p1, const f
     const auto l = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], minus_one, p0), __builtin_fmaf((float)h[1], minus_one, p1));
     lo = __builtin_bit_cast(unsigned, l);
 }
+
+// The same for d0 g and d1 g, g a power of two, each piece rounded to nearest: what is lost of d g is unbiased and at most 2^-22
+// of it or 2^-25.
+__device__ __forceinline__ void cut_scaled(const float d0, const float d1, const float g, unsigned &hi, unsigned &lo) {
+    hi = pack_f16_pinned(d0 * g, d1 * g);
+    lo = pack_f16(__builtin_fmaf(d0, g, -f16_lo(hi)), __builtin_fmaf(d1, g, -f16_hi(hi)));
+}
+
+__device__ __forceinline__ float power_inverse(const float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
 
 // BACK = false: pass 1 (stationary X, streaming Y).  BACK = true: pass 2 (stationary Y, streaming X, lists).
 // A wave owns one stationary tile (32 rows: operands and result in registers); the WAVES waves of a workgroup share the
@@ -360,6 +370,10 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         for (int r = 0; r < 16; ++r) O[q][r] = 0.f;
     const float k = a.scales[0];
     float m = -__builtin_inff(), z = 0.f;
+    // pass 2: O is sum_u (q - t) g x_u.  One g for all items would leave the q of a large catalogue, 10^-6 of the t's, few bits
+    // (16 at a million items); so each item (a lane and its other half's lane) has its own, which follows its largest
+    // |q - t| downwards and leaves that one its 22 bits (f = 64: 433 us, 425 with one g; f = 128: 887 and 875).
+    float g = 0x1p126f;                                  // |q - t| <= 1: a new one is 2^8 at the least
     float minus_one = -1.f;
     asm volatile("" : "+s"(minus_one));
 
@@ -373,7 +387,6 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
     const uint16_t *offs = BACK ? a.offs + block : nullptr;
     struct Entries { int b, e, item; float t, bias; };
     Entries now{0, 0, 0, 0.f, NEVER}, old = now;
-    int64_t old_user = 0;
     auto fetch = [&](const int64_t t) {                  // the first LPR entries of the row's user in stage t
         Entries x{0, 0, 0, 0.f, NEVER};
         const int64_t u = t * TILE + row;
@@ -388,13 +401,12 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
     };
     auto place = [&](const int64_t t) {                  // writes `now`, the entries of stage t
         if (old.b + sub < old.e) t_tile[(old.item - i_first) * T_STRIDE + row] = 0.f;
-        for (int q = old.b + sub + LPR; q < old.e; q += LPR) t_tile[(a.s_item[old_user * a.k + q] - i_first) * T_STRIDE + row] = 0.f;
         const int64_t u = t * TILE + row;
+        for (int q = old.b + sub + LPR; q < old.e; q += LPR) t_tile[(a.s_item[(u - TILE) * a.k + q] - i_first) * T_STRIDE + row] = 0.f;
         if (now.b + sub < now.e) t_tile[(now.item - i_first) * T_STRIDE + row] = now.t;
         for (int q = now.b + sub + LPR; q < now.e; q += LPR)
             t_tile[(a.s_item[u * a.k + q] - i_first) * T_STRIDE + row] = a.s_t[u * a.k + q];
         old = now;
-        old_user = u;
         if (sub == 0) bias[row] = now.bias;
     };
 
@@ -466,15 +478,32 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         } else {
             const f32x4 *tt = reinterpret_cast<const f32x4 *>(t_tile + (wave * 32 + j) * T_STRIDE) + h;
             const f32x4 *bb = reinterpret_cast<const f32x4 *>(bias) + h;
+            float top = 0.f;
 #pragma unroll
-            for (int g = 0; g < 4; ++g) {
-                const f32x4 tv = tt[2 * g], bv = bb[2 * g];
+            for (int b = 0; b < 4; ++b) {
+                const f32x4 tv = tt[2 * b], bv = bb[2 * b];
 #pragma unroll
-                for (int e = 0; e < 4; e += 2) {
-                    const float p0 = exp2_fast(__builtin_fmaf(S[4 * g + e], k, -bv[e])) - tv[e];
-                    const float p1 = exp2_fast(__builtin_fmaf(S[4 * g + e + 1], k, -bv[e + 1])) - tv[e + 1];
-                    cut_pair(p0, p1, minus_one, PH[2 * g + e / 2], PL[2 * g + e / 2]);
+                for (int e = 0; e < 4; ++e) {
+                    S[4 * b + e] = exp2_fast(__builtin_fmaf(S[4 * b + e], k, -bv[e])) - tv[e];
+                    top = fmaxf(top, fabsf(S[4 * b + e]));
                 }
+                if (F == 64) __builtin_amdgcn_sched_barrier(0);     // these two keep the form of four waves per SIMD from spilling
+            }
+            if (__any(top * g > (float)(1 << Q_TOP))) {
+                top = fmaxf(top, __shfl_xor(top, 32));
+                // 2^(Q_TOP - Q_ROOM - 1) <= top next < twice that; the power from the exponent's bits
+                const float next = __uint_as_float((unsigned)(253 + Q_TOP - Q_ROOM) * 0x800000u - (__float_as_uint(top) & 0x7f800000u));
+                const float scale = top * g > (float)(1 << Q_TOP) ? next * power_inverse(g) : 1.f;
+                g *= scale;
+#pragma unroll
+                for (int q = 0; q < FT; ++q)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) O[q][r] *= scale;
+            }
+#pragma unroll
+            for (int r = 0; r < 16; r += 2) {
+                cut_scaled(S[r], S[r + 1], g, PH[r / 2], PL[r / 2]);
+                if (F == 64) __builtin_amdgcn_sched_barrier(0);
             }
         }
 #pragma unroll
@@ -506,20 +535,21 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
 #pragma unroll
             for (int q = 0; q < FT; ++q)
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<f32x4 *>(a.o_part + at * F + 32 * q + 8 * g + 4 * h) =
-                        f32x4{O[q][4 * g], O[q][4 * g + 1], O[q][4 * g + 2], O[q][4 * g + 3]};
+                for (int b = 0; b < 4; ++b)
+                    *reinterpret_cast<f32x4 *>(a.o_part + at * F + 32 * q + 8 * b + 4 * h) =
+                        f32x4{O[q][4 * b], O[q][4 * b + 1], O[q][4 * b + 2], O[q][4 * b + 3]};
         }
     } else if (r < a.M) {
+        const float inv_g = power_inverse(g);
         if (splits == 1) {
-            const float inv = a.scales[2];
+            const float inv = a.scales[2] * inv_g;
             const bool quads = a.f % 4 == 0 && (uintptr_t)a.dY % 16 == 0;
 #pragma unroll
             for (int q = 0; q < FT; ++q)
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {
-                    const int c = 32 * q + 8 * g + 4 * h;
-                    const f32x4 v{O[q][4 * g] * inv, O[q][4 * g + 1] * inv, O[q][4 * g + 2] * inv, O[q][4 * g + 3] * inv};
+                for (int b = 0; b < 4; ++b) {
+                    const int c = 32 * q + 8 * b + 4 * h;
+                    const f32x4 v{O[q][4 * b] * inv, O[q][4 * b + 1] * inv, O[q][4 * b + 2] * inv, O[q][4 * b + 3] * inv};
                     float *dst = a.dY + r * a.f + c;
                     if (quads) {
                         if (c < a.f) *reinterpret_cast<f32x4 *>(dst) = v;
@@ -534,9 +564,9 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
 #pragma unroll
             for (int q = 0; q < FT; ++q)
 #pragma unroll
-                for (int g = 0; g < 4; ++g)
-                    *reinterpret_cast<f32x4 *>(a.dy_part + at * F + 32 * q + 8 * g + 4 * h) =
-                        f32x4{O[q][4 * g], O[q][4 * g + 1], O[q][4 * g + 2], O[q][4 * g + 3]};
+                for (int b = 0; b < 4; ++b)
+                    *reinterpret_cast<f32x4 *>(a.dy_part + at * F + 32 * q + 8 * b + 4 * h) =
+                        f32x4{O[q][4 * b] * inv_g, O[q][4 * b + 1] * inv_g, O[q][4 * b + 2] * inv_g, O[q][4 * b + 3] * inv_g};
         }
     }
 }
@@ -674,7 +704,7 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
         sorted[rank[b]] = (int32_t)(own[b] >> 32);
         sorted_t[rank[b]] = t;
         a.s_item[u * a.k + rank[b]] = (int32_t)(own[b] >> 32);
-        a.s_t[u * a.k + rank[b]] = t * exp2f(Q_OFFSET);
+        a.s_t[u * a.k + rank[b]] = t;
     }
     __syncthreads();
     for (int64_t b = tid; b <= a.item_blocks; b += 256) {
@@ -688,7 +718,7 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
         a.offs[u * (a.item_blocks + 1) + b] = (uint16_t)lo;
     }
     // a list without weight: c (q - t) must be 0 for all items, so its user's q is switched off
-    if (tid == 0) a.bias[u] = any ? hi + log2f(z) - P_OFFSET - Q_OFFSET : NEVER;
+    if (tid == 0) a.bias[u] = any ? hi + log2f(z) - P_OFFSET : NEVER;
     const float lse = (hi + log2f(z) - P_OFFSET) * 0.69314718f;      // ln Z of s / T
     // the listed items: t y summed, <x, y> for the loss
     const int group = tid >> 4, l = tid & 15;
