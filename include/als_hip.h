@@ -446,10 +446,12 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  *                        dY_out [M, f]:       sum_u slope_ui X[user_ids[u]],
  *                    both dense row major.  A user id outside [0, x_rows) gives NaN for its loss and dX row and adds nothing
  *                    to dY.  Any f <= ALS_MAX_FACTORS and alignment; temperature in [1e-6, 1e6];
- *                    n_users, M <= 2^27; the factors must be finite.  Products of 22-bit operands (two fp16 pieces of a value scaled by one power
- *                    of two per factor; values below 2^-18 of the factor's largest lose bits; q - t of dY by one per item, so
- *                    those below 2^-10 of the item's largest over the users lose bits, and none more than 2^-33 of that)
- *                    accumulated in float32.
+ *                    n_users, M <= 2^27; the factors must be finite.  Products of 22-bit operands accumulated in float32: two
+ *                    fp16 pieces of a value scaled by one power of two per factor (values below 2^-18 of the factor's
+ *                    largest lose bits); of c x by one per user (below 2^-18 of the user's largest); of q - t in dY by one per
+ *                    item (below 2^-10 of the item's largest over the users, none by more than 2^-33 of that).  Weights
+ *                    may be of any size: what a user adds to dY is right beside any other's, down to 2^-126 of the
+ *                    largest c x.  The weight of a user whose list is empty, or unknown, is not looked at.
  *                    8 n M f operations, three products each.  Workspace: about 8 (n + M) F bytes, F = f rounded up to 32,
  *                    64, 128 or 256, plus the parts of split sums.  Up to 4 users (8 where M >= 65536 and f <= 128) are
  *                    computed in float32 products from one read of the item factor, with 4 n M bytes of workspace.

@@ -60,6 +60,8 @@ constexpr float LAZY = 6.f;             // the running maximum follows when it l
 constexpr int Q_TOP = 15, Q_ROOM = 6;   // pass 2: an item's q - t times a power of two that keeps them below 2^Q_TOP; when one passes
                                         // that, the power is set so that Q_ROOM bits are free above it
 constexpr float NEVER = 1e30f;          // bias of a padding user: q = 0
+constexpr int NO_SHARE = -(1 << 20);    // in place of an exponent: a user whose row adds nothing to dY
+constexpr int CX_TOP = 15;              // a user's c x, as an operand, times the power of two that keeps it below 2^CX_TOP
 constexpr int T_STRIDE = 36;            // floats per item column of the list tile: 16-byte aligned, columns on different banks
 
 struct FactorArgs {
@@ -76,14 +78,15 @@ struct FactorArgs {
     const float *weight;
     float *loss, *dX, *dY;
     // workspace
-    float *maxima;        // Y_MAX_BLOCKS of |y|, X_MAX_BLOCKS of |x|, X_MAX_BLOCKS of |c x|
-    float *scales;        // {1 / (s_x s_y), 1 / s_y, 1 / s_cx}
+    float *maxima;        // Y_MAX_BLOCKS of |y|, X_MAX_BLOCKS of |x|, X_MAX_BLOCKS of user_exp
+    float *scales;        // {1 / (s_x s_y), 1 / s_y, exponent of dY's unit, largest user_exp}
+    int32_t *user_exp;    // |c_u x_uk| < 2^user_exp[u], or NO_SHARE; NULL in the form for few users
     char *xt, *yt;        // the factors as tiles
     float *o_part;        // [split, user, F]
     float *stat_part;     // [split, user, 2]: running maximum (log2), sum
-    float *bias;          // log2 Z_u, per user, NEVER for padding
+    float *bias;          // log2 Z_u less what the user's q carries, NEVER for padding
     int32_t *s_item;      // lists in item order [user, k]
-    float *s_t;           // t
+    float *s_t;           // t, times what it carries
     uint16_t *offs;       // [user, item blocks + 1] first list entry at or behind the block
     float *dy_part;       // [split, item, F]
     int64_t n_tiles, m_tiles;
@@ -143,14 +146,55 @@ __device__ __forceinline__ float block_sum256(float v, float *red) {
 }
 
 // ----------------------------------------------------------------------------- laying the factors out
-// Largest |y|, |x| and |c x| (finite ones), one value per block: the reader takes the maximum over blocks.
+// Over the sixteen lanes that share a row, in all of them.
+__device__ __forceinline__ float max16(float v) {
+#pragma unroll
+    for (int o = 8; o >= 1; o >>= 1) v = fmaxf(v, __shfl_xor(v, o));
+    return v;
+}
+__device__ __forceinline__ bool any16(const bool v) { return (__ballot(v) >> (threadIdx.x & 48) & 0xffffu) != 0; }
+
+// Whether a user's list has an entry that counts: of an item listed twice the first stands.  By the sixteen lanes of its row.
+__device__ bool list_counts(const FactorArgs &a, const int64_t u, const int l) {
+    const int32_t *idx = a.t_idx + u * a.ldt;
+    const float *val = a.t_val + u * a.ldt;
+    bool good = false, masked = false;
+#pragma unroll 4
+    for (int p = l; p < a.k; p += 16) {
+        const bool in = idx[p] >= 0 && idx[p] < a.M, low = val[p] == -__builtin_inff();
+        good |= in && !low;
+        masked |= in && low;
+    }
+    good = any16(good);
+    if (!good || !any16(masked)) return good;
+    good = false;                                        // rare: only an item's first entry may count, and that may be a masked one
+    for (int p = l; p < a.k && !good; p += 16) {
+        if (idx[p] < 0 || idx[p] >= a.M || val[p] == -__builtin_inff()) continue;
+        good = true;
+        for (int q = 0; q < p && good; ++q) good = idx[q] != idx[p];
+    }
+    return any16(good);
+}
+
+// Exponents of the parts of c x: v = m 2^e, 0.5 <= |m| < 1; 0 for what is 0 or not finite.
+__device__ __forceinline__ int exponent(const float v) {
+    int e = 0;
+    if (fabsf(v) < __builtin_inff() && v != 0.f) (void)frexpf(v, &e);
+    return e;
+}
+
+// Largest |y| and |x| (finite ones) and largest user_exp, one value per block: the reader takes the maximum over blocks.
+//
+// A user's weight, and with it the size of c_u x_u, is the caller's choice: one power of two for all users would let the
+// largest weight, which may be that of an empty list, take the others' bits.  So every user has its own, which pass 2 carries in
+// q and t instead: (q - t) 2^(user_exp - largest) times c x 2^-user_exp.
 template <bool VEC>
 __global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
     __shared__ float red[4];
     const bool is_y = blockIdx.x < Y_MAX_BLOCKS;
     const int b = is_y ? blockIdx.x : blockIdx.x - Y_MAX_BLOCKS, nb = is_y ? Y_MAX_BLOCKS : X_MAX_BLOCKS;
     const int64_t rows = is_y ? a.M : a.n;
-    float m = 0.f, mc = 0.f;
+    float m = 0.f, mc = (float)NO_SHARE;
     // rows without gaps are one long row (500 000 x 33: 36 us otherwise); of others sixteen lanes take a row at a time
     const bool flat = is_y && a.ldy == a.f && (uintptr_t)a.Y % 16 == 0;
     if (flat) {
@@ -166,16 +210,23 @@ __global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
     }
     if (!flat) for (int64_t r = (int64_t)b * 16 + (threadIdx.x >> 4); r < rows; r += (int64_t)nb * 16) {
         const float *row = is_y ? a.Y + r * a.ldy : user_row(a, r);
-        if (!row) continue;
-        const float c = is_y || !a.weight ? 1.f : fabsf(a.weight[r]);
+        const float w = !is_y && a.weight ? a.weight[r] : 1.f;
+        const bool counts = !is_y && list_counts(a, r, threadIdx.x & 15);      // beside the user's id, not behind its row
         float mr = 0.f;
-        for (int k = 4 * (threadIdx.x & 15); k < a.f; k += 64) {
-            const f32x4 v = load4<VEC>(row, k, a.f);
+        if (row)
+            for (int k = 4 * (threadIdx.x & 15); k < a.f; k += 64) {
+                const f32x4 v = load4<VEC>(row, k, a.f);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) mr = fmaxf(mr, finite_abs(v[e]));
-        }
+                for (int e = 0; e < 4; ++e) mr = fmaxf(mr, finite_abs(v[e]));
+            }
         m = fmaxf(m, mr);
-        mc = fmaxf(mc, finite_abs(mr * c * a.inv_t));
+        if (!is_y) {                                     // all sixteen lanes: r is one for them
+            mr = max16(mr);
+            const bool share = row && counts && mr > 0.f && w != 0.f;
+            const int e = share ? exponent(mr) + exponent(w) + exponent(a.inv_t) : NO_SHARE;
+            if ((threadIdx.x & 15) == 0) a.user_exp[r] = e;
+            if (fabsf(w) < __builtin_inff()) mc = fmaxf(mc, (float)e);
+        }
     }
     m = block_max256(m, red);
     mc = block_max256(mc, red);
@@ -185,32 +236,24 @@ __global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
     }
 }
 
-// Whether a user's list has an entry that counts: of an item listed twice the first stands.  (For the few whose weight is
-// not finite, by one thread.)
-__device__ bool list_has_weight(const FactorArgs &a, const int64_t u) {
-    const int32_t *idx = a.t_idx + u * a.ldt;
-    for (int p = 0; p < a.k; ++p) {
-        if (idx[p] < 0 || idx[p] >= a.M || a.t_val[u * a.ldt + p] == -__builtin_inff()) continue;
-        bool first = true;
-        for (int q = 0; q < p && first; ++q) first = idx[q] != idx[p];
-        if (first) return true;
-    }
-    return false;
-}
-// hi and lo fp16 pieces of s x
-__device__ __forceinline__ void cut(const float x, const float s, _Float16 &hi, _Float16 &lo) {
-    const float v = x * s;
+// hi and lo fp16 pieces of v.  (Of the float32 v: left to itself the compiler takes a product into the conversion, and hi is
+// then that of another rounding than the v whose rest is lo.)
+__device__ __forceinline__ void cut(float v, _Float16 &hi, _Float16 &lo) {
+    asm volatile("" : "+v"(v));
     hi = (_Float16)v;
     lo = (_Float16)(v - (float)hi);
 }
 
+__device__ __forceinline__ float power(const int e) { return ldexpf(1.f, e < -126 ? -126 : e > 126 ? 126 : e); }      // 2^e
+
 // One tile of 32 rows per workgroup: through LDS, then both forms.  Tiles of Y first, then of X (whose row form carries
-// log2(e) / T and whose transposed form carries c_u).
+// log2(e) / T and whose transposed form carries c_u 2^-user_exp).
 template <int F>
 __global__ __launch_bounds__(256) void prepare_kernel(const FactorArgs a) {
     constexpr int KS = F / 16, FT = F / 32;
     __shared__ float tile[TILE][F + 1];
     __shared__ float red[4], cs[TILE];
+    __shared__ int xe[TILE];
     const int tid = threadIdx.x;
     const bool is_y = blockIdx.x < a.m_tiles;
     const int64_t T = is_y ? blockIdx.x : blockIdx.x - a.m_tiles;
@@ -226,33 +269,42 @@ __global__ __launch_bounds__(256) void prepare_kernel(const FactorArgs a) {
     }
     if (tid < TILE) {
         const int64_t r = T * TILE + tid;
-        float c = is_y ? 1.f : 0.f;
-        if (!is_y && r < rows) {
-            c = (a.weight ? a.weight[r] : 1.f) * a.inv_t;
-            // a mean over the list's own length weights an empty list by infinity: it asks for nothing all the same
-            if (!(fabsf(c) < 3e38f) && !(user_row(a, r) && list_has_weight(a, r))) c = 0.f;
+        const bool user = !is_y && r < rows;
+        const int own_exp = user ? a.user_exp[r] : NO_SHARE;
+        const float w = user && a.weight ? a.weight[r] : 1.f;
+        const int ew = exponent(w), et = exponent(a.inv_t);
+        float c = 0.f;                                   // users without a share, whatever their weight: 0
+        int e = 0;
+        if (own_exp != NO_SHARE) {
+            e = ew + et - own_exp;                       // of x alone
+            c = ldexpf(w, -ew) * ldexpf(a.inv_t, CX_TOP - et);
         }
         cs[tid] = c;
+        xe[tid] = e;
     }
     my = block_max256(my, red);                          // the first of them waits for the tile as well
     mx = block_max256(mx, red);
     mc = block_max256(mc, red);
+    // both factors times a power of two that keeps them below 2^15, X times log2(e) / T besides
     const float to_log2 = a.inv_t * 1.44269504f;
-    const float sy = op_scale(my).s, sx = op_scale(mx * to_log2).s, sc = op_scale(mc).s;
+    const int ex = exponent(mx), ey = exponent(my), el = exponent(to_log2);
+    const float sy = power(15 - ey), sx = ldexpf(to_log2, -el) * power(15 - ex);
     if (blockIdx.x == 0 && tid == 0) {
-        a.scales[0] = 1.f / (sx * sy);
-        a.scales[1] = 1.f / sy;
-        a.scales[2] = 1.f / sc;
+        const int top = mc > (float)NO_SHARE ? (int)mc : 0;
+        a.scales[0] = power(ex + el + ey - 30);
+        a.scales[1] = power(ey - 15);
+        a.scales[2] = (float)(top - CX_TOP);
+        a.scales[3] = (float)top;
     }
     char *out = (is_y ? a.yt : a.xt) + T * (F * 256);
-    const float s_row = is_y ? sy : sx, m_row = is_y ? 1.f : to_log2, s_tr = is_y ? sy : sc;
+    const float s_row = is_y ? sy : sx;
     for (int q = tid; q < KS * 64; q += 256) {
         const int ks = q >> 6, lane = q & 63, h = lane >> 5, i = lane & 31;
         f16x8 hi, lo;
 #pragma unroll
         for (int e = 0; e < 8; ++e) {
             _Float16 x, y;
-            cut(tile[i][16 * ks + 8 * h + e] * m_row, s_row, x, y);
+            cut(tile[i][16 * ks + 8 * h + e] * s_row, x, y);
             hi[e] = x; lo[e] = y;
         }
         *reinterpret_cast<f16x8 *>(out + (2 * ks) * 1024 + lane * 16) = hi;
@@ -265,7 +317,7 @@ __global__ __launch_bounds__(256) void prepare_kernel(const FactorArgs a) {
         for (int e = 0; e < 8; ++e) {
             const int row = 16 * kk + 8 * (e / 4) + 4 * h + e % 4;
             _Float16 x, y;
-            cut(tile[row][32 * ft + i] * cs[row], s_tr, x, y);
+            cut(is_y ? tile[row][32 * ft + i] * sy : ldexpf(tile[row][32 * ft + i], xe[row]) * cs[row], x, y);
             hi[e] = x; lo[e] = y;
         }
         *reinterpret_cast<f16x8 *>(out + (2 * KS + 2 * fk) * 1024 + lane * 16) = hi;
@@ -542,14 +594,15 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
     } else if (r < a.M) {
         const float inv_g = power_inverse(g);
         if (splits == 1) {
-            const float inv = a.scales[2] * inv_g;
+            const int unit = (int)a.scales[2];
             const bool quads = a.f % 4 == 0 && (uintptr_t)a.dY % 16 == 0;
 #pragma unroll
             for (int q = 0; q < FT; ++q)
 #pragma unroll
                 for (int b = 0; b < 4; ++b) {
                     const int c = 32 * q + 8 * b + 4 * h;
-                    const f32x4 v{O[q][4 * b] * inv, O[q][4 * b + 1] * inv, O[q][4 * b + 2] * inv, O[q][4 * b + 3] * inv};
+                    const f32x4 v{ldexpf(O[q][4 * b] * inv_g, unit), ldexpf(O[q][4 * b + 1] * inv_g, unit),
+                                  ldexpf(O[q][4 * b + 2] * inv_g, unit), ldexpf(O[q][4 * b + 3] * inv_g, unit)};
                     float *dst = a.dY + r * a.f + c;
                     if (quads) {
                         if (c < a.f) *reinterpret_cast<f32x4 *>(dst) = v;
@@ -573,14 +626,14 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
 
 // dY from the parts of pass 2, in split order.
 __global__ __launch_bounds__(256) void join_items_kernel(const FactorArgs a, const int F) {
-    const float inv = a.scales[2];
+    const int unit = (int)a.scales[2];
     const int64_t total = a.M * a.f;
     for (int64_t q = (int64_t)blockIdx.x * 256 + threadIdx.x; q < total; q += (int64_t)gridDim.x * 256) {
         const int64_t i = q / a.f;
         const int c = (int)(q - i * a.f);
         float v = 0.f;
         for (int s = 0; s < a.splits2; ++s) v += a.dy_part[((int64_t)s * a.M + i) * F + c];
-        a.dY[q] = v * inv;
+        a.dY[q] = ldexpf(v, unit);
     }
 }
 
@@ -624,6 +677,9 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
     const int quad = tid % QUADS, o_first = tid / QUADS;
     const float *o_src = a.o_part + u * F + 4 * quad;
     const float x_own = tid < f ? xrow[tid] : 0.f;
+    // what the user's row of the c x operand carries less than the largest, its q and t in pass 2 carry
+    const int own_exp = a.user_exp ? a.user_exp[u] : 0;
+    const int shift = a.user_exp && own_exp != NO_SHARE ? own_exp - (int)a.scales[3] : 0;
     uint64_t own[OWN];
     float own_val[OWN], m_own[S_OWN], z_own[S_OWN];
 #pragma unroll
@@ -704,7 +760,7 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
         sorted[rank[b]] = (int32_t)(own[b] >> 32);
         sorted_t[rank[b]] = t;
         a.s_item[u * a.k + rank[b]] = (int32_t)(own[b] >> 32);
-        a.s_t[u * a.k + rank[b]] = t;
+        a.s_t[u * a.k + rank[b]] = own_exp != NO_SHARE ? ldexpf(t, shift) : 0.f * t;
     }
     __syncthreads();
     for (int64_t b = tid; b <= a.item_blocks; b += 256) {
@@ -718,7 +774,7 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
         a.offs[u * (a.item_blocks + 1) + b] = (uint16_t)lo;
     }
     // a list without weight: c (q - t) must be 0 for all items, so its user's q is switched off
-    if (tid == 0) a.bias[u] = any ? hi + log2f(z) - P_OFFSET : NEVER;
+    if (tid == 0) a.bias[u] = any && own_exp != NO_SHARE ? hi + log2f(z) - P_OFFSET - (float)shift : NEVER;
     const float lse = (hi + log2f(z) - P_OFFSET) * 0.69314718f;      // ln Z of s / T
     // the listed items: t y summed, <x, y> for the loss
     const int group = tid >> 4, l = tid & 15;
@@ -799,7 +855,7 @@ struct Plan {
     int F, waves, splits1, splits2, item_blocks;
     bool few;
     int64_t n_tiles, m_tiles;
-    size_t off_scales, off_xt, off_yt, off_o, off_stat, off_bias, off_item, off_t, off_offs, off_dy, total;
+    size_t off_scales, off_xt, off_yt, off_o, off_stat, off_bias, off_item, off_t, off_offs, off_dy, off_exp, total;
 };
 
 // Splits of a pass over `stream` tiles for `blocks` workgroups: enough workgroups for 512 (two per compute unit), at least
@@ -844,6 +900,7 @@ Plan make_plan(const int64_t n, const int64_t M, const int32_t f, const int32_t 
     p.off_t = take((size_t)n * k * 4);
     p.off_offs = take((size_t)n * (p.item_blocks + 1) * 2);
     p.off_dy = take(p.splits2 > 1 ? (size_t)p.splits2 * M * p.F * 4 : 0);
+    p.off_exp = take(p.few ? 0 : (size_t)n * 4);
     p.total = at;
     return p;
 }
@@ -955,6 +1012,7 @@ int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const 
     a.o_part = (float *)(ws + p.off_o); a.stat_part = (float *)(ws + p.off_stat); a.bias = (float *)(ws + p.off_bias);
     a.s_item = (int32_t *)(ws + p.off_item); a.s_t = (float *)(ws + p.off_t); a.offs = (uint16_t *)(ws + p.off_offs);
     a.dy_part = (float *)(ws + p.off_dy);
+    a.user_exp = p.few ? nullptr : (int32_t *)(ws + p.off_exp);
     a.n_tiles = p.n_tiles; a.m_tiles = p.m_tiles; a.splits1 = p.splits1; a.splits2 = p.splits2; a.item_blocks = p.item_blocks;
     a.block_items = p.waves * TILE;
     hipStream_t st = (hipStream_t)stream;

@@ -97,3 +97,83 @@ def test_items_that_nobody_lists_have_gradients_as_good_as_the_listed(ops, n, M,
     tol = (mag * rel_tolerance(d, n)).T.contiguous() @ X.double().abs()
     tol += 2.0 ** -33 * mag.amax(0)[:, None] * X.double().abs().sum(0)
     assert off_over_tolerance(dY, want, tol) <= 1.0
+
+
+# ----------------------------------------------------------------------------- weights
+def check_formula(ops, X, Y, idx, val, T, w):
+    """Every element of dX and dY against the magnitudes of its own terms."""
+    loss, dX, dY = ops.distill_topk(X, Y, None, idx, val, temperature=T, weight=w)
+    wl, wx, wy, mag, d = formula(X, Y, idx, val, T, w)
+    n, M = len(X), len(Y)
+    ty = (mag * rel_tolerance(d, n)).T.contiguous() @ X.double().abs()
+    # pieces of q - t, a user's row and its share's float32 (below 2^-126 of the largest): one part in 2^33 of an item's largest
+    ty += 2.0 ** -33 * (mag * X.double().abs().amax(1, keepdim=True)).sum(0)[:, None]
+    tx = rel_tolerance(d, M) * (mag @ Y.double().abs())
+    tx += 2.0 ** -30 * mag.sum(1, keepdim=True) * Y.double().abs().max()
+    assert off_over_tolerance(dY, wy, ty + 1e-300) <= 1.0 and off_over_tolerance(dX, wx, tx + 1e-300) <= 1.0
+    assert off_over_tolerance(loss, wl, 1e-4 + 2e-5 * wl.abs()) <= 1.0
+    return loss, dX, dY
+
+
+@pytest.mark.parametrize("n", [3, 8, 40, 300])
+@pytest.mark.parametrize("bad", [1e8, 1e12, 1e25, 3e38, -1e30, INF, NAN])
+def test_the_weight_of_an_empty_list_reaches_nobody(ops, n, bad):
+    """1 / (length + 1e-12) as a weight, say: the same bits as with weight 0."""
+    X, Y, idx, val = inputs(n, n, 9000, 24, 20)
+    X *= 20.0
+    none = [1] if n == 3 else [1, 4, n - 1]
+    idx[1] = -1
+    if n > 3:
+        val[4] = -INF
+        idx[n - 1] = 7; val[n - 1, 0] = -INF             # one item, and its first entry asks for nothing
+    w = torch.rand(n, generator=gen(6), device="cuda") + 0.5
+    w[none] = 0.0
+    want = ops.distill_topk(X, Y, None, idx, val, temperature=20.0, weight=w)
+    w[none] = bad
+    got = ops.distill_topk(X, Y, None, idx, val, temperature=20.0, weight=w)
+    for g, v in zip(got, want):
+        assert torch.equal(g, v)
+    assert torch.isfinite(want[2]).all() and bool(want[2].any())
+
+
+@pytest.mark.parametrize("n", [8, 40, 700])
+@pytest.mark.parametrize("power", [-100, -70, -40, 1, 33, 57, 90])
+def test_weights_times_a_power_of_two(ops, n, power):
+    """Gradients times the same power of two, bit for bit: nothing about them is relative to 1."""
+    X, Y, idx, val = inputs(n + 1, n, 5000, 24, 20)
+    w = torch.rand(n, generator=gen(6), device="cuda") + 0.5
+    loss, dX, dY = ops.distill_topk(X, Y, None, idx, val, weight=w)
+    l2, x2, y2 = ops.distill_topk(X, Y, None, idx, val, weight=w * 2.0 ** power)
+    assert torch.equal(loss, l2)
+    assert torch.equal(x2.double(), dX.double() * 2.0 ** power) or power < -60      # below float32's normal range
+    off = (y2.double() - dY.double() * 2.0 ** power).abs()
+    assert bool((off <= 2.0 ** -149).all()) if power < -60 else not off.any()
+
+
+@pytest.mark.parametrize("n", [8, 40, 300])
+@pytest.mark.parametrize("spread", [1.0, 2.0 ** 30, 2.0 ** 60])
+def test_users_of_very_different_weight(ops, n, spread):
+    """Weights from 1 to `spread`, of either sign.  Half of the users' scores leave some items alone (30 to 80 temperatures below
+    the top), so that there the light users' share is what counts."""
+    X, Y, idx, val = inputs(n + 2, n, 6000, 16, 20)
+    g = gen(7)
+    w = spread ** torch.rand(n, generator=g, device="cuda") * torch.where(torch.rand(n, generator=g, device="cuda") < 0.3, -1.0, 1.0)
+    w[0], w[1] = 1.0, spread
+    Y[:, 0] = 0.0
+    Y[1000:1010, 0] = 60.0                               # what the light half ranks first, and the heavy half last
+    light = w.abs() < spread ** 0.5
+    X[:, 0] = torch.where(light, 0.1, -1.0)
+    check_formula(ops, X, Y, idx, val, 1.0, w)
+
+
+def test_factors_far_from_one_with_weights_that_make_up_for_it(ops):
+    for n in (8, 40):
+        X, Y, idx, val = inputs(n + 3, n, 5000, 20, 20)
+        w = torch.rand(n, generator=gen(6), device="cuda") + 0.5
+        for a, b in ((2.0 ** -60, 2.0 ** 60), (2.0 ** 50, 2.0 ** -50)):
+            want = ops.distill_topk(X, Y, None, idx, val, weight=w)
+            loss, dX, dY = ops.distill_topk(X * a, Y * b, None, idx, val, weight=w)
+            assert torch.equal(loss, want[0])
+            assert torch.equal(dX, want[1] * b) and torch.equal(dY, want[2] * a)
+            _, dX, dY = ops.distill_topk(X * a, Y * b, None, idx, val, weight=w * b)
+            assert torch.equal(dY, want[2])
