@@ -448,8 +448,11 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  *                    to dY.  Any f <= ALS_MAX_FACTORS and alignment; temperature in [1e-6, 1e6];
  *                    n_users, M <= 2^27; the factors must be finite.  Products of 22-bit operands accumulated in float32: two
  *                    fp16 pieces of a value scaled by one power of two per factor (values below 2^-18 of the factor's
- *                    largest lose bits); of c x by one per user (below 2^-18 of the user's largest); of q - t in dY by one per
- *                    item (below 2^-10 of the item's largest over the users, none by more than 2^-33 of that).  Weights
+ *                    largest lose bits); of c x by one per user (below 2^-18 of the user's largest); of q in dX by one per user
+ *                    (below 2^-14 of the user's largest, none by more than 2^-37 of that), of q - t in dY by one per item (below
+ *                    2^-10 of the item's largest over the users, none by more than 2^-33 of that).  Gradients are summed over
+ *                    parts of at most 32768 items or users (as long as that makes 512 parts or fewer), ln Z in float32
+ *                    over 16 items and float64 above; the parts are joined in float32.  Weights
  *                    may be of any size: what a user adds to dY is right beside any other's, down to 2^-126 of the
  *                    largest c x.  The weight of a user whose list is empty, or unknown, is not looked at.
  *                    8 n M f operations, three products each.  Workspace: about 8 (n + M) F bytes, F = f rounded up to 32,

@@ -55,8 +55,10 @@ constexpr int TILE = 32;                // rows per tile, of either factor
 constexpr int Y_MAX_BLOCKS = 1024, X_MAX_BLOCKS = 256;
 constexpr int64_t ROWS_MAX = 1 << 27;   // of either factor: a launch takes fewer than 2^32 threads along x, here 256 per tile
 constexpr int64_t GRID_X = 1 << 21;     // a workgroup per user: beyond that along y
-constexpr float P_OFFSET = 8.f;         // pass 1: p 2^8, and at most 2^6 above the running maximum's: below 2^15
-constexpr float LAZY = 6.f;             // the running maximum follows when it lags by more than 2^6
+constexpr float P_OFFSET = 12.f;        // pass 1: p 2^12, and at most 2^3 above the running maximum's: below 2^16, fp16's largest
+constexpr float LAZY = 3.f;             // the running maximum follows when it lags by more than 2^3.  Offset and lag set what the
+                                        // lower piece still holds of a user's tail, 2^-37 of the largest; 2^-33 with 8 and 6, and
+                                        // fewer corrections, takes 0 to 1 % less time
 constexpr int Q_TOP = 15, Q_ROOM = 6;   // pass 2: an item's q - t times a power of two that keeps them below 2^Q_TOP; when one passes
                                         // that, the power is set so that Q_ROOM bits are free above it
 constexpr float NEVER = 1e30f;          // bias of a padding user: q = 0
@@ -337,22 +339,15 @@ __device__ __forceinline__ void dma16(const void *g, const unsigned lds) {
 __device__ __forceinline__ f32x16 mfma32(const u32x4 &a, const u32x4 &b, const f32x16 &c) {
     return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
 }
-// Two float32 values as fp16 pairs of both pieces.  Toward zero: the rest is exact and of one sign.
-// minus_one: -1 in a register that the compiler does not look into, so that p - h is one instruction which reads h as it lies.
-__device__ __forceinline__ void cut_pair(const float p0, const float p1, const float minus_one, unsigned &hi, unsigned &lo) {
-    const auto h = __builtin_amdgcn_cvt_pkrtz(p0, p1);
-    hi = __builtin_bit_cast(unsigned, h);
-    const auto l = __builtin_amdgcn_cvt_pkrtz(__builtin_fmaf((float)h[0], minus_one, p0), __builtin_fmaf((float)h[1], minus_one, p1));
-    lo = __builtin_bit_cast(unsigned, l);
+// p0 g and p1 g, g a power of two, as fp16 pairs of both pieces, each rounded to nearest: what is lost of p g is unbiased and at
+// most 2^-22 of it or 2^-25.  g is in a register that the compiler does not look into, so that p g - hi is one instruction
+// also where g is 1; and the rests are made opaque too: taken into the conversion, as two instructions that leave a half each, they
+// take longer (443 us for 437 at f = 64).
+__device__ __forceinline__ void cut_rest(const float p0, const float p1, const float g, const unsigned hi, unsigned &lo) {
+    float r0 = __builtin_fmaf(p0, g, -f16_lo(hi)), r1 = __builtin_fmaf(p1, g, -f16_hi(hi));
+    asm volatile("" : "+v"(r0), "+v"(r1));
+    lo = pack_f16(r0, r1);
 }
-
-// The same for d0 g and d1 g, g a power of two, each piece rounded to nearest: what is lost of d g is unbiased and at most 2^-22
-// of it or 2^-25.
-__device__ __forceinline__ void cut_scaled(const float d0, const float d1, const float g, unsigned &hi, unsigned &lo) {
-    hi = pack_f16_pinned(d0 * g, d1 * g);
-    lo = pack_f16(__builtin_fmaf(d0, g, -f16_lo(hi)), __builtin_fmaf(d1, g, -f16_hi(hi)));
-}
-
 __device__ __forceinline__ float power_inverse(const float p) { return __uint_as_float(0x7f000000u - __float_as_uint(p)); }
 
 // BACK = false: pass 1 (stationary X, streaming Y).  BACK = true: pass 2 (stationary Y, streaming X, lists).
@@ -421,13 +416,14 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
 #pragma unroll
         for (int r = 0; r < 16; ++r) O[q][r] = 0.f;
     const float k = a.scales[0];
-    float m = -__builtin_inff(), z = 0.f;
+    float m = -__builtin_inff();
+    double z = 0.0;                                      // of a lane: up to half of all items, a tile's sixteen in float32
+    float one = 1.f;
+    asm volatile("" : "+s"(one));
     // pass 2: O is sum_u (q - t) g x_u.  One g for all items would leave the q of a large catalogue, 10^-6 of the t's, few bits
     // (16 at a million items); so each item (a lane and its other half's lane) has its own, which follows its largest
     // |q - t| downwards and leaves that one its 22 bits (f = 64: 433 us, 425 with one g; f = 128: 887 and 875).
     float g = 0x1p126f;                                  // |q - t| <= 1: a new one is 2^8 at the least
-    float minus_one = -1.f;
-    asm volatile("" : "+s"(minus_one));
 
     // ---- pass 2: the lists of the streaming users, as a dense tile [item of the block, user of the stage] that is zero but
     // for the listed pairs.  LPR lanes of a wave own a user's row: between two barriers they clear what they wrote there for
@@ -510,23 +506,27 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
             for (int r = 1; r < 16; ++r) top = fmaxf(top, S[r]);
             top *= k;
             if (__any(top > m + LAZY)) {
-                const float other = __shfl_xor(top, 32);
-                const float next = fmaxf(m, fmaxf(top, other));
+                // only where it lags: a user's sums must not depend on what else its wave works on
+                top = fmaxf(top, __shfl_xor(top, 32));
+                const float next = top > m + LAZY ? top : m;
                 const float scale = m == -__builtin_inff() ? 0.f : exp2_fast(m - next);
                 m = next;
-                z *= scale;
+                z *= (double)scale;
 #pragma unroll
                 for (int q = 0; q < FT; ++q)
 #pragma unroll
                     for (int r = 0; r < 16; ++r) O[q][r] *= scale;
             }
             const float c = P_OFFSET - m;
+            float sum = 0.f;
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
                 const float p0 = exp2_fast(__builtin_fmaf(S[r], k, c)), p1 = exp2_fast(__builtin_fmaf(S[r + 1], k, c));
-                z += p0 + p1;
-                cut_pair(p0, p1, minus_one, PH[r / 2], PL[r / 2]);
+                sum += p0 + p1;
+                PH[r / 2] = pack_f16_pinned(p0, p1);
+                cut_rest(p0, p1, one, PH[r / 2], PL[r / 2]);
             }
+            z += (double)sum;
         } else {
             const f32x4 *tt = reinterpret_cast<const f32x4 *>(t_tile + (wave * 32 + j) * T_STRIDE) + h;
             const f32x4 *bb = reinterpret_cast<const f32x4 *>(bias) + h;
@@ -554,7 +554,8 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
             }
 #pragma unroll
             for (int r = 0; r < 16; r += 2) {
-                cut_scaled(S[r], S[r + 1], g, PH[r / 2], PL[r / 2]);
+                PH[r / 2] = pack_f16_pinned(S[r] * g, S[r + 1] * g);
+                cut_rest(S[r], S[r + 1], g, PH[r / 2], PL[r / 2]);
                 if (F == 64) __builtin_amdgcn_sched_barrier(0);
             }
         }
@@ -583,7 +584,7 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
         z += __shfl_xor(z, 32);
         if (r < a.n) {
             const int64_t at = (int64_t)split * a.n + r;
-            if (h == 0) { a.stat_part[2 * at] = m; a.stat_part[2 * at + 1] = z; }
+            if (h == 0) { a.stat_part[2 * at] = m; a.stat_part[2 * at + 1] = (float)z; }
 #pragma unroll
             for (int q = 0; q < FT; ++q)
 #pragma unroll
@@ -860,10 +861,15 @@ struct Plan {
 
 // Splits of a pass over `stream` tiles for `blocks` workgroups: enough workgroups for 512 (two per compute unit), at least
 // 8 tiles each (fewer do not end sooner: a workgroup's start takes as long as 8 tiles), a multiple of 8 from 8 on (one XCD
-// per split), none empty.
+// per split), none empty.  And at most SPLIT_TILES each, as long as a launch takes them: a float32 sum that has grown long loses
+// whatever small terms follow.
+constexpr int64_t SPLIT_TILES = 1024;
 int split_count(const int64_t blocks, const int64_t stream) {
     int64_t s = std::max<int64_t>(1, std::min<int64_t>(MAX_SPLITS / std::max<int64_t>(blocks, 1), stream / 8));
     if (s > 8) s = s / 8 * 8;
+    int64_t least = std::min<int64_t>({MAX_SPLITS, (stream + SPLIT_TILES - 1) / SPLIT_TILES, (1 << 22) / std::max<int64_t>(blocks, 1)});
+    if (least > 8) least = (least + 7) / 8 * 8;
+    s = std::max(s, least);
     while (s > 1) {
         const int64_t per = (stream + s - 1) / s;
         if ((s - 1) * per < stream) break;

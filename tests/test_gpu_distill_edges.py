@@ -177,3 +177,44 @@ def test_factors_far_from_one_with_weights_that_make_up_for_it(ops):
             assert torch.equal(dX, want[1] * b) and torch.equal(dY, want[2] * a)
             _, dX, dY = ops.distill_topk(X * a, Y * b, None, idx, val, weight=w * b)
             assert torch.equal(dY, want[2])
+
+
+# ----------------------------------------------------------------------------- long sums
+@pytest.mark.parametrize("n", [2, 12, 1 << 16])
+def test_a_long_tail_far_below_the_top(ops, n):
+    """One item far above a million others at 2^-32 to 2^-34 of it, and a column of Y that is 1: there dX is weight (1 - 1),
+    whatever the q are.  An item's q loses at most 2^-37 of the largest; a sum of 2^15 items, the part that the top is in, may
+    lose its other terms beside that one; q and t sums take 2^-20 more."""
+    M = (1 << 20) + 3
+    Y = torch.zeros(M, 8, device="cuda")
+    Y[:, 0] = 1.0
+    Y[:, 1] = -math.log(2.0) * (32 + 2 * torch.rand(M, generator=gen(3), device="cuda"))
+    Y[5, 1] = 0.0
+    X = torch.zeros(16, 8, device="cuda")
+    X[:, 1] = torch.linspace(0.98, 1.0, 16)
+    users = torch.arange(n, device="cuda") % 16
+    idx = torch.tensor([[5, 9]], dtype=torch.int32, device="cuda").repeat(n, 1)
+    val = torch.zeros(n, 2, device="cuda")
+    loss, dX, dY = ops.distill_topk(X, Y, users, idx, val)
+    assert float(dX[:, 0].abs().max()) <= M * 2.0 ** -37 + 2.0 ** 15 * 2.0 ** -32 + 2.0 ** -20
+    s = X.double() @ Y.double().T.contiguous()
+    want = -math.log(2.0) - torch.log_softmax(s, 1)[:, [5, 9]].mean(1)
+    assert float((loss.double() - want[users]).abs().max()) <= 2.0 ** -16          # of terms up to 24, scores within 2^-18
+
+
+def test_ln_z_of_many_users(ops):
+    """Of so many users that a lane sums half of the items: equal terms, whose roundings in float32 would all fall one way."""
+    n, M = 1 << 17, 120001
+    Y = torch.zeros(M, 8, device="cuda")
+    Y[:, 0] = 1.0
+    Y[0, 0] = 4.0
+    X = torch.zeros(8, 8, device="cuda")
+    X[:, 0] = torch.linspace(0.05, 0.6, 8)
+    users = torch.arange(n, device="cuda") % 8
+    idx = torch.tensor([[0, 9]], dtype=torch.int32, device="cuda").repeat(n, 1)
+    val = torch.zeros(n, 2, device="cuda")
+    loss, _, _ = ops.distill_topk(X, Y, users, idx, val)
+    x = X[:, 0].double()
+    want = -math.log(2.0) - 2.5 * x + torch.log(torch.exp(4 * x) + (M - 1) * torch.exp(x))
+    # scores within 2^-20 of up to 2.4, both in ln Z and in the terms; logarithms and sums of float32 numbers up to 16
+    assert float((loss.double() - want[users]).abs().max()) <= 2 * 2.4 * 2.0 ** -20 + 4 * 16 * 2.0 ** -24
