@@ -455,26 +455,62 @@ struct ListedRow {
     }
 };
 
-// Column of the m-th item (from 0, in column order) whose key is `key`, an item per thread and round: for the +inf of a row.
+// Items of one score stand in column order.  Counted once per block of columns (running sums in sh.csub; returns their log2
+// width, at least a wave's 64), any number of draws among them cost a look at one block each.
 template <class G, int TYPE>
-__device__ __forceinline__ int32_t nth_of_key(const RowView<TYPE> &view, const uint32_t key, const u64 m, SampleShared<G> &sh) {
+__device__ __forceinline__ int count_columns(const RowView<TYPE> &view, const uint32_t key, SampleShared<G> &sh) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    if (tid == 0) sh.picked.index = -1;
-    u64 seen = 0;
-    for (int64_t i0 = 0; i0 < view.M; i0 += G::THREADS) {
-        const int64_t i = i0 + tid;
-        const bool hit = i < view.M && rank_key(view.at(i)) == key;
-        const u64 mask = __ballot(hit);
-        __syncthreads();                                     // the last round's wave sums have been read
-        if (lane == 0) sh.wave_c[wave] = __popcll(mask);
-        __syncthreads();
-        const u64 before = seen + __popcll(mask & ((1ull << lane) - 1)) + sum_of_first<G>(sh.wave_c, wave);
-        seen += sum_of_first<G>(sh.wave_c, G::WAVES);
-        if (hit && before == m) sh.picked.index = (int32_t)i;
-        if (m < seen) break;                                 // uniform: `seen` is the same in every thread
+    int shift = 6;
+    while ((view.M - 1) >> shift >= G::BUCKETS) ++shift;
+#pragma unroll
+    for (int q = 0; q < G::OWN; ++q) { sh.csub[G::OWN * tid + q] = 0; sh.wsub[G::OWN * tid + q] = 0; }
+    __syncthreads();
+#pragma unroll 1
+    for (int32_t i0 = 64 * wave; i0 < view.M; i0 += 4 * G::THREADS) {       // a wave's 64 columns lie in one block
+        u64 mask[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int32_t i = i0 + k * G::THREADS + lane;
+            mask[k] = __ballot(i < view.M && rank_key(view.at(i)) == key);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k)
+            if (lane == 0 && mask[k]) atomicAdd(&sh.csub[(i0 + k * G::THREADS) >> shift], (uint32_t)__popcll(mask[k]));
     }
     __syncthreads();
-    return sh.picked.index;
+    scan_buckets(sh.csub, sh.wsub, sh);
+    return shift;
+}
+// Column of the m-th of them, from 0; by one wave, m below their number.
+template <class G, int TYPE>
+__device__ __forceinline__ int32_t nth_column(const RowView<TYPE> &view, const uint32_t key, const int shift, uint32_t m,
+                                              const SampleShared<G> &sh) {
+    constexpr int SEGMENT = G::BUCKETS / 64;
+    const int lane = threadIdx.x & 63;
+    const int seg = __ffsll(__ballot(sh.csub[SEGMENT * lane + SEGMENT - 1] > m)) - 1;
+    if (seg < 0) return -1;                                  // not so: m is below the last sum
+    const int b = SEGMENT * seg + __ffsll(__ballot(sh.csub[SEGMENT * seg + (lane & (SEGMENT - 1))] > m)) - 1;
+    m -= b ? sh.csub[b - 1] : 0;
+    const int64_t end = min((int64_t)view.M, (int64_t)(b + 1) << shift);
+#pragma unroll 1
+    for (int64_t i0 = (int64_t)b << shift; i0 < end; i0 += 256) {
+        u64 mask[4];
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const int64_t i = i0 + 64 * k + lane;
+            mask[k] = __ballot(i < end && rank_key(view.at(i)) == key);
+        }
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            const uint32_t here = (uint32_t)__popcll(mask[k]);
+            if (m < here) {
+                const uint32_t before = __builtin_amdgcn_mbcnt_hi((uint32_t)(mask[k] >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)mask[k], 0u));
+                return (int32_t)(i0 + 64 * k + __ffsll(__ballot((mask[k] >> lane & 1) != 0 && before == m)) - 1);
+            }
+            m -= here;
+        }
+    }
+    return -1;
 }
 
 // ----------------------------------------------------------------------------- the question
@@ -845,18 +881,15 @@ __device__ __forceinline__ void answer_all(const SampleArgs &a, const int64_t r,
 template <class G, int TYPE>
 __device__ __forceinline__ void answer_infinite(const SampleArgs &a, const int64_t r, const RowView<TYPE> &view, const RowParams &p,
                                 SampleShared<G> &sh) {
-    if (threadIdx.x == 0) sh.n_list = 0;
-    __syncthreads();
-    each_again<G>(view, [&](const float s, const int32_t) { if (s == __builtin_inff()) atomicAdd(&sh.n_list, 1u); });
-    __syncthreads();
-    u64 n = sh.n_list;
+    const uint32_t key = rank_key(__builtin_inff());
+    const int shift = count_columns<G>(view, key, sh);
+    u64 n = sh.csub[G::BUCKETS - 1];
     if (p.top_k > 0 && (u64)p.top_k < n) n = (u64)p.top_k;
     if (p.top_p < 1.f) n = top_p_target(p.top_p, n) + 1;
-    for (int d = 0; d < a.n_draws; ++d) {
+    for (int d = threadIdx.x >> 6; d < a.n_draws; d += G::WAVES) {
         const int64_t at = r * a.n_draws + d;
-        const int32_t i = nth_of_key<G>(view, rank_key(__builtin_inff()), draw_target(drawn_number(a, at), n), sh);
-        __syncthreads();
-        if (threadIdx.x == 0) { a.idx[at] = i; a.logp[at] = -logf((float)n); }
+        const int32_t i = nth_column<G>(view, key, shift, (uint32_t)draw_target(drawn_number(a, at), n), sh);
+        if ((threadIdx.x & 63) == 0) { a.idx[at] = i; a.logp[at] = -logf((float)n); }
     }
 }
 
