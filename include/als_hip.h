@@ -398,7 +398,7 @@ int32_t als_recommend_topk_prepared_f32(const float *X, int64_t ldx, const int64
  * column -1 and logp -inf.  +inf scores share all the weight.  Weights are summed as integers of 2^-Q of the largest,
  * Q = min(51, 62 - ceil(log2 M)); an item below half of that counts as dropped.  The answer depends on the row and its
  * parameters alone.
- * Rows of at most 2^31 - 2^16 columns, at most 2^16 draws per row (they are made one after the other).
+ * Rows of at most 2^31 - 2^16 columns, at most 2^16 draws per row.
  * opts      [host] one value for all rows, or a [device] array with one per row where the pointer is not NULL.
  * ex_*      as als_topk_rows_f32: those columns are set to -inf first, in place; columns outside [0, M) are ignored.
  * All other pointers are [device].  Few long rows need a workspace of als_sample_rows_workspace_bytes bytes (0: none, the

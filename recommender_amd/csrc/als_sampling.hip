@@ -64,7 +64,10 @@ typedef Group<512, 2048> Large;
 constexpr int CUT_BUCKETS = Large::BUCKETS;
 constexpr int LISTED = 2048;          // items collected in LDS
 constexpr int SR_LISTED = 16384;      // cut rows: items collected per row
-constexpr int32_t DRAWS_MAX = 1 << 16;      // a row's draws are made one after the other: some microseconds each
+// A row's draws: some microseconds each from a list in LDS, several of them side by side; where thousands of items matter, a share
+// of the passes over the row that a window takes (draw_from_windows).  65 536 draws, ms: 13 of a row of 1 000 003 equal scores,
+// 23 of five different ones, 250 of a normal distribution's, 1800 where all of it lies within one bucket of the histogram.
+constexpr int32_t DRAWS_MAX = 1 << 16;
 
 struct Found {            // an item collected by a workgroup of a cut row
     float score;
@@ -126,7 +129,10 @@ struct SampleShared {
                 u64 ranked[G::RANKED][2];           // (key << 32 | ~column, weight)
                 u64 wave_ranked[G::WAVES][G::WAVE_ITEMS][2];
             };
-            Found found[LISTED];
+            union {
+                Found found[LISTED];
+                u64 sorted[LISTED];                 // rank key << 32 | ~column
+            };
         };
         uint32_t values[VALUES];                    // how often a 16-bit value and its negative occur
     };
@@ -135,7 +141,7 @@ struct SampleShared {
     uint32_t wave_c[G::WAVES];
     float wave_f[G::WAVES], wave_g[G::WAVES];
     Picked picked;
-    uint32_t bucket, n_list, n_focus, k_lo, k_hi;
+    uint32_t bucket, n_list, k_lo, k_hi;
     u64 base_w, kept;
     uint32_t base_c, in_bucket;
 };
@@ -412,25 +418,30 @@ __device__ __forceinline__ void each_again(const RowView<TYPE> &view, F f) {
     for (int32_t i = threadIdx.x; i < view.M; i += G::THREADS) f(view.at(i), i);
 }
 
-// Collected in a list.  Where that does not hold them (whole) the row is read again for every answer's bucket alone (focus), and
-// only if that is still too much - thousands of equal scores - for every look at the items.  (600 x 65000, 8 draws of rows at
-// T up to 1: 303 us with a focus, 1552 looking at the whole row every time.)
+// The items the answers can be, in LDS.
+struct Listed {
+    const Found *found;
+    uint32_t n;
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+#pragma unroll 1
+        for (uint32_t q = threadIdx.x; q < n; q += blockDim.x) f(found[q].score, found[q].index);
+    }
+};
+// The same where LDS does not hold them: a list in memory or, if that does not either (whole), the row itself.
 template <class G, int TYPE>
-struct ListedRow {
+struct Unlisted {
     const RowView<TYPE> &view;
     const Found *found;
     uint32_t n;
     bool whole;
-    __device__ __forceinline__ void focus(const uint32_t b, const RowScale &c, SampleShared<G> &sh) {
-        if (!whole) return;
-        __syncthreads();
-        if (threadIdx.x == 0) sh.n_focus = 0;
-        __syncthreads();
-        auto see = [&](const float s, const int32_t i) {
-            if (bucket_of<G::BUCKETS>(s, c) != b) return;
-            const uint32_t at = atomicAdd(&sh.n_focus, 1u);
-            if (at < (uint32_t)LISTED) sh.found[at] = Found{s, i};
-        };
+    template <class F>
+    __device__ __forceinline__ void each(F f) const {
+        if (!whole) {
+#pragma unroll 1
+            for (uint32_t q = threadIdx.x; q < n; q += G::THREADS) f(found[q].score, found[q].index);
+            return;
+        }
         row_u32x4 v, next = RowView<TYPE>::nothing();
         if ((int32_t)threadIdx.x < view.n_chunks) next = view.load(threadIdx.x);
 #pragma unroll 1
@@ -438,20 +449,10 @@ struct ListedRow {
             v = next;
             if (q + G::THREADS < view.n_chunks) next = view.load(q + G::THREADS);
 #pragma unroll
-            for (int e = 0; e < RowView<TYPE>::VEC; ++e) see(RowView<TYPE>::value(v, e), view.index0(q) + e);
+            for (int e = 0; e < RowView<TYPE>::VEC; ++e) f(RowView<TYPE>::value(v, e), view.index0(q) + e);
         }
         const int32_t x = view.extra(threadIdx.x);
-        if (x >= 0) see(view.at(x), x);
-        __syncthreads();
-        found = sh.found;
-        n = uniform(sh.n_focus);
-    }
-    template <class F>
-    __device__ __forceinline__ void each(F f) {
-        if (whole && n > (uint32_t)LISTED) each_again<G>(view, f);
-        else
-#pragma unroll 1
-            for (uint32_t q = threadIdx.x; q < n; q += G::THREADS) f(found[q].score, found[q].index);
+        if (x >= 0) f(view.at(x), x);
     }
 };
 
@@ -516,13 +517,12 @@ __device__ __forceinline__ int32_t nth_column(const RowView<TYPE> &view, const u
 // ----------------------------------------------------------------------------- the question
 // The item, in rank order, at which the running sum of ones (by_count) or of weights passes `target`; the caller has
 // made sure that it does.  Every thread returns the same.
-template <class G, int TYPE, class Row>
-__device__ __forceinline__ Picked find(Row &row, const RowView<TYPE> &view, const RowScale &c, const bool by_count, const u64 target,
+template <class G, int TYPE>
+__device__ __forceinline__ Picked find(const Listed &row, const RowView<TYPE> &view, const RowScale &c, const bool by_count, const u64 target,
                        const bool counted, SampleShared<G> &sh) {
     const int tid = threadIdx.x;
     pick_bucket(sh.cnt, sh.wsum, by_count, target, 0, 0, sh);
     const uint32_t b = uniform(sh.bucket);
-    row.focus(b, c, sh);
     uint32_t n = counted ? uniform(sh.in_bucket) : 0, base_c = uniform(sh.base_c);      // 0: not known, tried
     u64 base_w = uniform(sh.base_w);
     // the bucket's keys [k_lo, k_hi] that are still in question: to begin with its scores and a bucket's width more on either
@@ -738,8 +738,8 @@ __device__ __forceinline__ u64 draw_target(const double u, const u64 W) {
 }
 
 // First bucket whose running sum exceeds the target (the last one if none does).
-template <class G>
-__device__ __forceinline__ int bucket_passing(const u64 *sums, const u64 target) {
+template <class G, class V>
+__device__ __forceinline__ int bucket_passing(const V *sums, const u64 target) {
     int lo = 0, hi = G::BUCKETS - 1;
     while (lo < hi) {
         const int mid = (lo + hi) >> 1;
@@ -821,12 +821,197 @@ __device__ __forceinline__ void wanted_buckets(const SampleArgs &a, const int64_
     __syncthreads();
 }
 
+// ----------------------------------------------------------------------------- rows that LDS has no list of
+// Thousands of items can matter: many draws of a flat row, equal scores, a temperature far above the scores' spread.  An answer
+// then takes passes over the list in memory or the row; but what they find is a whole window of the rank order around it - as
+// many items as are sorted in LDS, or all items of one score -, and every other draw that falls into it is answered with it.
+// A row of M items has some M / BUCKETS such windows, however many draws.
+struct Window {
+    u64 base_w, end_w;        // running weight in front of it and behind it
+    u64 each;                 // 0: items sorted in sh.sorted, their running weights in sh.wsub; else the weight of every item of score `key`
+    uint32_t base_c, n, key;
+    int shift;                // of count_columns
+};
+// sh.sorted[0, n) in descending order, and their running weights.
+template <class G>
+__device__ __forceinline__ void sort_window(const uint32_t n, const RowScale &c, SampleShared<G> &sh) {
+    const int tid = threadIdx.x;
+    uint32_t size = 2;
+    while (size < n) size *= 2;                              // at most BUCKETS
+    for (uint32_t q = n + tid; q < size; q += G::THREADS) sh.sorted[q] = 0;
+    __syncthreads();
+#pragma unroll 1
+    for (uint32_t run = 2; run <= size; run *= 2)
+#pragma unroll 1
+        for (uint32_t step = run / 2; step > 0; step /= 2) {
+            for (uint32_t q = tid; q < size / 2; q += G::THREADS) {
+                const uint32_t lo = 2 * q - (q & (step - 1)), hi = lo + step;
+                const u64 x = sh.sorted[lo], y = sh.sorted[hi];
+                if ((lo & run) == 0 ? x < y : x > y) { sh.sorted[lo] = y; sh.sorted[hi] = x; }
+            }
+            __syncthreads();
+        }
+#pragma unroll 1
+    for (int q = tid; q < G::BUCKETS; q += G::THREADS) {
+        u64 w = 0;
+        if ((uint32_t)q < n) weigh(key_score((uint32_t)(sh.sorted[q] >> 32)), c, sh.pow2, w);
+        sh.wsub[q] = w; sh.csub[q] = 0;
+    }
+    __syncthreads();
+    scan_buckets(sh.csub, sh.wsub, sh);
+}
+// From bucket (or part) b on, the last one up to which all items are sorted together; b itself if not even its own are.
+template <class G>
+__device__ __forceinline__ uint32_t sorted_with(const uint32_t *cnt, const uint32_t b) {
+    const uint32_t before = b ? cnt[b - 1] : 0;
+    const uint32_t e = (uint32_t)bucket_passing<G>(cnt, (u64)before + G::BUCKETS);
+    return cnt[e] - before <= (uint32_t)G::BUCKETS ? e : max(b, e ? e - 1 : 0);
+}
+// The items of the bucket that `target` lies in, into sh.found; more than LISTED: too many.
+template <class G, int TYPE>
+__device__ __forceinline__ uint32_t bucket_into_lds(const Unlisted<G, TYPE> &row, const RowScale &c, const bool by_count, const u64 target,
+                                                    SampleShared<G> &sh) {
+    if (threadIdx.x == 0) sh.n_list = 0;
+    pick_bucket(sh.cnt, sh.wsum, by_count, target, 0, 0, sh);
+    const uint32_t b = uniform(sh.bucket);
+    row.each([&](const float s, const int32_t i) {
+        if (bucket_of<G::BUCKETS>(s, c) != b) return;
+        const uint32_t at = atomicAdd(&sh.n_list, 1u);
+        if (at < (uint32_t)LISTED) sh.found[at] = Found{s, i};
+    });
+    __syncthreads();
+    return uniform(sh.n_list);
+}
+// The window that holds the item at which the running sum passes `target` (see find).
+template <class G, int TYPE>
+__device__ __forceinline__ Window window_of(const Unlisted<G, TYPE> &row, const RowView<TYPE> &view, const RowScale &c, const bool by_count,
+                                            const u64 target, const bool counted, const bool wide, SampleShared<G> &sh) {
+    const int tid = threadIdx.x;
+    pick_bucket(sh.cnt, sh.wsum, by_count, target, 0, 0, sh);
+    const uint32_t b = uniform(sh.bucket);
+    uint32_t n = 0, base_c = uniform(sh.base_c);             // 0: not known, tried
+    u64 base_w = uniform(sh.base_w);
+    uint32_t last = b;                                       // buckets b to last
+    if (counted) {
+        // as many buckets as are sorted, where a look at the items costs more than that: of the row, a list need not have them all
+        if (wide) last = uniform(sorted_with<G>(sh.cnt, b));
+        n = uniform(sh.cnt[last] - (b ? sh.cnt[b - 1] : 0));
+    }
+    const float width = 1.f / c.per_score;                   // keys in question as in find
+    uint32_t k_hi = uniform(rank_key(fminf(c.top_f - (float)((int)b - 1) * width, c.top_f)));
+    uint32_t k_lo = uniform(last == G::BUCKETS - 1 ? 0 : rank_key(c.top_f - (float)(last + 2) * width));
+#pragma unroll 1
+    for (;;) {
+        __syncthreads();
+        const bool take = n <= (uint32_t)G::BUCKETS;
+        if (!take && k_lo == k_hi) break;
+        const int bits = 32 - __clz(k_hi - k_lo), part_bits = 31 - __clz(G::BUCKETS), shift = bits > part_bits ? bits - part_bits : 0;
+#pragma unroll
+        for (int q = 0; q < G::OWN; ++q) { sh.csub[G::OWN * tid + q] = 0; sh.wsub[G::OWN * tid + q] = 0; }
+        if (tid == 0) sh.n_list = 0;
+        __syncthreads();
+        bool full = false;                                   // one item too many says enough
+        row.each([&](const float s, const int32_t i) {
+            if (full || bucket_of<G::BUCKETS>(s, c) - b > last - b) return;
+            const uint32_t key = rank_key(s);
+            u64 w;
+            if (key < k_lo || key > k_hi || !weigh(s, c, sh.pow2, w)) return;
+            if (take) {
+                const uint32_t at = atomicAdd(&sh.n_list, 1u);
+                full = at >= (uint32_t)G::BUCKETS;
+                if (!full) sh.sorted[at] = (u64)key << 32 | (uint32_t)~(uint32_t)i;
+            } else {
+                const uint32_t d = (k_hi - key) >> shift;    // in rank order
+                atomicAdd(&sh.csub[d], 1u);
+                atomicAdd(&sh.wsub[d], w);
+            }
+        });
+        __syncthreads();
+        if (take) {
+            n = uniform(sh.n_list);
+            if (n > (uint32_t)G::BUCKETS) continue;
+            sort_window(n, c, sh);
+            return Window{base_w, base_w + sh.wsub[G::BUCKETS - 1], 0, base_c, n, 0, 0};
+        }
+        scan_buckets(sh.csub, sh.wsub, sh);
+        pick_bucket(sh.csub, sh.wsub, by_count, target, base_c, base_w, sh);
+        const uint32_t d = uniform(sh.bucket), d_last = uniform(sorted_with<G>(sh.csub, d));
+        const uint64_t behind = (uint64_t)(d_last + 1) << shift;           // keys down to the last part's end
+        k_lo = behind > k_hi - k_lo ? k_lo : k_hi - (uint32_t)behind + 1;
+        k_hi = k_hi - (d << shift);
+        n = uniform(sh.csub[d_last] - (d ? sh.csub[d - 1] : 0)); base_c = uniform(sh.base_c); base_w = uniform(sh.base_w);
+    }
+    u64 each;
+    weigh(key_score(k_lo), c, sh.pow2, each);
+    const int shift = count_columns<G>(view, k_lo, sh);
+    n = sh.csub[G::BUCKETS - 1];
+    return Window{base_w, base_w + n * each, each, base_c, n, k_lo, shift};
+}
+// The item of a sorted window at place e.
+template <class G>
+__device__ __forceinline__ Picked item_at(const Window &x, const uint32_t e, const SampleShared<G> &sh) {
+    const u64 before = e ? sh.wsub[e - 1] : 0, key = sh.sorted[e];
+    return Picked{x.base_w + before, sh.wsub[e] - before, (int32_t)~(uint32_t)key, key_score((uint32_t)(key >> 32))};
+}
+// A threshold's item (its column only if the window is a sorted one).
+template <class G>
+__device__ __forceinline__ Picked threshold_in(const Window &x, const bool by_count, const u64 target, const SampleShared<G> &sh) {
+    const u64 over = target - (by_count ? x.base_c : x.base_w);
+    if (x.each) return Picked{x.base_w + (by_count ? over : over / x.each) * x.each, x.each, -1, key_score(x.key)};
+    return item_at(x, min(by_count ? (uint32_t)over : (uint32_t)bucket_passing<G>(sh.wsub, over), x.n - 1), sh);
+}
+// The draws from `from` on.  target_of(draw), finish(draw, item); a draw that is still open has column OPEN.
+constexpr int32_t OPEN = -2;
+template <class G, int TYPE, class T, class F>
+__device__ __forceinline__ void draw_from_windows(const SampleArgs &a, const int64_t r, const int from, const Unlisted<G, TYPE> &row, const RowView<TYPE> &view,
+                                                  const RowScale &c, const bool counted, T target_of, F finish, SampleShared<G> &sh) {
+    const int tid = threadIdx.x;
+    int32_t *idx = a.idx + r * a.n_draws;                    // thread t writes and reads the draws from + t, from + t + THREADS, ...
+    for (int d = from + tid; d < a.n_draws; d += G::THREADS) idx[d] = OPEN;
+#pragma unroll 1
+    for (int d0 = from; d0 < a.n_draws;) {
+        __syncthreads();
+        if (tid == 0) sh.k_lo = ~0u;
+        __syncthreads();
+        if (d0 + tid < a.n_draws && idx[d0 + tid] == OPEN) atomicMin(&sh.k_lo, (uint32_t)(d0 + tid));
+        __syncthreads();
+        const uint32_t first = uniform(sh.k_lo);
+        if (first == ~0u) {
+            d0 += G::THREADS;
+            continue;
+        }
+        const Window x = window_of(row, view, c, false, target_of((int)first), counted, row.whole, sh);
+#pragma unroll 1
+        for (int d = d0 + tid; d - tid < a.n_draws; d += G::THREADS) {
+            u64 over = 0;
+            bool in = d < a.n_draws && idx[d] == OPEN;
+            if (in) {
+                const u64 target = target_of(d);
+                in = (target >= x.base_w && target < x.end_w) || d == (int)first;        // the first is: it ends the loop
+                over = target - x.base_w;
+            }
+            if (x.each == 0) {
+                if (in) finish(d, item_at(x, min((uint32_t)bucket_passing<G>(sh.wsub, over), x.n - 1), sh));
+                continue;
+            }
+            const uint32_t m = in ? (uint32_t)min(over / x.each, (u64)x.n - 1) : 0;
+            int32_t column = -1;
+            for (u64 mask = __ballot(in); mask; mask &= mask - 1) {      // a wave for one of its draws at a time
+                const int lane = __ffsll(mask) - 1;
+                const int32_t i = nth_column<G>(view, x.key, x.shift, (uint32_t)__builtin_amdgcn_readlane((int)m, lane), sh);
+                if ((tid & 63) == lane) column = i;
+            }
+            if (in) finish(d, Picked{x.base_w + (u64)m * x.each, x.each, column, key_score(x.key)});
+        }
+    }
+}
+
 // Steps 2 to 4 from the running sums in sh.cnt / sh.wsum.  in_lds: the row's items are a list in LDS; then of several draws a
 // wave makes one each, and the workgroup together those that a wave does not (one alone takes a wave as long: 19.7 and 20.2 us
 // for a row of 59 047 at n = 1, but 36 against 31 for 300 rows of 9 724).
-template <class G, int TYPE, class Row>
-__device__ __forceinline__ void answer(const SampleArgs &a, const int64_t r, Row &row, const bool in_lds, const bool counted, const RowView<TYPE> &view, const RowScale &c,
-                       const RowParams &p, SampleShared<G> &sh) {
+template <class G, int TYPE, bool CUT>
+__device__ __forceinline__ void answer(const SampleArgs &a, const int64_t r, const Unlisted<G, TYPE> &row, const bool in_lds, const bool counted,
+                                       const RowView<TYPE> &view, const RowScale &c, const RowParams &p, SampleShared<G> &sh) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     u64 W = uniform(sh.wsum[G::BUCKETS - 1]);
     const bool by_k = top_k_asked(a, p) && (uint32_t)p.top_k < sh.cnt[G::BUCKETS - 1], by_p = p.top_p < 1.f;
@@ -843,19 +1028,43 @@ __device__ __forceinline__ void answer(const SampleArgs &a, const int64_t r, Row
         a.idx[at] = f.index;
         a.logp[at] = (float)(x - (log_of(W, sh.pow2, a.q_bits) - 0.69314718055994530942 * a.q_bits));
     };
+    // Few answers from a list in memory: of each one's bucket alone, as from a list in LDS, if that holds it (64 draws of
+    // a row of a million: 428 us, 780 from windows; 1000, whose list does not fit: 116 and 22 ms).
+    auto from_windows = [&](int step) {                      // this and all later steps
+        for (; step < 0; ++step) {
+            if (step == -1 && !by_p) continue;
+            const u64 target = target_of(step);
+            const Window x = window_of(row, view, c, step == -2, target, counted, false, sh);
+            const Picked f = threshold_in(x, step == -2, target, sh);
+            W = uniform(f.before + f.weight);
+        }
+        draw_from_windows(a, r, step, row, view, c, counted, target_of, finish, sh);
+    };
     int step = by_k ? -2 : by_p ? -1 : 0;
+    if (!in_lds && (!CUT || row.whole || a.n_draws > 256)) {
+        from_windows(step);
+        return;
+    }
+    Listed list{sh.found, row.n};
     while (step < a.n_draws) {                               // uniform
         if (step == -1 && !by_p) {
             step = 0;
             continue;
         }
-        const int many = step < 0 ? 1 : min(G::WAVES, a.n_draws - step);
+        if (CUT && !in_lds) {
+            list.n = bucket_into_lds(row, c, step == -2, target_of(step), sh);
+            if (list.n > (uint32_t)LISTED) {
+                from_windows(step);
+                return;
+            }
+        }
+        const int many = step < 0 || (CUT && !in_lds) ? 1 : min(G::WAVES, a.n_draws - step);
         uint32_t open = (1u << many) - 1;
-        if (in_lds && many > 1) {
+        if (many > 1) {
             bool done = true;
             if (wave < many) {
                 Picked f;
-                done = wave_find<G>(row.found, row.n, c, step == -2, target_of(step + wave), sh, f);
+                done = wave_find<G>(list.found, list.n, c, step == -2, target_of(step + wave), sh, f);
                 if (done && lane == 0) finish(step + wave, f);
             }
             if (lane == 0) sh.wave_c[wave] = !done;
@@ -865,7 +1074,7 @@ __device__ __forceinline__ void answer(const SampleArgs &a, const int64_t r, Row
         while (open) {
             const int mine = step + __ffs(open) - 1;
             open &= open - 1;
-            const Picked f = find<G>(row, view, c, step == -2, target_of(mine), counted, sh);
+            const Picked f = find<G>(list, view, c, step == -2, target_of(mine), counted, sh);
             if (threadIdx.x == 0) finish(mine, f);
         }
         __syncthreads();
@@ -1258,8 +1467,8 @@ __global__ __launch_bounds__(G::THREADS, 4) void sample_rows_kernel(const Sample
         __syncthreads();
     }
     const bool whole = n_found > (uint32_t)LISTED;           // more than the list holds: the answers come from memory
-    ListedRow<G, TYPE> list{view, sh.found, n_found, whole};
-    answer<G>(a, r, list, !whole, counted, view, c, p, sh);
+    const Unlisted<G, TYPE> list{view, sh.found, n_found, whole};
+    answer<G, TYPE, false>(a, r, list, !whole, counted, view, c, p, sh);
 }
 
 // ----------------------------------------------------------------------------- cut rows
@@ -1448,8 +1657,8 @@ __global__ __launch_bounds__(G::THREADS) void part_answer_kernel(const SampleArg
         for (uint32_t q = threadIdx.x; q < n; q += G::THREADS) sh.found[q] = a.found[r * SR_LISTED + q];
         __syncthreads();
     }
-    ListedRow<G, TYPE> row{view, in_lds ? sh.found : a.found + r * SR_LISTED, n, n > SR_LISTED};      // more than the list holds: from memory
-    answer<G>(a, r, row, in_lds, true, view, c, p, sh);
+    const Unlisted<G, TYPE> row{view, a.found + r * SR_LISTED, n, n > SR_LISTED};       // more than the list holds: from the row
+    answer<G, TYPE, true>(a, r, row, in_lds, true, view, c, p, sh);
 }
 
 // ----------------------------------------------------------------------------- host

@@ -63,3 +63,76 @@ def test_many_draws_of_infinite_scores(ops, dtype, n, M, some):
         for r in range(n):
             check_equal_items(idx[r], logp[r], u[r], places, kept)
         assert ms < 50.0, ms                             # a pass over a million items per draw: some hundred
+
+
+def definition(s, u, T, top_k=0, top_p=1.0):
+    """One row in float64: columns, ln q, and whether u W lies clear of a border (weights are integers of 2^-39 of the largest
+    at the least, sums of a million of them within 2^-20 of that)."""
+    s = s.double()
+    rank = torch.sort(s, descending=True, stable=True)
+    w = torch.exp((rank.values - rank.values[0]) / T)
+    w[torch.isnan(w) | (rank.values == -INF)] = 0.0
+    if top_k:
+        w[top_k:] = 0.0
+    sure = True
+    if top_p < 1:
+        cum = torch.cumsum(w, 0)
+        p = float(torch.tensor(top_p, dtype=torch.float32))
+        sure = float(((cum - p * cum[-1]).abs() / cum[-1]).min()) > 1e-12 or bool((w == w[0]).all())
+        w = torch.where(cum - w < p * cum[-1], w, 0.0)
+    cum = torch.cumsum(w, 0)
+    at = torch.searchsorted(cum, u * cum[-1], right=True).clamp(max=int((w > 0).sum()) - 1)
+    gap = torch.minimum((cum[at] - u * cum[-1]).abs(), (u * cum[-1] - (cum[at] - w[at])).abs()) / cum[-1]
+    return rank.indices[at], torch.log(w[at] / cum[-1]), (gap > 1e-11) & sure
+
+
+def rows_of_kind(kind, n, M, g):
+    if kind == "equal":                                  # a user whose factors are 0
+        S = torch.full((n, M), 0.25, device="cuda")
+    elif kind == "five":                                 # quantised scores
+        S = torch.randint(0, 5, (n, M), generator=g, device="cuda").float() * 0.125
+    elif kind == "close":                                # all within a bucket of the histogram, one far below
+        S = 1.0 + 1e-3 * torch.rand(n, M, generator=g, device="cuda")
+        S[:, 3] = -1e20
+    elif kind == "signs":                                # zeros of either sign are one score
+        S = torch.where(torch.rand(n, M, generator=g, device="cuda") < 0.5, -0.0, 0.0)
+    else:
+        S = torch.randn(n, M, generator=g, device="cuda")
+    S[torch.rand(n, M, generator=g, device="cuda") < 0.01] = -INF
+    return S
+
+
+@pytest.mark.parametrize("dtype", sorted(TYPES))
+@pytest.mark.parametrize("kind", ["equal", "five", "close", "signs", "normal"])
+@pytest.mark.parametrize("n, M", [(3, 3001), (2, 40001), (1, 200003), (2, 600001)])
+def test_many_draws_where_thousands_of_items_matter(ops, dtype, kind, n, M):
+    g = gen(M)
+    S = rows_of_kind(kind, n, M, g).to(TYPES[dtype])
+    T = 1e22 if kind == "close" else 1.0
+    draws = 700
+    u = torch.rand(n, draws, generator=g, device="cuda", dtype=torch.float64)
+    u[0, 0], u[0, 1] = 0.0, 1.0 - 2.0 ** -53
+    for kw in (dict(), dict(top_k=M // 3), dict(top_p=0.6), dict(top_k=M // 2, top_p=0.7), dict(top_k=M), dict(top_k=5000)):
+        idx, logp = ops.sample_rows(S, u, temperature=T, **kw)
+        for r in range(n):
+            want, wl, sure = definition(S[r].float(), u[r], T, **kw)
+            assert bool(sure.float().mean() > 0.95) or kw.get("top_p"), (kw, r)
+            assert torch.equal(idx[r][sure].long(), want[sure]), (kw, r)
+            assert torch.allclose(logp[r][sure].double(), wl[sure], rtol=2.0 ** -23, atol=1e-7), (kw, r)
+        one, _ = ops.sample_rows(S, u[:, 5].contiguous(), temperature=T, **kw)     # the same draws, however many are made
+        assert torch.equal(one, idx[:, 5])
+
+
+@pytest.mark.parametrize("kind", ["equal", "five", "normal", "close"])
+def test_a_draw_does_not_cost_a_pass(ops, kind):
+    """As many draws as are taken, of long rows: a second or two at the most (one pass per draw would be minutes)."""
+    g = gen(8)
+    for n, M in ((1, 1000003), (4, 70001)):
+        S = rows_of_kind(kind, n, M, g)
+        u = torch.rand(n, 1 << 16, generator=g, device="cuda", dtype=torch.float64)
+        (idx, _), ms = timed(lambda: ops.sample_rows(S, u, temperature=1.0))
+        print(kind, n, M, "%.1f ms" % ms)
+        for r in range(n):
+            want, _, sure = definition(S[r], u[r], 1.0)
+            assert torch.equal(idx[r][sure].long(), want[sure])
+        assert ms < 5000.0, ms
