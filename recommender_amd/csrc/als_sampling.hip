@@ -66,7 +66,7 @@ constexpr int LISTED = 2048;          // items collected in LDS
 constexpr int SR_LISTED = 16384;      // cut rows: items collected per row
 // A row's draws: some microseconds each from a list in LDS, several of them side by side; where thousands of items matter, a share
 // of the passes over the row that a window takes (draw_from_windows).  65 536 draws, ms: 13 of a row of 1 000 003 equal scores,
-// 23 of five different ones, 250 of a normal distribution's, 1800 where all of it lies within one bucket of the histogram.
+// 23 of five different ones, 210 of a normal distribution's, 1500 where all of it lies within one bucket of the histogram.
 constexpr int32_t DRAWS_MAX = 1 << 16;
 
 struct Found {            // an item collected by a workgroup of a cut row
@@ -849,8 +849,14 @@ __device__ __forceinline__ void sort_window(const uint32_t n, const RowScale &c,
                 const u64 x = sh.sorted[lo], y = sh.sorted[hi];
                 if ((lo & run) == 0 ? x < y : x > y) { sh.sorted[lo] = y; sh.sorted[hi] = x; }
             }
-            __syncthreads();
+            // a wave's 64 pairs of up to 64 apart are 128 neighbours: until pairs are further apart no other wave touches them
+            if (step > 64 || (step == 1 && run > 64)) __syncthreads();
+            else {
+                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_wave_barrier();
+            }
         }
+    __syncthreads();
 #pragma unroll 1
     for (int q = tid; q < G::BUCKETS; q += G::THREADS) {
         u64 w = 0;
@@ -900,6 +906,9 @@ __device__ __forceinline__ Window window_of(const Unlisted<G, TYPE> &row, const 
     const float width = 1.f / c.per_score;                   // keys in question as in find
     uint32_t k_hi = uniform(rank_key(fminf(c.top_f - (float)((int)b - 1) * width, c.top_f)));
     uint32_t k_lo = uniform(last == G::BUCKETS - 1 ? 0 : rank_key(c.top_f - (float)(last + 2) * width));
+    // Scores well above the cut have a weight.  (2 % above it, and a min_p that is not within 10^-4 of 1: then 0.98 of the way to
+    // it leaves more than min_p.)
+    const bool all_weigh = last < (uint32_t)(G::BUCKETS * 49 / 50) && c.cut > 0.1;
 #pragma unroll 1
     for (;;) {
         __syncthreads();
@@ -910,16 +919,18 @@ __device__ __forceinline__ Window window_of(const Unlisted<G, TYPE> &row, const 
         for (int q = 0; q < G::OWN; ++q) { sh.csub[G::OWN * tid + q] = 0; sh.wsub[G::OWN * tid + q] = 0; }
         if (tid == 0) sh.n_list = 0;
         __syncthreads();
-        bool full = false;                                   // one item too many says enough
+        // by the scores first, which is the same as by their keys: two comparisons are all that most items of a pass cost
+        float lo = k_lo > rank_key(-__builtin_inff()) ? key_score(k_lo) : -__builtin_inff();
+        const float hi = key_score(k_hi);
         row.each([&](const float s, const int32_t i) {
-            if (full || bucket_of<G::BUCKETS>(s, c) - b > last - b) return;
-            const uint32_t key = rank_key(s);
+            if (!(s >= lo && s <= hi)) return;
             u64 w;
-            if (key < k_lo || key > k_hi || !weigh(s, c, sh.pow2, w)) return;
+            if (bucket_of<G::BUCKETS>(s, c) - b > last - b || (!(take && all_weigh) && !weigh(s, c, sh.pow2, w))) return;
+            const uint32_t key = rank_key(s);
             if (take) {
                 const uint32_t at = atomicAdd(&sh.n_list, 1u);
-                full = at >= (uint32_t)G::BUCKETS;
-                if (!full) sh.sorted[at] = (u64)key << 32 | (uint32_t)~(uint32_t)i;
+                if (at >= (uint32_t)G::BUCKETS) lo = __builtin_inff();      // one item too many says enough
+                else sh.sorted[at] = (u64)key << 32 | (uint32_t)~(uint32_t)i;
             } else {
                 const uint32_t d = (k_hi - key) >> shift;    // in rank order
                 atomicAdd(&sh.csub[d], 1u);
@@ -1029,7 +1040,7 @@ __device__ __forceinline__ void answer(const SampleArgs &a, const int64_t r, con
         a.logp[at] = (float)(x - (log_of(W, sh.pow2, a.q_bits) - 0.69314718055994530942 * a.q_bits));
     };
     // Few answers from a list in memory: of each one's bucket alone, as from a list in LDS, if that holds it (64 draws of
-    // a row of a million: 428 us, 780 from windows; 1000, whose list does not fit: 116 and 22 ms).
+    // a row of a million: 438 us, 780 from windows; 1000, whose list does not fit: 116 ms so, 15 from windows).
     auto from_windows = [&](int step) {                      // this and all later steps
         for (; step < 0; ++step) {
             if (step == -1 && !by_p) continue;
