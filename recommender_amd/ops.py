@@ -648,6 +648,28 @@ def _row_param(v, n, dtype, name, like):
     return (int(v) if dtype == torch.int32 else float(v)), None
 
 
+def _draw_args(u, temperature, top_k, top_p, min_p, n, like):
+    """The checked (scalar, per-row tensor) pairs of the four parameters of n rows, and u checked."""
+    if not isinstance(u, torch.Tensor) or u.dtype not in (torch.float32, torch.float64):
+        raise ValueError("u must be a float32 or float64 tensor")
+    if u.dim() not in (1, 2) or u.shape[0] != n or (u.dim() == 2 and u.shape[1] < 1):
+        raise ValueError("u must be [n_rows] or [n_rows, n_draws]")
+    if u.dim() == 2 and u.shape[1] > 1 << 16:
+        raise ValueError("at most 2^16 draws per row, got %d" % u.shape[1])
+    if not u.is_cuda or not u.is_contiguous():
+        raise ValueError("u must be a contiguous CUDA/HIP tensor")
+    pairs = (_row_param(temperature, n, torch.float32, "temperature", like), _row_param(top_k, n, torch.int32, "top_k", like),
+             _row_param(top_p, n, torch.float32, "top_p", like), _row_param(min_p, n, torch.float32, "min_p", like))
+    (t, _), (k, _), (p, _), (m, _) = pairs
+    if not t >= 0:
+        raise ValueError("temperature must be >= 0")
+    if not 0 <= k < 2 ** 31:
+        raise ValueError("top_k must be >= 0 (0: off)")
+    if not (0 <= p <= 1 and 0 <= m <= 1):
+        raise ValueError("top_p and min_p must lie in [0, 1]")
+    return pairs
+
+
 def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, exclude=None, exclude_rows=None):
     """Random columns of every score row (float32, float16 or bfloat16), drawn from the row's softmax at `temperature` cut
     by min_p, top_k and top_p in this order (als_sample_rows in include/als_hip.h has the definition).  u: the random
@@ -660,24 +682,7 @@ def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, e
     holds."""
     dtype, ld = _score_rows(score_rows, "score_rows")
     n, M = score_rows.shape
-    if not isinstance(u, torch.Tensor) or u.dtype not in (torch.float32, torch.float64):
-        raise ValueError("u must be a float32 or float64 tensor")
-    if u.dim() not in (1, 2) or u.shape[0] != n or (u.dim() == 2 and u.shape[1] < 1):
-        raise ValueError("u must be [n_rows] or [n_rows, n_draws]")
-    if u.dim() == 2 and u.shape[1] > 1 << 16:
-        raise ValueError("at most 2^16 draws per row, got %d" % u.shape[1])
-    if not u.is_cuda or not u.is_contiguous():
-        raise ValueError("u must be a contiguous CUDA/HIP tensor")
-    t, t_rows = _row_param(temperature, n, torch.float32, "temperature", score_rows)
-    k, k_rows = _row_param(top_k, n, torch.int32, "top_k", score_rows)
-    p, p_rows = _row_param(top_p, n, torch.float32, "top_p", score_rows)
-    m, m_rows = _row_param(min_p, n, torch.float32, "min_p", score_rows)
-    if not t >= 0:
-        raise ValueError("temperature must be >= 0")
-    if not 0 <= k < 2 ** 31:
-        raise ValueError("top_k must be >= 0 (0: off)")
-    if not (0 <= p <= 1 and 0 <= m <= 1):
-        raise ValueError("top_p and min_p must lie in [0, 1]")
+    (t, t_rows), (k, k_rows), (p, p_rows), (m, m_rows) = _draw_args(u, temperature, top_k, top_p, min_p, n, score_rows)
     ex_ptr = ex_col = None
     if exclude is not None:
         ex_ptr, ex_col = exclude
@@ -938,8 +943,7 @@ def recommend_sample(X, Y, users, u, temperature=1.0, top_k=0, top_p=1.0, min_p=
     M = Y.shape[0] if M is None else int(M)
     _index(users, torch.int64, "users")
     nu = users.shape[0]
-    if not isinstance(u, torch.Tensor) or u.dim() not in (1, 2) or u.shape[0] != nu:
-        raise ValueError("u must be [n_users] or [n_users, n_draws]")
+    _draw_args(u, temperature, top_k, top_p, min_p, nu, X)
     _same_device(X, users, u)
     idx = torch.empty(u.shape, dtype=torch.int32, device=X.device)
     logp = torch.empty(u.shape, dtype=torch.float32, device=X.device)

@@ -1,0 +1,54 @@
+"""GPU tests of what the softmax operators make of their arguments: refusals at the entry, whatever path a call takes."""
+import warnings
+
+import numpy as np
+import pytest
+
+torch = pytest.importorskip("torch")
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def ops():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    from recommender_amd import ops
+    return ops
+
+
+@pytest.fixture
+def model(ops):
+    g = torch.Generator(device="cuda")
+    g.manual_seed(1)
+    X = torch.randn(90, 16, generator=g, device="cuda")
+    Y = torch.randn(1500, 16, generator=g, device="cuda")
+    users = torch.randint(0, 90, (70,), generator=g, device="cuda")
+    u = torch.rand(70, 3, generator=g, device="cuda")
+    return X, Y, users, u
+
+
+@pytest.mark.parametrize("block", [4096, 16])
+@pytest.mark.parametrize("length", [69, 71, 1, 140])
+@pytest.mark.parametrize("name", ["temperature", "top_k", "top_p", "min_p"])
+@pytest.mark.parametrize("top_k", [0, 20])
+def test_recommend_sample_refuses_parameters_of_another_length(ops, model, name, length, block, top_k):
+    """On the path through the list (one top_k) and through the scores, and whichever block a parameter would end in."""
+    X, Y, users, u = model
+    kw = dict(top_k=top_k, block_users=block)
+    kw[name] = torch.full((length,), 3, dtype=torch.int32, device="cuda") if name == "top_k" else torch.full((length,), 0.5, device="cuda")
+    with pytest.raises(ValueError):
+        ops.recommend_sample(X, Y, users, u, **kw)
+
+
+@pytest.mark.parametrize("top_k", [0, 20])
+def test_recommend_sample_refuses_at_the_entry(ops, model, top_k):
+    X, Y, users, u = model
+    rows = torch.ones(70, device="cuda")
+    for kw in (dict(u=u.half()), dict(u=u[:69]), dict(u=u.cpu()), dict(u=u.t().contiguous().t()), dict(u=u[:, :0]),
+               dict(u=torch.zeros(70, (1 << 16) + 1, device="cuda")), dict(temperature=-1.0), dict(temperature=float("nan")),
+               dict(top_p=1.5), dict(min_p=-0.1), dict(temperature=rows.double()), dict(temperature=rows.cpu()),
+               dict(top_p=torch.ones(140, device="cuda")[::2]), dict(top_k=-1), dict(users=users.int()), dict(users=users + 50)):
+        args = dict(dict(users=users, u=u, top_k=top_k), **kw)
+        with pytest.raises(ValueError):
+            ops.recommend_sample(X, Y, args.pop("users"), args.pop("u"), **args)
