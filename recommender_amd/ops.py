@@ -573,9 +573,15 @@ def scores(X, Y, user_ids=None, M=None, out=None):
     if out.shape[0] < nu or out.shape[1] < M or out.stride(1) != 1:
         raise ValueError("out too small or not row-major")
     _same_device(X, prepared.table if prepared else Y, user_ids, out)
+    return _launch_scores(X, ldx, Y, ldy, user_ids, nu, M, out)
+
+
+def _launch_scores(X, ldx, Y, ldy, user_ids, nu, M, out):
+    """scores() of checked arguments."""
+    f = X.shape[1]
     with torch.cuda.device(X.device):
-        if prepared:
-            check(lib.als_scores_prepared_f32(_ptr(X), ldx, _ptr(user_ids), nu, _ptr(prepared.table), prepared.shape[0], M,
+        if isinstance(Y, PreparedItems):
+            check(lib.als_scores_prepared_f32(_ptr(X), ldx, _ptr(user_ids), nu, _ptr(Y.table), Y.shape[0], M,
                                               f, _ptr(out), out.stride(0), _stream()), "als_scores_prepared_f32")
         else:
             check(lib.als_scores_f32(_ptr(X), ldx, _ptr(user_ids), nu, _ptr(Y), ldy, M, f, _ptr(out), out.stride(0),
@@ -699,6 +705,13 @@ def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, e
     elif exclude_rows is not None:
         raise ValueError("exclude_rows without exclude")
     _same_device(score_rows, u, ex_ptr, ex_col, exclude_rows)
+    return _launch_draws(score_rows, dtype, ld, u, (t, t_rows), (k, k_rows), (p, p_rows), (m, m_rows), ex_ptr, ex_col, exclude_rows)
+
+
+def _launch_draws(score_rows, dtype, ld, u, temperature, top_k, top_p, min_p, ex_ptr, ex_col, exclude_rows):
+    """sample_rows() of checked arguments, the parameters as _draw_args leaves them."""
+    n, M = score_rows.shape
+    (t, t_rows), (k, k_rows), (p, p_rows), (m, m_rows) = temperature, top_k, top_p, min_p
     idx = u.new_empty(u.shape, dtype=torch.int32)
     logp = u.new_empty(u.shape, dtype=torch.float32)
     if n == 0:
@@ -940,32 +953,40 @@ def recommend_sample(X, Y, users, u, temperature=1.0, top_k=0, top_p=1.0, min_p=
 
     A single top_k of 1 to 1024 draws from recommend_topk's list (no score matrix): the kept items are the same, being the
     first in rank order either way.  Otherwise the scores of a block are materialised, at most 4 GiB at a time."""
+    prepared = isinstance(Y, PreparedItems)
+    ldx = _factor_ld(X, "X"); ldy = 0 if prepared else _factor_ld(Y, "Y")
     M = Y.shape[0] if M is None else int(M)
+    if Y.shape[1] != X.shape[1] or not (1 <= M <= Y.shape[0]):
+        raise ValueError("factor counts differ or M out of range")
     _index(users, torch.int64, "users")
     nu = users.shape[0]
-    _draw_args(u, temperature, top_k, top_p, min_p, nu, X)
-    _same_device(X, users, u)
-    idx = torch.empty(u.shape, dtype=torch.int32, device=X.device)
-    logp = torch.empty(u.shape, dtype=torch.float32, device=X.device)
+    pairs = _draw_args(u, temperature, top_k, top_p, min_p, nu, X)
+    _same_device(X, Y.table if prepared else Y, users, u)
     if nu == 0:
-        return idx, logp
-    part = lambda v, s, e: v[s:e] if torch.is_tensor(v) and v.dim() else v  # noqa: E731
-    if not (torch.is_tensor(top_k) and top_k.dim()) and 1 <= int(top_k) <= min(1024, M):
-        items, val = recommend_topk(X, Y, users, int(top_k), M, exclude_csr, block_users)
+        return torch.empty(u.shape, dtype=torch.int32, device=X.device), torch.empty(u.shape, dtype=torch.float32, device=X.device)
+    (k, k_rows) = pairs[1]
+    if k_rows is None and 1 <= k <= min(1024, M):
+        items, val = recommend_topk(X, Y, users, k, M, exclude_csr, block_users)
         at, logp = sample_rows(val, u, temperature, 0, top_p, min_p)
         got = torch.gather(items, 1, at.reshape(nu, -1).clamp(min=0).long()).reshape(u.shape)
         return torch.where(at < 0, at, got), logp
-    ex = None
+    # ids are looked at once, not per block: a look waits for the device
+    top = int(users.max())
+    if int(users.min()) < 0 or top >= X.shape[0]:
+        raise ValueError("user id out of range")
+    ex_ptr = ex_col = None
     if exclude_csr is not None:
-        ex = device_exclusions(exclude_csr, X.device)
-    rows_per = max(1, min(block_users, max(nu, 1), (1 << 30) // max(M, 1)))
-    buf = None
+        ex_ptr, ex_col = device_exclusions(exclude_csr, X.device)
+        if top + 1 >= ex_ptr.shape[0]:
+            raise ValueError("a user id lies outside the exclusion CSR")
+    idx = torch.empty(u.shape, dtype=torch.int32, device=X.device)
+    logp = torch.empty(u.shape, dtype=torch.float32, device=X.device)
+    rows_per = max(1, min(block_users, nu, (1 << 30) // M))
+    buf = torch.empty((min(rows_per, nu), M), dtype=torch.float32, device=X.device)
     for s in range(0, nu, rows_per):
         e = min(nu, s + rows_per)
-        if buf is None:
-            buf = torch.empty((min(rows_per, nu), M), dtype=torch.float32, device=X.device)
-        sc = scores(X, Y, users[s:e], M, out=buf)
-        i_, l_ = sample_rows(sc, u[s:e], part(temperature, s, e), part(top_k, s, e), part(top_p, s, e), part(min_p, s, e), ex,
-                             users[s:e] if ex else None)
-        idx[s:e] = i_; logp[s:e] = l_
+        sc = _launch_scores(X, ldx, Y, ldy, users[s:e], e - s, M, buf)
+        part = [(v, None if rows is None else rows[s:e]) for v, rows in pairs]
+        idx[s:e], logp[s:e] = _launch_draws(sc, _lib.DTYPES[torch.float32], M, u[s:e], *part, ex_ptr, ex_col,
+                                            None if ex_ptr is None else users[s:e])
     return idx, logp

@@ -1,6 +1,8 @@
 """GPU tests of what the softmax operators make of their arguments: refusals at the entry, whatever path a call takes."""
 import warnings
 
+import warnings
+
 import numpy as np
 import pytest
 
@@ -52,3 +54,34 @@ def test_recommend_sample_refuses_at_the_entry(ops, model, top_k):
         args = dict(dict(users=users, u=u, top_k=top_k), **kw)
         with pytest.raises(ValueError):
             ops.recommend_sample(X, Y, args.pop("users"), args.pop("u"), **args)
+
+
+def waits_for_the_device(call):
+    torch.cuda.synchronize()
+    with warnings.catch_warnings(record=True) as seen:
+        warnings.simplefilter("always")
+        torch.cuda.set_sync_debug_mode("warn")
+        try:
+            call()
+        finally:
+            torch.cuda.set_sync_debug_mode("default")
+    return sum("called a synchronizing" in str(w.message) for w in seen)
+
+
+@pytest.mark.parametrize("excluded", [False, True])
+def test_recommend_sample_waits_as_often_for_many_blocks_as_for_one(ops, model, excluded):
+    X, Y, users, u = model
+    ex = ops.device_exclusions((np.arange(91, dtype=np.int64) * 5, np.tile(np.arange(5, dtype=np.int32), 90)), X.device) if excluded else None
+    counts = []
+    answers = []
+    for block in (4096, 7):
+        call = lambda: answers.append(ops.recommend_sample(X, Y, users, u, top_p=0.9, exclude_csr=ex, block_users=block))  # noqa: E731
+        call()
+        counts.append(waits_for_the_device(call))
+    assert counts[0] == counts[1], counts
+    assert torch.equal(answers[0][0], answers[-1][0]) and torch.equal(answers[0][1], answers[-1][1])
+    if excluded:
+        assert int(answers[0][0].min()) >= 5
+        short = ops.device_exclusions((np.zeros(50, dtype=np.int64), np.zeros(0, dtype=np.int32)), X.device)
+        with pytest.raises(ValueError):
+            ops.recommend_sample(X, Y, users, u, top_p=0.9, exclude_csr=short)
