@@ -776,9 +776,10 @@ def distill_rows(score_rows, teacher_idx, teacher_val, temperature=1.0, weight=N
         if ldo != ld:
             raise ValueError("out is laid over score_rows with another row stride")
     elif n and out.untyped_storage().data_ptr() == score_rows.untyped_storage().data_ptr():
-        a, b = score_rows.data_ptr(), out.data_ptr()
-        size = score_rows.element_size()
-        if a < b + ((n - 1) * ldo + M) * size and b < a + ((n - 1) * ld + M) * size:
+        # elements from a score to out's at the same place, and to the row of scores at or in front of that
+        gap = (out.data_ptr() - score_rows.data_ptr()) // score_rows.element_size()
+        apart = gap >= (n - 1) * ld + M or -gap >= (n - 1) * ldo + M
+        if not apart and (ldo != ld or gap % ld < M or gap % ld > ld - M):
             raise ValueError("out overlaps score_rows without being it")
     _same_device(score_rows, weight, out)
     loss = teacher_val.new_empty(n)

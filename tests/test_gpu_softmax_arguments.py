@@ -85,3 +85,32 @@ def test_recommend_sample_waits_as_often_for_many_blocks_as_for_one(ops, model, 
         short = ops.device_exclusions((np.zeros(50, dtype=np.int64), np.zeros(0, dtype=np.int32)), X.device)
         with pytest.raises(ValueError):
             ops.recommend_sample(X, Y, users, u, top_p=0.9, exclude_csr=short)
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.float16, torch.bfloat16])
+@pytest.mark.parametrize("swap", [False, True])
+def test_distill_rows_writes_beside_the_scores_in_one_buffer(ops, dtype, swap):
+    """Scores and gradient as two column blocks of one buffer share no element; any that do are refused."""
+    n, M = 9, 701
+    buf = torch.randn(n, 2 * M + 3, device="cuda").to(dtype)
+    idx = torch.randint(0, M, (n, 20), device="cuda", dtype=torch.int32)
+    val = torch.randn(n, 20, device="cuda")
+    S, out = buf[:, :M], buf[:, M + 3:]
+    if swap:
+        S, out = out, S
+    kept = S.clone()
+    want = ops.distill_rows(kept, idx, val)
+    loss, grad = ops.distill_rows(S, idx, val, out=out)
+    assert grad is out and torch.equal(S, kept) and torch.equal(loss, want[0])
+    assert torch.allclose(out.float(), want[1].float(), rtol=2.0 ** -7, atol=1e-6)
+    for a in (1, M // 2, M - 1):
+        with pytest.raises(ValueError):
+            ops.distill_rows(buf[:, :M], idx, val, out=buf[:, a:a + M])
+        with pytest.raises(ValueError):
+            ops.distill_rows(buf[:, a:a + M], idx, val, out=buf[:, :M])
+    with pytest.raises(ValueError):                      # a row further down
+        ops.distill_rows(buf[:-1, :M], idx[:-1], val[:-1], out=buf[1:, :M])
+    flat = buf.flatten()
+    with pytest.raises(ValueError):                      # other row strides, which meet somewhere
+        ops.distill_rows(flat[: 4 * 1000].view(4, 1000)[:, :M], idx[:4], val[:4], out=flat[M: M + 4 * 1100].view(4, 1100)[:, :M])
+    ops.distill_rows(flat[: 4 * M].view(4, M), idx[:4], val[:4], out=flat[4 * M: 8 * M].view(4, M))
