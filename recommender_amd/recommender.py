@@ -64,6 +64,7 @@ class RecommenderALS:
         self._eval_keys = None         # sorted (user, item) keys of the training pairs / relevant test pairs, on the device
         self.engine = None
         self._foldin_cache = None
+        self._distilled = False        # whether the item factor has been changed since the engine's Gram was taken
         self._exclusions = None
         self._prepared = None          # the item factor in the score kernel's operand form, built on the first recommend()
         self.start_epoch = 0
@@ -140,6 +141,7 @@ class RecommenderALS:
         for epoch in range(self.start_epoch, epochs):
             self.engine.step()
             self._prepared = None                     # the item factor has changed
+            self._distilled = False
             self.trace.append(self.engine.last_delta())
             if do_eval:
                 self.eval_epochs.append(epoch); self.eval_scores.append(self.evaluate())
@@ -214,6 +216,7 @@ class RecommenderALS:
                 self.trace = [float(t) for t in fp.read().strip().split("\n")[1:]][: self.start_epoch]
         self.engine = None
         self._foldin_cache = None
+        self._distilled = False
         self._prepared = None
         return self
 
@@ -299,8 +302,9 @@ class RecommenderALS:
         loss, dX, dY = ops.distill_topk(self.X, self.Y, uid, ti, tv, temperature=temperature, weight=w, M=self.n_items)
         self.X.index_add_(0, uid, dX, alpha=-float(lr))
         self.Y[: self.n_items].add_(dY, alpha=-float(lr))
-        self._prepared = None                             # the item factor has changed
+        self._prepared = None                             # the item factor has changed, and no Gram taken before is its
         self._foldin_cache = None
+        self._distilled = True
         return float(loss.double().mean().item())
 
     def _rated(self):
@@ -365,7 +369,7 @@ class RecommenderALS:
         refresh_gram=True (default) computes the item Gram from the current Y first.  refresh_gram=False
         reproduces the reference: the cached Gram is used as it stands (ALS.py:385 passes the cache 'Y2' and never
         refreshes it) - after train() that is the Gram taken before the last item sweep (ALS.py:345-349), after a
-        load it is fresh (ALS.py:301-308), and later fold-ins keep using it."""
+        load or a distill() it is fresh (ALS.py:301-308), and later fold-ins keep using it."""
         csr = rows if (cols is None and vals is None) else self.make_update_data((rows, cols, vals))
         if isinstance(csr, list) and not csr:
             return
@@ -373,7 +377,7 @@ class RecommenderALS:
             raise ValueError("update_user takes (rows, cols, vals) or the result of make_update_data")
         if refresh_gram:
             cache = ops.gram(self.Y, self.config["lamb"])
-        elif self.engine is not None and self.trace:
+        elif self.engine is not None and self.trace and not self._distilled:
             cache = self.engine.cache_Y                # as the last training epoch left it
         else:                                          # nothing trained in this object: computed once, then reused
             if self._foldin_cache is None:
