@@ -792,6 +792,11 @@ def distill_rows(score_rows, teacher_idx, teacher_val, temperature=1.0, weight=N
     return loss, out
 
 
+def distill_topk_workspace(n, M, f, k):
+    """Bytes of device memory that a distill_topk call of these sizes takes for itself (0: sizes it refuses)."""
+    return lib.als_distill_topk_workspace_bytes(int(n), int(M), int(f), int(k))
+
+
 def distill_topk(X, Y, users, teacher_idx, teacher_val, temperature=1.0, weight=None, M=None):
     """distill_rows for the scores <X[users], Y[:M]> of two float32 factors, without the score matrix, and with the
     gradients of the factors instead of the scores' (als_distill_topk_f32 in include/als_hip.h).  users: int64 device
@@ -822,7 +827,7 @@ def distill_topk(X, Y, users, teacher_idx, teacher_val, temperature=1.0, weight=
     if n == 0:
         return loss, dX, X.new_zeros((M, f))
     dY = X.new_empty((M, f))
-    need = lib.als_distill_topk_workspace_bytes(n, M, f, k)
+    need = distill_topk_workspace(n, M, f, k)
     ws = torch.empty(need, dtype=torch.uint8, device=X.device)
     _enqueue("als_distill_topk_f32", X.device, _addr(X), X.shape[0], ldx, _addr(users), n, _addr(Y), ldy, M, f, _addr(teacher_idx),
              _addr(teacher_val), ldt, k, T, _addr(weight), _addr(loss), _addr(dX), _addr(dY), _addr(ws), need)

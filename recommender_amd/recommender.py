@@ -41,6 +41,8 @@ DEFAULTS = dict(f=20,           # ALS.json.template:26 (the reference's layer wi
 
 
 class RecommenderALS:
+    DISTILL_BYTES = 4 << 30            # of workspace for a step of distill(): more users than that takes go in several calls
+
     def __init__(self, mode="train", n_users=None, n_items=None, als_kwargs=None, model_path=None, device=None):
         if mode not in ("train", "predict"):
             raise ValueError("mode must be 'train' or 'predict'")
@@ -295,11 +297,24 @@ class RecommenderALS:
             raise ValueError("user id outside the model")
         ti = teacher_idx.cpu().numpy() if torch.is_tensor(teacher_idx) else np.asarray(teacher_idx)
         tv = teacher_scores.cpu().numpy() if torch.is_tensor(teacher_scores) else np.asarray(teacher_scores)
+        if ti.ndim != 2 or tv.shape != ti.shape or len(ti) != len(users):
+            raise ValueError("teacher_idx and teacher_scores must both be [n_users, k]")
         ti = torch.as_tensor(np.where((ti >= 0) & (ti < self.n_items), ti, -1).astype(np.int32), device=self.device)
         tv = torch.as_tensor(np.ascontiguousarray(tv, dtype=np.float32), device=self.device)
         uid = self._idx(users)
         w = torch.full((len(users),), 1.0 / len(users), dtype=torch.float32, device=self.device)
-        loss, dX, dY = ops.distill_topk(self.X, self.Y, uid, ti, tv, temperature=temperature, weight=w, M=self.n_items)
+        # as many users a call as its workspace (its list offsets grow with users times items) leaves memory for
+        step = len(users)
+        while step > 32 and ops.distill_topk_workspace(step, self.n_items, self.X.shape[1], ti.shape[-1]) > self.DISTILL_BYTES:
+            step = (step + 1) // 2
+        losses, grads, dY = [], [], None
+        for s in range(0, len(users), step):
+            part = slice(s, s + step)
+            loss, dX, d = ops.distill_topk(self.X, self.Y, uid[part], ti[part], tv[part], temperature=temperature, weight=w[part],
+                                           M=self.n_items)
+            losses.append(loss); grads.append(dX)
+            dY = d if dY is None else dY.add_(d)
+        loss, dX = (losses[0], grads[0]) if len(grads) == 1 else (torch.cat(losses), torch.cat(grads))
         self.X.index_add_(0, uid, dX, alpha=-float(lr))
         self.Y[: self.n_items].add_(dY, alpha=-float(lr))
         self._prepared = None                             # the item factor has changed, and no Gram taken before is its
