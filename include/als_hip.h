@@ -451,16 +451,16 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  *                    largest lose bits); of c x by one per user (below 2^-18 of the user's largest); of q in dX by one per user
  *                    (below 2^-14 of the user's largest, none by more than 2^-37 of that), of q - t in dY by one per item (below
  *                    2^-10 of the item's largest over the users, none by more than 2^-33 of that).  Gradients are summed over
- *                    parts of at most 32768 items or users (as long as that makes 512 parts or fewer), ln Z in float32
- *                    over 16 items and float64 above; the parts are joined in float32.  Weights
- *                    may be of any size: what a user adds to dY is right beside any other's, down to 2^-126 of the
+ *                    parts of at most 32768 items or users (while that makes 512 parts or fewer), ln Z in float32 over 16
+ *                    items and float64 above; the parts are joined in float32.  Weights may be of any size: what a user adds to dY is right beside any other's, down to 2^-126 of the
  *                    largest c x.  The weight of a user whose list is empty, or unknown, is not looked at.
  *                    8 n M f operations, three products each.  Workspace, with F = f rounded up to 32, 64, 128 or 256: the
- *                    operands, 8 (n + M) F bytes; the parts of split sums, 4 F n and, where pass 2 is split, 4 F M times the
- *                    parts; the lists, 8 n k; and where each list enters each block of 256 items (128 for F = 256), 2 n M / 256:
- *                    the largest where both are large, 8 GB for a million users of a million items (call for blocks of
- *                    users and add up dY).  Up to 4 users (8 where M >= 65536 and f <= 128) are
- *                    computed in float32 products from one read of the item factor, with 4 n M bytes of workspace.
+ *                    operands, 8 (n + M) F bytes; the parts of split sums, 4 F n each and, where pass 2 has more than one,
+ *                    4 F M each; the lists, 8 n k; and where each list enters each block of 256 items (128 for F = 256),
+ *                    2 n M / 256.  Parts and lists' places grow with users times items: 26 GB for a million users of a
+ *                    million items at f = 64, 4 GB for 131072 (call for blocks of users, and add up dY).  Up to 4 users (8
+ *                    where M >= 65536 and f <= 128) are computed in float32 products from one read of the item factor,
+ *                    with 4 n M bytes of workspace.
  * ------------------------------------------------------------------------------------ */
 size_t als_distill_topk_workspace_bytes(int64_t n_users, int64_t M, int32_t f, int32_t k);
 int32_t als_distill_topk_f32(const float *X, int64_t x_rows, int64_t ldx, const int64_t *user_ids, int64_t n_users, const float *Y,

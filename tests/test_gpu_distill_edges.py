@@ -218,3 +218,25 @@ def test_ln_z_of_many_users(ops):
     want = -math.log(2.0) - 2.5 * x + torch.log(torch.exp(4 * x) + (M - 1) * torch.exp(x))
     # scores within 2^-20 of up to 2.4, both in ln Z and in the terms; logarithms and sums of float32 numbers up to 16
     assert float((loss.double() - want[users]).abs().max()) <= 2 * 2.4 * 2.0 ** -20 + 4 * 16 * 2.0 ** -24
+
+
+@pytest.mark.parametrize("first", [(1 << 21) - 40, (1 << 21) + 45 - 80, 1_000_003])
+def test_the_items_gradients_of_users_on_every_axis_of_a_launch(ops, first):
+    """More users than one launch axis takes, of which 80 weigh anything: dY is theirs, to what 80 terms allow.  (All weighted
+    alike, what the users behind the first axis add would be lost in the tolerance of a sum over two million.)"""
+    n, M, f, k = (1 << 21) + 45, 40, 8, 3
+    g = gen(52)
+    X = torch.rand(n, f, generator=g, device="cuda") * 2 - 1
+    Y = torch.rand(M, f, generator=g, device="cuda") * 2 - 1
+    idx = (torch.randint(0, M - k, (n, 1), generator=g, device="cuda") + torch.arange(k, device="cuda")).to(torch.int32)
+    val = torch.randn(n, k, generator=g, device="cuda")
+    part = slice(first, first + 80)
+    w = torch.zeros(n, device="cuda")
+    w[part] = torch.rand(80, generator=g, device="cuda") + 0.5
+    loss, dX, dY = ops.distill_topk(X, Y, None, idx, val, weight=w)
+    wl, wx, wy, mag, d = formula(X[part], Y, idx[part], val[part], 1.0, w[part])
+    tol = (mag * rel_tolerance(d, 80)).T.contiguous() @ X[part].double().abs() + 2.0 ** -33 * mag.sum(0)[:, None]
+    assert off_over_tolerance(dY, wy, tol) <= 1.0
+    assert off_over_tolerance(dX[part], wx, rel_tolerance(d, M) * (mag @ Y.double().abs())) <= 1.0
+    assert not dX[: first].any() and not dX[first + 80:].any()
+    assert off_over_tolerance(loss[part], wl, 1e-5 + 1e-5 * wl.abs()) <= 1.0
