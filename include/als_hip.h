@@ -399,7 +399,8 @@ int32_t als_recommend_topk_prepared_f32(const float *X, int64_t ldx, const int64
  * Q = min(51, 62 - ceil(log2 M)); an item below half of that counts as dropped.  The answer depends on the row and its
  * parameters alone.
  * Rows of at most 2^31 - 2^16 columns, at most 2^16 draws per row.
- * opts      [host] one value for all rows, or a [device] array with one per row where the pointer is not NULL.
+ * opts      [host] one value for all rows, or a [device] array with one per row where the pointer is not NULL.  float32 either
+ *           way: top_p = 0.3f is a little more than three tenths, which ten equal items share as four.
  * ex_*      as als_topk_rows_f32: those columns are set to -inf first, in place; columns outside [0, M) are ignored.
  * All other pointers are [device].  Few long rows need a workspace of als_sample_rows_workspace_bytes bytes (0: none, the
  * pointer may be NULL).
@@ -426,7 +427,7 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
 /* ------------------------------------------------------------------------------------
  * Following a teacher's ranked lists (no reference counterpart): how far a student's softmax over all items is from a
  * teacher's softmax over the few items it lists (what als_recommend_topk_f32 returned for a larger model, say), and the
- * gradient of that.  Per row, at temperature T (> 0, finite):
+ * gradient of that.  Per row, at temperature T (in [1e-30, 1e30]):
  *     t_j = softmax of teacher_val / T over the row's list,   q_i = softmax of the student's scores / T over all M items
  *     loss = sum_j t_j (ln t_j - ln q_j),                     slope_i = weight (q_i - t_i) / T   (t_i = 0 off the list)
  * teacher_idx / teacher_val [n_rows, ld_teacher] int32 / float32, the first k (<= 1024) of a row; an index outside [0, M)

@@ -367,8 +367,8 @@ int32_t als_distill_rows(const void *scores, int32_t dtype, int64_t lds, int64_t
         return als_fail_(ALS_ERR_UNSUPPORTED, "als_distill_rows: dtype %d (0 float32, 1 float16, 2 bfloat16)", dtype);
     if (((uintptr_t)scores | (uintptr_t)grad_out) % (dtype == ALS_DTYPE_F32 ? 4 : 2))
         return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_rows: scores or gradient are not aligned to their type");
-    if (!(temperature > 0.f) || !(1.f / temperature > 0.f) || !(1.f / temperature < 3e38f))
-        return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_rows: temperature %g", (double)temperature);
+    if (!(temperature >= 1e-30f && temperature <= 1e30f))     // 1 / T and its product with log2(e) are ordinary numbers
+        return als_fail_(ALS_ERR_INVALID_ARG, "als_distill_rows: temperature %g outside [1e-30, 1e30]", (double)temperature);
     const size_t need = als_distill_rows_workspace_bytes(dtype, n_rows, M, k);
     if (need && (!workspace || ws_bytes < need || (uintptr_t)workspace % 8))
         return als_fail_(ALS_ERR_WORKSPACE, "als_distill_rows: workspace too small or not 8-byte aligned: %zu < %zu", ws_bytes, need);

@@ -680,7 +680,8 @@ def sample_rows(score_rows, u, temperature=1.0, top_k=0, top_p=1.0, min_p=0.0, e
     """Random columns of every score row (float32, float16 or bfloat16), drawn from the row's softmax at `temperature` cut
     by min_p, top_k and top_p in this order (als_sample_rows in include/als_hip.h has the definition).  u: the random
     numbers, float32 or float64 in [0, 1), [n] for one draw per row or [n, d] for d draws with replacement.
-    temperature, top_k, top_p, min_p: one value for all rows, or a device tensor with one per row (float32; top_k int32);
+    temperature, top_k, top_p, min_p: one value for all rows, or a device tensor with one per row (float32; top_k int32).  A
+    single value is taken as a float32 too, as if a row's tensor held it (0.3 is then a little more than 0.3);
     top_k = 0, top_p = 1 and min_p = 0 are off, temperature = 0 takes the best item.
     exclude / exclude_rows: as topk_rows (those columns are set to -inf in the score rows first).
     Returns (idx int32, logp float32), shaped like u: the column and the logarithm of its probability; a row with
