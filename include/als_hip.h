@@ -453,8 +453,10 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  *                    (below 2^-14 of the user's largest, none by more than 2^-37 of that), of q - t in dY by one per item (below
  *                    2^-10 of the item's largest over the users, none by more than 2^-33 of that).  Gradients are summed over
  *                    parts of at most 32768 items or users (while that makes 512 parts or fewer), ln Z in float32 over 16
- *                    items and float64 above; the parts are joined in float32.  Weights may be of any size: what a user adds to dY is right beside any other's, down to 2^-126 of the
- *                    largest c x.  The weight of a user whose list is empty, or unknown, is not looked at.
+ *                    items and float64 above; the parts are joined in float32.  Weights may be of any size:
+ *                    what a user adds to dY is right beside any other's, down to 2^-126 of the largest c x (one 2^-e of the
+ *                    largest carries e in its exponentials' arguments: another e 2^-24 of its q).  The weight of a user whose
+ *                    list is empty, or who is unknown, is not looked at.
  *                    8 n M f operations, three products each.  Workspace, with F = f rounded up to 32, 64, 128 or 256: the
  *                    operands, 8 (n + M) F bytes; the parts of split sums, 4 F n each and, where pass 2 has more than one,
  *                    4 F M each; the lists, 8 n k; and where each list enters each block of 256 items (128 for F = 256),

@@ -287,6 +287,8 @@ class RecommenderALS:
         if self.mode != "train":
             raise RuntimeError("cannot call distill() when mode is not 'train'")
         if self.X is None:
+            if self.n_users is None or self.n_items is None:
+                raise RuntimeError("call input_data() first, or declare n_users and n_items")
             self._ensure_factors()
         users = np.asarray(users, dtype=np.int64).reshape(-1)
         if len(users) == 0:

@@ -80,3 +80,13 @@ def test_a_step_of_many_users_goes_in_several_calls(monkeypatch):
         model.distill(lists[:2], values[:2, :5], [1, 2], lr=0.1)
     with pytest.raises(ValueError):
         model.distill(lists[:2, 0], values[:2, 0], [1, 2], lr=0.1)
+
+
+def test_a_model_without_sizes_is_refused():
+    if not torch.cuda.is_available():
+        pytest.skip("needs a GPU")
+    import recommender_amd as ra
+    with pytest.raises(RuntimeError):
+        ra.RecommenderALS(als_kwargs=dict(f=8)).distill([[1]], [[1.0]], [0], lr=0.1)
+    model = ra.RecommenderALS(n_users=5, n_items=9, als_kwargs=dict(f=8))
+    assert np.isfinite(model.distill([[1, 2]], [[1.0, 0.5]], [3], lr=0.1))
