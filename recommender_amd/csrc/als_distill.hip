@@ -10,7 +10,8 @@
 // passes (maximum, sum, gradient) and its gradient written once.  1024 threads hold 65 536 float32 or 131 072 16-bit items;
 // longer rows are cut into parts of half that and take two launches, the second of which reads them again.  Whole calls on one
 // MI355X: 4096 x 59047 float32 398 us = 4.9 TB/s, what a copy of them takes; 2048 x 59047 bfloat16 119 us = 4.1 TB/s (a copy
-// 101: the exponentials of 16-bit rows cost twice as much per byte, two workgroups per compute unit hide most of it);
+// 101: the exponentials of 16-bit rows cost twice as much per byte, two workgroups per compute unit hide most of it, and at the
+// 64 registers that takes 7 to 9 of them spill, 32 to 40 bytes of scratch a lane);
 // 61 x 1000003 float32 124 us where one read and one write take 102.
 #include <hip/hip_runtime.h>
 
@@ -191,7 +192,7 @@ struct RowPart {
 #pragma unroll
             for (int e = 0; e < VEC; ++e) part += exp2_fast((RowView<TYPE>::value(held[q], e) - m) * c2);
             z += (double)part;
-            __builtin_amdgcn_sched_barrier(0);          // a chunk at a time: unrolled together they spill
+            __builtin_amdgcn_sched_barrier(0);          // a chunk at a time: unrolled together they spill more (NV = 8 spills 7 to 9 even so)
         }
         return z;
     }

@@ -7,8 +7,10 @@
 //   lists   per user: joins the parts, ln Z, the teacher's softmax, the loss, dX; and the list in item order.
 //   pass 2  items stationary, users streaming: s again, q = exp(s - ln Z_u), minus the listed t, dY += (q - t) (c_u x_u).
 // 8 n M f multiplications and additions, of which three products each: operands are two fp16 pieces of a value scaled by a
-// power of two (22 mantissa bits) and hi hi + hi lo + lo hi are accumulated in float32 - the accuracy of float32 products
-// at several times their rate.
+// power of two (22 mantissa bits) and hi hi + hi lo + lo hi are accumulated in float32 - about the accuracy of float32 products
+// at several times their rate.  A power of two for each factor, and where the values' range is not the factors' own each has its
+// own: a user's weights exp(s - maximum) in pass 1, a user's c x, and an item's q - t in pass 2 (cut to pieces times a power that
+// follows its largest; user_exp, and g in pass_kernel).
 //
 // A handful of users leaves such tiles mostly empty: they take als_distill_few.inc's vector kernels instead.
 //
@@ -21,12 +23,13 @@
 // 64 lanes x 16 bytes.  A stage is one tile: F / 4 KB, contiguous, copied to LDS by LDS-DMA.
 //
 // What bounds it (one MI355X).  24 n M f operations at the 1.18 PFLOP/s a large fp16 library product reaches here (at 1.6 GHz:
-// power) are 315 us at 4096 x 59047, f = 64, and 666 us at 1023 x 250001, f = 128; whole calls take 411 and 853.  Under a
-// profiler, which makes them 490 and 1020, the passes are 181 + 238 and 401 + 478 us: the matrix pipe is busy 68 and 46 % of their cycles at f = 64, 58 and 45 % at 128, and
+// power) are 315 us at 4096 x 59047, f = 64, and 666 us at 1023 x 250001, f = 128; whole calls take 437 to 455 and 882 to 921,
+// by box.  Under a profiler, which makes them 525 and 1056, the passes are 192 + 256 and 414 + 498 us: the matrix pipe is busy 64
+// and 44 % of their cycles at f = 64, 55 and 44 % at 128, and
 // vector instructions take the rest (per tile and wave at f = 64: 24 matrix instructions of 32 cycles, 16 exponentials of 16,
-// some 90 others of 4, which do not overlap them).  Pass 2 has the lists on top, and 231 blocks of items for 256 compute units.
-// The other launches are memory: laying out 14 and 86 us, lists 40 and 23, the maxima 5 and 32.  Small calls are launches
-// and latency: 64 x 9724, f = 20, 33 us in five launches.
+// some 100 others of 4, which do not overlap them).  Pass 2 has the lists on top, and 231 blocks of items for 256 compute units.
+// The other launches are memory: laying out 14 and 86 us, lists 43 and 25, the maxima 9 and 34.  Small calls are launches
+// and latency: 64 x 9724, f = 20, 37 us in five launches.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>

@@ -226,8 +226,9 @@ struct SplitOps {
 
 // Pieces of the GS k-steps of one stage into fragment registers [QB/2, QB/2 + GS/2); also bacc.
 // st.w holds sqrt(alpha r) here.
-// The elementwise work runs on pairs of adjacent factor indices (v_pk_mul_f32 / v_pk_add_f32 /
-// v_pk_fma_f32: two float32 operations per instruction, bit-identical to the scalar forms).
+// The bf16 form's elementwise work is written on pairs of adjacent factor indices where registers allow it.  (The pairs were laid
+// out for packed float32 instructions, which this library is built without, see the Makefile; as two single instructions
+// each they return the same bits.)
 __device__ __forceinline__ f32x2 trunc_bf16(const f32x2 x) { return f32x2{trunc_bf16(x.x), trunc_bf16(x.y)}; }
 template <int VW, int MODE = ALS_MODE_BF16X3>
 __device__ __forceinline__ void split_stage(const Stage<VW> &st, const int QB, SplitOps<VW> &o, float (&bacc)[VW]) {
@@ -437,7 +438,8 @@ __device__ __forceinline__ void reduce_b(float (&bacc)[VW]) {
 template <int VW>
 __device__ __forceinline__ void sym_tiles_matvec(const f32x4 (&T)[Geo<VW>::NT], const float (&v)[VW], float (&y)[VW],
                                                  const int lane) {
-    // register pairs: two multiply-adds per v_pk_fma_f32
+    // register pairs, as two multiply-adds each (packed ones, which this library is built without, halve their number: of 22
+    // steps per row at f = 128 the user half-sweep then takes 42.9 ms for 56.3)
     f32x4 vrow[VW];
     f32x2 olo[VW], ohi[VW], ocol[VW];
 #pragma unroll

@@ -8,7 +8,7 @@
 //      weight exceeds u W; its ln(w_i / W) is returned beside it.
 // Every step asks the same question - at which item, in rank order, does a running sum (of ones, or of weights) pass a
 // target - and the kernels have one answer to it (find): a histogram of the row over 512 or 2048 buckets of equal width in
-// the score gives the bucket, the bucket's few items are collected in LDS and ranked against each other.  Nothing is sorted.
+// the score gives the bucket, the bucket's few items are collected in LDS and ranked against each other.  Rows are not sorted.
 //
 // Weights are held as integers, round(w 2^Q) with Q = min(51, 62 - ceil(log2 M)): their sums are exact whatever the order,
 // so integer atomics do not make the result depend on timing, and a draw differs from the definition's only where u W lies
@@ -18,15 +18,17 @@
 // k + r, 2^(k mod 256 / 256) from a table, a polynomial of degree 4 in r; error below 1e-15.
 //
 // Two forms.  sample_rows_kernel: one workgroup per row, one launch; the row is read from memory for its maximum and for the
-// items that can matter, in one pass if they are few (filtered rows), and otherwise, mostly from the caches, twice more.
+// items that can matter, in one pass if they are few (filtered rows), and otherwise, mostly from the caches, twice more (and
+// once or more per window of the rank order where those are too many for LDS).
 // Few long rows are cut into parts, one workgroup each, in four launches: maximum; histogram; items of the buckets the
 // answers can lie in, collected in a list; the answers from the list.
 //
 // What bounds it (whole calls on one MI355X).  Filtered rows: the read, 4096 x 59047 float32 in 181 us = 5.3 TB/s (a plain
 // sum over them reads 4.0).  Rows of which much counts: vector instructions and LDS atomics; 1021 x 131071 bfloat16 with
-// 8 draws each takes 192 us, 185 000 cycles a row with two rows on a compute unit: about 40 000 for the maximum, 55 000 for
+// 8 draws each takes 190 us, 185 000 cycles a row with two rows on a compute unit: about 40 000 for the maximum, 55 000 for
 // counting the values, 40 000 for collecting, 40 000 for the draws.  Single rows: a chain of memory round trips and some
-// forty barriers, 19 us for 59 047 items; 10^6 items in four launches 37 us (5 + 9 + 11 + 13 and their gaps).
+// forty barriers, 19 us for 59 047 items; 10^6 items in four launches 37 us (under a profiler 5 + 9 + 11 + 13).  Rows of which
+// thousands of items matter to many draws: windows, see there.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
