@@ -249,7 +249,8 @@ __device__ __forceinline__ void cut(float v, _Float16 &hi, _Float16 &lo) {
     lo = (_Float16)(v - (float)hi);
 }
 
-__device__ __forceinline__ float power(const int e) { return ldexpf(1.f, e < -126 ? -126 : e > 126 ? 126 : e); }      // 2^e
+__device__ __forceinline__ int within(const int e) { return e < -126 ? -126 : e > 126 ? 126 : e; }
+__device__ __forceinline__ float power(const int e) { return ldexpf(1.f, within(e)); }      // 2^e
 
 // One tile of 32 rows per workgroup: through LDS, then both forms.  Tiles of Y first, then of X (whose row form carries
 // log2(e) / T and whose transposed form carries c_u 2^-user_exp).
@@ -292,12 +293,12 @@ __global__ __launch_bounds__(256) void prepare_kernel(const FactorArgs a) {
     mc = block_max256(mc, red);
     // both factors times a power of two that keeps them below 2^15, X times log2(e) / T besides
     const float to_log2 = a.inv_t * 1.44269504f;
-    const int ex = exponent(mx), ey = exponent(my), el = exponent(to_log2);
-    const float sy = power(15 - ey), sx = ldexpf(to_log2, -el) * power(15 - ex);
+    const int ex = within(15 - exponent(mx)), ey = within(15 - exponent(my)), el = exponent(to_log2);
+    const float sy = power(ey), sx = ldexpf(to_log2, -el) * power(ex);
     if (blockIdx.x == 0 && tid == 0) {
         const int top = mc > (float)NO_SHARE ? (int)mc : 0;
-        a.scales[0] = power(ex + el + ey - 30);
-        a.scales[1] = power(ey - 15);
+        a.scales[0] = power(el - ex - ey);
+        a.scales[1] = power(-ey);
         a.scales[2] = (float)(top - CX_TOP);
         a.scales[3] = (float)top;
     }
@@ -838,10 +839,10 @@ __global__ __launch_bounds__(256) void lists_kernel(const FactorArgs a) {
         for (int g = 1; g < GROUPS; ++g) o += o_sum[g][tid];
 #pragma unroll 3
         for (int g = 1; g < 16; ++g) listed += part[g][tid];
-        const float c = (a.weight ? a.weight[u] : 1.f) * a.inv_t, inv = a.scales[1] / z;
+        const float c = (a.weight ? a.weight[u] : 1.f) * a.inv_t, inv = 1.f / z, unit = a.scales[1];
 #pragma unroll
         for (int e = 0; e < 4; ++e)
-            if (4 * tid + e < f) a.dX[u * f + 4 * tid + e] = any ? c * (o[e] * inv - listed[e]) : 0.f;
+            if (4 * tid + e < f) a.dX[u * f + 4 * tid + e] = any ? c * (o[e] * inv * unit - listed[e]) : 0.f;
     }
 }
 
