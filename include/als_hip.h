@@ -398,7 +398,8 @@ int32_t als_recommend_topk_prepared_f32(const float *X, int64_t ldx, const int64
  * column -1 and logp -inf.  +inf scores share all the weight.  Weights are summed as integers of 2^-Q of the largest,
  * Q = min(51, 62 - ceil(log2 M)); an item below half of that counts as dropped.  The answer depends on the row and its
  * parameters alone.
- * Rows of at most 2^31 - 2^16 columns, at most 2^16 draws per row.
+ * Rows of at most 2^31 - 2^16 columns, at most als_sample_rows_max_draws draws per row: 2^16, and 2^34 / M of rows of more
+ * than 2^22 columns (what a draw costs where no list of candidates is short: up to a pass over the row by one workgroup).
  * opts      [host] one value for all rows, or a [device] array with one per row where the pointer is not NULL.  float32 either
  *           way: top_p = 0.3f is a little more than three tenths, which ten equal items share as four.
  * ex_*      as als_topk_rows_f32: those columns are set to -inf first, in place; columns outside [0, M) are ignored.
@@ -419,6 +420,7 @@ typedef struct {
     const float *min_p_rows;
 } als_sample_opts_t;
 size_t als_sample_rows_workspace_bytes(int32_t dtype, int64_t n_rows, int64_t M);
+int32_t als_sample_rows_max_draws(int64_t M);
 int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows, int64_t M, const int64_t *ex_rowptr,
                         const int32_t *ex_col, const int64_t *ex_row_ids, const als_sample_opts_t *opts, const void *u,
                         int32_t u_is_f64, int32_t n_draws, int32_t *idx_out, float *logp_out, void *workspace, size_t ws_bytes,

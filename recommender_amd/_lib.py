@@ -56,6 +56,7 @@ SIGNATURES = {
     "als_sample_rows": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_vp, c_vp, c_vp, c_i32, c_i32, c_vp, c_vp, c_vp,
                                 c_sz, c_vp]),
     "als_sample_rows_workspace_bytes": (c_sz, [c_i32, c_i64, c_i64]),
+    "als_sample_rows_max_draws": (c_i32, [c_i64]),
     "als_distill_rows": (c_i32, [c_vp, c_i32, c_i64, c_i64, c_i64, c_vp, c_vp, c_i64, c_i32, c_f32, c_vp, c_vp, c_vp, c_i64, c_vp, c_sz,
                                  c_vp]),
     "als_distill_topk_workspace_bytes": (c_sz, [c_i64, c_i64, c_i32, c_i32]),

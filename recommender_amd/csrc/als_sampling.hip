@@ -69,7 +69,10 @@ constexpr int SR_LISTED = 16384;      // cut rows: items collected per row
 // A row's draws: some microseconds each from a list in LDS, several of them side by side; where thousands of items matter, a share
 // of the passes over the row that a window takes (draw_from_windows).  65 536 draws, ms: 13 of a row of 1 000 003 equal scores,
 // 23 of five different ones, 210 of a normal distribution's, 1500 where all of it lies within one bucket of the histogram.
+// A window takes a pass of one workgroup, 0.3 ns an item (1.2 at the worst), and there are no more windows than draws or some
+// M / 1024: so that a launch ends within seconds, rows of more than 2^22 items are drawn from 2^34 / M times a call.
 constexpr int32_t DRAWS_MAX = 1 << 16;
+int32_t draws_max(const int64_t M) { return M <= (1 << 22) ? DRAWS_MAX : (int32_t)std::max<int64_t>(1, (1LL << 34) / M); }
 
 struct Found {            // an item collected by a workgroup of a cut row
     float score;
@@ -854,7 +857,7 @@ __device__ __forceinline__ void sort_window(const uint32_t n, const RowScale &c,
             // a wave's 64 pairs of up to 64 apart are 128 neighbours: until pairs are further apart no other wave touches them
             if (step > 64 || (step == 1 && run > 64)) __syncthreads();
             else {
-                __builtin_amdgcn_fence(__ATOMIC_RELEASE, "wavefront");
+                __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 __builtin_amdgcn_wave_barrier();
             }
         }
@@ -1735,13 +1738,15 @@ size_t als_sample_rows_workspace_bytes(int32_t dtype, int64_t n_rows, int64_t M)
     return cut_plan(dtype, n_rows, M).total;
 }
 
+int32_t als_sample_rows_max_draws(int64_t M) { return M < 1 || M > ROW_MAX ? 0 : draws_max(M); }
+
 int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows, int64_t M, const int64_t *ex_rowptr,
                         const int32_t *ex_col, const int64_t *ex_row_ids, const als_sample_opts_t *opts, const void *u,
                         int32_t u_is_f64, int32_t n_draws, int32_t *idx_out, float *logp_out, void *workspace, size_t ws_bytes,
                         void *stream) {
     if (!scores || !opts || !u || !idx_out || !logp_out)
         return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: null pointer");
-    if (n_rows < 1 || M < 1 || lds < M || M > ROW_MAX || n_rows > INT32_MAX || n_draws < 1 || n_draws > DRAWS_MAX)
+    if (n_rows < 1 || M < 1 || lds < M || M > ROW_MAX || n_rows > INT32_MAX || n_draws < 1 || n_draws > draws_max(M))
         return als_fail_(ALS_ERR_INVALID_ARG, "als_sample_rows: bad sizes (n_rows=%lld M=%lld lds=%lld n_draws=%d)", (long long)n_rows,
                          (long long)M, (long long)lds, n_draws);
     if (dtype < ALS_DTYPE_F32 || dtype > ALS_DTYPE_BF16)

@@ -717,6 +717,13 @@ def _launch_draws(score_rows, dtype, ld, u, temperature, top_k, top_p, min_p, ex
     logp = u.new_empty(u.shape, dtype=torch.float32)
     if n == 0:
         return idx, logp
+    if M > 1 << 22 and u.dim() == 2:                     # rows so long that a call takes fewer draws: in several
+        most = lib.als_sample_rows_max_draws(M)
+        if u.shape[1] > most:
+            for s in range(0, u.shape[1], most):
+                idx[:, s:s + most], logp[:, s:s + most] = _launch_draws(score_rows, dtype, ld, u[:, s:s + most].contiguous(), temperature,
+                                                                        top_k, top_p, min_p, ex_ptr, ex_col, exclude_rows)
+            return idx, logp
     need = lib.als_sample_rows_workspace_bytes(dtype, n, M)
     ws = torch.empty(need, dtype=torch.uint8, device=score_rows.device) if need else None
     opts = _lib.SampleOpts(t, k, p, m, _addr(t_rows), _addr(k_rows), _addr(p_rows), _addr(m_rows))

@@ -136,3 +136,20 @@ def test_a_draw_does_not_cost_a_pass(ops, kind):
             want, _, sure = definition(S[r], u[r], 1.0)
             assert torch.equal(idx[r][sure].long(), want[sure])
         assert ms < 5000.0, ms
+
+
+def test_more_draws_of_a_long_row_than_a_call_takes(ops):
+    """They go in several calls: the same answers as by hand, the exclusions made once or more."""
+    M, draws = (1 << 22) + 77, 5000
+    g = gen(11)
+    S = torch.randn(1, M, generator=g, device="cuda")
+    u = torch.rand(1, draws, generator=g, device="cuda", dtype=torch.float64)
+    ex = (torch.tensor([0, 3], device="cuda"), torch.tensor([5, 6, 7], dtype=torch.int32, device="cuda"))
+    S[0, 5:8] = 50.0
+    idx, logp = ops.sample_rows(S, u, temperature=0.5, top_k=3000, exclude=ex)
+    assert bool((S[0, 5:8] == -INF).all())
+    for a, b in ((0, 100), (4050, 4150), (4900, 5000)):
+        i, l = ops.sample_rows(S, u[:, a:b].contiguous(), temperature=0.5, top_k=3000)
+        assert torch.equal(i, idx[:, a:b]) and torch.equal(l, logp[:, a:b])
+    want, wl, sure = definition(S[0], u[0], 0.5, top_k=3000)
+    assert torch.equal(idx[0][sure].long(), want[sure]) and bool(sure.float().mean() > 0.95)
