@@ -452,7 +452,7 @@ int32_t als_sample_rows(void *scores, int32_t dtype, int64_t lds, int64_t n_rows
  *                    n_users, M <= 2^27; the factors must be finite.  Products of 22-bit operands accumulated in float32: two
  *                    fp16 pieces of a value scaled by one power of two per factor (values below 2^-18 of the factor's
  *                    largest lose bits); of c x by one per user (below 2^-18 of the user's largest); of q in dX by one per user
- *                    (below 2^-14 of the user's largest, none by more than 2^-37 of that), of q - t in dY by one per item (below
+ *                    (below 2^-11 of the largest of the part summed, none by more than 2^-34 of that), of q - t in dY by one per item (below
  *                    2^-10 of the item's largest over the users, none by more than 2^-33 of that).  Gradients are summed over
  *                    parts of at most 32768 items or users (while that makes 512 parts or fewer), ln Z in float32 over 16
  *                    items and float64 above; the parts are joined in float32.  Weights may be of any size:

@@ -23,8 +23,8 @@
 // 64 lanes x 16 bytes.  A stage is one tile: F / 4 KB, contiguous, copied to LDS by LDS-DMA.
 //
 // What bounds it (one MI355X).  24 n M f operations at the 1.18 PFLOP/s a large fp16 library product reaches here (at 1.6 GHz:
-// power) are 315 us at 4096 x 59047, f = 64, and 666 us at 1023 x 250001, f = 128; whole calls take 437 to 455 and 882 to 921,
-// by box.  Under a profiler, which makes them 525 and 1056, the passes are 192 + 256 and 414 + 498 us: the matrix pipe is busy 64
+// power) are 315 us at 4096 x 59047, f = 64, and 666 us at 1023 x 250001, f = 128; whole calls take 437 to 455 and 882 to 921
+// from card to card.  Under a profiler, which makes them 525 and 1056, the passes are 192 + 256 and 414 + 498 us: the matrix pipe is busy 64
 // and 44 % of their cycles at f = 64, 55 and 44 % at 128, and
 // vector instructions take the rest (per tile and wave at f = 64: 24 matrix instructions of 32 cycles, 16 exponentials of 16,
 // some 100 others of 4, which do not overlap them).  Pass 2 has the lists on top, and 231 blocks of items for 256 compute units.
@@ -58,10 +58,10 @@ constexpr int TILE = 32;                // rows per tile, of either factor
 constexpr int Y_MAX_BLOCKS = 1024, X_MAX_BLOCKS = 256;
 constexpr int64_t ROWS_MAX = 1 << 27;   // of either factor: a launch takes fewer than 2^32 threads along x, here 256 per tile
 constexpr int64_t GRID_X = 1 << 21;     // a workgroup per user: beyond that along y
-constexpr float P_OFFSET = 12.f;        // pass 1: p 2^12, and at most 2^3 above the running maximum's: below 2^16, fp16's largest
-constexpr float LAZY = 3.f;             // the running maximum follows when it lags by more than 2^3.  Offset and lag set what the
-                                        // lower piece still holds of a user's tail, 2^-37 of the largest; 2^-33 with 8 and 6, and
-                                        // fewer corrections, takes 0 to 1 % less time
+constexpr float P_OFFSET = 9.f;         // pass 1: p 2^9, and at most 2^6 above the running maximum's: below 2^16, fp16's largest
+constexpr float LAZY = 6.f;             // the running maximum follows when it lags by more than 2^6.  The lower piece holds a user's
+                                        // weights to 2^-34 of the largest in its part, which a part's 32768 items make 2^-19 of the
+                                        // sum.  (12 and 3, with more corrections: 2^-22 and 1 to 2 % more time)
 constexpr int Q_TOP = 15, Q_ROOM = 6;   // pass 2: an item's q - t times a power of two that keeps them below 2^Q_TOP; when one passes
                                         // that, the power is set so that Q_ROOM bits are free above it
 constexpr float NEVER = 1e30f;          // bias of a padding user: q = 0
@@ -160,16 +160,21 @@ __device__ __forceinline__ float max16(float v) {
 __device__ __forceinline__ bool any16(const bool v) { return (__ballot(v) >> (threadIdx.x & 48) & 0xffffu) != 0; }
 
 // Whether a user's list has an entry that counts: of an item listed twice the first stands.  By the sixteen lanes of its row.
-__device__ bool list_counts(const FactorArgs &a, const int64_t u, const int l) {
+// first / first_val: entries l, l + 16, .., which the caller has loaded (-1 behind the list's end).
+constexpr int FIRST = 8;
+__device__ bool list_counts(const FactorArgs &a, const int64_t u, const int l, const int32_t (&first)[FIRST], const float (&first_val)[FIRST]) {
     const int32_t *idx = a.t_idx + u * a.ldt;
     const float *val = a.t_val + u * a.ldt;
     bool good = false, masked = false;
-#pragma unroll 4
-    for (int p = l; p < a.k; p += 16) {
-        const bool in = idx[p] >= 0 && idx[p] < a.M, low = val[p] == -__builtin_inff();
+    auto see = [&](const int32_t i, const float v) {
+        const bool in = i >= 0 && i < a.M, low = v == -__builtin_inff();
         good |= in && !low;
         masked |= in && low;
-    }
+    };
+#pragma unroll
+    for (int q = 0; q < FIRST; ++q) see(first[q], first_val[q]);
+#pragma unroll 4
+    for (int p = l + 16 * FIRST; p < a.k; p += 16) see(idx[p], val[p]);
     good = any16(good);
     if (!good || !any16(masked)) return good;
     good = false;                                        // rare: only an item's first entry may count, and that may be a masked one
@@ -196,8 +201,9 @@ __device__ __forceinline__ int exponent(const float v) {
 template <bool VEC>
 __global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
     __shared__ float red[4];
-    const bool is_y = blockIdx.x < Y_MAX_BLOCKS;
-    const int b = is_y ? blockIdx.x : blockIdx.x - Y_MAX_BLOCKS, nb = is_y ? Y_MAX_BLOCKS : X_MAX_BLOCKS;
+    // the users' blocks first: theirs are chains of loads, beside which the items stream
+    const bool is_y = blockIdx.x >= X_MAX_BLOCKS;
+    const int b = is_y ? blockIdx.x - X_MAX_BLOCKS : blockIdx.x, nb = is_y ? Y_MAX_BLOCKS : X_MAX_BLOCKS;
     const int64_t rows = is_y ? a.M : a.n;
     float m = 0.f, mc = (float)NO_SHARE;
     // rows without gaps are one long row (500 000 x 33: 36 us otherwise); of others sixteen lanes take a row at a time
@@ -214,9 +220,19 @@ __global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
         if (b == 0 && rest < a.M * a.f) m = fmaxf(m, finite_abs(a.Y[rest]));
     }
     if (!flat) for (int64_t r = (int64_t)b * 16 + (threadIdx.x >> 4); r < rows; r += (int64_t)nb * 16) {
-        const float *row = is_y ? a.Y + r * a.ldy : user_row(a, r);
+        const int l = threadIdx.x & 15;
         const float w = !is_y && a.weight ? a.weight[r] : 1.f;
-        const bool counts = !is_y && list_counts(a, r, threadIdx.x & 15);      // beside the user's id, not behind its row
+        int32_t first[FIRST];
+        float first_val[FIRST];
+        if (!is_y) {                                     // under way beside the user's id
+#pragma unroll
+            for (int q = 0; q < FIRST; ++q) {
+                const int p = l + 16 * q;
+                first[q] = p < a.k ? a.t_idx[r * a.ldt + p] : -1;
+                first_val[q] = p < a.k ? a.t_val[r * a.ldt + p] : 0.f;
+            }
+        }
+        const float *row = is_y ? a.Y + r * a.ldy : user_row(a, r);
         float mr = 0.f;
         if (row)
             for (int k = 4 * (threadIdx.x & 15); k < a.f; k += 64) {
@@ -227,17 +243,17 @@ __global__ __launch_bounds__(256) void maxima_kernel(const FactorArgs a) {
         m = fmaxf(m, mr);
         if (!is_y) {                                     // all sixteen lanes: r is one for them
             mr = max16(mr);
-            const bool share = row && counts && mr > 0.f && w != 0.f;
+            const bool share = list_counts(a, r, l, first, first_val) && row && mr > 0.f && w != 0.f;
             const int e = share ? exponent(mr) + exponent(w) + exponent(a.inv_t) : NO_SHARE;
-            if ((threadIdx.x & 15) == 0) a.user_exp[r] = e;
+            if (l == 0) a.user_exp[r] = e;
             if (fabsf(w) < __builtin_inff()) mc = fmaxf(mc, (float)e);
         }
     }
     m = block_max256(m, red);
     mc = block_max256(mc, red);
     if (threadIdx.x == 0) {
-        a.maxima[blockIdx.x] = m;
-        if (!is_y) a.maxima[blockIdx.x + X_MAX_BLOCKS] = mc;
+        a.maxima[is_y ? b : Y_MAX_BLOCKS + b] = m;
+        if (!is_y) a.maxima[Y_MAX_BLOCKS + X_MAX_BLOCKS + b] = mc;
     }
 }
 
