@@ -153,3 +153,34 @@ def test_more_draws_of_a_long_row_than_a_call_takes(ops):
         assert torch.equal(i, idx[:, a:b]) and torch.equal(l, logp[:, a:b])
     want, wl, sure = definition(S[0], u[0], 0.5, top_k=3000)
     assert torch.equal(idx[0][sure].long(), want[sure]) and bool(sure.float().mean() > 0.95)
+
+
+def test_windows_in_a_graph_and_on_two_streams(ops):
+    """Rows cut over workgroups and rows of one, many draws each; replays with the program's own work between them."""
+    g = gen(12)
+    cases = []
+    for n, M, kind in ((1, 200003, "equal"), (2, 300007, "normal"), (3, 40001, "five"), (2, 40001, "normal")):
+        S = rows_of_kind(kind, n, M, g)
+        u = torch.rand(n, 500, generator=g, device="cuda")
+        cases.append((S, u))
+    calls = [lambda S=S, u=u: ops.sample_rows(S, u, temperature=1.0, top_p=0.99) for S, u in cases]
+    want = [c() for c in calls]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = [c() for c in calls]
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for _ in range(4):
+        graph.replay()
+        (torch.randn(700, 700, device="cuda") * 2).sum()
+        torch.cuda.synchronize()
+        for (i, l), (wi, wl) in zip(out, want):
+            assert torch.equal(i, wi) and torch.equal(l, wl)
+            i.zero_(); l.zero_()
+        got = []
+        for k, c in enumerate(calls):
+            with torch.cuda.stream(streams[k % 2]):
+                got.append(c())
+        torch.cuda.synchronize()
+        for (i, l), (wi, wl) in zip(got, want):
+            assert torch.equal(i, wi) and torch.equal(l, wl)
