@@ -23,13 +23,13 @@
 // 64 lanes x 16 bytes.  A stage is one tile: F / 4 KB, contiguous, copied to LDS by LDS-DMA.
 //
 // What bounds it (one MI355X).  24 n M f operations at the 1.18 PFLOP/s a large fp16 library product reaches here (at 1.6 GHz:
-// power) are 315 us at 4096 x 59047, f = 64, and 666 us at 1023 x 250001, f = 128; whole calls take 437 to 455 and 882 to 921
-// from card to card.  Under a profiler, which makes them 525 and 1056, the passes are 192 + 256 and 414 + 498 us: the matrix pipe is busy 64
-// and 44 % of their cycles at f = 64, 55 and 44 % at 128, and
+// power) are 315 us at 4096 x 59047, f = 64, and 666 us at 1023 x 250001, f = 128; whole calls take 423 to 436 and 873 to 882
+// from card to card.  Under a profiler, which makes them 497 and 1018, the passes are 178 + 247 and 396 + 479 us: the matrix pipe is
+// busy 66 and 44 % of their cycles at f = 64, 57 and 44 % at 128, and
 // vector instructions take the rest (per tile and wave at f = 64: 24 matrix instructions of 32 cycles, 16 exponentials of 16,
 // some 100 others of 4, which do not overlap them).  Pass 2 has the lists on top, and 231 blocks of items for 256 compute units.
-// The other launches are memory: laying out 14 and 86 us, lists 43 and 25, the maxima 9 and 34.  Small calls are launches
-// and latency: 64 x 9724, f = 20, 37 us in five launches.
+// The other launches are memory: laying out 14 and 86 us, lists 42 and 25, the maxima 6 and 32.  Small calls are launches
+// and latency: 64 x 9724, f = 20, 36 us in five launches.
 #include <hip/hip_runtime.h>
 
 #include <algorithm>
@@ -442,7 +442,7 @@ __global__ __launch_bounds__(WAVES * 64, F <= 64 ? 4 : 1) void pass_kernel(const
     asm volatile("" : "+s"(one));
     // pass 2: O is sum_u (q - t) g x_u.  One g for all items would leave the q of a large catalogue, 10^-6 of the t's, few bits
     // (16 at a million items); so each item (a lane and its other half's lane) has its own, which follows its largest
-    // |q - t| downwards and leaves that one its 22 bits (f = 64: 433 us, 425 with one g; f = 128: 887 and 875).
+    // |q - t| downwards and leaves that one its 22 bits (f = 64: 433 us a call, 425 with one g; f = 128: 887 and 875).
     float g = 0x1p126f;                                  // |q - t| <= 1: a new one is 2^8 at the least
 
     // ---- pass 2: the lists of the streaming users, as a dense tile [item of the block, user of the stage] that is zero but
