@@ -16,6 +16,7 @@ import re
 import subprocess
 import sys
 import tempfile
+from concurrent.futures import ThreadPoolExecutor
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 CSRC = os.path.join(ROOT, "recommender_amd", "csrc")
@@ -146,7 +147,11 @@ def assembly_of(src):
 
 
 def main(argv):
-    texts = [(p, open(p).read()) for p in argv] if argv else [(s, assembly_of(os.path.join(CSRC, s))) for s in SOURCES]
+    if argv:
+        texts = [(p, open(p).read()) for p in argv]
+    else:
+        with ThreadPoolExecutor(len(SOURCES)) as pool:           # the compiler is another process each
+            texts = list(zip(SOURCES, pool.map(lambda s: assembly_of(os.path.join(CSRC, s)), SOURCES)))
     total = n_dpp = 0
     for name, text in texts:
         n_dpp += len(re.findall(r"^\s*v_\w+_dpp\s", text, flags=re.M))
